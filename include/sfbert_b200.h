@@ -275,6 +275,52 @@ int sfb_linear_residual(sfb_stream_t stream, void *out, const void *x, const voi
 int sfb_embedding(sfb_stream_t stream, void *out, const void *table, const int32_t *ids, const void *pos,
                   uint32_t batch, uint32_t seq_len, uint32_t hidden, uint32_t vocab, int dtype, uint32_t *bad_ids);
 
+/* ---- what logits are turned into: scores, losses, answers ---------------------------------------------- */
+
+/* Rows of logits [rows, vocab] of type dtype, `pitch` elements from row to row (any alignment of whole elements); scale > 0
+ * multiplies every logit (1 / temperature).  With m the largest logit of a row and l = log sum_j exp(scale (x_j - m)):
+ *   stats [rows][2] = m, l                                      (-inf, -inf where every logit is -inf)
+ *   logp [rows] = scale (x_t - m) - l for t = targets[row]      (targets and logp NULL: not asked for)
+ *   entropy [rows] = -sum_j p_j log p_j                          (NULL: not asked for; 0 where every logit is -inf)
+ *   top_logp, top_ids [rows][top_k]: the top_k (0 to 128) largest, in descending order, equal ones by ascending index; where fewer
+ *     tokens have a logit above -inf the rest is -inf and -1
+ * all fp32 (ids int32).  A target outside [0, vocab) -- a row without one -- gives a logp of 0; it is counted in *missed
+ * (device uint32, may be NULL), and unless entropy or alternatives are asked for its row is not read and its stats are 0.  A NaN
+ * or +inf among a row's logits makes its results NaN (its alternatives' ids -1).  Sums are fp32.  vocab is at most 2^30, with
+ * alternatives 2^19. */
+int sfb_token_logprobs(sfb_stream_t stream, const void *logits, uint64_t pitch, const int32_t *targets, uint32_t rows,
+                       uint32_t vocab, int dtype, float scale, float *logp, float *stats, float *entropy,
+                       float *top_logp, int32_t *top_ids, uint32_t top_k, uint32_t *missed);
+
+/* The gradient of the above: out [rows, width] (type dtype, out_pitch elements from row to row, may be logits itself)
+ *   = scale (dlogp (d_jt - p_j) - dentropy p_j (log p_j + entropy))       for j < vocab, 0 for vocab <= j < width.
+ * stats, entropy as sfb_token_logprobs gave them; entropy and dentropy may both be NULL.  A row without a target has no
+ * dlogp term; without dentropy it is zeros and not read.  targets and dlogp are required. */
+int sfb_token_logprobs_grad(sfb_stream_t stream, const void *logits, uint64_t pitch, const int32_t *targets, const float *stats,
+                            const float *dlogp, const float *entropy, const float *dentropy, void *out, uint64_t out_pitch,
+                            uint32_t rows, uint32_t vocab, uint32_t width, int dtype, float scale);
+
+/* Distillation from a teacher's list of k (1 to 128) tokens per row: ids int32 [rows][k], teacher fp32 [rows][k] their log
+ * probabilities at the temperature (what sfb_token_logprobs gives as alternatives); logits are the student's, p their softmax:
+ *   tail 0: q = softmax(teacher) over the list,            loss = sum_k q_k (log q_k - log p_k)
+ *   tail 1: q = exp(teacher), q_r = max(0, 1 - sum_k q_k),  loss = sum_k q_k (log q_k - log p_k) + q_r (log q_r - log p_r)
+ * with p_r what the student leaves to the tokens that are not listed (summed over them; where that is nothing the term is
+ * left out).  An id outside [0, vocab) is no entry: its weight is 0, it is counted in *missed (may be NULL).  The same id
+ * twice is two entries of one token.  stats [rows][2 + tail] = m, l and with tail the log of the unlisted tokens' sum beside m.
+ * The loss carries no factor for the temperature.  vocab is at most 2^30, with tail 2^20. */
+int sfb_distill_topk(sfb_stream_t stream, const void *logits, uint64_t pitch, const int32_t *ids, const float *teacher,
+                     uint32_t rows, uint32_t vocab, uint32_t k, int dtype, float scale, int tail, float *loss, float *stats,
+                     uint32_t *missed);
+
+/* Its gradient: out = scale dloss (Q p_j - q_j), Q the sum of the q; with tail, for tokens that are not listed, scale dloss
+ * p_j (Q - q_r / p_r).  targets, token_stats and dlogp (all or none): + dlogp (d_jt - p1_j), the hard label's share with p1 the
+ * softmax at scale 1 and token_stats its stats [rows][2] from sfb_token_logprobs.  Columns from vocab to width: 0.  out may be
+ * logits itself. */
+int sfb_distill_topk_grad(sfb_stream_t stream, const void *logits, uint64_t pitch, const int32_t *ids, const float *teacher,
+                          const float *stats, const float *dloss, const int32_t *targets, const float *token_stats,
+                          const float *dlogp, void *out, uint64_t out_pitch, uint32_t rows, uint32_t vocab, uint32_t width,
+                          uint32_t k, int dtype, float scale, int tail);
+
 /* ---- element-sparse (CSR) attention: the alternative format the reference prototypes ------------------ */
 
 /* The CSR pattern of a block layout (ONE head, uint8 [nb][nb]): every element of every kept block, columns ascending.

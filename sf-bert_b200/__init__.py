@@ -28,7 +28,7 @@ SYMBOLS = [
     "sfb_masked_softmax_grad", "sfb_linear", "sfb_linear_nt", "sfb_embedding", "sfb_csr_from_layout",
     "sfb_csr_attention", "sfb_rowdot", "sfb_fused_sddmm_softmax_grad", "sfb_fused_attention_slice", "sfb_device_status_clear",
     "sfb_linear_residual", "sfb_attention_backward", "sfb_csr_workspace",
-    "sfb_csr_attention_planned",
+    "sfb_csr_attention_planned", "sfb_token_logprobs", "sfb_token_logprobs_grad", "sfb_distill_topk", "sfb_distill_topk_grad",
 ]
 
 if not os.path.exists(LIB_PATH):
@@ -77,6 +77,10 @@ lib.sfb_attention_backward.argtypes = [_vp] * 13 + [_i32] + [_u32] * 10 + [_f32]
 lib.sfb_csr_workspace.argtypes = [_u32, _u32]
 lib.sfb_csr_workspace.restype = _u64
 lib.sfb_csr_attention_planned.argtypes = [_vp, _vp, _vp, _u32, _vp, _vp, _vp, _vp, _i32, _u32, _u32, _u32, _u32, _f32, _vp, _vp]
+lib.sfb_token_logprobs.argtypes = [_vp, _vp, _u64, _vp, _u32, _u32, _i32, _f32] + [_vp] * 5 + [_u32, _vp]
+lib.sfb_token_logprobs_grad.argtypes = [_vp, _vp, _u64] + [_vp] * 6 + [_u64, _u32, _u32, _u32, _i32, _f32]
+lib.sfb_distill_topk.argtypes = [_vp, _vp, _u64, _vp, _vp, _u32, _u32, _u32, _i32, _f32, _i32, _vp, _vp, _vp]
+lib.sfb_distill_topk_grad.argtypes = [_vp, _vp, _u64] + [_vp] * 8 + [_u64, _u32, _u32, _u32, _u32, _i32, _f32, _i32]
 
 
 def device_status():
@@ -304,6 +308,42 @@ def bias_residual_layernorm(x, bias, resid, gain, beta, want_sum=False, out=None
 def bias_gelu(x, bias, out=None):
     """(x + bias) * sigmoid(1.702 (x + bias)) (tensor_add_vector_gpu_2048 + gelu_gpu_v2, cuda_kernels.h:471,561)."""
     return _host.bias_gelu(x, bias, out)
+
+
+def token_logprobs(logits, targets=None, vocab=None, scale=1.0, entropy=False, top_k=0):
+    """Log probabilities of given tokens under softmax(scale * logits), with entropy and the top_k (at most 128) most probable
+    tokens, in one pass over the logits: what linear_nt's result is scored by.
+
+    logits [..., width] (fp32, bf16 or fp16; rows contiguous and at one pitch), targets int32 [...] or None.  vocab: how many
+    columns are tokens (the rest is padding, as a table padded to a multiple of 16 leaves it).  Returns (logp, stats, entropy,
+    top_logp, top_ids, missed), fp32 and int32, None for what was not asked for: stats [..., 2] holds each row's largest logit m
+    and log sum exp(scale (x - m)), which the gradient needs.  Alternatives are in descending order, equal ones by ascending index; tokens at
+    -inf are none (id -1, -inf).  A target outside [0, vocab) gives 0 and is counted in missed; such rows are not
+    read (stats 0) unless entropy or alternatives are asked for."""
+    return _host.token_logprobs(logits, targets, vocab, scale, entropy, top_k)
+
+
+def token_logprobs_grad(logits, targets, stats, dlogp, entropy=None, dentropy=None, vocab=None, scale=1.0, out=None):
+    """The gradient of token_logprobs' logp and entropy with respect to the logits (in their type and layout; out may be logits):
+    scale * (dlogp * (onehot - p) - dentropy * p * (log p + entropy)).  dlogp and dentropy are fp32 [...]; columns from vocab on
+    get 0.  The alternatives' log probabilities have no gradient."""
+    return _host.token_logprobs_grad(logits, targets, stats, dlogp, entropy, dentropy, vocab, scale, out)
+
+
+def distill_topk(logits, ids, teacher, vocab=None, scale=1.0, tail=False):
+    """KL divergence of the student's softmax(scale * logits) from a teacher's list of at most 128 tokens: ids int32 [..., k] and
+    teacher fp32 [..., k], their log probabilities at the temperature (token_logprobs(teacher_logits, scale=scale, top_k=k)).
+    The list is renormalised, or with tail=True what it leaves is one more class beside what the student leaves to unlisted
+    tokens.  Ids outside [0, vocab) are no entries (lists of uneven length) and are counted.  Returns (loss [...],
+    stats [..., 2] or with tail [..., 3], missed).  The loss has no factor for the temperature."""
+    return _host.distill_topk(logits, ids, teacher, vocab, scale, tail)
+
+
+def distill_topk_grad(logits, ids, teacher, stats, dloss, vocab=None, scale=1.0, tail=False, targets=None, token_stats=None, dlogp=None,
+                      out=None):
+    """The gradient of distill_topk's loss with respect to the student's logits (out may be logits).  With targets, token_stats and dlogp
+    (token_logprobs' stats at scale 1) the hard label's gradient dlogp * (onehot - softmax(logits)) is added in the same pass."""
+    return _host.distill_topk_grad(logits, ids, teacher, stats, dloss, vocab, scale, tail, targets, token_stats, dlogp, out)
 
 
 def encoder_layer_tensor(x2d, w, lay, heads, ln_order, scale):

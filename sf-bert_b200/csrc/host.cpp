@@ -7,6 +7,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 #include <ATen/ATen.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <cmath>
 #include <string>
@@ -19,7 +20,8 @@ namespace {
     X(sfb_last_error) X(sfb_bst_sgemm_nt) X(sfb_masked_softmax) X(sfb_bst_sgemm_xn) X(sfb_masked_softmax_grad) X(sfb_linear) \
     X(sfb_linear_nt) X(sfb_linear_residual) X(sfb_embedding) X(sfb_csr_attention) X(sfb_csr_attention_planned) X(sfb_csr_workspace) X(sfb_rowdot) X(sfb_fused_sddmm_softmax_grad)                  \
     X(sfb_fused_sddmm_softmax) X(sfb_fused_attention) X(sfb_fused_attention_slice) X(sfb_bias_residual_layernorm)         \
-    X(sfb_bias_gelu) X(sfb_attention_backward)
+    X(sfb_bias_gelu) X(sfb_attention_backward) X(sfb_token_logprobs) X(sfb_token_logprobs_grad) X(sfb_distill_topk)      \
+    X(sfb_distill_topk_grad)
 struct Lib {
 #define DECL(f) decltype(&::f) f = nullptr;
     SFB_FUNCTIONS(DECL)
@@ -532,6 +534,181 @@ FUNCTION(py_attention_backward, 8)
     return PyTuple_Pack(3, x.o, y.o, z.o);
 }
 
+// ---- logits ------------------------------------------------------------------------------------------------------------------
+// [..., width] logits as rows at one pitch
+struct LogitRows {
+    const at::Tensor &t;
+    int64_t rows = 1, width, pitch;
+    explicit LogitRows(const at::Tensor &x) : t(x)
+    {
+        require(x.dim() >= 1, "logits must have a last dimension");
+        width = x.size(-1);
+        pitch = width;
+        require(width >= 1 && width <= (1ll << 30) && (x.stride(-1) == 1 || width == 1), "a row of logits must be contiguous, of 1 to 2^30 elements");
+        bool inner = true;                    // no dimension of more than one row so far
+        int64_t next = 0;
+        for (int64_t i = x.dim() - 2; i >= 0; i--) {
+            const int64_t n = x.size(i);
+            if (n != 1 && x.numel()) {
+                require(inner ? x.stride(i) >= width : x.stride(i) == next, "the rows of logits must lie at one pitch");
+                if (inner) pitch = x.stride(i);
+                next = x.stride(i) * n;
+                inner = false;
+            }
+            rows *= n;
+        }
+        require(rows < (1ll << 27), "too many rows of logits");
+    }
+    at::IntArrayRef lead() const { return t.sizes().slice(0, t.dim() - 1); }
+    int64_t bytes() const { return rows ? ((rows - 1) * pitch + width) * t.element_size() : 0; }
+};
+// a tensor that goes with the rows: contiguous, of this type, its sizes those of the rows and then `last` (0: nothing more)
+const at::Tensor &beside(PyObject *o, const LogitRows &x, at::ScalarType type, int64_t last, const char *text)
+{
+    const at::Tensor &t = tensor(o);
+    const int64_t dims = x.t.dim() - 1 + (last ? 1 : 0);
+    require(t.scalar_type() == type && t.is_contiguous() && t.dim() == dims && t.device() == x.t.device() &&
+                t.sizes().slice(0, x.t.dim() - 1) == x.lead() && (!last || t.size(-1) == last), text);
+    return t;
+}
+template <typename T> inline T *ptr_of(PyObject *o, const LogitRows &x, at::ScalarType type, int64_t last, const char *text)
+{
+    return o == Py_None ? nullptr : (T *)ptr(beside(o, x, type, last, text));
+}
+inline int64_t vocab_or_width(PyObject *o, const LogitRows &x)
+{
+    const int64_t v = o == Py_None ? x.width : (int64_t)integer(o);
+    require(v >= 1 && v <= x.width, "vocab must be 1 to the number of columns");
+    return v;
+}
+inline void require_cuda(const at::Tensor &t) { require(t.is_cuda(), "expected a tensor on a CUDA device"); }
+// The calls below run on the device of their tensors, on its current stream, whichever device is the current one.
+inline sfb_stream_t stream_of(const at::Tensor &t) { return (sfb_stream_t)c10::cuda::getCurrentCUDAStream(t.device().index()).stream(); }
+inline at::Tensor rows_like(const LogitRows &x, int64_t last, at::ScalarType type)
+{
+    std::vector<int64_t> size(x.lead().begin(), x.lead().end());
+    if (last) size.push_back(last);
+    return empty(size, type, x.t);
+}
+// the gradient's tensor: laid out as the logits, or the caller's
+at::Tensor grad_out(PyObject *out, const LogitRows &x)
+{
+    if (out == Py_None) return x.t.is_contiguous() ? empty(x.t.sizes(), x.t.scalar_type(), x.t) : at::empty_strided(x.t.sizes(), x.t.strides(), x.t.options());
+    const at::Tensor &o = tensor(out);
+    require(o.sizes() == x.t.sizes() && o.scalar_type() == x.t.scalar_type() && o.device() == x.t.device(), "out must be like the logits");
+    const LogitRows r(o);
+    const char *a = (const char *)ptr(o), *b = (const char *)ptr(x.t);
+    require((a == b && r.pitch == x.pitch) || a + r.bytes() <= b || b + x.bytes() <= a, "out must be the logits themselves or memory of its own");
+    return o;
+}
+inline float positive_scale(PyObject *o)
+{
+    const float s = (float)number(o);
+    require(s > 0.f && s <= 1e6f, "scale must be positive (and at most 1e6)");
+    return s;
+}
+const char *const bad_targets = "targets must be contiguous int32, one per row of logits, on their device";
+const char *const bad_floats = "a float tensor does not go with the logits (contiguous fp32, one element per row, on their device)";
+const char *const bad_stats = "stats must be the contiguous fp32 tensor that the forward call gave, on the logits' device";
+const char *const bad_lists = "ids and teacher must be contiguous int32 and fp32 [..., k] tensors, one list per row of logits, on their device";
+
+// (logits, targets, vocab, scale, entropy, top_k) -> (logp, stats, entropy, top_logp, top_ids, missed)
+FUNCTION(py_token_logprobs, 6)
+{
+    const LogitRows x(tensor(a[0]));
+    const int64_t vocab = vocab_or_width(a[2], x);
+    const float scale = positive_scale(a[3]);
+    const bool ent = truth(a[4]);
+    const long k = integer(a[5]);
+    const int t = tag(x.t);
+    require(k >= 0 && k <= 128 && k <= vocab, "top_k must be 0 to 128 and at most vocab");
+    require(k == 0 || vocab <= (1 << 19), "alternatives need a vocab of at most 2^19");
+    const int32_t *targets = ptr_of<int32_t>(a[1], x, at::kInt, 0, bad_targets);
+    require_cuda(x.t);
+    const c10::cuda::CUDAGuard on(x.t.device());
+    at::Tensor stats = rows_like(x, 2, at::kFloat), missed = empty({1}, at::kInt, x.t), logp, entropy, top_logp, top_ids;
+    if (a[1] != Py_None) logp = rows_like(x, 0, at::kFloat);
+    if (ent) entropy = rows_like(x, 0, at::kFloat);
+    if (k) { top_logp = rows_like(x, k, at::kFloat); top_ids = rows_like(x, k, at::kInt); }
+    auto p = [](const at::Tensor &o) { return o.defined() ? (float *)ptr(o) : nullptr; };
+    call(L.sfb_token_logprobs, stream_of(x.t), ptr(x.t), (uint64_t)x.pitch, targets, (uint32_t)x.rows, (uint32_t)vocab, t, scale, p(logp), p(stats),
+         p(entropy), p(top_logp), k ? (int32_t *)ptr(top_ids) : nullptr, (uint32_t)k, (uint32_t *)ptr(missed));
+    PyObject *r = PyTuple_New(6);
+    if (!r) throw Raised();
+    const at::Tensor *all[6] = {&logp, &stats, &entropy, &top_logp, &top_ids, &missed};
+    for (int i = 0; i < 6; i++) {
+        PyObject *o = all[i]->defined() ? wrap(*all[i]) : Py_NewRef(Py_None);
+        if (!o) { Py_DECREF(r); throw Raised(); }
+        PyTuple_SET_ITEM(r, i, o);
+    }
+    return r;
+}
+// (logits, targets, stats, dlogp, entropy, dentropy, vocab, scale, out) -> dlogits
+FUNCTION(py_token_logprobs_grad, 9)
+{
+    const LogitRows x(tensor(a[0]));
+    const int64_t vocab = vocab_or_width(a[6], x);
+    const float scale = positive_scale(a[7]);
+    const int t = tag(x.t);
+    const int32_t *targets = (int32_t *)ptr(beside(a[1], x, at::kInt, 0, bad_targets));
+    const float *stats = (float *)ptr(beside(a[2], x, at::kFloat, 2, bad_stats)), *dlogp = (float *)ptr(beside(a[3], x, at::kFloat, 0, bad_floats));
+    const float *entropy = ptr_of<float>(a[4], x, at::kFloat, 0, bad_floats), *dentropy = ptr_of<float>(a[5], x, at::kFloat, 0, bad_floats);
+    require((a[4] == Py_None) == (a[5] == Py_None), "entropy and dentropy go together");
+    require_cuda(x.t);
+    const c10::cuda::CUDAGuard on(x.t.device());
+    at::Tensor out = grad_out(a[8], x);
+    call(L.sfb_token_logprobs_grad, stream_of(x.t), ptr(x.t), (uint64_t)x.pitch, targets, stats, dlogp, entropy, dentropy, ptr(out),
+         (uint64_t)LogitRows(out).pitch, (uint32_t)x.rows, (uint32_t)vocab, (uint32_t)x.width, t, scale);
+    return wrap(out);
+}
+// the length of the lists: ids [..., k]
+inline int64_t list_length(PyObject *ids)
+{
+    const at::Tensor &t = tensor(ids);
+    require(t.dim() >= 1 && t.size(-1) >= 1 && t.size(-1) <= 128, "a list must have 1 to 128 entries");
+    return t.size(-1);
+}
+// (logits, ids, teacher, vocab, scale, tail) -> (loss, stats, missed)
+FUNCTION(py_distill_topk, 6)
+{
+    const LogitRows x(tensor(a[0]));
+    const int64_t vocab = vocab_or_width(a[3], x), k = list_length(a[1]);
+    const float scale = positive_scale(a[4]);
+    const bool tail = truth(a[5]);
+    const int t = tag(x.t);
+    require(!tail || vocab <= (1 << 20), "the remainder needs a vocab of at most 2^20");
+    const int32_t *ids = (int32_t *)ptr(beside(a[1], x, at::kInt, k, bad_lists));
+    const float *teacher = (float *)ptr(beside(a[2], x, at::kFloat, k, bad_lists));
+    require_cuda(x.t);
+    const c10::cuda::CUDAGuard on(x.t.device());
+    at::Tensor loss = rows_like(x, 0, at::kFloat), stats = rows_like(x, tail ? 3 : 2, at::kFloat), missed = empty({1}, at::kInt, x.t);
+    call(L.sfb_distill_topk, stream_of(x.t), ptr(x.t), (uint64_t)x.pitch, ids, teacher, (uint32_t)x.rows, (uint32_t)vocab, (uint32_t)k, t, scale,
+         (int)tail, (float *)ptr(loss), (float *)ptr(stats), (uint32_t *)ptr(missed));
+    Ref l(wrap(loss)), s(wrap(stats)), n(wrap(missed));
+    return PyTuple_Pack(3, l.o, s.o, n.o);
+}
+// (logits, ids, teacher, stats, dloss, vocab, scale, tail, targets, token_stats, dlogp, out) -> dlogits
+FUNCTION(py_distill_topk_grad, 12)
+{
+    const LogitRows x(tensor(a[0]));
+    const int64_t vocab = vocab_or_width(a[5], x), k = list_length(a[1]);
+    const float scale = positive_scale(a[6]);
+    const bool tail = truth(a[7]);
+    const int t = tag(x.t);
+    const int32_t *ids = (int32_t *)ptr(beside(a[1], x, at::kInt, k, bad_lists));
+    const float *teacher = (float *)ptr(beside(a[2], x, at::kFloat, k, bad_lists));
+    const float *stats = (float *)ptr(beside(a[3], x, at::kFloat, tail ? 3 : 2, bad_stats)), *dloss = (float *)ptr(beside(a[4], x, at::kFloat, 0, bad_floats));
+    require((a[8] == Py_None) == (a[9] == Py_None) && (a[8] == Py_None) == (a[10] == Py_None), "targets, token_stats and dlogp go together");
+    const int32_t *targets = ptr_of<int32_t>(a[8], x, at::kInt, 0, bad_targets);
+    const float *token_stats = ptr_of<float>(a[9], x, at::kFloat, 2, bad_stats), *dlogp = ptr_of<float>(a[10], x, at::kFloat, 0, bad_floats);
+    require_cuda(x.t);
+    const c10::cuda::CUDAGuard on(x.t.device());
+    at::Tensor out = grad_out(a[11], x);
+    call(L.sfb_distill_topk_grad, stream_of(x.t), ptr(x.t), (uint64_t)x.pitch, ids, teacher, stats, dloss, targets, token_stats, dlogp, ptr(out),
+         (uint64_t)LogitRows(out).pitch, (uint32_t)x.rows, (uint32_t)vocab, (uint32_t)x.width, (uint32_t)k, t, scale, (int)tail);
+    return wrap(out);
+}
+
 // bind(addresses by name): which build of the library the functions call
 PyObject *py_bind(PyObject *, PyObject *args)
 {
@@ -562,6 +739,7 @@ PyMethodDef methods[] = {
     ENTRY(bst_sgemm_nt), ENTRY(masked_softmax), ENTRY(bst_sgemm), ENTRY(masked_softmax_grad), ENTRY(rowdot), ENTRY(fused_sddmm_softmax_grad),
     ENTRY(fused_sddmm_softmax), ENTRY(linear), ENTRY(embedding), ENTRY(csr_attention), ENTRY(fused_attention), ENTRY(fused_attention_slice),
     ENTRY(bias_residual_layernorm), ENTRY(bias_gelu), ENTRY(encoder_layer), ENTRY(attention_backward_fused), ENTRY(attention_backward),
+    ENTRY(token_logprobs), ENTRY(token_logprobs_grad), ENTRY(distill_topk), ENTRY(distill_topk_grad),
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -1,0 +1,834 @@
+// Operators on rows of logits: log probabilities of given tokens with entropy and top alternatives, distillation from a
+// teacher's top tokens, and their gradients.
+//
+// With m = max_j x_j, S = sum_j exp(s (x_j - m)), l = ln S and p_j = exp(s (x_j - m) - l):
+//   log probability    s (x_t - m) - l
+//   entropy            l - sum_j p_j s (x_j - m)
+//   distillation       sum_k q_k (ln q_k - ln p_k) over the teacher's list, with or without one more class for what it leaves
+//   gradients          s g (d_jt - p_j) - s h p_j (ln p_j + H)      and      s w (Q p_j - q_j)
+// All of it is bound by the one pass over the logits (and the one over their gradient); the kernels are built so that
+// each element is read once, whole windows of 16 bytes at a time, several on their way per thread.
+#include "logits.cuh"
+#include <cooperative_groups.h>
+
+namespace cg = cooperative_groups;
+
+namespace sfb {
+static int set_zero(const char *who, uint32_t *counter, cudaStream_t s)
+{
+    const cudaError_t e = counter ? cudaMemsetAsync(counter, 0, sizeof(uint32_t), s) : cudaSuccess;
+    SFB_REQUIRE(e == cudaSuccess, "%s: %s", who, cudaGetErrorString(e));
+    clear_error();
+    return 0;
+}
+
+namespace lg {
+
+constexpr uint32_t kThreads = 256;
+constexpr int kU = 4;                     // windows that a thread has on their way at a time
+constexpr uint32_t kCap = 1024;           // candidates for a row's alternatives
+constexpr uint32_t kMaxList = 128;        // alternatives, entries of a teacher's list
+constexpr uint32_t kMaxCluster = 8;
+
+struct StatParams {
+    const void *x;
+    uint64_t pitch;                       // elements from row to row
+    uint32_t rows, vocab;
+    float scale, s2;                      // s2 = scale * log2(e)
+    const int32_t *targets;
+    float *logp, *stats, *entropy, *top_logp;
+    int32_t *top_ids;
+    uint32_t k;                           // alternatives, or entries of the lists
+    const int32_t *ids;                   // the lists [rows][k]
+    const float *teacher;
+    float *loss;
+    uint32_t *missed;
+    uint32_t count_here;                  // targets (entries) counted by one CTA behind the rows'; 0: each row adds its own
+};
+
+__device__ __forceinline__ uint32_t cluster_rank()
+{
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ uint32_t cluster_size()
+{
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+    return r;
+}
+
+// bits in the order of the values (-0 is 0)
+__device__ __forceinline__ uint32_t ordered(float v)
+{
+    const uint32_t u = __float_as_uint(v + 0.f);
+    return u ^ (uint32_t)((int32_t)u >> 31 | (int32_t)0x80000000);
+}
+__device__ __forceinline__ float from_ordered(uint32_t o) { return __uint_as_float(o & 0x80000000u ? o ^ 0x80000000u : ~o); }
+// larger for larger values, and among equal ones for the lower index
+__device__ __forceinline__ unsigned long long rank_key(float v, uint32_t index) { return (unsigned long long)ordered(v) << 32 | (0xffffffffu - index); }
+
+__device__ __forceinline__ float warp_max_nan(float v)
+{
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v = max_nan(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+}
+
+// the sums of a warp's threads, beside the largest of their maxima
+template <bool ENT> __device__ __forceinline__ void warp_sums(Sums &a, float &mx, float s2)
+{
+    mx = warp_max_nan(mx);
+    a.move_to(mx, s2);
+    a.s = warp_sum(a.s);
+    if (ENT) a.e = warp_sum(a.e);
+}
+
+template <int DT, bool ENT> __device__ __forceinline__ void add_window(Sums &a, const uint4 &v, float s2)
+{
+    float x[Win<DT>::kElems];
+    unpack<DT>(v, x);
+    float s = 0.f, e = 0.f;
+#pragma unroll
+    for (uint32_t j = 0; j < Win<DT>::kElems; j++) {
+        const float t = s2 * (x[j] - a.r), y = ex2(t);
+        s += y;
+        if (ENT) e = fmaf(y, fmaxf(t, kFar), e);
+    }
+    a.s += s;
+    if (ENT) a.e += e;
+}
+
+// listed tokens of a window (bit j: element j) become -inf
+template <int DT> __device__ __forceinline__ void drop_listed(uint4 &v, uint32_t bits)
+{
+    uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        if (DT == SFB_F32) {
+            if (bits >> j & 1) u[j] = Win<DT>::kInf;
+        } else {
+            if (bits >> (2 * j) & 1) u[j] = (u[j] & 0xffff0000u) | Win<DT>::kInf;
+            if (bits >> (2 * j + 1) & 1) u[j] = (u[j] & 0xffffu) | Win<DT>::kInf << 16;
+        }
+    }
+    v = make_uint4(u[0], u[1], u[2], u[3]);
+}
+
+struct Part { float m, s, e; };
+
+// ids outside [0, vocab), counted by one CTA
+__device__ __forceinline__ void count_missed(const int32_t *ids, uint32_t n, uint32_t vocab, uint32_t *missed, uint32_t *part)
+{
+    uint32_t bad = 0;
+    for (uint32_t i = threadIdx.x; i < n; i += blockDim.x * 8) {
+        int32_t v[8];
+#pragma unroll
+        for (int u = 0; u < 8; u++) v[u] = i + u * blockDim.x < n ? ids[i + u * blockDim.x] : 0;
+#pragma unroll
+        for (int u = 0; u < 8; u++) bad += (uint32_t)v[u] >= vocab;
+    }
+    bad = __reduce_add_sync(0xffffffffu, bad);
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = bad;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (uint32_t w = 1; w < blockDim.x / 32; w++) bad += part[w];
+        *missed = bad;
+    }
+}
+
+// The largest t such that at least k of the n (at most 256) values have the upper 16 bits of their ordered form at or
+// above it, as an ordered value.  One warp.
+__device__ __forceinline__ uint32_t kth_largest(const float *values, uint32_t n, uint32_t k)
+{
+    const uint32_t lane = threadIdx.x & 31;
+    uint32_t o[8];
+#pragma unroll
+    for (int j = 0; j < 8; j++) o[j] = lane + 32 * j < n ? ordered(values[lane + 32 * j]) >> 16 : 0u;
+    uint32_t t = 0;
+    for (uint32_t bit = 0x8000u; bit; bit >>= 1) {
+        uint32_t c = 0;
+#pragma unroll
+        for (int j = 0; j < 8; j++) c += o[j] >= (t | bit);
+        if (__reduce_add_sync(0xffffffffu, c) >= k) t |= bit;
+    }
+    return t << 16;
+}
+
+struct TopShared {
+    float gm[kThreads];                   // largest values of the groups of threads
+    unsigned long long cand[kCap];
+    uint32_t hits[kCap];
+    uint32_t cnt, n_hits, tau, part[8];
+    float m, l;
+};
+
+// sum over the CTA's threads
+__device__ __forceinline__ uint32_t block_sum(uint32_t v, uint32_t *part)
+{
+    v = __reduce_add_sync(0xffffffffu, v);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = 0;
+    for (uint32_t w = 0; w < blockDim.x / 32; w++) v += part[w];
+    return v;
+}
+
+// The candidates when too many values reach the bound (values tie, or most of the large ones went to a few threads): the bound is
+// bisected over the values and their indices, a pass over the row (by now in L2) for each step.  One CTA, the whole row.
+template <int DT> __device__ __noinline__ void bisect_candidates(const Row<DT> row, uint32_t k, TopShared *sh)
+{
+    unsigned long long lo = (unsigned long long)sh->tau << 32, hi = ~0ull, x = lo;      // more than kCap reach lo, fewer than k hi
+    const uint32_t windows = row.windows();
+    for (;;) {
+        const unsigned long long mid = lo + (hi - lo) / 2;
+        if (mid == lo) { x = hi; break; }
+        uint32_t c = 0;
+        for (uint32_t w = threadIdx.x; w < windows; w += blockDim.x) {
+            float v[Win<DT>::kElems];
+            unpack<DT>(load_window(row, w), v);
+#pragma unroll
+            for (uint32_t j = 0; j < Win<DT>::kElems; j++) c += v[j] > neg_inf() && rank_key(v[j], w * Win<DT>::kElems + j - row.head) >= mid;
+        }
+        c = block_sum(c, sh->part);
+        if (c < k) hi = mid;
+        else if (c > kCap) lo = mid;
+        else { x = mid; break; }
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) sh->cnt = 0;
+    __syncthreads();
+    for (uint32_t w = threadIdx.x; w < windows; w += blockDim.x) {
+        float v[Win<DT>::kElems];
+        unpack<DT>(load_window(row, w), v);
+#pragma unroll
+        for (uint32_t j = 0; j < Win<DT>::kElems; j++) {
+            const unsigned long long key = rank_key(v[j], w * Win<DT>::kElems + j - row.head);
+            if (v[j] > neg_inf() && key >= x) {
+                const uint32_t at = atomicAdd(&sh->cnt, 1u);
+                if (at < kCap) sh->cand[at] = key;
+            }
+        }
+    }
+    __syncthreads();
+}
+
+// A row's statistics, and what is made of them.  One CTA per row, or a cluster of CTAs where there are few rows: each
+// takes every C-th piece, and CTA 0 joins the parts.  KD: 0 tokens, 1 lists, 2 lists with the remainder as one more class.
+template <int DT, bool ENT, bool TOP, int KD>
+__global__ void __launch_bounds__(kThreads, 4) row_stats_kernel(const StatParams p)
+{
+    extern __shared__ __align__(16) uint8_t dyn[];       // TOP: the largest value of each group of windows; KD 2: a bit per position
+    __shared__ Part parts[kMaxCluster * 8];
+    __shared__ __align__(16) uint8_t top_raw[TOP ? sizeof(TopShared) : 16];
+    TopShared *const top_s = (TopShared *)top_raw;
+    __shared__ int32_t l_id[KD ? kMaxList : 1];
+    __shared__ float l_q[KD ? kMaxList : 1], l_x[KD ? kMaxList : 1];
+    __shared__ uint32_t l_twice;
+
+    const uint32_t T = blockDim.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const uint32_t C = cluster_size(), rank = cluster_rank();
+    const uint32_t r = blockIdx.x / C;
+    if (C > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");    // waited for before the first word into another CTA
+    grid_dependency_wait();
+    grid_launch_dependents();
+
+    bool skip = false;
+    int32_t target = -1;
+    if (r >= p.rows) {
+        if (rank == 0) count_missed(KD ? p.ids : p.targets, p.count_here, p.vocab, p.missed, (uint32_t *)parts);
+        skip = true;
+    } else if (KD == 0 && p.targets) {
+        target = p.targets[r];
+        const bool inside = (uint32_t)target < p.vocab;
+        if (!inside && rank == 0 && tid == 0 && p.missed && !p.count_here) atomicAdd(p.missed, 1u);
+        if (!inside) {
+            target = -1;
+            if (!ENT && !TOP) {              // nothing of this row is asked for
+                if (rank == 0 && tid == 0) { p.logp[r] = 0.f; p.stats[2 * (size_t)r] = p.stats[2 * (size_t)r + 1] = 0.f; }
+                skip = true;
+            }
+        }
+    }
+    if (skip) {
+        __syncwarp();
+        if (C > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+        return;
+    }
+
+    const void *x = (const char *)p.x + (size_t)r * p.pitch * Win<DT>::kSize;
+    const Row<DT> row(x, p.vocab);
+    const uint32_t windows = row.windows();
+    float x_target = 0.f;
+    if (KD == 0 && target >= 0 && rank == 0 && tid < 64) x_target = load_element<DT>(x, (uint32_t)target);
+
+    if (TOP && tid == 0) { top_s->cnt = 0; top_s->n_hits = 0; }
+    if (KD) {
+        uint32_t *bits = (uint32_t *)dyn;
+        if (KD == 2) {
+            for (uint32_t i = tid; i < (row.end + 31) / 32; i += T) bits[i] = 0;
+            if (tid == 0) l_twice = 0;
+            __syncthreads();
+        }
+        uint32_t bad = 0;
+        for (uint32_t i = tid; i < p.k; i += T) {
+            const int32_t id = p.ids[(size_t)r * p.k + i];
+            const bool ok = (uint32_t)id < p.vocab;
+            bad += !ok;
+            l_id[i] = ok ? id : -1;
+            l_q[i] = ok ? p.teacher[(size_t)r * p.k + i] : neg_inf();
+            l_x[i] = ok ? load_element<DT>(x, (uint32_t)id) : neg_inf();
+            if (KD == 2 && ok) {
+                const uint32_t pos = row.head + (uint32_t)id, bit = 1u << (pos & 31);
+                if (atomicOr(&bits[pos >> 5], bit) & bit) l_twice = 1;
+            }
+        }
+        if (p.missed && !p.count_here && rank == 0) {
+            bad = __reduce_add_sync(0xffffffffu, bad);
+            if (lane == 0 && bad) atomicAdd(p.missed, bad);
+        }
+        __syncthreads();
+    }
+
+    // ---- the pass ----
+    Sums a;
+    float mx = neg_inf();
+    const float gap = 40.f / p.s2;
+    const uint32_t step = C * kU * T, first = rank * kU * T + tid;
+    float *keys = (float *)dyn;
+    uint4 v[kU], next[kU];
+#pragma unroll
+    for (int u = 0; u < kU; u++) next[u] = load_window(row, first + u * T);
+    for (uint32_t w0 = first, g = 0; w0 - tid < windows; w0 += step, g++) {
+#pragma unroll
+        for (int u = 0; u < kU; u++) v[u] = next[u];
+        if (w0 - tid + step < windows) {
+#pragma unroll
+            for (int u = 0; u < kU; u++) next[u] = load_window(row, w0 + step + u * T);
+        }
+        if (KD == 2) {
+#pragma unroll
+            for (int u = 0; u < kU; u++) {
+                const uint32_t w = w0 + u * T;
+                uint32_t b = 0;
+                if (w < windows) b = DT == SFB_F32 ? dyn[w >> 1] >> ((w & 1) * 4) & 15u : dyn[w];
+                if (b) drop_listed<DT>(v[u], b);
+            }
+        }
+        const float m = max_windows<DT, kU>(v);
+        if (TOP) keys[g * T + tid] = m;
+        mx = max_nan(mx, m);
+        if (a.prepare(m, p.s2, gap)) {
+#pragma unroll
+            for (int u = 0; u < kU; u++) add_window<DT, ENT>(a, v[u], p.s2);
+        }
+    }
+
+    // ---- the parts of the warps (and CTAs) meet in CTA 0 ----
+    const float own_mx = mx;
+    warp_sums<ENT>(a, mx, p.s2);
+    if (C > 1) {
+        asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+        const cg::cluster_group cl = cg::this_cluster();
+        if (lane == 0) cl.map_shared_rank(parts, 0)[rank * 8 + warp] = Part{mx, a.s, a.e};
+        if (TOP) {
+            float gmx = own_mx;
+            for (uint32_t o = 1; o < C; o <<= 1) gmx = max_nan(gmx, __shfl_xor_sync(0xffffffffu, gmx, o));
+            cl.map_shared_rank(top_s->gm, tid & (C - 1))[rank * (T / C) + tid / C] = gmx;
+        }
+        cl.sync();
+        if (!TOP && rank) return;
+    } else {
+        if (lane == 0) parts[warp] = Part{mx, a.s, a.e};
+        if (TOP) top_s->gm[tid] = own_mx;
+        __syncthreads();
+    }
+
+    const uint32_t merger = TOP ? 1 : 0;          // with alternatives, warp 0 looks for their bound meanwhile
+    if (rank == 0 && warp == merger) {
+        const uint32_t warps = T / 32, n = C * warps;
+        Sums b;
+        float bm = neg_inf();
+        for (uint32_t i = lane; i < n; i += 32) {
+            const Part q = parts[i / warps * 8 + i % warps];
+            Sums c;
+            c.r = q.m; c.s = q.s; c.e = q.e;
+            const float m2 = max_nan(bm, q.m);
+            b.move_to(m2, p.s2);
+            c.move_to(m2, p.s2);
+            b.s += c.s; b.e += c.e;
+            bm = m2;
+        }
+        if (KD == 2) {
+            for (uint32_t i = lane; i < p.k; i += 32) {
+                if (l_id[i] < 0) continue;
+                bm = max_nan(bm, l_x[i]);
+            }
+        }
+        warp_sums<ENT>(b, bm, p.s2);
+        const float m = bm;
+        float s = b.s, rest = s;
+        if (KD == 2) {
+            float listed = 0.f;
+            for (uint32_t i = lane; i < p.k; i += 32) {
+                if (l_id[i] < 0 || !(l_x[i] > neg_inf() || l_x[i] != l_x[i])) continue;
+                bool again = false;
+                if (l_twice)
+                    for (uint32_t j = 0; j < i; j++) again |= l_id[j] == l_id[i];
+                if (!again) listed += ex2(p.s2 * (l_x[i] - m));
+            }
+            s = rest + warp_sum(listed);
+        }
+        const bool empty = m == neg_inf();
+        const float l = empty ? neg_inf() : logf(s);
+        if (KD == 0) {
+            if (TOP && lane == 0) { top_s->m = m; top_s->l = l; }
+            if (lane == 0) {
+                p.stats[2 * (size_t)r] = m;
+                p.stats[2 * (size_t)r + 1] = l;
+                if (p.logp) p.logp[r] = target < 0 ? 0.f : empty ? neg_inf() : p.scale * (x_target - m) - l;
+                if (ENT) p.entropy[r] = empty ? 0.f : l - kLn2 * (b.e / s);
+            }
+        } else {
+            // the teacher's probabilities
+            float mq = neg_inf(), zq = 0.f;
+            if (KD == 1) {
+                for (uint32_t i = lane; i < p.k; i += 32) mq = max_nan(mq, l_q[i]);
+                mq = warp_max_nan(mq);
+            } else {
+                mq = 0.f;
+            }
+            if (mq != neg_inf())
+                for (uint32_t i = lane; i < p.k; i += 32) zq += expf(l_q[i] - mq);
+            zq = warp_sum(zq);
+            const float lz = KD == 1 ? mq + logf(zq) : 0.f;
+            float loss = 0.f;
+            if (mq != neg_inf()) {
+                for (uint32_t i = lane; i < p.k; i += 32) {
+                    const float lq = l_q[i] - lz, q = expf(lq);
+                    const float lp = l_x[i] == neg_inf() ? neg_inf() : p.scale * (l_x[i] - m) - l;
+                    if (!(q <= 0.f)) loss += q * (lq - lp);
+                }
+            }
+            loss = warp_sum(loss);
+            if (lane == 0) {
+                float *st = p.stats + (KD == 2 ? 3 : 2) * (size_t)r;
+                st[0] = m;
+                st[1] = l;
+                if (KD == 2) {
+                    const float left = fmaxf(0.f, 1.f - zq), lr = rest > 0.f || rest != rest ? logf(rest) : neg_inf();
+                    if (left > 0.f && !(lr == neg_inf())) loss += left * (logf(left) - (lr - l));
+                    st[2] = lr;
+                }
+                p.loss[r] = loss;
+            }
+        }
+    }
+    if (!TOP) return;
+
+    // ---- alternatives ----
+    // At least k groups of threads have a value at or above the k-th largest of the groups' maxima, so every one of the k
+    // largest values of the row is: only groups of windows whose maximum reaches that bound are looked at again.
+    if (warp == 0) {
+        const uint32_t t = kth_largest(top_s->gm, T, p.k);
+        if (lane == 0) top_s->tau = t;
+    }
+    __syncthreads();
+    const uint32_t tau = top_s->tau;
+    for (uint32_t w0 = first, g = 0; w0 - tid < windows; w0 += step, g++) {
+        const float m = keys[g * T + tid];
+        if (m > neg_inf() && ordered(m) >= tau) {
+            const uint32_t at = atomicAdd(&top_s->n_hits, 1u);
+            if (at < kCap) top_s->hits[at] = w0;
+        }
+    }
+    __syncthreads();
+    TopShared *first_cta = C > 1 ? cg::this_cluster().map_shared_rank(top_s, 0) : top_s;
+    const uint32_t n_hits = top_s->n_hits;
+    if (n_hits > kCap) {
+        if (tid == 0) atomicAdd(&first_cta->cnt, kCap + 1);
+    } else {
+        for (uint32_t i = tid; i < n_hits * kU; i += T) {
+            const uint32_t w = top_s->hits[i / kU] + (i % kU) * T;
+            if (w >= windows) continue;
+            float e[Win<DT>::kElems];
+            unpack<DT>(load_window(row, w), e);
+#pragma unroll
+            for (uint32_t j = 0; j < Win<DT>::kElems; j++) {
+                if (e[j] > neg_inf() && ordered(e[j]) >= tau) {
+                    const uint32_t at = atomicAdd(&first_cta->cnt, 1u);
+                    if (at < kCap) first_cta->cand[at] = rank_key(e[j], w * Win<DT>::kElems + j - row.head);
+                }
+            }
+        }
+    }
+    if (C > 1) {
+        cg::this_cluster().sync();
+        if (rank) return;
+    } else {
+        __syncthreads();
+    }
+    const float m = top_s->m, l = top_s->l;
+    const bool sound = l == l;                  // no NaN in the row
+    if (sound && top_s->cnt > kCap) bisect_candidates<DT>(row, p.k, top_s);
+    const uint32_t cnt = sound ? top_s->cnt : 0u;
+    float *out_logp = p.top_logp + (size_t)r * p.k;
+    int32_t *out_ids = p.top_ids + (size_t)r * p.k;
+    for (uint32_t i = tid; i < cnt; i += T) {
+        const unsigned long long key = top_s->cand[i];
+        uint32_t above = 0;
+        for (uint32_t j = 0; j < cnt; j++) above += top_s->cand[j] > key;
+        if (above < p.k) {
+            out_logp[above] = p.scale * (from_ordered((uint32_t)(key >> 32)) - m) - l;
+            out_ids[above] = (int32_t)(0xffffffffu - (uint32_t)key);
+        }
+    }
+    for (uint32_t i = cnt + tid; i < p.k; i += T) {
+        out_logp[i] = sound ? neg_inf() : l;
+        out_ids[i] = -1;
+    }
+}
+
+// ---- gradients --------------------------------------------------------------------------------------------------------
+struct GradParams {
+    const void *x;
+    void *out;
+    uint64_t pitch, out_pitch;
+    uint32_t rows, vocab, width;
+    uint32_t parts, per;                  // CTAs per row, windows of each
+    float scale, s2;
+    const int32_t *targets;
+    const float *stats, *dlogp, *entropy, *dentropy;
+    const int32_t *ids;
+    const float *teacher, *dloss, *token_stats;
+    uint32_t k;
+    int tail;
+};
+
+// windows of x that start where those of out do not
+template <int DT> __device__ __forceinline__ uint4 load_shifted(const void *x, uint32_t head, uint32_t n, uint32_t w)
+{
+    uint32_t v[4];
+#pragma unroll
+    for (uint32_t j = 0; j < 4; j++) {
+        const uint32_t i = w * Win<DT>::kElems + j * (Win<DT>::kElems / 4) - head;       // below the row's start: wraps, and is no index
+        if (DT == SFB_F32) {
+            v[j] = i < n ? ((const uint32_t *)x)[i] : Win<DT>::kInf;
+        } else {
+            const uint32_t lo = i < n ? ((const uint16_t *)x)[i] : Win<DT>::kInf, hi = i + 1 < n ? ((const uint16_t *)x)[i + 1] : Win<DT>::kInf;
+            v[j] = lo | hi << 16;
+        }
+    }
+    return make_uint4(v[0], v[1], v[2], v[3]);
+}
+
+// dx = p (c0 + c1 t) with t the base-2 logarithm of p, plus the given target's share (KD 0, ENT: c1 is not 0);
+// dx = c0 2^t + c2 2^t2, what is listed made again by itself (KD 1; HARD: c2 is not 0).
+template <int DT, bool ENT, bool KD, bool HARD, bool SAME>
+__global__ void __launch_bounds__(kThreads) row_grad_kernel(const GradParams p)
+{
+    __shared__ int32_t l_id[KD ? kMaxList : 1];
+    __shared__ float l_q[KD ? kMaxList : 1];
+    __shared__ float coef[4];
+    constexpr uint32_t E = Win<DT>::kElems;
+    const uint32_t T = blockDim.x, tid = threadIdx.x, lane = tid & 31;
+    const uint32_t r = blockIdx.x / p.parts, part = blockIdx.x - r * p.parts;
+    grid_dependency_wait();
+    grid_launch_dependents();
+
+    const void *x = (const char *)p.x + (size_t)r * p.pitch * Win<DT>::kSize;
+    void *out = (char *)p.out + (size_t)r * p.out_pitch * Win<DT>::kSize;
+    const Row<DT> orow(out, p.width), row(x, p.vocab);        // SAME: both start at the same place of their windows
+    const uint32_t w_begin = part * p.per, w_end = min(orow.windows(), w_begin + p.per);
+    const int32_t i_begin = (int32_t)(w_begin * E) - (int32_t)orow.head, i_end = (int32_t)(w_end * E) - (int32_t)orow.head;
+
+    const float *st = p.stats + (KD && p.tail ? 3 : 2) * (size_t)r;
+    const float m = st[0];
+    float c0, c1 = 0.f, c2 = 0.f, l2, l2b = 0.f, target_share = 0.f;
+    int32_t target = p.targets ? p.targets[r] : -1;
+    if ((uint32_t)target >= p.vocab) target = -1;
+    bool zero = m == neg_inf();                               // no token is left: every probability is 0
+
+    constexpr uint32_t kSlots = 2;                            // KD: a thread's share of the list and the target (at least 128 threads)
+    float x_listed[kSlots], listed_w = 0.f, listed_c = 0.f;
+    if (!KD) {
+        const float g = target >= 0 ? p.dlogp[r] : 0.f;
+        l2 = st[1] * kLog2e;
+        if (ENT) {
+            const float h = p.dentropy[r];
+            c0 = -p.scale * (g + h * p.entropy[r]);
+            c1 = -p.scale * h * kLn2;
+        } else {
+            c0 = -p.scale * g;
+            zero |= target < 0;
+        }
+        target_share = p.scale * g;
+    } else {
+        if (tid < 32) {
+            float mq = p.tail ? 0.f : neg_inf(), zq = 0.f;
+            for (uint32_t i = lane; i < p.k; i += 32) {
+                const int32_t id = p.ids[(size_t)r * p.k + i];
+                const bool ok = (uint32_t)id < p.vocab;
+                const float lq = ok ? p.teacher[(size_t)r * p.k + i] : neg_inf();
+                l_id[i] = ok ? id : -1;
+                l_q[i] = lq;
+                if (!p.tail) mq = max_nan(mq, lq);
+            }
+            mq = warp_max_nan(mq);
+            __syncwarp();
+            if (mq != neg_inf())
+                for (uint32_t i = lane; i < p.k; i += 32) zq += expf(l_q[i] - mq);
+            zq = warp_sum(zq);
+            const float inv = p.tail ? 1.f : 1.f / zq;
+            for (uint32_t i = lane; i < p.k; i += 32) l_q[i] = mq == neg_inf() ? 0.f : expf(l_q[i] - mq) * inv;
+            if (lane == 0) {
+                const float sum = p.tail ? zq : mq == neg_inf() ? 0.f : 1.f, left = p.tail ? fmaxf(0.f, 1.f - zq) : 0.f;
+                coef[0] = sum + left;
+                coef[1] = left;
+            }
+        }
+        __syncthreads();
+        const float sw = p.scale * p.dloss[r], all = coef[0], left = coef[1];
+        listed_w = sw;
+        listed_c = sw * all;
+        l2 = st[1] * kLog2e;
+        c0 = sw * all;
+        if (p.tail) {
+            // unlisted tokens: all * p - left * p / p_rest, as a multiple of their share of the remainder
+            const float lr = st[2];
+            if (lr == neg_inf()) {
+                c0 = 0.f;                                     // every unlisted one has a probability of 0
+            } else {
+                c0 = sw * (all * expf(lr - st[1]) - left);
+                l2 = lr * kLog2e;
+            }
+        }
+        if (HARD) {
+            const float g = target >= 0 ? p.dlogp[r] : 0.f;
+            c2 = -g;
+            l2b = p.token_stats[2 * (size_t)r + 1] * kLog2e;
+            target_share = g;
+        }
+#pragma unroll
+        for (uint32_t n = 0; n < kSlots; n++) {
+            const uint32_t i = tid + n * T;
+            const int32_t id = i < p.k ? l_id[i] : i == p.k && HARD ? target : -1;
+            x_listed[n] = id >= 0 && id >= i_begin && id < i_end ? load_element<DT>(x, (uint32_t)id) : 0.f;
+        }
+        __syncthreads();                                      // out may be x: nothing is written before what is listed has been read
+    }
+
+    const uint32_t w_target = !KD && target >= 0 ? ((uint32_t)target + orow.head) / E : 0xffffffffu;
+    const uint32_t e_target = ((uint32_t)target + orow.head) % E;
+    for (uint32_t w0 = w_begin + tid; w0 - tid < w_end; w0 += kU * T) {
+        uint4 v[kU];
+        if (!zero) {
+#pragma unroll
+            for (int u = 0; u < kU; u++) {
+                const uint32_t w = w0 + u * T;
+                if (w < w_end) v[u] = SAME ? load_window(row, w) : load_shifted<DT>(x, orow.head, p.vocab, w);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < kU; u++) {
+            const uint32_t w = w0 + u * T;
+            if (w >= w_end) break;
+            float y[E];
+            if (zero) {
+#pragma unroll
+                for (uint32_t j = 0; j < E; j++) y[j] = 0.f;
+            } else {
+                unpack<DT>(v[u], y);
+#pragma unroll
+                for (uint32_t j = 0; j < E; j++) {
+                    const float d = y[j] - m;
+                    const float t = fmaf(p.s2, d, -l2), e = ex2(t);
+                    y[j] = ENT ? e * fmaf(c1, fmaxf(t, kFar), c0) : e * c0;
+                    if (HARD) y[j] = fmaf(c2, ex2(fmaf(kLog2e, d, -l2b)), y[j]);
+                }
+            }
+            if (w == w_target) {
+#pragma unroll
+                for (uint32_t j = 0; j < E; j++)
+                    if (j == e_target) y[j] += target_share;
+            }
+            if (orow.whole(w)) {
+                ((uint4 *)orow.base)[w] = pack<DT>(y);
+            } else {
+#pragma unroll
+                for (uint32_t j = 0; j < E; j++) {
+                    const uint32_t pos = w * E + j;
+                    if (pos >= orow.head && pos < orow.end) store_element<DT>(out, pos - orow.head, y[j]);
+                }
+            }
+        }
+    }
+    if (!KD) return;
+    // What is listed, and the target: made again from all the shares it has.  An index that stands in the list twice is
+    // written twice, with the same value.
+    __syncthreads();
+#pragma unroll
+    for (uint32_t n = 0; n < kSlots; n++) {
+        const uint32_t i = tid + n * T;
+        const int32_t id = i < p.k ? l_id[i] : i == p.k && HARD ? target : -1;
+        if (id < 0 || id < i_begin || id >= i_end) continue;
+        float q = 0.f;
+        bool listed = false;
+        for (uint32_t j = 0; j < p.k; j++)
+            if (l_id[j] == id) { q += l_q[j]; listed = true; }
+        const float d = x_listed[n] - m;
+        float y = 0.f;
+        if (!zero) y = listed ? listed_c * ex2(fmaf(p.s2, d, -st[1] * kLog2e)) : c0 * ex2(fmaf(p.s2, d, -l2));
+        y -= listed_w * q;
+        if (HARD) {
+            if (!zero) y = fmaf(c2, ex2(fmaf(kLog2e, d, -l2b)), y);
+            if (id == target) y += target_share;
+        }
+        store_element<DT>(out, (uint32_t)id, y);
+    }
+}
+
+// ---- launches -----------------------------------------------------------------------------------------------------------
+static uint32_t stat_threads(uint32_t windows, bool top) { return windows > 512 ? 256 : windows > 256 || top ? 128 : 64; }
+
+template <int DT, bool ENT, bool TOP, int KD> static int launch_stats(cudaStream_t s, StatParams &p, const char *who)
+{
+    const int dev = current_device(), sms = device_sm_count(dev);
+    SFB_REQUIRE(sms > 0, "%s: cannot query the device", who);
+    const uint32_t windows = p.vocab / Win<DT>::kElems + 2;      // at most, wherever a row starts
+    const uint32_t T = stat_threads(windows, TOP);
+    uint32_t C = 1;
+    while (C < kMaxCluster && (uint64_t)p.rows * C * 2 <= (uint64_t)sms * 2 && windows > C * T * 2) C *= 2;
+    const uint64_t entries = p.missed ? KD ? (uint64_t)p.rows * p.k : p.targets ? p.rows : 0 : 0;
+    p.count_here = entries <= T * 32u ? (uint32_t)entries : 0;
+    if (!p.count_here && set_zero(who, p.missed, s)) return 1;
+    for (;; C = 1) {
+        const uint32_t groups = (windows + C * kU * T - 1) / (C * kU * T);
+        const size_t smem = TOP ? (size_t)groups * T * sizeof(float) : KD == 2 ? ((size_t)windows * Win<DT>::kElems + 31) / 32 * 4 : 0;
+        SFB_REQUIRE(smem <= 200 * 1024, "%s: vocab=%u is too large", who, p.vocab);
+        static DeviceOnce once;
+        if (!once.done(dev)) {
+            SFB_REQUIRE(cudaFuncSetAttribute(row_stats_kernel<DT, ENT, TOP, KD>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024) == cudaSuccess,
+                        "%s: cannot reserve shared memory", who);
+            once.mark(dev);
+        }
+        const uint32_t grid = (p.rows + (p.count_here ? 1 : 0)) * C;
+        const cudaError_t e = launch_overlapped_cluster(row_stats_kernel<DT, ENT, TOP, KD>, dim3(grid), dim3(T), smem, s, C, p);
+        if (e == cudaSuccess || C == 1) break;
+        (void)cudaGetLastError();                // a device or a partition that cannot place clusters
+    }
+    return check_launch(who);
+}
+
+template <int DT, bool ENT, bool KD, bool HARD> static int launch_grad(cudaStream_t s, GradParams &p, const char *who)
+{
+    const int sms = device_sm_count(current_device());
+    SFB_REQUIRE(sms > 0, "%s: cannot query the device", who);
+    const uint32_t windows = p.width / Win<DT>::kElems + 2;
+    const uint32_t T = windows > 512 ? 256 : windows > 256 || KD ? 128 : 64;
+    const uint32_t round = T * kU;
+    uint32_t rounds = (windows + round - 1) / round;
+    // whole rows per CTA once there are several CTAs for every SM, a round each before that
+    uint32_t per = 1;
+    while (per < rounds && (uint64_t)p.rows * ((rounds + per * 2 - 1) / (per * 2)) >= (uint64_t)sms * 16) per *= 2;
+    p.per = per * round;
+    p.parts = (windows + p.per - 1) / p.per;
+    SFB_REQUIRE((uint64_t)p.rows * p.parts < (1ull << 31), "%s: too many rows", who);
+    const uint64_t size = Win<DT>::kSize;
+    const bool same = ((uintptr_t)p.x & 15) == ((uintptr_t)p.out & 15) && (p.pitch * size & 15) == (p.out_pitch * size & 15);
+    const dim3 grid(p.rows * p.parts);
+    if (same) launch_overlapped(row_grad_kernel<DT, ENT, KD, HARD, true>, grid, dim3(T), 0, s, p);
+    else launch_overlapped(row_grad_kernel<DT, ENT, KD, HARD, false>, grid, dim3(T), 0, s, p);
+    return check_launch(who);
+}
+
+}  // namespace lg
+
+#define BY_TYPE(dtype, f, ...)                                                                         \
+    ((dtype) == SFB_F32 ? f<SFB_F32, __VA_ARGS__> : (dtype) == SFB_BF16 ? f<SFB_BF16, __VA_ARGS__> : f<SFB_F16, __VA_ARGS__>)
+
+static int check_rows(const char *who, const void *x, uint64_t pitch, uint32_t rows, uint32_t vocab, uint32_t width, int dtype, float scale)
+{
+    SFB_REQUIRE(valid_dtype(dtype), "%s: unknown dtype %d", who, dtype);
+    SFB_REQUIRE(x && ((uintptr_t)x & (elem_size(dtype) - 1)) == 0, "%s: logits are NULL or not aligned to their elements", who);
+    SFB_REQUIRE(vocab >= 1 && vocab <= width && width <= (1u << 30), "%s: vocab=%u of width=%u out of range", who, vocab, width);
+    SFB_REQUIRE(pitch >= width || rows <= 1, "%s: a row pitch smaller than the rows", who);
+    SFB_REQUIRE(rows < (1u << 27), "%s: too many rows", who);
+    SFB_REQUIRE(scale > 0.f && scale <= 1e6f, "%s: scale must be positive (and at most 1e6)", who);
+    return 0;
+}
+
+}  // namespace sfb
+
+using namespace sfb;
+
+extern "C" int sfb_token_logprobs(sfb_stream_t stream, const void *logits, uint64_t pitch, const int32_t *targets, uint32_t rows, uint32_t vocab,
+                                  int dtype, float scale, float *logp, float *stats, float *entropy, float *top_logp, int32_t *top_ids,
+                                  uint32_t top_k, uint32_t *missed)
+{
+    const char *who = "sfb_token_logprobs";
+    if (rows == 0) return set_zero(who, missed, as_stream(stream));
+    if (check_rows(who, logits, pitch, rows, vocab, vocab, dtype, scale)) return 1;
+    SFB_REQUIRE(stats, "%s: NULL pointer", who);
+    SFB_REQUIRE(!targets == !logp, "%s: targets and logp go together", who);
+    SFB_REQUIRE(top_k <= lg::kMaxList && top_k <= vocab, "%s: top_k=%u must be at most %u and vocab=%u", who, top_k, lg::kMaxList, vocab);
+    SFB_REQUIRE(top_k == 0 || (top_logp && top_ids), "%s: NULL pointer", who);
+    SFB_REQUIRE(top_k == 0 || vocab <= (1u << 19), "%s: vocab=%u is too large for alternatives (%u)", who, vocab, 1u << 19);
+    lg::StatParams p = {logits, pitch, rows, vocab, scale, scale * lg::kLog2e, targets, logp, stats, entropy, top_logp, top_ids, top_k,
+                        nullptr, nullptr, nullptr, targets ? missed : nullptr, 0};
+    cudaStream_t s = as_stream(stream);
+    if (!targets && set_zero(who, missed, s)) return 1;
+    if (top_k) return entropy ? BY_TYPE(dtype, lg::launch_stats, true, true, 0)(s, p, who) : BY_TYPE(dtype, lg::launch_stats, false, true, 0)(s, p, who);
+    return entropy ? BY_TYPE(dtype, lg::launch_stats, true, false, 0)(s, p, who) : BY_TYPE(dtype, lg::launch_stats, false, false, 0)(s, p, who);
+}
+
+extern "C" int sfb_token_logprobs_grad(sfb_stream_t stream, const void *logits, uint64_t pitch, const int32_t *targets, const float *stats,
+                                       const float *dlogp, const float *entropy, const float *dentropy, void *out, uint64_t out_pitch, uint32_t rows,
+                                       uint32_t vocab, uint32_t width, int dtype, float scale)
+{
+    const char *who = "sfb_token_logprobs_grad";
+    if (rows == 0) { clear_error(); return 0; }
+    if (check_rows(who, logits, pitch, rows, vocab, width, dtype, scale)) return 1;
+    SFB_REQUIRE(targets && stats && dlogp && out, "%s: NULL pointer", who);
+    SFB_REQUIRE(!entropy == !dentropy, "%s: entropy and dentropy go together", who);
+    SFB_REQUIRE(((uintptr_t)out & (elem_size(dtype) - 1)) == 0 && (out_pitch >= width || rows <= 1), "%s: out is misaligned or its rows overlap", who);
+    lg::GradParams p = {logits, out, pitch, out_pitch, rows, vocab, width, 0, 0, scale, scale * lg::kLog2e, targets, stats, dlogp, entropy, dentropy,
+                        nullptr, nullptr, nullptr, nullptr, 0, 0};
+    cudaStream_t s = as_stream(stream);
+    return dentropy ? BY_TYPE(dtype, lg::launch_grad, true, false, false)(s, p, who) : BY_TYPE(dtype, lg::launch_grad, false, false, false)(s, p, who);
+}
+
+extern "C" int sfb_distill_topk(sfb_stream_t stream, const void *logits, uint64_t pitch, const int32_t *ids, const float *teacher, uint32_t rows,
+                                uint32_t vocab, uint32_t k, int dtype, float scale, int tail, float *loss, float *stats, uint32_t *missed)
+{
+    const char *who = "sfb_distill_topk";
+    if (rows == 0) return set_zero(who, missed, as_stream(stream));
+    if (check_rows(who, logits, pitch, rows, vocab, vocab, dtype, scale)) return 1;
+    SFB_REQUIRE(ids && teacher && loss && stats, "%s: NULL pointer", who);
+    SFB_REQUIRE(k >= 1 && k <= lg::kMaxList, "%s: %u entries per list (1 to %u)", who, k, lg::kMaxList);
+    SFB_REQUIRE(!tail || vocab <= (1u << 20), "%s: vocab=%u is too large for the remainder (%u)", who, vocab, 1u << 20);
+    lg::StatParams p = {logits, pitch, rows, vocab, scale, scale * lg::kLog2e, nullptr, nullptr, stats, nullptr, nullptr, nullptr, k,
+                        ids, teacher, loss, missed, 0};
+    cudaStream_t s = as_stream(stream);
+    return tail ? BY_TYPE(dtype, lg::launch_stats, false, false, 2)(s, p, who) : BY_TYPE(dtype, lg::launch_stats, false, false, 1)(s, p, who);
+}
+
+extern "C" int sfb_distill_topk_grad(sfb_stream_t stream, const void *logits, uint64_t pitch, const int32_t *ids, const float *teacher,
+                                     const float *stats, const float *dloss, const int32_t *targets, const float *token_stats, const float *dlogp,
+                                     void *out, uint64_t out_pitch, uint32_t rows, uint32_t vocab, uint32_t width, uint32_t k, int dtype, float scale,
+                                     int tail)
+{
+    const char *who = "sfb_distill_topk_grad";
+    if (rows == 0) { clear_error(); return 0; }
+    if (check_rows(who, logits, pitch, rows, vocab, width, dtype, scale)) return 1;
+    SFB_REQUIRE(ids && teacher && stats && dloss && out, "%s: NULL pointer", who);
+    SFB_REQUIRE(!targets == !token_stats && !targets == !dlogp, "%s: targets, token_stats and dlogp go together", who);
+    SFB_REQUIRE(k >= 1 && k <= lg::kMaxList, "%s: %u entries per list (1 to %u)", who, k, lg::kMaxList);
+    SFB_REQUIRE(((uintptr_t)out & (elem_size(dtype) - 1)) == 0 && (out_pitch >= width || rows <= 1), "%s: out is misaligned or its rows overlap", who);
+    lg::GradParams p = {logits, out, pitch, out_pitch, rows, vocab, width, 0, 0, scale, scale * lg::kLog2e, targets, stats, dlogp, nullptr, nullptr,
+                        ids, teacher, dloss, token_stats, k, tail};
+    cudaStream_t s = as_stream(stream);
+    return targets ? BY_TYPE(dtype, lg::launch_grad, false, true, true)(s, p, who) : BY_TYPE(dtype, lg::launch_grad, false, true, false)(s, p, who);
+}
