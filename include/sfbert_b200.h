@@ -321,6 +321,15 @@ int sfb_distill_topk_grad(sfb_stream_t stream, const void *logits, uint64_t pitc
                           const float *dlogp, void *out, uint64_t out_pitch, uint32_t rows, uint32_t vocab, uint32_t width,
                           uint32_t k, int dtype, float scale, int tail);
 
+/* sfb_token_logprobs of logits = x . table^T + bias that are never written (nor rounded to 16 bits): x [m, k] and table [vocab, k] of
+ * type dtype (SFB_BF16 or SFB_F16), row-major, 16-byte aligned, k a multiple of 8; bias fp32 [vocab] or NULL; any vocab of at least 1.
+ * logp, stats, entropy (or NULL) and *missed (or NULL) as there, without alternatives.  workspace: device memory of
+ * sfb_linear_logprobs_workspace(m, vocab) bytes, 16-byte aligned, for this call alone. */
+uint64_t sfb_linear_logprobs_workspace(uint32_t m, uint32_t vocab);
+int sfb_linear_logprobs(sfb_stream_t stream, const void *x, const void *table, const float *bias, const int32_t *targets,
+                        uint32_t m, uint32_t vocab, uint32_t k, int dtype, float scale, float *logp, float *stats,
+                        float *entropy, uint32_t *missed, void *workspace);
+
 /* ---- element-sparse (CSR) attention: the alternative format the reference prototypes ------------------ */
 
 /* The CSR pattern of a block layout (ONE head, uint8 [nb][nb]): every element of every kept block, columns ascending.

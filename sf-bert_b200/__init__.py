@@ -29,6 +29,7 @@ SYMBOLS = [
     "sfb_csr_attention", "sfb_rowdot", "sfb_fused_sddmm_softmax_grad", "sfb_fused_attention_slice", "sfb_device_status_clear",
     "sfb_linear_residual", "sfb_attention_backward", "sfb_csr_workspace",
     "sfb_csr_attention_planned", "sfb_token_logprobs", "sfb_token_logprobs_grad", "sfb_distill_topk", "sfb_distill_topk_grad",
+    "sfb_linear_logprobs", "sfb_linear_logprobs_workspace",
 ]
 
 if not os.path.exists(LIB_PATH):
@@ -81,6 +82,10 @@ lib.sfb_token_logprobs.argtypes = [_vp, _vp, _u64, _vp, _u32, _u32, _i32, _f32] 
 lib.sfb_token_logprobs_grad.argtypes = [_vp, _vp, _u64] + [_vp] * 6 + [_u64, _u32, _u32, _u32, _i32, _f32]
 lib.sfb_distill_topk.argtypes = [_vp, _vp, _u64, _vp, _vp, _u32, _u32, _u32, _i32, _f32, _i32, _vp, _vp, _vp]
 lib.sfb_distill_topk_grad.argtypes = [_vp, _vp, _u64] + [_vp] * 8 + [_u64, _u32, _u32, _u32, _u32, _i32, _f32, _i32]
+
+lib.sfb_linear_logprobs_workspace.argtypes = [_u32, _u32]
+lib.sfb_linear_logprobs_workspace.restype = _u64
+lib.sfb_linear_logprobs.argtypes = [_vp] * 5 + [_u32, _u32, _u32, _i32, _f32] + [_vp] * 5
 
 
 def device_status():
@@ -344,6 +349,14 @@ def distill_topk_grad(logits, ids, teacher, stats, dloss, vocab=None, scale=1.0,
     """The gradient of distill_topk's loss with respect to the student's logits (out may be logits).  With targets, token_stats and dlogp
     (token_logprobs' stats at scale 1) the hard label's gradient dlogp * (onehot - softmax(logits)) is added in the same pass."""
     return _host.distill_topk_grad(logits, ids, teacher, stats, dloss, vocab, scale, tail, targets, token_stats, dlogp, out)
+
+
+def linear_logprobs(x, table, targets, bias=None, vocab=None, scale=1.0, entropy=False):
+    """token_logprobs(linear_nt(x, table, bias), targets) without the logits: scores of given tokens straight from hidden states
+    x [..., k] over the (tied) table [n, k], 16-bit, k a multiple of 8.  Only the first vocab rows of the table are tokens (None: all;
+    any number).  The logits are fp32 sums that are neither rounded nor stored.  Returns (logp, stats, entropy or
+    None, missed) as token_logprobs does."""
+    return _host.linear_logprobs(x, table, targets, bias, vocab, scale, entropy)
 
 
 def encoder_layer_tensor(x2d, w, lay, heads, ln_order, scale):

@@ -56,6 +56,9 @@ int tc_linear(cudaStream_t s, void *out, const void *x, const void *w, const flo
               int dtype, int act, bool w_transposed, const void *resid);
 int embedding_lookup(cudaStream_t s, void *out, const void *table, const int32_t *ids, const void *pos, uint32_t batch,
                      uint32_t seq_len, uint32_t hidden, uint32_t vocab, int dtype, uint32_t *bad_ids);
+uint64_t tc_linear_logprobs_workspace(uint32_t m, uint32_t n);
+int tc_linear_logprobs(cudaStream_t s, const void *x, const void *table, const float *bias, const int32_t *targets, uint32_t m, uint32_t n,
+                       uint32_t k, int dtype, float scale, float *logp, float *stats, float *entropy, uint32_t *missed, void *workspace);
 int tc_status_gemm(uint32_t *out);
 int tc_status_clear_gemm();
 

@@ -12,6 +12,7 @@
 // Every wait on an mbarrier is bounded; on a timeout the CTA records a status word and leaves through the
 // common teardown.
 #include "tc_common.cuh"
+#include "logits.cuh"
 
 namespace sfb {
 namespace tc {
@@ -38,6 +39,11 @@ struct GParams {
     int w_transposed;   // w is [n, k] row-major (out = x . w^T, the tied-embedding logits): its tile is a K-major B operand
     uint32_t band;      // CTA-pair kernel: column tiles per band of the tile order (tile_coords)
     const void *resid;  // split kernel: [m, n] of x's type, added to the product (not out itself), or NULL
+    // scores: what is kept of each row's 128 columns in place of the columns themselves
+    float4 *score_parts;       // [ceil(n / 128)][m]: largest, sum of the powers, sum of them times their exponents
+    float *target_logit;       // [m]
+    const int32_t *targets;    // [m]
+    float s2;                  // scale * log2(e)
 };
 
 // Tile t of the CTA-pair kernel -> (row tile, column tile).  The tiles run band by band, a band being `band` column
@@ -62,6 +68,15 @@ __device__ __forceinline__ void tile_coords(const GParams &p, uint32_t t, uint32
 __device__ __forceinline__ float4 fetch_bias(const GParams &p, uint32_t n0, uint32_t lane)
 {
     return p.bias && n0 + lane * 4 < p.N ? __ldg((const float4 *)(p.bias + n0 + lane * 4)) : make_float4(0.f, 0.f, 0.f, 0.f);
+}
+
+// The same where n need not be a multiple of 16 and the bias starts anywhere.
+__device__ __forceinline__ float4 fetch_bias_any(const GParams &p, uint32_t n0, uint32_t lane)
+{
+    float b[4];
+#pragma unroll
+    for (uint32_t j = 0; j < 4; j++) b[j] = p.bias && n0 + lane * 4 + j < p.N ? __ldg(p.bias + n0 + lane * 4 + j) : 0.f;
+    return make_float4(b[0], b[1], b[2], b[3]);
 }
 
 __device__ __forceinline__ float gelu_ref(float t)
@@ -175,6 +190,71 @@ __device__ __forceinline__ void drain_rows_staged(const GParams &p, const CUtens
     }
 }
 
+// The same share of an accumulator as logits that are never stored: the largest, the sum of 2^(s2 (x - r)) beside it and
+// (ENT) the sum of those times their exponents go to the row's part for these 128 columns, the target's logit to its
+// place.  A thread has a whole row of the tile, so nothing is exchanged.  128 columns cost a thread about 128 x 6
+// instructions and the SM 2048 cycles of exponentials per 256-column tile; the tile's MMAs take 2048 cycles per 256 of k.
+template <bool ENT>
+__device__ __forceinline__ void score_rows(const GParams &p, uint32_t tcol, const float *bias, uint32_t row, uint32_t n0)
+{
+    const bool row_ok = row < p.M;
+    const uint32_t target = row_ok ? (uint32_t)p.targets[row] : 0xffffffffu;
+    lg::Sums a;
+    float mx = lg::neg_inf();
+    const float gap = 40.f / p.s2;
+    uint32_t v[2][32];
+    TMEM_LD_32((v[0]), tcol);
+#pragma unroll
+    for (uint32_t c = 0; c < 4; c++) {
+        const uint32_t c0 = c * 32, col = n0 + c0;
+        __syncwarp();                        // the lanes parted over targets and references
+        tmem_wait_ld();
+        if (c + 1 < 4) TMEM_LD_32((v[(c + 1) & 1]), tcol + c0 + 32);
+        uint32_t(&cur)[32] = v[c & 1];
+        float x[32];
+#pragma unroll
+        for (int j = 0; j < 32; j++) x[j] = __uint_as_float(cur[j]);
+        if (p.bias) {
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const float4 bb = *(const float4 *)(bias + c0 + 4 * j);
+                x[4 * j] += bb.x; x[4 * j + 1] += bb.y; x[4 * j + 2] += bb.z; x[4 * j + 3] += bb.w;
+            }
+        }
+        if (col + 32 > p.N) {
+#pragma unroll
+            for (uint32_t j = 0; j < 32; j++)
+                if (col + j >= p.N) x[j] = lg::neg_inf();
+        }
+        if (target - col < 32u && target < p.N) {
+            float xt = x[0];
+#pragma unroll
+            for (uint32_t j = 1; j < 32; j++)
+                if (target - col == j) xt = x[j];
+            p.target_logit[row] = xt;
+        }
+        float m = x[0];
+#pragma unroll
+        for (int j = 1; j < 32; j++) m = lg::max_nan(m, x[j]);
+        mx = lg::max_nan(mx, m);
+        if (a.prepare(m, p.s2, gap)) {
+            float s[4] = {0.f, 0.f, 0.f, 0.f}, e[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int j = 0; j < 32; j++) {
+                const float t = p.s2 * (x[j] - a.r), y = lg::ex2(t);
+                s[j & 3] += y;
+                if (ENT) e[j & 3] = fmaf(y, fmaxf(t, lg::kFar), e[j & 3]);
+            }
+            a.s += (s[0] + s[1]) + (s[2] + s[3]);
+            if (ENT) a.e += (e[0] + e[1]) + (e[2] + e[3]);
+        }
+    }
+    a.move_to(mx, p.s2);
+    if (row_ok && n0 < p.N) p.score_parts[(size_t)(n0 / 128) * p.M + row] = make_float4(mx, a.s, a.e, 0.f);
+}
+
+// SCORE: 0 the product itself, 1 scores of its rows, 2 with the sum that the entropy takes
+template <int SCORE>
 __global__ void __launch_bounds__(320, 1)
 linear_tc_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap bmap, const GParams p)
 {
@@ -271,7 +351,8 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant
         const uint32_t r = quarter * 32 + lane;
         const uint32_t lane_field = (quarter * 32) << 16;
         uint32_t i = 0;
-        float4 next = fetch_bias(p, (blockIdx.x / p.tiles_m) * kGBN + chalf * 128, lane);
+        auto bias_of = [&](uint32_t n0) { return SCORE ? fetch_bias_any(p, n0, lane) : fetch_bias(p, n0, lane); };
+        float4 next = bias_of((blockIdx.x / p.tiles_m) * kGBN + chalf * 128);
         for (uint32_t t = blockIdx.x; t < n_tiles; t += gridDim.x, i++) {
             const uint32_t buf = i % kGBufs;
             const uint32_t n0 = (t / p.tiles_m) * kGBN + chalf * 128;
@@ -279,9 +360,10 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant
             if (!mbar_wait_warp(&st->acc_full[buf], (i / kGBufs) & 1, abort_flag, 44)) break;
             *(float4 *)(bias + lane * 4) = next;
             __syncwarp();
-            if (t + gridDim.x < n_tiles) next = fetch_bias(p, ((t + gridDim.x) / p.tiles_m) * kGBN + chalf * 128, lane);
+            if (t + gridDim.x < n_tiles) next = bias_of(((t + gridDim.x) / p.tiles_m) * kGBN + chalf * 128);
             tcgen05_fence_after();
-            drain_rows(p, tmem + buf * kGBN + chalf * 128 + lane_field, bias, (t % p.tiles_m) * kGBM + r, n0);
+            if (SCORE) score_rows<SCORE == 2>(p, tmem + buf * kGBN + chalf * 128 + lane_field, bias, (t % p.tiles_m) * kGBM + r, n0);
+            else drain_rows(p, tmem + buf * kGBN + chalf * 128 + lane_field, bias, (t % p.tiles_m) * kGBM + r, n0);
             tcgen05_fence_before();
             mbar_arrive(&st->acc_empty[buf]);
         }
@@ -391,6 +473,7 @@ __device__ __forceinline__ void umma_commit_pair(uint64_t *bar)
                  : "memory");
 }
 
+template <int SCORE>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(320, 1)
 linear_tc_pair_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap bmap,
                       const __grid_constant__ CUtensorMap omap, const GParams p)
@@ -496,7 +579,8 @@ linear_tc_pair_kernel(const __grid_constant__ CUtensorMap amap, const __grid_con
         const uint32_t acc_empty0[2] = {mapa_rank(smem_u32(&st->acc_empty[0]), 0), mapa_rank(smem_u32(&st->acc_empty[1]), 0)};
         uint32_t i = 0, tm, tn;
         tile_coords(p, pair, tm, tn);
-        float4 next = fetch_bias(p, tn * kGBN + chalf * 128, lane);
+        auto bias_of = [&](uint32_t n0) { return SCORE ? fetch_bias_any(p, n0, lane) : fetch_bias(p, n0, lane); };
+        float4 next = bias_of(tn * kGBN + chalf * 128);
         for (uint32_t t = pair; t < n_tiles; t += pairs, i++) {
             const uint32_t buf = i & 1;
             const uint32_t n0 = tn * kGBN + chalf * 128;
@@ -507,10 +591,11 @@ linear_tc_pair_kernel(const __grid_constant__ CUtensorMap amap, const __grid_con
             __syncwarp();
             if (t + pairs < n_tiles) {
                 tile_coords(p, t + pairs, tm, tn);
-                next = fetch_bias(p, tn * kGBN + chalf * 128, lane);
+                next = bias_of(tn * kGBN + chalf * 128);
             }
             tcgen05_fence_after();
-            drain_rows_staged(p, &omap, tmem + buf * kGBN + chalf * 128 + lane_field, staging + (warp - 2) * 4096, bias, m0 + quarter * 32, n0, lane);
+            if (SCORE) score_rows<SCORE == 2>(p, tmem + buf * kGBN + chalf * 128 + lane_field, bias, m0 + quarter * 32 + lane, n0);
+            else drain_rows_staged(p, &omap, tmem + buf * kGBN + chalf * 128 + lane_field, staging + (warp - 2) * 4096, bias, m0 + quarter * 32, n0, lane);
             tcgen05_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive_cluster(buf ? acc_empty0[1] : acc_empty0[0]);
@@ -880,7 +965,7 @@ static int linear_product(cudaStream_t s, void *out, const void *x, const void *
         if (w_transposed ? make_map_2d(&bp, w, n, k, is_bf16, kGBN / 2) : make_map_2d(&bp, w, k, n, is_bf16, kGBK)) return 1;
         static DeviceOnce once_pair;
         if (!once_pair.done(dev)) {
-            if (cudaFuncSetAttribute(linear_tc_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kPSmem) != cudaSuccess)
+            if (cudaFuncSetAttribute(linear_tc_pair_kernel<0>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kPSmem) != cudaSuccess)
                 return fail("sfb_linear: cannot reserve %zu bytes of shared memory", kPSmem);
             once_pair.mark(dev);
         }
@@ -890,14 +975,14 @@ static int linear_product(cudaStream_t s, void *out, const void *x, const void *
         prm.band = tiles_n < kPBand ? tiles_n : kPBand;
         const uint64_t pair_tiles = (uint64_t)prm.tiles_m * tiles_n;
         const uint32_t pairs = pair_tiles < (uint64_t)(sms / 2) ? (uint32_t)pair_tiles : (uint32_t)(sms / 2);
-        if (launch_overlapped(linear_tc_pair_kernel, dim3(2 * pairs), dim3(320), kPSmem, s, am, bp, om, prm) == cudaSuccess)
+        if (launch_overlapped(linear_tc_pair_kernel<0>, dim3(2 * pairs), dim3(320), kPSmem, s, am, bp, om, prm) == cudaSuccess)
             return check_launch("sfb_linear");
         (void)cudaGetLastError();
     }
     if (w_transposed ? make_map_2d(&bm, w, n, k, is_bf16, kGBN) : make_map_2d(&bm, w, k, n, is_bf16, kGBK)) return 1;
     static DeviceOnce once;
     if (!once.done(dev)) {
-        if (cudaFuncSetAttribute(linear_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kGSmem) != cudaSuccess)
+        if (cudaFuncSetAttribute(linear_tc_kernel<0>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kGSmem) != cudaSuccess)
             return fail("sfb_linear: cannot reserve %zu bytes of shared memory", kGSmem);
         once.mark(dev);
     }
@@ -905,7 +990,7 @@ static int linear_product(cudaStream_t s, void *out, const void *x, const void *
     prm.band = 1;
     const uint64_t tiles = (uint64_t)prm.tiles_m * prm.tiles_n;
     const uint32_t grid = tiles < (uint64_t)sms ? (uint32_t)tiles : (uint32_t)sms;
-    launch_overlapped(linear_tc_kernel, dim3(grid), dim3(320), kGSmem, s, am, bm, prm);
+    launch_overlapped(linear_tc_kernel<0>, dim3(grid), dim3(320), kGSmem, s, am, bm, prm);
     return check_launch("sfb_linear");
 }
 
@@ -922,6 +1007,125 @@ int tc_linear(cudaStream_t s, void *out, const void *x, const void *w, const flo
     if (dtype == SFB_BF16) launch_overlapped(add_residual_kernel<true>, grid, dim3(256), 0, s, out, resid, pieces);
     else launch_overlapped(add_residual_kernel<false>, grid, dim3(256), 0, s, out, resid, pieces);
     return check_launch("sfb_linear_residual");
+}
+
+// ---- scores ---------------------------------------------------------------------------------------------------------------
+// A row's parts joined: R rows per CTA, its other threads spread over the parts.
+template <bool ENT>
+__global__ void __launch_bounds__(256) score_join_kernel(const float4 *parts, const float *target_logit, const int32_t *targets, uint32_t n_parts,
+                                                         uint32_t m, uint32_t vocab, uint32_t R, float scale, float s2, float *logp, float *stats,
+                                                         float *entropy, uint32_t *missed)
+{
+    using namespace lg;
+    __shared__ float sh[3][256];
+    const uint32_t tid = threadIdx.x, lr = tid % R, row = blockIdx.x * R + lr, groups = 256 / R;
+    grid_dependency_wait();
+    grid_launch_dependents();
+    if (blockIdx.x * R >= m) {                   // the CTA behind the rows' counts the targets that are none
+        uint32_t bad = 0;
+        for (uint32_t i = tid; i < m; i += 256) bad += (uint32_t)targets[i] >= vocab;
+        bad = __reduce_add_sync(0xffffffffu, bad);
+        if (tid % 32 == 0) ((uint32_t *)sh)[tid / 32] = bad;
+        __syncthreads();
+        for (uint32_t w = 1; w < 8; w++) bad += ((const uint32_t *)sh)[w];
+        if (tid == 0) *missed = bad;
+        return;
+    }
+    Sums a;
+    float mx = neg_inf();
+    if (row < m) {
+        for (uint32_t i = tid / R; i < n_parts; i += groups) {
+            const float4 q = parts[(size_t)i * m + row];
+            Sums b;
+            b.r = q.x; b.s = q.y; b.e = q.z;
+            const float top = max_nan(mx, q.x);
+            a.move_to(top, s2);
+            b.move_to(top, s2);
+            a.s += b.s; a.e += b.e;
+            mx = top;
+        }
+    }
+    sh[0][tid] = mx; sh[1][tid] = a.s; sh[2][tid] = a.e;
+    for (uint32_t half = 128; half >= R; half >>= 1) {
+        __syncthreads();
+        if (tid < half) {
+            Sums x, y;
+            x.r = sh[0][tid]; x.s = sh[1][tid]; x.e = sh[2][tid];
+            y.r = sh[0][tid + half]; y.s = sh[1][tid + half]; y.e = sh[2][tid + half];
+            const float top = max_nan(x.r, y.r);
+            x.move_to(top, s2);
+            y.move_to(top, s2);
+            sh[0][tid] = top; sh[1][tid] = x.s + y.s; sh[2][tid] = x.e + y.e;
+        }
+    }
+    __syncthreads();
+    if (tid >= R || row >= m) return;
+    const float top = sh[0][tid], s = sh[1][tid];
+    const bool empty = top == neg_inf(), inside = (uint32_t)targets[row] < vocab;
+    const float l = empty ? neg_inf() : logf(s);
+    const bool asked = inside || ENT;
+    stats[2 * (size_t)row] = asked ? top : 0.f;
+    stats[2 * (size_t)row + 1] = asked ? l : 0.f;
+    logp[row] = !inside ? 0.f : empty ? neg_inf() : scale * (target_logit[row] - top) - l;
+    if (ENT) entropy[row] = empty ? 0.f : l - kLn2 * (sh[2][tid] / s);
+}
+
+uint64_t tc_linear_logprobs_workspace(uint32_t m, uint32_t n) { return ((uint64_t)((n + 127) / 128) * 16 + 4) * m; }
+
+template <bool ENT> static int linear_logprobs(cudaStream_t s, const void *x, const void *table, const float *bias, const int32_t *targets, uint32_t m,
+                                               uint32_t n, uint32_t k, int dtype, float scale, float *logp, float *stats, float *entropy,
+                                               uint32_t *missed, void *workspace)
+{
+    using namespace tc;
+    const char *who = "sfb_linear_logprobs";
+    const int is_bf16 = dtype == SFB_BF16;
+    constexpr int kScore = ENT ? 2 : 1;
+    const int dev = current_device(), sms = device_sm_count(dev);
+    if (sms <= 0) return fail("%s: cannot read the SM count", who);
+    const uint32_t tiles_n = (n + kGBN - 1) / kGBN, n_parts = (n + 127) / 128;
+    float4 *parts = (float4 *)workspace;
+    float *target_logit = (float *)(parts + (size_t)n_parts * m);
+    GParams prm = {nullptr, bias, m, n, k, 0, tiles_n, is_bf16, SFB_ACT_NONE, 1, 1, nullptr, parts, target_logit, targets, scale * lg::kLog2e};
+    CUtensorMap am, bm;
+    if (make_map_2d(&am, x, m, k, is_bf16, kGBM)) return 1;
+    static DeviceOnce once;
+    if (!once.done(dev)) {
+        if (cudaFuncSetAttribute(linear_tc_pair_kernel<kScore>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kPSmem) != cudaSuccess ||
+            cudaFuncSetAttribute(linear_tc_kernel<kScore>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kGSmem) != cudaSuccess)
+            return fail("%s: cannot reserve %zu bytes of shared memory", who, kPSmem);
+        once.mark(dev);
+    }
+    bool launched = false;
+    if (kUsePairs && sms >= 2 && m > kGBM) {
+        if (make_map_2d(&bm, table, n, k, is_bf16, kGBN / 2)) return 1;
+        prm.tiles_m = (m + 255) / 256;
+        prm.band = tiles_n < kPBand ? tiles_n : kPBand;
+        const uint64_t tiles = (uint64_t)prm.tiles_m * tiles_n;
+        const uint32_t pairs = tiles < (uint64_t)(sms / 2) ? (uint32_t)tiles : (uint32_t)(sms / 2);
+        launched = launch_overlapped(linear_tc_pair_kernel<kScore>, dim3(2 * pairs), dim3(320), kPSmem, s, am, bm, am, prm) == cudaSuccess;
+        if (!launched) (void)cudaGetLastError();
+    }
+    if (!launched) {
+        if (make_map_2d(&bm, table, n, k, is_bf16, kGBN)) return 1;
+        prm.tiles_m = (m + kGBM - 1) / kGBM;
+        prm.band = 1;
+        const uint64_t tiles = (uint64_t)prm.tiles_m * tiles_n;
+        launch_overlapped(linear_tc_kernel<kScore>, dim3(tiles < (uint64_t)sms ? (uint32_t)tiles : (uint32_t)sms), dim3(320), kGSmem, s, am, bm, prm);
+    }
+    if (check_launch(who)) return 1;
+    // as many rows per CTA (up to 32, a warp's) as leave a CTA for every SM
+    uint32_t R = 1;
+    while (R < 32 && m / (2 * R) >= (uint32_t)sms) R *= 2;
+    launch_overlapped(score_join_kernel<ENT>, dim3((m + R - 1) / R + (missed ? 1 : 0)), dim3(256), 0, s, (const float4 *)parts, (const float *)target_logit,
+                      targets, n_parts, m, n, R, scale, prm.s2, logp, stats, entropy, missed);
+    return check_launch(who);
+}
+
+int tc_linear_logprobs(cudaStream_t s, const void *x, const void *table, const float *bias, const int32_t *targets, uint32_t m, uint32_t n,
+                       uint32_t k, int dtype, float scale, float *logp, float *stats, float *entropy, uint32_t *missed, void *workspace)
+{
+    return entropy ? linear_logprobs<true>(s, x, table, bias, targets, m, n, k, dtype, scale, logp, stats, entropy, missed, workspace)
+                   : linear_logprobs<false>(s, x, table, bias, targets, m, n, k, dtype, scale, logp, stats, entropy, missed, workspace);
 }
 
 int tc_status_clear_gemm()

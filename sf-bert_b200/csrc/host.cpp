@@ -21,7 +21,7 @@ namespace {
     X(sfb_linear_nt) X(sfb_linear_residual) X(sfb_embedding) X(sfb_csr_attention) X(sfb_csr_attention_planned) X(sfb_csr_workspace) X(sfb_rowdot) X(sfb_fused_sddmm_softmax_grad)                  \
     X(sfb_fused_sddmm_softmax) X(sfb_fused_attention) X(sfb_fused_attention_slice) X(sfb_bias_residual_layernorm)         \
     X(sfb_bias_gelu) X(sfb_attention_backward) X(sfb_token_logprobs) X(sfb_token_logprobs_grad) X(sfb_distill_topk)      \
-    X(sfb_distill_topk_grad)
+    X(sfb_distill_topk_grad) X(sfb_linear_logprobs) X(sfb_linear_logprobs_workspace)
 struct Lib {
 #define DECL(f) decltype(&::f) f = nullptr;
     SFB_FUNCTIONS(DECL)
@@ -708,6 +708,39 @@ FUNCTION(py_distill_topk_grad, 12)
          (uint64_t)LogitRows(out).pitch, (uint32_t)x.rows, (uint32_t)vocab, (uint32_t)x.width, (uint32_t)k, t, scale, (int)tail);
     return wrap(out);
 }
+// (x, table, targets, bias, vocab, scale, entropy) -> (logp, stats, entropy, missed)
+FUNCTION(py_linear_logprobs, 7)
+{
+    const LogitRows x(tensor(a[0]));
+    const at::Tensor &table = tensor(a[1]);
+    require(table.dim() == 2 && table.size(1) == x.width && table.scalar_type() == x.t.scalar_type() && table.device() == x.t.device() &&
+                x.t.is_contiguous() && table.is_contiguous(),
+            "x and table must be contiguous, of one type, on one device and of matching sizes");
+    const int64_t vocab = a[4] == Py_None ? table.size(0) : (int64_t)integer(a[4]);
+    require(vocab >= 1 && vocab <= table.size(0) && vocab <= (1ll << 30), "vocab must be 1 to the number of rows of the table");
+    const float scale = positive_scale(a[5]);
+    const bool ent = truth(a[6]);
+    const int t = tag(x.t);
+    const int32_t *targets = (int32_t *)ptr(beside(a[2], x, at::kInt, 0, bad_targets));
+    const float *bias = nullptr;
+    if (a[3] != Py_None) {
+        const at::Tensor &b = tensor(a[3]);
+        require(b.scalar_type() == at::kFloat && b.dim() == 1 && b.size(0) >= vocab && b.is_contiguous() && b.device() == x.t.device(),
+                "bias must be a contiguous fp32 vector of an element per token");
+        bias = (const float *)ptr(b);
+    }
+    require_cuda(x.t);
+    const c10::cuda::CUDAGuard on(x.t.device());
+    at::Tensor logp = rows_like(x, 0, at::kFloat), stats = rows_like(x, 2, at::kFloat), missed = empty({1}, at::kInt, x.t), entropy;
+    if (ent) entropy = rows_like(x, 0, at::kFloat);
+    at::Tensor ws = empty({(int64_t)L.sfb_linear_logprobs_workspace((uint32_t)x.rows, (uint32_t)vocab)}, at::kByte, x.t);
+    call(L.sfb_linear_logprobs, stream_of(x.t), ptr(x.t), ptr(table), bias, targets, (uint32_t)x.rows, (uint32_t)vocab, (uint32_t)x.width, t, scale,
+         (float *)ptr(logp), (float *)ptr(stats), ent ? (float *)ptr(entropy) : nullptr, (uint32_t *)ptr(missed), ptr(ws));
+    Ref l(wrap(logp)), s(wrap(stats)), n(wrap(missed));
+    if (!ent) return PyTuple_Pack(4, l.o, s.o, Py_None, n.o);
+    Ref e(wrap(entropy));
+    return PyTuple_Pack(4, l.o, s.o, e.o, n.o);
+}
 
 // bind(addresses by name): which build of the library the functions call
 PyObject *py_bind(PyObject *, PyObject *args)
@@ -739,7 +772,7 @@ PyMethodDef methods[] = {
     ENTRY(bst_sgemm_nt), ENTRY(masked_softmax), ENTRY(bst_sgemm), ENTRY(masked_softmax_grad), ENTRY(rowdot), ENTRY(fused_sddmm_softmax_grad),
     ENTRY(fused_sddmm_softmax), ENTRY(linear), ENTRY(embedding), ENTRY(csr_attention), ENTRY(fused_attention), ENTRY(fused_attention_slice),
     ENTRY(bias_residual_layernorm), ENTRY(bias_gelu), ENTRY(encoder_layer), ENTRY(attention_backward_fused), ENTRY(attention_backward),
-    ENTRY(token_logprobs), ENTRY(token_logprobs_grad), ENTRY(distill_topk), ENTRY(distill_topk_grad),
+    ENTRY(token_logprobs), ENTRY(token_logprobs_grad), ENTRY(distill_topk), ENTRY(distill_topk_grad), ENTRY(linear_logprobs),
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -832,3 +832,20 @@ extern "C" int sfb_distill_topk_grad(sfb_stream_t stream, const void *logits, ui
     cudaStream_t s = as_stream(stream);
     return targets ? BY_TYPE(dtype, lg::launch_grad, false, true, true)(s, p, who) : BY_TYPE(dtype, lg::launch_grad, false, true, false)(s, p, who);
 }
+
+extern "C" uint64_t sfb_linear_logprobs_workspace(uint32_t m, uint32_t vocab) { return tc_linear_logprobs_workspace(m, vocab); }
+
+extern "C" int sfb_linear_logprobs(sfb_stream_t stream, const void *x, const void *table, const float *bias, const int32_t *targets, uint32_t m,
+                                   uint32_t vocab, uint32_t k, int dtype, float scale, float *logp, float *stats, float *entropy, uint32_t *missed,
+                                   void *workspace)
+{
+    const char *who = "sfb_linear_logprobs";
+    if (m == 0) return set_zero(who, missed, as_stream(stream));
+    SFB_REQUIRE(x && table && targets && logp && stats && workspace, "%s: NULL pointer", who);
+    SFB_REQUIRE(dtype == SFB_BF16 || dtype == SFB_F16, "%s: x and table must be bf16 or fp16", who);
+    SFB_REQUIRE(vocab >= 1 && vocab <= (1u << 30) && k >= 8 && k % 8 == 0 && k <= (1u << 30), "%s: vocab=%u must be at least 1, k=%u a multiple of 8", who, vocab, k);
+    SFB_REQUIRE(m < (1u << 27), "%s: too many rows", who);
+    SFB_REQUIRE((((uintptr_t)x | (uintptr_t)table | (uintptr_t)workspace) & 15) == 0, "%s: x, table and workspace must be 16-byte aligned", who);
+    SFB_REQUIRE(scale > 0.f && scale <= 1e6f, "%s: scale must be positive (and at most 1e6)", who);
+    return tc_linear_logprobs(as_stream(stream), x, table, bias, targets, m, vocab, k, dtype, scale, logp, stats, entropy, missed, workspace);
+}

@@ -406,3 +406,83 @@ def test_no_rows(sfb):
     loss, st, missed = sfb.distill_topk(x, ids, teacher, tail=True)
     assert loss.shape == (0,) and st.shape == (0, 3) and int(missed) == 0
     assert sfb.distill_topk_grad(x, ids, teacher, st, f, tail=True).shape == (0, 50)
+
+
+# ---- scores without logits -------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("m,vocab,rows,k", [(1, 1, 1, 8), (1, 30522, 30528, 768), (7, 1000, 1000, 72), (128, 129, 129, 64), (129, 255, 256, 128), (300, 5003, 5003, 264),
+                                            (700, 30522, 30528, 768), (2000, 2049, 2049, 40), (5000, 260, 260, 1024)])
+def test_linear_logprobs(sfb, m, vocab, rows, k, dtype):
+    """A logit is a sum of k exact products, rounded at most once per 16 of them and in the accumulator: off by 2^-22 (k / 16 + 4)
+    of the sum of their sizes; a logarithm of a sum of exponentials by the largest such error, on top of the bounds above (a
+    thread adds 128 terms, a row's parts are joined in at most vocab / 128 steps)."""
+    g = gen(m + vocab)
+    x = torch.randn(m, k, device="cuda", generator=g).to(TYPES[dtype])
+    table = (2.0 / math.sqrt(k) * torch.randn(rows, k, device="cuda", generator=g)).to(TYPES[dtype])
+    table[vocab:] = INF
+    t = torch.randint(-1, vocab + 1, (m,), device="cuda", generator=g, dtype=torch.int32)
+    t[0] = vocab - 1
+    for scale, entropy, bias in [(1.0, False, None), (0.7, True, torch.randn(rows + 1, device="cuda", generator=g)[1:])]:
+        logp, stats, ent, missed = sfb.linear_logprobs(x, table, t, bias=bias, vocab=vocab, scale=scale, entropy=entropy)
+        assert sfb.device_status() == 0
+        z = x.double() @ table[:vocab].double().t() + (0 if bias is None else bias[:vocab].double())
+        off = scale * 2.0 ** -22 * (k / 16 + 4) * float((x.double().abs() @ table[:vocab].double().abs().t()).amax() + 4)
+        want = R.token_logprobs(z, t, vocab, scale)
+        d = R.bounds(vocab) + 2.0 ** -24 * 128 + 2 * off
+        nothing = torch.zeros_like(want["m"], dtype=torch.bool) if entropy else (t < 0) | (t >= vocab)
+        assert int(missed) == want["missed"]
+        same(logp, want["logp"], d + 2.0 ** -22 * want["logp"].abs(), "logp")
+        same(stats[:, 0], torch.where(nothing, 0.0, want["m"]), off / scale, "m")
+        same(stats[:, 1], torch.where(nothing, 0.0, want["l"]), d, "l")
+        if entropy:
+            same(ent, want["entropy"], 2 * d * (1 + 2 * want["entropy"].abs()), "entropy")
+        else:
+            assert ent is None
+        again = sfb.linear_logprobs(x, table, t, bias=bias, vocab=vocab, scale=scale, entropy=entropy)
+        assert torch.equal(logp, again[0]) and torch.equal(stats, again[1])
+
+
+def test_linear_logprobs_of_what_is_not_finite(sfb):
+    m, vocab, k = 200, 1000, 64
+    g = gen(3)
+    x = torch.randn(m, k, device="cuda", generator=g).to(torch.bfloat16)
+    table = torch.randn(vocab, k, device="cuda", generator=g).to(torch.bfloat16)
+    t = torch.full((m,), 5, device="cuda", dtype=torch.int32)
+    t[1] = 900
+    bias = torch.zeros(vocab, device="cuda")
+    bias[700:] = -INF                                                    # banned tokens
+    logp, stats, ent, _ = sfb.linear_logprobs(x, table, t, bias=bias, entropy=True)
+    z = x.double() @ table.double().t() + bias.double()
+    want = R.token_logprobs(z, t, vocab, 1.0)
+    same(logp, want["logp"], 1e-4, "logp")                               # 64 products of size 1: off by 2^-22 * 8 * 64
+    same(ent, want["entropy"], 1e-3, "entropy")
+    bias[:] = -INF
+    logp, stats, ent, _ = sfb.linear_logprobs(x, table, t, bias=bias, entropy=True)
+    assert bool((logp == -INF).all()) and bool((stats == -INF).all()) and not bool(ent.any())
+    x[3, 0] = math.nan
+    logp, stats, _, _ = sfb.linear_logprobs(x, table, t)
+    assert bool(logp[3].isnan()) and int(logp.isnan().sum()) == 1
+    assert sfb.device_status() == 0
+
+
+def test_linear_logprobs_captured_beside_another(sfb):
+    """Two captured calls and an eager one between them: each has a workspace of its own."""
+    g = gen(4)
+    x = [torch.randn(2, 150, 256, device="cuda", generator=g).to(torch.float16) for _ in range(2)]
+    table = (0.1 * torch.randn(7000, 256, device="cuda", generator=g)).to(torch.float16)
+    t = torch.randint(0, 7000, (2, 150), device="cuda", generator=g, dtype=torch.int32)
+    want = [sfb.linear_logprobs(y, table, t, entropy=True) for y in x]
+    torch.cuda.synchronize()
+    graphs, held = [torch.cuda.CUDAGraph() for _ in x], []
+    for n in (0, 1):
+        with torch.cuda.graph(graphs[n]):
+            held.append(sfb.linear_logprobs(x[n], table, t, entropy=True))
+    streams = [torch.cuda.Stream() for _ in x]
+    for _ in range(5):
+        for n in (0, 1):
+            with torch.cuda.stream(streams[n]):
+                graphs[n].replay()
+        sfb.linear_logprobs(x[0], table, t)
+    torch.cuda.synchronize()
+    for a, b in zip(held, want):
+        assert all(torch.equal(p, q) for p, q in zip(a, b)) and a[0].shape == (2, 150)
