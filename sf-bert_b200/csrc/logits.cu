@@ -85,19 +85,32 @@ template <bool ENT> __device__ __forceinline__ void warp_sums(Sums &a, float &mx
     if (ENT) a.e = warp_sum(a.e);
 }
 
-template <int DT, bool ENT> __device__ __forceinline__ void add_window(Sums &a, const uint4 &v, float s2)
+// N windows into the sums
+template <int DT, bool ENT, int N> __device__ __forceinline__ void add_windows(Sums &a, const uint4 (&v)[N], float s2)
 {
-    float x[Win<DT>::kElems];
-    unpack<DT>(v, x);
-    float s = 0.f, e = 0.f;
+    const Pair minus_r = pair(-a.r, -a.r), factor = pair(s2, s2);
+    Pair s = pair(a.s, 0.f), e = pair(a.e, 0.f);
 #pragma unroll
-    for (uint32_t j = 0; j < Win<DT>::kElems; j++) {
-        const float t = s2 * (x[j] - a.r), y = ex2(t);
-        s += y;
-        if (ENT) e = fmaf(y, fmaxf(t, kFar), e);
+    for (int u = 0; u < N; u++) {
+        float x[Win<DT>::kElems];
+        unpack<DT>(v[u], x);
+#pragma unroll
+        for (uint32_t j = 0; j < Win<DT>::kElems; j += 2) {
+            const Pair t = mul2(factor, add2(pair(x[j], x[j + 1]), minus_r));
+            float t0, t1;
+            halves(t, t0, t1);
+            const Pair y = pair(ex2(t0), ex2(t1));
+            s = add2(s, y);
+            if (ENT) e = fma2(y, pair(fmaxf(t0, kFar), fmaxf(t1, kFar)), e);
+        }
     }
-    a.s += s;
-    if (ENT) a.e += e;
+    float s0, s1;
+    halves(s, s0, s1);
+    a.s = s0 + s1;
+    if (ENT) {
+        halves(e, s0, s1);
+        a.e = s0 + s1;
+    }
 }
 
 // listed tokens of a window (bit j: element j) become -inf
@@ -215,6 +228,81 @@ template <int DT> __device__ __noinline__ void bisect_candidates(const Row<DT> r
     __syncthreads();
 }
 
+template <int DT> __device__ __forceinline__ uint32_t listed_bits(const uint8_t *bits, uint32_t w)
+{
+    return DT == SFB_F32 ? bits[w >> 1] >> ((w & 1) * 4) & 15u : bits[w];
+}
+// a window that is not in the row as a whole; returns its largest element
+template <int DT, bool ENT, int KD> __device__ __forceinline__ float add_edge(Sums &a, const Row<DT> &row, uint32_t w, const uint8_t *bits, float s2, float gap)
+{
+    uint4 v[1] = {edge_window<DT>(row.base, row.head, row.end, w)};
+    if (KD == 2 && listed_bits<DT>(bits, w)) drop_listed<DT>(v[0], listed_bits<DT>(bits, w));
+    const float m = max_windows<DT, 1>(v);
+    if (a.prepare(m, s2, gap)) add_windows<DT, ENT, 1>(a, v, s2);
+    return m;
+}
+
+// a row of tokens, its sums known beside m
+template <bool ENT> __device__ __forceinline__ void finish_tokens(const StatParams &p, uint32_t r, int32_t target, float x_target, float m, float s, float e)
+{
+    const bool empty = m == neg_inf();
+    const float l = empty ? neg_inf() : logf(s);
+    p.stats[2 * (size_t)r] = m;
+    p.stats[2 * (size_t)r + 1] = l;
+    if (p.logp) p.logp[r] = target < 0 ? 0.f : empty ? neg_inf() : p.scale * (x_target - m) - l;
+    if (ENT) p.entropy[r] = empty ? 0.f : l - kLn2 * (e / s);
+}
+
+// What one warp makes of a row of lists, its sums known: m and s beside it, rest = s without the listed tokens.
+template <int KD> __device__ __forceinline__ void finish_lists(const StatParams &p, uint32_t r, const int32_t *l_id, const float *l_q, const float *l_x,
+                                                               bool twice, float m, float rest)
+{
+    const uint32_t lane = threadIdx.x & 31;
+    float s = rest;
+    if (KD == 2) {
+        float listed = 0.f;
+        for (uint32_t i = lane; i < p.k; i += 32) {
+            if (l_id[i] < 0 || l_x[i] == neg_inf()) continue;
+            bool again = false;
+            if (twice)
+                for (uint32_t j = 0; j < i; j++) again |= l_id[j] == l_id[i];
+            if (!again) listed += ex2(p.s2 * (l_x[i] - m));
+        }
+        s = rest + warp_sum(listed);
+    }
+    const float l = m == neg_inf() ? neg_inf() : logf(s);
+    // the teacher's probabilities
+    float mq = KD == 1 ? neg_inf() : 0.f, zq = 0.f;
+    if (KD == 1) {
+        for (uint32_t i = lane; i < p.k; i += 32) mq = max_nan(mq, l_q[i]);
+        mq = warp_max_nan(mq);
+    }
+    if (mq != neg_inf())
+        for (uint32_t i = lane; i < p.k; i += 32) zq += expf(l_q[i] - mq);
+    zq = warp_sum(zq);
+    const float lz = KD == 1 ? mq + logf(zq) : 0.f;
+    float loss = 0.f;
+    if (mq != neg_inf()) {
+        for (uint32_t i = lane; i < p.k; i += 32) {
+            const float lq = l_q[i] - lz, q = expf(lq);
+            const float lp = l_x[i] == neg_inf() ? neg_inf() : p.scale * (l_x[i] - m) - l;
+            if (!(q <= 0.f)) loss += q * (lq - lp);
+        }
+    }
+    loss = warp_sum(loss);
+    if (lane == 0) {
+        float *st = p.stats + (KD == 2 ? 3 : 2) * (size_t)r;
+        st[0] = m;
+        st[1] = l;
+        if (KD == 2) {
+            const float left = fmaxf(0.f, 1.f - zq), lr = rest == 0.f ? neg_inf() : logf(rest);
+            if (left > 0.f && !(lr == neg_inf())) loss += left * (logf(left) - (lr - l));
+            st[2] = lr;
+        }
+        p.loss[r] = loss;
+    }
+}
+
 // A row's statistics, and what is made of them.  One CTA per row, or a cluster of CTAs where there are few rows: each
 // takes every C-th piece, and CTA 0 joins the parts.  KD: 0 tokens, 1 lists, 2 lists with the remainder as one more class.
 template <int DT, bool ENT, bool TOP, int KD>
@@ -260,7 +348,25 @@ __global__ void __launch_bounds__(kThreads, 4) row_stats_kernel(const StatParams
 
     const void *x = (const char *)p.x + (size_t)r * p.pitch * Win<DT>::kSize;
     const Row<DT> row(x, p.vocab);
-    const uint32_t windows = row.windows();
+    // The pass goes by groups of kU windows per thread, the next group on its way while one is added up; the first sets out here.
+    Sums a;
+    float mx = neg_inf();
+    const float gap = 40.f / p.s2;
+    const uint32_t n_whole = row.whole_count(), step = C * kU * T, first = rank * kU * T;
+    const uint4 *src = row.base + row.first_whole() + tid;
+    const bool edges = rank == 0 && tid == 0 && row.windows() != n_whole;       // what is not a whole window: thread 0's
+    float *keys = (float *)dyn;
+    auto load = [&](uint4 (&v)[kU], uint32_t i0) {
+        if (i0 + kU * T <= n_whole) {
+#pragma unroll
+            for (int u = 0; u < kU; u++) v[u] = load16(src + i0 + u * T);
+        } else {
+#pragma unroll
+            for (int u = 0; u < kU; u++) v[u] = i0 + u * T + tid < n_whole ? load16(src + i0 + u * T) : no_elements<DT>();
+        }
+    };
+    uint4 v[kU], next[kU];
+    if (first < n_whole) load(next, first);
     float x_target = 0.f;
     if (KD == 0 && target >= 0 && rank == 0 && tid < 64) x_target = load_element<DT>(x, (uint32_t)target);
 
@@ -293,37 +399,32 @@ __global__ void __launch_bounds__(kThreads, 4) row_stats_kernel(const StatParams
     }
 
     // ---- the pass ----
-    Sums a;
-    float mx = neg_inf();
-    const float gap = 40.f / p.s2;
-    const uint32_t step = C * kU * T, first = rank * kU * T + tid;
-    float *keys = (float *)dyn;
-    uint4 v[kU], next[kU];
-#pragma unroll
-    for (int u = 0; u < kU; u++) next[u] = load_window(row, first + u * T);
-    for (uint32_t w0 = first, g = 0; w0 - tid < windows; w0 += step, g++) {
+    uint32_t groups = 0;
+    for (uint32_t i0 = first; i0 < n_whole; i0 += step, groups++) {
 #pragma unroll
         for (int u = 0; u < kU; u++) v[u] = next[u];
-        if (w0 - tid + step < windows) {
-#pragma unroll
-            for (int u = 0; u < kU; u++) next[u] = load_window(row, w0 + step + u * T);
-        }
+        if (i0 + step < n_whole) load(next, i0 + step);
         if (KD == 2) {
 #pragma unroll
             for (int u = 0; u < kU; u++) {
-                const uint32_t w = w0 + u * T;
-                uint32_t b = 0;
-                if (w < windows) b = DT == SFB_F32 ? dyn[w >> 1] >> ((w & 1) * 4) & 15u : dyn[w];
+                const uint32_t i = i0 + u * T + tid;
+                const uint32_t b = i < n_whole ? listed_bits<DT>(dyn, row.first_whole() + i) : 0;
                 if (b) drop_listed<DT>(v[u], b);
             }
         }
         const float m = max_windows<DT, kU>(v);
-        if (TOP) keys[g * T + tid] = m;
+        if (TOP) keys[groups * T + tid] = m;
         mx = max_nan(mx, m);
-        if (a.prepare(m, p.s2, gap)) {
-#pragma unroll
-            for (int u = 0; u < kU; u++) add_window<DT, ENT>(a, v[u], p.s2);
+        if (a.prepare(m, p.s2, gap)) add_windows<DT, ENT, kU>(a, v, p.s2);
+    }
+    if (edges) {
+        float top = neg_inf();
+        for (int u = 0; u < 2; u++) {
+            const uint32_t w = u ? row.back() : row.front();
+            if (w != kNoWindow) top = max_nan(top, add_edge<DT, ENT, KD>(a, row, w, dyn, p.s2, gap));
         }
+        mx = max_nan(mx, top);
+        if (TOP) keys[groups * T] = top;
     }
 
     // ---- the parts of the warps (and CTAs) meet in CTA 0 ----
@@ -361,69 +462,14 @@ __global__ void __launch_bounds__(kThreads, 4) row_stats_kernel(const StatParams
             b.s += c.s; b.e += c.e;
             bm = m2;
         }
-        if (KD == 2) {
-            for (uint32_t i = lane; i < p.k; i += 32) {
-                if (l_id[i] < 0) continue;
-                bm = max_nan(bm, l_x[i]);
-            }
-        }
+        if (KD == 2)
+            for (uint32_t i = lane; i < p.k; i += 32) bm = max_nan(bm, l_x[i]);
         warp_sums<ENT>(b, bm, p.s2);
-        const float m = bm;
-        float s = b.s, rest = s;
-        if (KD == 2) {
-            float listed = 0.f;
-            for (uint32_t i = lane; i < p.k; i += 32) {
-                if (l_id[i] < 0 || !(l_x[i] > neg_inf() || l_x[i] != l_x[i])) continue;
-                bool again = false;
-                if (l_twice)
-                    for (uint32_t j = 0; j < i; j++) again |= l_id[j] == l_id[i];
-                if (!again) listed += ex2(p.s2 * (l_x[i] - m));
-            }
-            s = rest + warp_sum(listed);
-        }
-        const bool empty = m == neg_inf();
-        const float l = empty ? neg_inf() : logf(s);
-        if (KD == 0) {
-            if (TOP && lane == 0) { top_s->m = m; top_s->l = l; }
-            if (lane == 0) {
-                p.stats[2 * (size_t)r] = m;
-                p.stats[2 * (size_t)r + 1] = l;
-                if (p.logp) p.logp[r] = target < 0 ? 0.f : empty ? neg_inf() : p.scale * (x_target - m) - l;
-                if (ENT) p.entropy[r] = empty ? 0.f : l - kLn2 * (b.e / s);
-            }
-        } else {
-            // the teacher's probabilities
-            float mq = neg_inf(), zq = 0.f;
-            if (KD == 1) {
-                for (uint32_t i = lane; i < p.k; i += 32) mq = max_nan(mq, l_q[i]);
-                mq = warp_max_nan(mq);
-            } else {
-                mq = 0.f;
-            }
-            if (mq != neg_inf())
-                for (uint32_t i = lane; i < p.k; i += 32) zq += expf(l_q[i] - mq);
-            zq = warp_sum(zq);
-            const float lz = KD == 1 ? mq + logf(zq) : 0.f;
-            float loss = 0.f;
-            if (mq != neg_inf()) {
-                for (uint32_t i = lane; i < p.k; i += 32) {
-                    const float lq = l_q[i] - lz, q = expf(lq);
-                    const float lp = l_x[i] == neg_inf() ? neg_inf() : p.scale * (l_x[i] - m) - l;
-                    if (!(q <= 0.f)) loss += q * (lq - lp);
-                }
-            }
-            loss = warp_sum(loss);
-            if (lane == 0) {
-                float *st = p.stats + (KD == 2 ? 3 : 2) * (size_t)r;
-                st[0] = m;
-                st[1] = l;
-                if (KD == 2) {
-                    const float left = fmaxf(0.f, 1.f - zq), lr = rest > 0.f || rest != rest ? logf(rest) : neg_inf();
-                    if (left > 0.f && !(lr == neg_inf())) loss += left * (logf(left) - (lr - l));
-                    st[2] = lr;
-                }
-                p.loss[r] = loss;
-            }
+        if (KD) {
+            finish_lists<KD>(p, r, l_id, l_q, l_x, l_twice, bm, b.s);
+        } else if (lane == 0) {
+            finish_tokens<ENT>(p, r, target, x_target, bm, b.s, b.e);
+            if (TOP) { top_s->m = bm; top_s->l = bm == neg_inf() ? neg_inf() : logf(b.s); }
         }
     }
     if (!TOP) return;
@@ -437,33 +483,37 @@ __global__ void __launch_bounds__(kThreads, 4) row_stats_kernel(const StatParams
     }
     __syncthreads();
     const uint32_t tau = top_s->tau;
-    for (uint32_t w0 = first, g = 0; w0 - tid < windows; w0 += step, g++) {
-        const float m = keys[g * T + tid];
-        if (m > neg_inf() && ordered(m) >= tau) {
-            const uint32_t at = atomicAdd(&top_s->n_hits, 1u);
-            if (at < kCap) top_s->hits[at] = w0;
-        }
-    }
-    __syncthreads();
-    TopShared *first_cta = C > 1 ? cg::this_cluster().map_shared_rank(top_s, 0) : top_s;
-    const uint32_t n_hits = top_s->n_hits;
-    if (n_hits > kCap) {
-        if (tid == 0) atomicAdd(&first_cta->cnt, kCap + 1);
-    } else {
-        for (uint32_t i = tid; i < n_hits * kU; i += T) {
-            const uint32_t w = top_s->hits[i / kU] + (i % kU) * T;
-            if (w >= windows) continue;
-            float e[Win<DT>::kElems];
-            unpack<DT>(load_window(row, w), e);
-#pragma unroll
-            for (uint32_t j = 0; j < Win<DT>::kElems; j++) {
-                if (e[j] > neg_inf() && ordered(e[j]) >= tau) {
-                    const uint32_t at = atomicAdd(&first_cta->cnt, 1u);
-                    if (at < kCap) first_cta->cand[at] = rank_key(e[j], w * Win<DT>::kElems + j - row.head);
+            for (uint32_t g = 0; g <= groups; g++) {
+                if (g == groups && !edges) break;
+                const float m = keys[g * T + tid];
+                if (m > neg_inf() && ordered(m) >= tau) {
+                    const uint32_t at = atomicAdd(&top_s->n_hits, 1u);
+                    if (at < kCap) top_s->hits[at] = g * T + tid;
                 }
             }
-        }
-    }
+            __syncthreads();
+            TopShared *first_cta = C > 1 ? cg::this_cluster().map_shared_rank(top_s, 0) : top_s;
+            const uint32_t n_hits = top_s->n_hits;
+            if (n_hits > kCap) {
+                if (tid == 0) atomicAdd(&first_cta->cnt, kCap + 1);
+            } else {
+                for (uint32_t i = tid; i < n_hits * kU; i += T) {
+                    const uint32_t h = top_s->hits[i / kU], u = i % kU, index = h / T * step + first + u * T + h % T;
+                    uint32_t w = row.first_whole() + index;
+                    if (h >= groups * T) w = u == 0 ? row.front() : u == 1 ? row.back() : kNoWindow;
+                    else if (index >= n_whole) w = kNoWindow;
+                    if (w == kNoWindow) continue;
+                    float e[Win<DT>::kElems];
+                    unpack<DT>(load_window(row, w), e);
+#pragma unroll
+                    for (uint32_t j = 0; j < Win<DT>::kElems; j++) {
+                        if (e[j] > neg_inf() && ordered(e[j]) >= tau) {
+                            const uint32_t at = atomicAdd(&first_cta->cnt, 1u);
+                            if (at < kCap) first_cta->cand[at] = rank_key(e[j], w * Win<DT>::kElems + j - row.head);
+                        }
+                    }
+                }
+            }
     if (C > 1) {
         cg::this_cluster().sync();
         if (rank) return;
@@ -706,7 +756,7 @@ template <int DT, bool ENT, bool TOP, int KD> static int launch_stats(cudaStream
     if (!p.count_here && set_zero(who, p.missed, s)) return 1;
     for (;; C = 1) {
         const uint32_t groups = (windows + C * kU * T - 1) / (C * kU * T);
-        const size_t smem = TOP ? (size_t)groups * T * sizeof(float) : KD == 2 ? ((size_t)windows * Win<DT>::kElems + 31) / 32 * 4 : 0;
+        const size_t smem = TOP ? ((size_t)groups * T + 1) * sizeof(float) : KD == 2 ? ((size_t)windows * Win<DT>::kElems + 31) / 32 * 4 : 0;
         SFB_REQUIRE(smem <= 200 * 1024, "%s: vocab=%u is too large", who, p.vocab);
         static DeviceOnce once;
         if (!once.done(dev)) {

@@ -10,6 +10,7 @@
 namespace sfb {
 namespace lg {
 
+constexpr uint32_t kNoWindow = 0xffffffffu;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kFar = -2000.f;       // an exponent (base 2) whose power is 0 and whose product with it is, too: keeps 0 * -inf out of sums
 
@@ -24,6 +25,33 @@ __device__ __forceinline__ float ex2(float x)
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+// two fp32 values as one operand of the packed instructions, which do both at the cost of one
+typedef unsigned long long Pair;
+__device__ __forceinline__ Pair pair(float a, float b)
+{
+    Pair p;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(a), "f"(b));
+    return p;
+}
+__device__ __forceinline__ void halves(Pair p, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p)); }
+__device__ __forceinline__ Pair add2(Pair a, Pair b)
+{
+    Pair p;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(p) : "l"(a), "l"(b));
+    return p;
+}
+__device__ __forceinline__ Pair mul2(Pair a, Pair b)
+{
+    Pair p;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(p) : "l"(a), "l"(b));
+    return p;
+}
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c)
+{
+    Pair p;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(p) : "l"(a), "l"(b), "l"(c));
+    return p;
 }
 // the larger one, NaN if either is NaN
 __device__ __forceinline__ float max_nan(float a, float b)
@@ -46,6 +74,19 @@ template <int DT> struct Row {
         end = head + n;
     }
     __device__ __forceinline__ uint32_t windows() const { return (end + Win<DT>::kElems - 1) / Win<DT>::kElems; }
+    // windows [first_whole, first_whole + whole_count) are inside the row; besides them there are at most two
+    __device__ __forceinline__ uint32_t first_whole() const { return head ? 1 : 0; }
+    __device__ __forceinline__ uint32_t whole_count() const
+    {
+        const uint32_t b = first_whole(), e = end / Win<DT>::kElems;
+        return e > b ? e - b : 0;
+    }
+    __device__ __forceinline__ uint32_t front() const { return head ? 0u : kNoWindow; }
+    __device__ __forceinline__ uint32_t back() const
+    {
+        const uint32_t w = end / Win<DT>::kElems;
+        return end % Win<DT>::kElems && !(w == 0 && head) ? w : kNoWindow;
+    }
     __device__ __forceinline__ bool whole(uint32_t w) const { return w * Win<DT>::kElems >= head && (w + 1) * Win<DT>::kElems <= end; }
 };
 
@@ -72,11 +113,15 @@ __device__ __forceinline__ uint4 load16(const uint4 *p)
     asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
     return v;
 }
+template <int DT> __device__ __forceinline__ uint4 no_elements()
+{
+    const uint32_t none = DT == SFB_F32 ? Win<DT>::kInf : Win<DT>::kInf << 16 | Win<DT>::kInf;
+    return make_uint4(none, none, none, none);
+}
 template <int DT> __device__ __forceinline__ uint4 load_window(const Row<DT> &r, uint32_t w)
 {
     if (r.whole(w)) return load16(r.base + w);
-    const uint32_t none = DT == SFB_F32 ? Win<DT>::kInf : Win<DT>::kInf << 16 | Win<DT>::kInf;
-    if (w * Win<DT>::kElems >= r.end) return make_uint4(none, none, none, none);
+    if (w * Win<DT>::kElems >= r.end) return no_elements<DT>();
     return edge_window<DT>(r.base, r.head, r.end, w);
 }
 
