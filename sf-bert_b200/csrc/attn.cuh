@@ -59,8 +59,6 @@ int embedding_lookup(cudaStream_t s, void *out, const void *table, const int32_t
 uint64_t tc_linear_logprobs_workspace(uint32_t m, uint32_t n);
 int tc_linear_logprobs(cudaStream_t s, const void *x, const void *table, const float *bias, const int32_t *targets, uint32_t m, uint32_t n,
                        uint32_t k, int dtype, float scale, float *logp, float *stats, float *entropy, uint32_t *missed, void *workspace);
-int status_logits(uint32_t *out);
-int status_clear_logits();
 int tc_status_gemm(uint32_t *out);
 int tc_status_clear_gemm();
 

@@ -232,14 +232,23 @@ template <int DT> __device__ __forceinline__ uint32_t listed_bits(const uint8_t 
 {
     return DT == SFB_F32 ? bits[w >> 1] >> ((w & 1) * 4) & 15u : bits[w];
 }
-// a window that is not in the row as a whole; returns its largest element
-template <int DT, bool ENT, int KD> __device__ __forceinline__ float add_edge(Sums &a, const Row<DT> &row, uint32_t w, const uint8_t *bits, float s2, float gap)
+// The elements of a row that are not in a whole window, one per thread of its first 2 * kElems: the window at its front, then
+// the one at its back.  Their position, kNoWindow for threads (and windows) without one.
+template <int DT> __device__ __forceinline__ uint32_t edge_position(const Row<DT> &row, uint32_t i)
 {
-    uint4 v[1] = {edge_window<DT>(row.base, row.head, row.end, w)};
-    if (KD == 2 && listed_bits<DT>(bits, w)) drop_listed<DT>(v[0], listed_bits<DT>(bits, w));
-    const float m = max_windows<DT, 1>(v);
-    if (a.prepare(m, s2, gap)) add_windows<DT, ENT, 1>(a, v, s2);
-    return m;
+    constexpr uint32_t E = Win<DT>::kElems;
+    if (i >= 2 * E) return kNoWindow;
+    const uint32_t w = i < E ? row.front() : row.back();
+    if (w == kNoWindow) return kNoWindow;
+    const uint32_t pos = w * E + i % E;
+    return pos >= row.head && pos < row.end ? pos : kNoWindow;
+}
+template <bool ENT> __device__ __forceinline__ void add_element(Sums &a, float x, float s2, float gap)
+{
+    if (!a.prepare(x, s2, gap)) return;
+    const float t = s2 * (x - a.r), y = ex2(t);
+    a.s += y;
+    if (ENT) a.e = fmaf(y, fmaxf(t, kFar), a.e);
 }
 
 // a row of tokens, its sums known beside m
@@ -354,7 +363,6 @@ __global__ void __launch_bounds__(kThreads, 4) row_stats_kernel(const StatParams
     const float gap = 40.f / p.s2;
     const uint32_t n_whole = row.whole_count(), step = C * kU * T, first = rank * kU * T;
     const uint4 *src = row.base + row.first_whole() + tid;
-    const bool edges = rank == 0 && tid == 0 && row.windows() != n_whole;       // what is not a whole window: thread 0's
     float *keys = (float *)dyn;
     auto load = [&](uint4 (&v)[kU], uint32_t i0) {
         if (i0 + kU * T <= n_whole) {
@@ -367,10 +375,14 @@ __global__ void __launch_bounds__(kThreads, 4) row_stats_kernel(const StatParams
     };
     uint4 v[kU], next[kU];
     if (first < n_whole) load(next, first);
+    const uint32_t edge = rank == 0 ? edge_position<DT>(row, tid) : kNoWindow;       // what is not in a whole window: an element each
+    float x_edge = edge != kNoWindow ? load_element<DT>(x, edge - row.head) : neg_inf();
     float x_target = 0.f;
     if (KD == 0 && target >= 0 && rank == 0 && tid < 64) x_target = load_element<DT>(x, (uint32_t)target);
 
     if (TOP && tid == 0) { top_s->cnt = 0; top_s->n_hits = 0; }
+    int32_t id = -1;                         // this thread's entry of the list
+    float x_listed = neg_inf();
     if (KD) {
         uint32_t *bits = (uint32_t *)dyn;
         if (KD == 2) {
@@ -378,24 +390,24 @@ __global__ void __launch_bounds__(kThreads, 4) row_stats_kernel(const StatParams
             if (tid == 0) l_twice = 0;
             __syncthreads();
         }
-        uint32_t bad = 0;
-        for (uint32_t i = tid; i < p.k; i += T) {
-            const int32_t id = p.ids[(size_t)r * p.k + i];
-            const bool ok = (uint32_t)id < p.vocab;
-            bad += !ok;
-            l_id[i] = ok ? id : -1;
-            l_q[i] = ok ? p.teacher[(size_t)r * p.k + i] : neg_inf();
-            l_x[i] = ok ? load_element<DT>(x, (uint32_t)id) : neg_inf();
-            if (KD == 2 && ok) {
+        bool missed = false;
+        if (tid < p.k) {
+            id = p.ids[(size_t)r * p.k + tid];
+            missed = (uint32_t)id >= p.vocab;
+            if (missed) id = -1;
+            l_id[tid] = id;
+            l_q[tid] = missed ? neg_inf() : p.teacher[(size_t)r * p.k + tid];
+            if (!missed) x_listed = load_element<DT>(x, (uint32_t)id);
+            if (KD == 2 && !missed) {
                 const uint32_t pos = row.head + (uint32_t)id, bit = 1u << (pos & 31);
                 if (atomicOr(&bits[pos >> 5], bit) & bit) l_twice = 1;
             }
         }
         if (p.missed && !p.count_here && rank == 0) {
-            bad = __reduce_add_sync(0xffffffffu, bad);
+            const uint32_t bad = __popc(__ballot_sync(0xffffffffu, missed));
             if (lane == 0 && bad) atomicAdd(p.missed, bad);
         }
-        __syncthreads();
+        if (KD == 2) __syncthreads();
     }
 
     // ---- the pass ----
@@ -417,18 +429,15 @@ __global__ void __launch_bounds__(kThreads, 4) row_stats_kernel(const StatParams
         mx = max_nan(mx, m);
         if (a.prepare(m, p.s2, gap)) add_windows<DT, ENT, kU>(a, v, p.s2);
     }
-    if (edges) {
-        float top = neg_inf();
-        for (int u = 0; u < 2; u++) {
-            const uint32_t w = u ? row.back() : row.front();
-            if (w != kNoWindow) top = max_nan(top, add_edge<DT, ENT, KD>(a, row, w, dyn, p.s2, gap));
-        }
-        mx = max_nan(mx, top);
-        if (TOP) keys[groups * T] = top;
+    if (edge != kNoWindow) {
+        if (KD == 2 && ((const uint32_t *)dyn)[edge >> 5] >> (edge & 31) & 1) x_edge = neg_inf();
+        mx = max_nan(mx, x_edge);
+        add_element<ENT>(a, x_edge, p.s2, gap);
     }
 
     // ---- the parts of the warps (and CTAs) meet in CTA 0 ----
     const float own_mx = mx;
+    if (KD && tid < p.k) l_x[tid] = x_listed;
     warp_sums<ENT>(a, mx, p.s2);
     if (C > 1) {
         asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
@@ -483,37 +492,35 @@ __global__ void __launch_bounds__(kThreads, 4) row_stats_kernel(const StatParams
     }
     __syncthreads();
     const uint32_t tau = top_s->tau;
-            for (uint32_t g = 0; g <= groups; g++) {
-                if (g == groups && !edges) break;
-                const float m = keys[g * T + tid];
-                if (m > neg_inf() && ordered(m) >= tau) {
-                    const uint32_t at = atomicAdd(&top_s->n_hits, 1u);
-                    if (at < kCap) top_s->hits[at] = g * T + tid;
-                }
-            }
-            __syncthreads();
-            TopShared *first_cta = C > 1 ? cg::this_cluster().map_shared_rank(top_s, 0) : top_s;
-            const uint32_t n_hits = top_s->n_hits;
-            if (n_hits > kCap) {
-                if (tid == 0) atomicAdd(&first_cta->cnt, kCap + 1);
-            } else {
-                for (uint32_t i = tid; i < n_hits * kU; i += T) {
-                    const uint32_t h = top_s->hits[i / kU], u = i % kU, index = h / T * step + first + u * T + h % T;
-                    uint32_t w = row.first_whole() + index;
-                    if (h >= groups * T) w = u == 0 ? row.front() : u == 1 ? row.back() : kNoWindow;
-                    else if (index >= n_whole) w = kNoWindow;
-                    if (w == kNoWindow) continue;
-                    float e[Win<DT>::kElems];
-                    unpack<DT>(load_window(row, w), e);
+    TopShared *first_cta = C > 1 ? cg::this_cluster().map_shared_rank(top_s, 0) : top_s;
+    auto candidate = [&](float v, uint32_t index) {
+        if (v > neg_inf() && ordered(v) >= tau) {
+            const uint32_t at = atomicAdd(&first_cta->cnt, 1u);
+            if (at < kCap) first_cta->cand[at] = rank_key(v, index);
+        }
+    };
+    if (edge != kNoWindow) candidate(x_edge, edge - row.head);
+    for (uint32_t g = 0; g < groups; g++) {
+        const float m = keys[g * T + tid];
+        if (m > neg_inf() && ordered(m) >= tau) {
+            const uint32_t at = atomicAdd(&top_s->n_hits, 1u);
+            if (at < kCap) top_s->hits[at] = g * T + tid;
+        }
+    }
+    __syncthreads();
+    const uint32_t n_hits = top_s->n_hits;
+    if (n_hits > kCap) {
+        if (tid == 0) atomicAdd(&first_cta->cnt, kCap + 1);
+    } else {
+        for (uint32_t i = tid; i < n_hits * kU; i += T) {
+            const uint32_t h = top_s->hits[i / kU], at = h / T * step + first + i % kU * T + h % T, w = row.first_whole() + at;
+            if (at >= n_whole) continue;
+            float e[Win<DT>::kElems];
+            unpack<DT>(load16(row.base + w), e);
 #pragma unroll
-                    for (uint32_t j = 0; j < Win<DT>::kElems; j++) {
-                        if (e[j] > neg_inf() && ordered(e[j]) >= tau) {
-                            const uint32_t at = atomicAdd(&first_cta->cnt, 1u);
-                            if (at < kCap) first_cta->cand[at] = rank_key(e[j], w * Win<DT>::kElems + j - row.head);
-                        }
-                    }
-                }
-            }
+            for (uint32_t j = 0; j < Win<DT>::kElems; j++) candidate(e[j], w * Win<DT>::kElems + j - row.head);
+        }
+    }
     if (C > 1) {
         cg::this_cluster().sync();
         if (rank) return;
@@ -741,14 +748,14 @@ __global__ void __launch_bounds__(kThreads) row_grad_kernel(const GradParams p)
 }
 
 // ---- launches -----------------------------------------------------------------------------------------------------------
-static uint32_t stat_threads(uint32_t windows, bool top) { return windows > 512 ? 256 : windows > 256 || top ? 128 : 64; }
-
 template <int DT, bool ENT, bool TOP, int KD> static int launch_stats(cudaStream_t s, StatParams &p, const char *who)
 {
     const int dev = current_device(), sms = device_sm_count(dev);
     SFB_REQUIRE(sms > 0, "%s: cannot query the device", who);
     const uint32_t windows = p.vocab / Win<DT>::kElems + 2;      // at most, wherever a row starts
-    const uint32_t T = stat_threads(windows, TOP);
+    // What a row's end costs is paid by each of its warps, so many rows have four of them each (4096 rows of 30522 bf16: 47 us,
+    // with eight 50), few rows eight (257 of 50021 fp32: 19 us, with four 25).
+    const uint32_t T = windows > 512 && (p.rows < (uint32_t)sms * 8 || (TOP && p.k > 32)) ? 256 : windows > 256 || TOP || KD ? 128 : 64;
     uint32_t C = 1;
     while (C < kMaxCluster && (uint64_t)p.rows * C * 2 <= (uint64_t)sms * 2 && windows > C * T * 2) C *= 2;
     const uint64_t entries = p.missed ? KD ? (uint64_t)p.rows * p.k : p.targets ? p.rows : 0 : 0;
@@ -756,7 +763,7 @@ template <int DT, bool ENT, bool TOP, int KD> static int launch_stats(cudaStream
     if (!p.count_here && set_zero(who, p.missed, s)) return 1;
     for (;; C = 1) {
         const uint32_t groups = (windows + C * kU * T - 1) / (C * kU * T);
-        const size_t smem = TOP ? ((size_t)groups * T + 1) * sizeof(float) : KD == 2 ? ((size_t)windows * Win<DT>::kElems + 31) / 32 * 4 : 0;
+        const size_t smem = TOP ? (size_t)groups * T * sizeof(float) : KD == 2 ? ((size_t)windows * Win<DT>::kElems + 31) / 32 * 4 : 0;
         SFB_REQUIRE(smem <= 200 * 1024, "%s: vocab=%u is too large", who, p.vocab);
         static DeviceOnce once;
         if (!once.done(dev)) {

@@ -249,7 +249,7 @@ extern "C" int sfb_attention_backward(sfb_stream_t stream, const void *nn_lut, c
 
 extern "C" int sfb_device_status_clear(void)
 {
-    if (tc_status_clear_backward() || tc_status_clear_fused() || tc_status_clear_unfused() || tc_status_clear_gemm() || status_clear_logits()) return 1;
+    if (tc_status_clear_backward() || tc_status_clear_fused() || tc_status_clear_unfused() || tc_status_clear_gemm()) return 1;
     clear_error();
     return 0;
 }
@@ -257,9 +257,9 @@ extern "C" int sfb_device_status_clear(void)
 extern "C" int sfb_device_status(uint32_t *status)
 {
     SFB_REQUIRE(status, "sfb_device_status: NULL pointer");
-    uint32_t a = 0, b = 0, c = 0, d = 0, e = 0;
-    if (tc_status_fused(&a) || tc_status_unfused(&b) || tc_status_gemm(&c) || tc_status_backward(&d) || status_logits(&e)) return 1;
-    *status = a ? a : b ? b : c ? c : d ? d : e;
+    uint32_t a = 0, b = 0, c = 0, d = 0;
+    if (tc_status_fused(&a) || tc_status_unfused(&b) || tc_status_gemm(&c) || tc_status_backward(&d)) return 1;
+    *status = a ? a : b ? b : c ? c : d;
     clear_error();
     return 0;
 }
