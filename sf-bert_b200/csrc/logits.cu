@@ -71,9 +71,9 @@ __device__ __forceinline__ unsigned long long rank_key(float v, uint32_t index) 
 
 __device__ __forceinline__ float warp_max_nan(float v)
 {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v = max_nan(v, __shfl_xor_sync(0xffffffffu, v, o));
-    return v;
+    float y;
+    asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(v));
+    return y;
 }
 
 // the sums of a warp's threads, beside the largest of their maxima
@@ -151,28 +151,12 @@ __device__ __forceinline__ void count_missed(const int32_t *ids, uint32_t n, uin
     }
 }
 
-// The largest t such that at least k of the n (at most 256) values have the upper 16 bits of their ordered form at or
-// above it, as an ordered value.  One warp.
-__device__ __forceinline__ uint32_t kth_largest(const float *values, uint32_t n, uint32_t k)
-{
-    const uint32_t lane = threadIdx.x & 31;
-    uint32_t o[8];
-#pragma unroll
-    for (int j = 0; j < 8; j++) o[j] = lane + 32 * j < n ? ordered(values[lane + 32 * j]) >> 16 : 0u;
-    uint32_t t = 0;
-    for (uint32_t bit = 0x8000u; bit; bit >>= 1) {
-        uint32_t c = 0;
-#pragma unroll
-        for (int j = 0; j < 8; j++) c += o[j] >= (t | bit);
-        if (__reduce_add_sync(0xffffffffu, c) >= k) t |= bit;
-    }
-    return t << 16;
-}
-
 struct TopShared {
-    float gm[kThreads];                   // largest values of the groups of threads
-    unsigned long long cand[kCap];
+    uint32_t gm[kThreads];                // largest values of the groups of threads: 24 bits in their order, then 255 - group
+    unsigned long long cand[kCap];        // candidates, kCap / C places for each CTA (in CTA 0)
+    uint32_t n_cand[kMaxCluster];
     uint32_t hits[kCap];
+    float best[kMaxList];
     uint32_t cnt, n_hits, tau, part[8];
     float m, l;
 };
@@ -190,10 +174,11 @@ __device__ __forceinline__ uint32_t block_sum(uint32_t v, uint32_t *part)
 }
 
 // The candidates when too many values reach the bound (values tie, or most of the large ones went to a few threads): the bound is
-// bisected over the values and their indices, a pass over the row (by now in L2) for each step.  One CTA, the whole row.
+// bisected over the values and their indices, a pass over the row (by now in L2) for each step.  One CTA, the whole row; the
+// candidates are then sh->cnt from the first place on.
 template <int DT> __device__ __noinline__ void bisect_candidates(const Row<DT> row, uint32_t k, TopShared *sh)
 {
-    unsigned long long lo = (unsigned long long)sh->tau << 32, hi = ~0ull, x = lo;      // more than kCap reach lo, fewer than k hi
+    unsigned long long lo = (unsigned long long)sh->tau << 32, hi = ~0ull, x = lo;      // at least k reach lo (or all there are), fewer than k hi
     const uint32_t windows = row.windows();
     for (;;) {
         const unsigned long long mid = lo + (hi - lo) / 2;
@@ -262,54 +247,55 @@ template <bool ENT> __device__ __forceinline__ void finish_tokens(const StatPara
     if (ENT) p.entropy[r] = empty ? 0.f : l - kLn2 * (e / s);
 }
 
-// What one warp makes of a row of lists, its sums known: m and s beside it, rest = s without the listed tokens.
-template <int KD> __device__ __forceinline__ void finish_lists(const StatParams &p, uint32_t r, const int32_t *l_id, const float *l_q, const float *l_x,
-                                                               bool twice, float m, float rest)
+// What a warp's entries of a row's list come to before the row's sums are known.  With q_k = e^(lq_k - mq) / Z and x_r the
+// largest listed logit, loss = sum_k q_k (ln q_k - s (x_k - m) + l) is linear in s (x_r - m) and l.
+struct ListPart {
+    float mq, z, u, v, x_r, listed;       // max lq, sum e = e^(lq - mq), sum e lq, sum e (x - x_r), max x, sum over distinct of 2^(s2 (x - x_r))
+};
+
+// One warp: its entries, one per lane.  again: the lane's token stands earlier in the list.
+template <int KD> __device__ __forceinline__ void sum_entries(float lq, float x, bool again, float s2, ListPart *out)
 {
-    const uint32_t lane = threadIdx.x & 31;
-    float s = rest;
-    if (KD == 2) {
-        float listed = 0.f;
-        for (uint32_t i = lane; i < p.k; i += 32) {
-            if (l_id[i] < 0 || l_x[i] == neg_inf()) continue;
-            bool again = false;
-            if (twice)
-                for (uint32_t j = 0; j < i; j++) again |= l_id[j] == l_id[i];
-            if (!again) listed += ex2(p.s2 * (l_x[i] - m));
-        }
-        s = rest + warp_sum(listed);
+    const float mq = KD == 1 ? warp_max_nan(lq) : 0.f, x_r = warp_max_nan(x), base = x_r == neg_inf() ? 0.f : x_r;
+    const float e = lq == neg_inf() ? 0.f : ex2(kLog2e * (lq - mq));
+    const float z = warp_sum(e), u = warp_sum(e > 0.f || e != e ? e * lq : 0.f), v = warp_sum(e > 0.f ? e * (x - base) : 0.f);
+    const float listed = KD == 2 ? warp_sum(again ? 0.f : ex2(s2 * (x - base))) : 0.f;
+    if ((threadIdx.x & 31) == 0) *out = {mq, z, u, v, x_r, x_r == neg_inf() ? 0.f : listed};
+}
+
+// One thread: the row's results, m and s (KD 2: without the listed tokens) known.
+template <int KD> __device__ __forceinline__ void finish_lists(const StatParams &p, uint32_t r, const ListPart *part, float m, float s)
+{
+    const uint32_t n = (p.k + 31) / 32;
+    float mq = KD == 1 ? neg_inf() : 0.f, z = 0.f, u = 0.f, v = 0.f, listed = 0.f;
+    const bool empty = m == neg_inf();
+    if (KD == 1)
+        for (uint32_t w = 0; w < n; w++) mq = max_nan(mq, part[w].mq);
+    for (uint32_t w = 0; w < n; w++) {
+        const ListPart g = part[w];
+        const float f = KD == 2 ? 1.f : g.mq == neg_inf() ? 0.f : ex2(kLog2e * (g.mq - mq)), base = g.x_r == neg_inf() ? 0.f : g.x_r;
+        z += f * g.z;
+        u += f * g.u;
+        if (f * g.z > 0.f) v += f * (g.v + g.z * (base - m));        // sum of e (x - m)
+        if (KD == 2 && g.x_r != neg_inf()) listed += g.listed * ex2(p.s2 * (base - m));
     }
-    const float l = m == neg_inf() ? neg_inf() : logf(s);
-    // the teacher's probabilities
-    float mq = KD == 1 ? neg_inf() : 0.f, zq = 0.f;
-    if (KD == 1) {
-        for (uint32_t i = lane; i < p.k; i += 32) mq = max_nan(mq, l_q[i]);
-        mq = warp_max_nan(mq);
-    }
-    if (mq != neg_inf())
-        for (uint32_t i = lane; i < p.k; i += 32) zq += expf(l_q[i] - mq);
-    zq = warp_sum(zq);
-    const float lz = KD == 1 ? mq + logf(zq) : 0.f;
+    const float rest = s;
+    if (KD == 2) s += listed;
+    const float l = empty ? neg_inf() : logf(s);
     float loss = 0.f;
-    if (mq != neg_inf()) {
-        for (uint32_t i = lane; i < p.k; i += 32) {
-            const float lq = l_q[i] - lz, q = expf(lq);
-            const float lp = l_x[i] == neg_inf() ? neg_inf() : p.scale * (l_x[i] - m) - l;
-            if (!(q <= 0.f)) loss += q * (lq - lp);
-        }
+    if (!(z <= 0.f)) {
+        if (KD == 1) loss = empty ? -neg_inf() : (u - p.scale * v) / z - (mq + logf(z)) + l;
+        else loss = empty ? -neg_inf() : u - p.scale * v + z * l;
     }
-    loss = warp_sum(loss);
-    if (lane == 0) {
-        float *st = p.stats + (KD == 2 ? 3 : 2) * (size_t)r;
-        st[0] = m;
-        st[1] = l;
-        if (KD == 2) {
-            const float left = fmaxf(0.f, 1.f - zq), lr = rest == 0.f ? neg_inf() : logf(rest);
-            if (left > 0.f && !(lr == neg_inf())) loss += left * (logf(left) - (lr - l));
-            st[2] = lr;
-        }
-        p.loss[r] = loss;
+    float *st = p.stats + (KD == 2 ? 3 : 2) * (size_t)r;
+    st[0] = m;
+    st[1] = l;
+    if (KD == 2) {
+        const float lr = rest == 0.f ? neg_inf() : logf(rest), left = fmaxf(0.f, 1.f - z);
+        if (left > 0.f && !(lr == neg_inf())) loss += left * (logf(left) - (lr - l));
+        st[2] = lr;
     }
+    p.loss[r] = loss;
 }
 
 // A row's statistics, and what is made of them.  One CTA per row, or a cluster of CTAs where there are few rows: each
@@ -321,32 +307,34 @@ __global__ void __launch_bounds__(kThreads, 4) row_stats_kernel(const StatParams
     __shared__ Part parts[kMaxCluster * 8];
     __shared__ __align__(16) uint8_t top_raw[TOP ? sizeof(TopShared) : 16];
     TopShared *const top_s = (TopShared *)top_raw;
-    __shared__ int32_t l_id[KD ? kMaxList : 1];
-    __shared__ float l_q[KD ? kMaxList : 1], l_x[KD ? kMaxList : 1];
+    __shared__ int32_t l_id[KD == 2 ? kMaxList : 1];
+    __shared__ ListPart list[kMaxList / 32];
     __shared__ uint32_t l_twice;
+    constexpr bool kMaySkip = KD == 0 && !ENT && !TOP;   // a row without a target has nothing to give
 
     const uint32_t T = blockDim.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t C = cluster_size(), rank = cluster_rank();
     const uint32_t r = blockIdx.x / C;
     if (C > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");    // waited for before the first word into another CTA
+    if (TOP && tid == 0) { top_s->cnt = 0; top_s->n_hits = 0; }
+    if (KD == 2)
+        for (uint32_t i = tid; i < (p.vocab + 2 * Win<DT>::kElems + 31) / 32; i += T) ((uint32_t *)dyn)[i] = 0;
     grid_dependency_wait();
     grid_launch_dependents();
 
-    bool skip = false;
+    bool skip = r >= p.rows;
     int32_t target = -1;
-    if (r >= p.rows) {
+    if (skip) {
         if (rank == 0) count_missed(KD ? p.ids : p.targets, p.count_here, p.vocab, p.missed, (uint32_t *)parts);
-        skip = true;
-    } else if (KD == 0 && p.targets) {
+    } else if (kMaySkip && p.targets) {
         target = p.targets[r];
-        const bool inside = (uint32_t)target < p.vocab;
-        if (!inside && rank == 0 && tid == 0 && p.missed && !p.count_here) atomicAdd(p.missed, 1u);
-        if (!inside) {
-            target = -1;
-            if (!ENT && !TOP) {              // nothing of this row is asked for
-                if (rank == 0 && tid == 0) { p.logp[r] = 0.f; p.stats[2 * (size_t)r] = p.stats[2 * (size_t)r + 1] = 0.f; }
-                skip = true;
+        if ((uint32_t)target >= p.vocab) {
+            if (rank == 0 && tid == 0) {
+                if (p.missed && !p.count_here) atomicAdd(p.missed, 1u);
+                p.logp[r] = 0.f;
+                p.stats[2 * (size_t)r] = p.stats[2 * (size_t)r + 1] = 0.f;
             }
+            skip = true;
         }
     }
     if (skip) {
@@ -355,11 +343,9 @@ __global__ void __launch_bounds__(kThreads, 4) row_stats_kernel(const StatParams
         return;
     }
 
+    // The pass goes by groups of kU windows per thread, the next group on its way while one is added up; the first sets out here.
     const void *x = (const char *)p.x + (size_t)r * p.pitch * Win<DT>::kSize;
     const Row<DT> row(x, p.vocab);
-    // The pass goes by groups of kU windows per thread, the next group on its way while one is added up; the first sets out here.
-    Sums a;
-    float mx = neg_inf();
     const float gap = 40.f / p.s2;
     const uint32_t n_whole = row.whole_count(), step = C * kU * T, first = rank * kU * T;
     const uint4 *src = row.base + row.first_whole() + tid;
@@ -377,40 +363,54 @@ __global__ void __launch_bounds__(kThreads, 4) row_stats_kernel(const StatParams
     if (first < n_whole) load(next, first);
     const uint32_t edge = rank == 0 ? edge_position<DT>(row, tid) : kNoWindow;       // what is not in a whole window: an element each
     float x_edge = edge != kNoWindow ? load_element<DT>(x, edge - row.head) : neg_inf();
+    const bool merges = rank == 0 && warp == (TOP ? T / 32 - 1 : 0);      // with alternatives, others look for their bound meanwhile
     float x_target = 0.f;
-    if (KD == 0 && target >= 0 && rank == 0 && tid < 64) x_target = load_element<DT>(x, (uint32_t)target);
-
-    if (TOP && tid == 0) { top_s->cnt = 0; top_s->n_hits = 0; }
-    int32_t id = -1;                         // this thread's entry of the list
-    float x_listed = neg_inf();
-    if (KD) {
-        uint32_t *bits = (uint32_t *)dyn;
-        if (KD == 2) {
-            for (uint32_t i = tid; i < (row.end + 31) / 32; i += T) bits[i] = 0;
-            if (tid == 0) l_twice = 0;
-            __syncthreads();
-        }
-        bool missed = false;
-        if (tid < p.k) {
-            id = p.ids[(size_t)r * p.k + tid];
-            missed = (uint32_t)id >= p.vocab;
-            if (missed) id = -1;
-            l_id[tid] = id;
-            l_q[tid] = missed ? neg_inf() : p.teacher[(size_t)r * p.k + tid];
-            if (!missed) x_listed = load_element<DT>(x, (uint32_t)id);
-            if (KD == 2 && !missed) {
-                const uint32_t pos = row.head + (uint32_t)id, bit = 1u << (pos & 31);
-                if (atomicOr(&bits[pos >> 5], bit) & bit) l_twice = 1;
+    if (KD == 0 && merges && p.targets) {
+        if (!kMaySkip) {
+            target = p.targets[r];
+            if ((uint32_t)target >= p.vocab) {
+                target = -1;
+                if (lane == 0 && p.missed && !p.count_here) atomicAdd(p.missed, 1u);
             }
         }
-        if (p.missed && !p.count_here && rank == 0) {
-            const uint32_t bad = __popc(__ballot_sync(0xffffffffu, missed));
-            if (lane == 0 && bad) atomicAdd(p.missed, bad);
+        if (target >= 0) x_target = load_element<DT>(x, (uint32_t)target);
+    }
+    if (KD) {
+        // an entry of the list per thread
+        int32_t id = -1;
+        float lq = neg_inf(), xl = neg_inf();
+        if (tid < p.k) {
+            id = p.ids[(size_t)r * p.k + tid];
+            lq = p.teacher[(size_t)r * p.k + tid];
         }
-        if (KD == 2) __syncthreads();
+        const bool ok = (uint32_t)id < p.vocab;
+        if (!ok) lq = neg_inf();
+        if (ok && rank == 0) xl = load_element<DT>(x, (uint32_t)id);
+        bool again = false;
+        if (KD == 2) {
+            if (tid == 0) l_twice = 0;
+            if (tid < p.k) l_id[tid] = ok ? id : -1;
+            __syncthreads();                              // the bits are clear
+            if (ok) {
+                const uint32_t pos = row.head + (uint32_t)id, bit = 1u << (pos & 31);
+                if (atomicOr((uint32_t *)dyn + (pos >> 5), bit) & bit) l_twice = 1;
+            }
+            __syncthreads();
+            if (l_twice && ok)                            // a token that is listed twice counts once in the sum of the listed
+                for (uint32_t j = 0; j < tid; j++) again |= l_id[j] == id;
+        }
+        if (rank == 0 && warp < (p.k + 31) / 32) {
+            if (p.missed && !p.count_here) {
+                const uint32_t bad = __popc(__ballot_sync(0xffffffffu, tid < p.k && !ok));
+                if (lane == 0 && bad) atomicAdd(p.missed, bad);
+            }
+            sum_entries<KD>(lq, xl, again, p.s2, &list[warp]);
+        }
     }
 
     // ---- the pass ----
+    Sums a;
+    float mx = neg_inf();
     uint32_t groups = 0;
     for (uint32_t i0 = first; i0 < n_whole; i0 += step, groups++) {
 #pragma unroll
@@ -436,32 +436,34 @@ __global__ void __launch_bounds__(kThreads, 4) row_stats_kernel(const StatParams
     }
 
     // ---- the parts of the warps (and CTAs) meet in CTA 0 ----
-    const float own_mx = mx;
-    if (KD && tid < p.k) l_x[tid] = x_listed;
+    uint32_t n_groups = 0;
+    if (TOP) {
+        // groups of neighbouring threads, as large as leaves 2 k of them (32 at least)
+        uint32_t g = 1;
+        while (g < 32 && T / (2 * g) >= max(32u, 2 * p.k)) g *= 2;
+        n_groups = T / g;
+        float gm = mx;
+        for (uint32_t o = 1; o < g; o <<= 1) gm = max_nan(gm, __shfl_xor_sync(0xffffffffu, gm, o));
+        if ((tid & (g - 1)) == 0) top_s->gm[tid / g] = (ordered(gm) & ~0xffu) | (255 - tid / g);
+    }
     warp_sums<ENT>(a, mx, p.s2);
     if (C > 1) {
         asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
-        const cg::cluster_group cl = cg::this_cluster();
-        if (lane == 0) cl.map_shared_rank(parts, 0)[rank * 8 + warp] = Part{mx, a.s, a.e};
-        if (TOP) {
-            float gmx = own_mx;
-            for (uint32_t o = 1; o < C; o <<= 1) gmx = max_nan(gmx, __shfl_xor_sync(0xffffffffu, gmx, o));
-            cl.map_shared_rank(top_s->gm, tid & (C - 1))[rank * (T / C) + tid / C] = gmx;
+        if (lane == 0) cg::this_cluster().map_shared_rank(parts, 0)[rank * 8 + warp] = Part{mx, a.s, a.e};
+        if (!TOP) {
+            cg::this_cluster().sync();
+            if (rank) return;
         }
-        cl.sync();
-        if (!TOP && rank) return;
-    } else {
-        if (lane == 0) parts[warp] = Part{mx, a.s, a.e};
-        if (TOP) top_s->gm[tid] = own_mx;
-        __syncthreads();
+    } else if (lane == 0) {
+        parts[warp] = Part{mx, a.s, a.e};
     }
+    if (TOP || C == 1) __syncthreads();
 
-    const uint32_t merger = TOP ? 1 : 0;          // with alternatives, warp 0 looks for their bound meanwhile
-    if (rank == 0 && warp == merger) {
-        const uint32_t warps = T / 32, n = C * warps;
+    auto merge = [&]() {
+        const uint32_t warps = T / 32;
         Sums b;
         float bm = neg_inf();
-        for (uint32_t i = lane; i < n; i += 32) {
+        for (uint32_t i = lane; i < C * warps; i += 32) {
             const Part q = parts[i / warps * 8 + i % warps];
             Sums c;
             c.r = q.m; c.s = q.s; c.e = q.e;
@@ -471,32 +473,41 @@ __global__ void __launch_bounds__(kThreads, 4) row_stats_kernel(const StatParams
             b.s += c.s; b.e += c.e;
             bm = m2;
         }
-        if (KD == 2)
-            for (uint32_t i = lane; i < p.k; i += 32) bm = max_nan(bm, l_x[i]);
+        if (KD == 2 && lane < (p.k + 31) / 32) bm = max_nan(bm, list[lane].x_r);
         warp_sums<ENT>(b, bm, p.s2);
-        if (KD) {
-            finish_lists<KD>(p, r, l_id, l_q, l_x, l_twice, bm, b.s);
-        } else if (lane == 0) {
-            finish_tokens<ENT>(p, r, target, x_target, bm, b.s, b.e);
+        if (lane == 0) {
+            if (KD) finish_lists<KD>(p, r, list, bm, b.s);
+            else finish_tokens<ENT>(p, r, target, x_target, bm, b.s, b.e);
             if (TOP) { top_s->m = bm; top_s->l = bm == neg_inf() ? neg_inf() : logf(b.s); }
         }
+    };
+    if (!TOP) {
+        if (merges) merge();
+        return;
     }
-    if (!TOP) return;
 
     // ---- alternatives ----
-    // At least k groups of threads have a value at or above the k-th largest of the groups' maxima, so every one of the k
-    // largest values of the row is: only groups of windows whose maximum reaches that bound are looked at again.
-    if (warp == 0) {
-        const uint32_t t = kth_largest(top_s->gm, T, p.k);
-        if (lane == 0) top_s->tau = t;
+    // At least k groups of threads of a CTA have a value at or above the k-th largest of the groups' maxima, so every one of the k
+    // largest values that the CTA has seen is: only windows whose maximum reaches that bound are looked at again.  CTA 0 ranks
+    // what all of them find.
+    if (tid < n_groups) {
+        const uint32_t own = top_s->gm[tid];
+        uint32_t above = 0;
+#pragma unroll 4
+        for (uint32_t j = 0; j < n_groups; j += 4) {
+            const uint4 o = *(const uint4 *)&top_s->gm[j];
+            above += (o.x > own) + (o.y > own) + (o.z > own) + (o.w > own);
+        }
+        if (above == min(p.k, n_groups) - 1) top_s->tau = n_groups < p.k ? 0 : own & ~0xffu;
     }
+    if (C == 1 && merges) merge();
     __syncthreads();
-    const uint32_t tau = top_s->tau;
-    TopShared *first_cta = C > 1 ? cg::this_cluster().map_shared_rank(top_s, 0) : top_s;
+    const uint32_t tau = top_s->tau, places = kCap / C;
+    unsigned long long *to = (C > 1 ? cg::this_cluster().map_shared_rank(top_s, 0) : top_s)->cand + rank * places;
     auto candidate = [&](float v, uint32_t index) {
         if (v > neg_inf() && ordered(v) >= tau) {
-            const uint32_t at = atomicAdd(&first_cta->cnt, 1u);
-            if (at < kCap) first_cta->cand[at] = rank_key(v, index);
+            const uint32_t at = atomicAdd(&top_s->cnt, 1u);
+            if (at < places) to[at] = rank_key(v, index);
         }
     };
     if (edge != kNoWindow) candidate(x_edge, edge - row.head);
@@ -510,41 +521,69 @@ __global__ void __launch_bounds__(kThreads, 4) row_stats_kernel(const StatParams
     __syncthreads();
     const uint32_t n_hits = top_s->n_hits;
     if (n_hits > kCap) {
-        if (tid == 0) atomicAdd(&first_cta->cnt, kCap + 1);
+        if (tid == 0) atomicAdd(&top_s->cnt, kCap + 1);
     } else {
-        for (uint32_t i = tid; i < n_hits * kU; i += T) {
-            const uint32_t h = top_s->hits[i / kU], at = h / T * step + first + i % kU * T + h % T, w = row.first_whole() + at;
-            if (at >= n_whole) continue;
-            float e[Win<DT>::kElems];
-            unpack<DT>(load16(row.base + w), e);
+        // an element each for the CTA's threads, four on their way at a time
+        constexpr uint32_t E = Win<DT>::kElems;
+        const uint32_t n = n_hits * kU * E;
+        for (uint32_t i0 = tid; i0 < n; i0 += 4 * T) {
+            float e[4];
+            uint32_t index[4];
 #pragma unroll
-            for (uint32_t j = 0; j < Win<DT>::kElems; j++) candidate(e[j], w * Win<DT>::kElems + j - row.head);
+            for (uint32_t j = 0; j < 4; j++) {
+                const uint32_t i = i0 + j * T, h = i < n ? top_s->hits[i / (kU * E)] : 0;
+                const uint32_t at = h / T * step + first + i / E % kU * T + h % T;
+                index[j] = (row.first_whole() + at) * E + i % E - row.head;
+                e[j] = i < n && at < n_whole ? load_element<DT>(x, index[j]) : neg_inf();
+            }
+#pragma unroll
+            for (uint32_t j = 0; j < 4; j++) candidate(e[j], index[j]);
         }
     }
+    __syncthreads();
+    if (tid == 0) (C > 1 ? cg::this_cluster().map_shared_rank(top_s, 0) : top_s)->n_cand[rank] = top_s->cnt;
     if (C > 1) {
         cg::this_cluster().sync();
         if (rank) return;
+        if (merges) merge();
     } else {
         __syncthreads();
     }
-    const float m = top_s->m, l = top_s->l;
-    const bool sound = l == l;                  // no NaN in the row
-    if (sound && top_s->cnt > kCap) bisect_candidates<DT>(row, p.k, top_s);
-    const uint32_t cnt = sound ? top_s->cnt : 0u;
-    float *out_logp = p.top_logp + (size_t)r * p.k;
+    bool few = true;
+    uint32_t total = 0, lists = C;
+    for (uint32_t c = 0; c < C; c++) {
+        few &= top_s->n_cand[c] <= places;
+        total += top_s->n_cand[c];
+    }
+    if (!few) {
+        bisect_candidates<DT>(row, p.k, top_s);
+        if (tid == 0) top_s->n_cand[0] = top_s->cnt;
+        __syncthreads();
+        lists = 1;
+        total = top_s->cnt;
+    }
     int32_t *out_ids = p.top_ids + (size_t)r * p.k;
-    for (uint32_t i = tid; i < cnt; i += T) {
-        const unsigned long long key = top_s->cand[i];
-        uint32_t above = 0;
-        for (uint32_t j = 0; j < cnt; j++) above += top_s->cand[j] > key;
+    for (uint32_t i = tid; i < total; i += T) {
+        uint32_t at = i, above = 0, c = 0;
+        for (uint32_t n = top_s->n_cand[0]; at >= n; n = top_s->n_cand[++c]) at -= n;
+        const unsigned long long key = top_s->cand[c * places + at];
+        for (uint32_t d = 0; d < lists; d++) {
+            const uint32_t n = top_s->n_cand[d];
+            const unsigned long long *others = top_s->cand + d * places;
+#pragma unroll 4
+            for (uint32_t j = 0; j < n; j++) above += others[j] > key;
+        }
         if (above < p.k) {
-            out_logp[above] = p.scale * (from_ordered((uint32_t)(key >> 32)) - m) - l;
+            top_s->best[above] = from_ordered((uint32_t)(key >> 32));
             out_ids[above] = (int32_t)(0xffffffffu - (uint32_t)key);
         }
     }
-    for (uint32_t i = cnt + tid; i < p.k; i += T) {
-        out_logp[i] = sound ? neg_inf() : l;
-        out_ids[i] = -1;
+    __syncthreads();
+    const float m = top_s->m, l = top_s->l;
+    const bool sound = l == l;                  // no NaN in the row
+    for (uint32_t i = tid; i < p.k; i += T) {
+        p.top_logp[(size_t)r * p.k + i] = !sound ? l : i < total ? p.scale * (top_s->best[i] - m) - l : neg_inf();
+        if (!sound || i >= total) out_ids[i] = -1;
     }
 }
 
@@ -757,13 +796,13 @@ template <int DT, bool ENT, bool TOP, int KD> static int launch_stats(cudaStream
     // with eight 50), few rows eight (257 of 50021 fp32: 19 us, with four 25).
     const uint32_t T = windows > 512 && (p.rows < (uint32_t)sms * 8 || (TOP && p.k > 32)) ? 256 : windows > 256 || TOP || KD ? 128 : 64;
     uint32_t C = 1;
-    while (C < kMaxCluster && (uint64_t)p.rows * C * 2 <= (uint64_t)sms * 2 && windows > C * T * 2) C *= 2;
+    while (C < kMaxCluster && (uint64_t)p.rows * C * 4 < (uint64_t)sms * 7 && windows > C * T * 2 && (!TOP || C * p.k <= 80)) C *= 2;
     const uint64_t entries = p.missed ? KD ? (uint64_t)p.rows * p.k : p.targets ? p.rows : 0 : 0;
     p.count_here = entries <= T * 32u ? (uint32_t)entries : 0;
     if (!p.count_here && set_zero(who, p.missed, s)) return 1;
     for (;; C = 1) {
         const uint32_t groups = (windows + C * kU * T - 1) / (C * kU * T);
-        const size_t smem = TOP ? (size_t)groups * T * sizeof(float) : KD == 2 ? ((size_t)windows * Win<DT>::kElems + 31) / 32 * 4 : 0;
+        const size_t smem = TOP ? (size_t)groups * T * sizeof(float) : KD == 2 ? ((size_t)p.vocab + 2 * Win<DT>::kElems + 31) / 32 * 4 : 0;
         SFB_REQUIRE(smem <= 200 * 1024, "%s: vocab=%u is too large", who, p.vocab);
         static DeviceOnce once;
         if (!once.done(dev)) {
