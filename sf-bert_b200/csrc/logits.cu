@@ -153,8 +153,7 @@ __device__ __forceinline__ void count_missed(const int32_t *ids, uint32_t n, uin
 
 struct TopShared {
     uint32_t gm[kThreads];                // largest values of the groups of threads: 24 bits in their order, then 255 - group
-    unsigned long long cand[kCap];        // candidates, kCap / C places for each CTA (in CTA 0)
-    uint32_t n_cand[kMaxCluster];
+    unsigned long long cand[kCap];        // candidates (in CTA 0)
     uint32_t hits[kCap];
     float best[kMaxList];
     uint32_t cnt, n_hits, tau, part[8];
@@ -502,12 +501,12 @@ __global__ void __launch_bounds__(kThreads, 4) row_stats_kernel(const StatParams
     }
     if (C == 1 && merges) merge();
     __syncthreads();
-    const uint32_t tau = top_s->tau, places = kCap / C;
-    unsigned long long *to = (C > 1 ? cg::this_cluster().map_shared_rank(top_s, 0) : top_s)->cand + rank * places;
+    const uint32_t tau = top_s->tau;
+    TopShared *const join = C > 1 ? cg::this_cluster().map_shared_rank(top_s, 0) : top_s;
     auto candidate = [&](float v, uint32_t index) {
         if (v > neg_inf() && ordered(v) >= tau) {
-            const uint32_t at = atomicAdd(&top_s->cnt, 1u);
-            if (at < places) to[at] = rank_key(v, index);
+            const uint32_t at = C > 1 ? atomicAdd(&join->cnt, 1u) : atomicAdd(&top_s->cnt, 1u);
+            if (at < kCap) join->cand[at] = rank_key(v, index);
         }
     };
     if (edge != kNoWindow) candidate(x_edge, edge - row.head);
@@ -515,33 +514,41 @@ __global__ void __launch_bounds__(kThreads, 4) row_stats_kernel(const StatParams
         const float m = keys[g * T + tid];
         if (m > neg_inf() && ordered(m) >= tau) {
             const uint32_t at = atomicAdd(&top_s->n_hits, 1u);
-            if (at < kCap) top_s->hits[at] = g * T + tid;
+            if (at < kCap) top_s->hits[at] = first + g * step + tid;
         }
     }
     __syncthreads();
     const uint32_t n_hits = top_s->n_hits;
     if (n_hits > kCap) {
-        if (tid == 0) atomicAdd(&top_s->cnt, kCap + 1);
+        if (tid == 0) atomicAdd(&join->cnt, kCap + 1);
     } else {
-        // an element each for the CTA's threads, four on their way at a time
         constexpr uint32_t E = Win<DT>::kElems;
         const uint32_t n = n_hits * kU * E;
-        for (uint32_t i0 = tid; i0 < n; i0 += 4 * T) {
+        if (n <= 4 * T) {
+            // few: an element each for the CTA's threads, four on their way (the shortest path of a row by itself)
             float e[4];
             uint32_t index[4];
 #pragma unroll
             for (uint32_t j = 0; j < 4; j++) {
-                const uint32_t i = i0 + j * T, h = i < n ? top_s->hits[i / (kU * E)] : 0;
-                const uint32_t at = h / T * step + first + i / E % kU * T + h % T;
+                const uint32_t i = tid + j * T, at = (i < n ? top_s->hits[i / (kU * E)] : 0) + i / E % kU * T;
                 index[j] = (row.first_whole() + at) * E + i % E - row.head;
                 e[j] = i < n && at < n_whole ? load_element<DT>(x, index[j]) : neg_inf();
             }
 #pragma unroll
             for (uint32_t j = 0; j < 4; j++) candidate(e[j], index[j]);
+        } else {
+            // a window each, most of which hold nothing (64 alternatives of 4096 rows of 30522 bf16: 98 -> 87 us)
+            for (uint32_t i = tid; i < n_hits * kU; i += T) {
+                const uint32_t at = top_s->hits[i / kU] + i % kU * T;
+                const uint4 one[1] = {at < n_whole ? load16(row.base + row.first_whole() + at) : no_elements<DT>()};
+                if (!(ordered(max_windows<DT, 1>(one)) >= tau)) continue;
+                float e[E];
+                unpack<DT>(one[0], e);
+#pragma unroll
+                for (uint32_t j = 0; j < E; j++) candidate(e[j], (row.first_whole() + at) * E + j - row.head);
+            }
         }
     }
-    __syncthreads();
-    if (tid == 0) (C > 1 ? cg::this_cluster().map_shared_rank(top_s, 0) : top_s)->n_cand[rank] = top_s->cnt;
     if (C > 1) {
         cg::this_cluster().sync();
         if (rank) return;
@@ -549,30 +556,14 @@ __global__ void __launch_bounds__(kThreads, 4) row_stats_kernel(const StatParams
     } else {
         __syncthreads();
     }
-    bool few = true;
-    uint32_t total = 0, lists = C;
-    for (uint32_t c = 0; c < C; c++) {
-        few &= top_s->n_cand[c] <= places;
-        total += top_s->n_cand[c];
-    }
-    if (!few) {
-        bisect_candidates<DT>(row, p.k, top_s);
-        if (tid == 0) top_s->n_cand[0] = top_s->cnt;
-        __syncthreads();
-        lists = 1;
-        total = top_s->cnt;
-    }
+    if (top_s->cnt > kCap) bisect_candidates<DT>(row, p.k, top_s);
+    const uint32_t total = top_s->cnt;
     int32_t *out_ids = p.top_ids + (size_t)r * p.k;
     for (uint32_t i = tid; i < total; i += T) {
-        uint32_t at = i, above = 0, c = 0;
-        for (uint32_t n = top_s->n_cand[0]; at >= n; n = top_s->n_cand[++c]) at -= n;
-        const unsigned long long key = top_s->cand[c * places + at];
-        for (uint32_t d = 0; d < lists; d++) {
-            const uint32_t n = top_s->n_cand[d];
-            const unsigned long long *others = top_s->cand + d * places;
-#pragma unroll 4
-            for (uint32_t j = 0; j < n; j++) above += others[j] > key;
-        }
+        const unsigned long long key = top_s->cand[i];
+        uint32_t above = 0;
+#pragma unroll 8
+        for (uint32_t j = 0; j < total; j++) above += top_s->cand[j] > key;
         if (above < p.k) {
             top_s->best[above] = from_ordered((uint32_t)(key >> 32));
             out_ids[above] = (int32_t)(0xffffffffu - (uint32_t)key);
@@ -796,7 +787,12 @@ template <int DT, bool ENT, bool TOP, int KD> static int launch_stats(cudaStream
     // with eight 50), few rows eight (257 of 50021 fp32: 19 us, with four 25).
     const uint32_t T = windows > 512 && (p.rows < (uint32_t)sms * 8 || (TOP && p.k > 32)) ? 256 : windows > 256 || TOP || KD ? 128 : 64;
     uint32_t C = 1;
-    while (C < kMaxCluster && (uint64_t)p.rows * C * 4 < (uint64_t)sms * 7 && windows > C * T * 2 && (!TOP || C * p.k <= 80)) C *= 2;
+    // CTAs per row: as many as there are SMs without one, and a few for every SM as long as each has two groups of windows
+    while (C < kMaxCluster && windows > C * T * 2 && (!TOP || C * p.k <= 80)) {
+        const uint64_t ctas = (uint64_t)p.rows * C * 2;
+        if (ctas > (uint64_t)sms && (2 * ctas > 7 * (uint64_t)sms || windows < 2 * C * 2 * kU * T)) break;
+        C *= 2;
+    }
     const uint64_t entries = p.missed ? KD ? (uint64_t)p.rows * p.k : p.targets ? p.rows : 0 : 0;
     p.count_here = entries <= T * 32u ? (uint32_t)entries : 0;
     if (!p.count_here && set_zero(who, p.missed, s)) return 1;
