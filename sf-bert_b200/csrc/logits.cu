@@ -26,6 +26,7 @@ namespace lg {
 
 constexpr uint32_t kThreads = 256;
 constexpr int kU = 4;                     // windows that a thread has on their way at a time
+constexpr int kG = 4;                     // the same for gradients
 constexpr uint32_t kCap = 1024;           // candidates for a row's alternatives
 constexpr uint32_t kMaxList = 128;        // alternatives, entries of a teacher's list
 constexpr uint32_t kMaxCluster = 8;
@@ -614,12 +615,13 @@ template <int DT> __device__ __forceinline__ uint4 load_shifted(const void *x, u
 // dx = p (c0 + c1 t) with t the base-2 logarithm of p, plus the given target's share (KD 0, ENT: c1 is not 0);
 // dx = c0 2^t + c2 2^t2, what is listed made again by itself (KD 1; HARD: c2 is not 0).
 template <int DT, bool ENT, bool KD, bool HARD, bool SAME>
-__global__ void __launch_bounds__(kThreads) row_grad_kernel(const GradParams p)
+__global__ void __launch_bounds__(kThreads, 5) row_grad_kernel(const GradParams p)
 {
-    __shared__ int32_t l_id[KD ? kMaxList : 1];
-    __shared__ float l_q[KD ? kMaxList : 1];
-    __shared__ float coef[4];
+    __shared__ __align__(16) int32_t l_id[KD ? kMaxList : 4];
+    __shared__ __align__(16) float l_q[KD ? kMaxList : 4];
+    __shared__ float2 l_part[kMaxList / 32];                  // a warp's entries: the largest teacher value, the sum of the powers beside it
     constexpr uint32_t E = Win<DT>::kElems;
+    constexpr bool kMaySkip = !KD && !ENT;                    // a row without a target is zeros
     const uint32_t T = blockDim.x, tid = threadIdx.x, lane = tid & 31;
     const uint32_t r = blockIdx.x / p.parts, part = blockIdx.x - r * p.parts;
     grid_dependency_wait();
@@ -631,95 +633,87 @@ __global__ void __launch_bounds__(kThreads) row_grad_kernel(const GradParams p)
     const uint32_t w_begin = part * p.per, w_end = min(orow.windows(), w_begin + p.per);
     const int32_t i_begin = (int32_t)(w_begin * E) - (int32_t)orow.head, i_end = (int32_t)(w_end * E) - (int32_t)orow.head;
 
-    const float *st = p.stats + (KD && p.tail ? 3 : 2) * (size_t)r;
-    const float m = st[0];
-    float c0, c1 = 0.f, c2 = 0.f, l2, l2b = 0.f, target_share = 0.f;
     int32_t target = p.targets ? p.targets[r] : -1;
     if ((uint32_t)target >= p.vocab) target = -1;
-    bool zero = m == neg_inf();                               // no token is left: every probability is 0
+    const float *st = p.stats + (KD && p.tail ? 3 : 2) * (size_t)r;
+    const float m = st[0];
+    const bool zero = m == neg_inf() || (kMaySkip && target < 0);       // no token is left (every probability is 0), or nothing is asked for
+    auto load = [&](uint32_t w) { return SAME ? load_window(row, w) : load_shifted<DT>(x, orow.head, p.vocab, w); };
+    uint4 v[kG];
+    auto load_round = [&](uint32_t w0) {
+#pragma unroll
+        for (int u = 0; u < kG; u++)
+            if (w0 + u * T < w_end) v[u] = load(w0 + u * T);
+    };
+    if (!zero) load_round(w_begin + tid);
 
-    constexpr uint32_t kSlots = 2;                            // KD: a thread's share of the list and the target (at least 128 threads)
-    float x_listed[kSlots], listed_w = 0.f, listed_c = 0.f;
+    float c0, c1 = 0.f, c2 = 0.f, l2, l2b = 0.f, target_share = 0.f;
+    int32_t id = -1;                                          // KD: this thread's entry of the list
+    float x_listed = 0.f, x_target = 0.f, listed_w = 0.f, listed_c = 0.f;
     if (!KD) {
         const float g = target >= 0 ? p.dlogp[r] : 0.f;
         l2 = st[1] * kLog2e;
+        c0 = -p.scale * g;
         if (ENT) {
             const float h = p.dentropy[r];
             c0 = -p.scale * (g + h * p.entropy[r]);
             c1 = -p.scale * h * kLn2;
-        } else {
-            c0 = -p.scale * g;
-            zero |= target < 0;
         }
         target_share = p.scale * g;
     } else {
-        if (tid < 32) {
-            float mq = p.tail ? 0.f : neg_inf(), zq = 0.f;
-            for (uint32_t i = lane; i < p.k; i += 32) {
-                const int32_t id = p.ids[(size_t)r * p.k + i];
-                const bool ok = (uint32_t)id < p.vocab;
-                const float lq = ok ? p.teacher[(size_t)r * p.k + i] : neg_inf();
-                l_id[i] = ok ? id : -1;
-                l_q[i] = lq;
-                if (!p.tail) mq = max_nan(mq, lq);
-            }
-            mq = warp_max_nan(mq);
-            __syncwarp();
-            if (mq != neg_inf())
-                for (uint32_t i = lane; i < p.k; i += 32) zq += expf(l_q[i] - mq);
-            zq = warp_sum(zq);
-            const float inv = p.tail ? 1.f : 1.f / zq;
-            for (uint32_t i = lane; i < p.k; i += 32) l_q[i] = mq == neg_inf() ? 0.f : expf(l_q[i] - mq) * inv;
-            if (lane == 0) {
-                const float sum = p.tail ? zq : mq == neg_inf() ? 0.f : 1.f, left = p.tail ? fmaxf(0.f, 1.f - zq) : 0.f;
-                coef[0] = sum + left;
-                coef[1] = left;
-            }
+        float lq = neg_inf();
+        if (tid < p.k) {
+            id = p.ids[(size_t)r * p.k + tid];
+            lq = p.teacher[(size_t)r * p.k + tid];
+            if ((uint32_t)id >= p.vocab) { id = -1; lq = neg_inf(); }
+            l_id[tid] = id;
+        } else if (tid < kMaxList) {
+            l_id[tid] = -1;
         }
-        __syncthreads();
-        const float sw = p.scale * p.dloss[r], all = coef[0], left = coef[1];
-        listed_w = sw;
-        listed_c = sw * all;
-        l2 = st[1] * kLog2e;
-        c0 = sw * all;
-        if (p.tail) {
-            // unlisted tokens: all * p - left * p / p_rest, as a multiple of their share of the remainder
-            const float lr = st[2];
-            if (lr == neg_inf()) {
-                c0 = 0.f;                                     // every unlisted one has a probability of 0
-            } else {
-                c0 = sw * (all * expf(lr - st[1]) - left);
-                l2 = lr * kLog2e;
-            }
+        const uint32_t n = (p.k + 31) / 32;
+        if (tid / 32 < n) {
+            const float mq = p.tail ? 0.f : warp_max_nan(lq), z = warp_sum(lq == neg_inf() ? 0.f : ex2(kLog2e * (lq - mq)));
+            if (lane == 0) l_part[tid / 32] = make_float2(mq, z);
         }
+        // out may be x: what is listed (and the target) is read before anything is written
+        if (id >= i_begin && id < i_end && id >= 0) x_listed = load_element<DT>(x, (uint32_t)id);
+        if (HARD && tid == 0 && target >= 0 && target >= i_begin && target < i_end) x_target = load_element<DT>(x, (uint32_t)target);
+        const float sw = p.scale * p.dloss[r], l = st[1], lr = p.tail ? st[2] : 0.f;
         if (HARD) {
             const float g = target >= 0 ? p.dlogp[r] : 0.f;
             c2 = -g;
             l2b = p.token_stats[2 * (size_t)r + 1] * kLog2e;
             target_share = g;
         }
-#pragma unroll
-        for (uint32_t n = 0; n < kSlots; n++) {
-            const uint32_t i = tid + n * T;
-            const int32_t id = i < p.k ? l_id[i] : i == p.k && HARD ? target : -1;
-            x_listed[n] = id >= 0 && id >= i_begin && id < i_end ? load_element<DT>(x, (uint32_t)id) : 0.f;
-        }
-        __syncthreads();                                      // out may be x: nothing is written before what is listed has been read
-    }
-
-    const uint32_t w_target = !KD && target >= 0 ? ((uint32_t)target + orow.head) / E : 0xffffffffu;
-    const uint32_t e_target = ((uint32_t)target + orow.head) % E;
-    for (uint32_t w0 = w_begin + tid; w0 - tid < w_end; w0 += kU * T) {
-        uint4 v[kU];
-        if (!zero) {
-#pragma unroll
-            for (int u = 0; u < kU; u++) {
-                const uint32_t w = w0 + u * T;
-                if (w < w_end) v[u] = SAME ? load_window(row, w) : load_shifted<DT>(x, orow.head, p.vocab, w);
+        __syncthreads();
+        float mq = p.tail ? 0.f : neg_inf(), z = 0.f;
+        if (!p.tail)
+            for (uint32_t w = 0; w < n; w++) mq = max_nan(mq, l_part[w].x);
+        for (uint32_t w = 0; w < n; w++) z += l_part[w].x == neg_inf() ? 0.f : l_part[w].y * (p.tail ? 1.f : ex2(kLog2e * (l_part[w].x - mq)));
+        const bool none = mq == neg_inf();
+        if (tid < kMaxList) l_q[tid] = lq == neg_inf() || none ? 0.f : ex2(kLog2e * (lq - mq)) * (p.tail ? 1.f : 1.f / z);
+        const float left = p.tail ? fmaxf(0.f, 1.f - z) : 0.f, all = p.tail ? z + left : none ? 0.f : 1.f;
+        listed_w = sw;
+        listed_c = sw * all;
+        l2 = l * kLog2e;
+        c0 = sw * all;
+        if (p.tail) {
+            // unlisted tokens: all * p - left * p / p_rest, as a multiple of their share of the remainder
+            if (lr == neg_inf()) {
+                c0 = 0.f;                                     // every unlisted one has a probability of 0
+            } else {
+                c0 = sw * (all * expf(lr - l) - left);
+                l2 = lr * kLog2e;
             }
         }
+    }
+
+    const uint32_t w_target = !KD && target >= 0 ? ((uint32_t)target + orow.head) / E : kNoWindow;
+    const Pair minus_m = pair(-m, -m), s2 = pair(p.s2, p.s2), minus_l = pair(-l2, -l2), k0 = pair(c0, c0), k1 = pair(c1, c1);
+    const Pair log2e = pair(kLog2e, kLog2e), minus_lb = pair(-l2b, -l2b), k2 = pair(c2, c2);
+    for (uint32_t w0 = w_begin + tid; w0 - tid < w_end; w0 += kG * T) {
 #pragma unroll
-        for (int u = 0; u < kU; u++) {
+        for (int u = 0; u < kG; u++) {
             const uint32_t w = w0 + u * T;
             if (w >= w_end) break;
             float y[E];
@@ -729,17 +723,24 @@ __global__ void __launch_bounds__(kThreads) row_grad_kernel(const GradParams p)
             } else {
                 unpack<DT>(v[u], y);
 #pragma unroll
-                for (uint32_t j = 0; j < E; j++) {
-                    const float d = y[j] - m;
-                    const float t = fmaf(p.s2, d, -l2), e = ex2(t);
-                    y[j] = ENT ? e * fmaf(c1, fmaxf(t, kFar), c0) : e * c0;
-                    if (HARD) y[j] = fmaf(c2, ex2(fmaf(kLog2e, d, -l2b)), y[j]);
+                for (uint32_t j = 0; j < E; j += 2) {
+                    const Pair d = add2(pair(y[j], y[j + 1]), minus_m), t = fma2(s2, d, minus_l);
+                    float t0, t1;
+                    halves(t, t0, t1);
+                    const Pair e = pair(ex2(t0), ex2(t1));
+                    Pair g = mul2(e, ENT ? fma2(k1, pair(fmaxf(t0, kFar), fmaxf(t1, kFar)), k0) : k0);
+                    if (HARD) {
+                        halves(fma2(log2e, d, minus_lb), t0, t1);
+                        g = fma2(k2, pair(ex2(t0), ex2(t1)), g);
+                    }
+                    halves(g, y[j], y[j + 1]);
                 }
             }
             if (w == w_target) {
+                const uint32_t at = ((uint32_t)target + orow.head) % E;
 #pragma unroll
                 for (uint32_t j = 0; j < E; j++)
-                    if (j == e_target) y[j] += target_share;
+                    if (j == at) y[j] += target_share;
             }
             if (orow.whole(w)) {
                 ((uint4 *)orow.base)[w] = pack<DT>(y);
@@ -751,30 +752,36 @@ __global__ void __launch_bounds__(kThreads) row_grad_kernel(const GradParams p)
                 }
             }
         }
+        // all of a round's loads after all of the last one's stores: taking turns window by window cost 20 % of the bandwidth
+        if (!zero) load_round(w0 + kG * T);
     }
     if (!KD) return;
-    // What is listed, and the target: made again from all the shares it has.  An index that stands in the list twice is
+    // What is listed, and the target: made again from all the shares it has.  A token that stands in the list twice is
     // written twice, with the same value.
     __syncthreads();
-#pragma unroll
-    for (uint32_t n = 0; n < kSlots; n++) {
-        const uint32_t i = tid + n * T;
-        const int32_t id = i < p.k ? l_id[i] : i == p.k && HARD ? target : -1;
-        if (id < 0 || id < i_begin || id >= i_end) continue;
+    auto again = [&](int32_t token, float xl) {
         float q = 0.f;
         bool listed = false;
-        for (uint32_t j = 0; j < p.k; j++)
-            if (l_id[j] == id) { q += l_q[j]; listed = true; }
-        const float d = x_listed[n] - m;
+        for (uint32_t j = 0; j < p.k; j += 4) {
+            const int4 o = *(const int4 *)&l_id[j];
+            const float4 w = *(const float4 *)&l_q[j];
+            if (o.x == token) { q += w.x; listed = true; }
+            if (o.y == token) { q += w.y; listed = true; }
+            if (o.z == token) { q += w.z; listed = true; }
+            if (o.w == token) { q += w.w; listed = true; }
+        }
+        const float d = xl - m;
         float y = 0.f;
         if (!zero) y = listed ? listed_c * ex2(fmaf(p.s2, d, -st[1] * kLog2e)) : c0 * ex2(fmaf(p.s2, d, -l2));
         y -= listed_w * q;
         if (HARD) {
             if (!zero) y = fmaf(c2, ex2(fmaf(kLog2e, d, -l2b)), y);
-            if (id == target) y += target_share;
+            if (token == target) y += target_share;
         }
-        store_element<DT>(out, (uint32_t)id, y);
-    }
+        store_element<DT>(out, (uint32_t)token, y);
+    };
+    if (id >= 0 && id >= i_begin && id < i_end) again(id, x_listed);
+    if (HARD && tid == 0 && target >= 0 && target >= i_begin && target < i_end) again(target, x_target);
 }
 
 // ---- launches -----------------------------------------------------------------------------------------------------------
@@ -820,11 +827,11 @@ template <int DT, bool ENT, bool KD, bool HARD> static int launch_grad(cudaStrea
     SFB_REQUIRE(sms > 0, "%s: cannot query the device", who);
     const uint32_t windows = p.width / Win<DT>::kElems + 2;
     const uint32_t T = windows > 512 ? 256 : windows > 256 || KD ? 128 : 64;
-    const uint32_t round = T * kU;
+    const uint32_t round = T * kG;
     uint32_t rounds = (windows + round - 1) / round;
-    // whole rows per CTA once there are several CTAs for every SM, a round each before that
+    // A CTA takes several rounds of windows where enough CTAs are left for every SM: lists cost each CTA a few thousand cycles.
     uint32_t per = 1;
-    while (per < rounds && (uint64_t)p.rows * ((rounds + per * 2 - 1) / (per * 2)) >= (uint64_t)sms * 16) per *= 2;
+    while (per < rounds && (uint64_t)p.rows * ((rounds + per * 2 - 1) / (per * 2)) >= (uint64_t)sms * (KD ? 4 : 32)) per *= 2;
     p.per = per * round;
     p.parts = (windows + p.per - 1) / p.per;
     SFB_REQUIRE((uint64_t)p.rows * p.parts < (1ull << 31), "%s: too many rows", who);
