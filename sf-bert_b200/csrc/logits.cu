@@ -360,7 +360,8 @@ __global__ void __launch_bounds__(kThreads, 4) row_stats_kernel(const StatParams
         }
     };
     uint4 v[kU], next[kU];
-    if (first < n_whole) load(next, first);
+    const uint32_t groups = first < n_whole ? (n_whole - first + step - 1) / step : 0;
+    if (groups) load(next, first);
     const uint32_t edge = rank == 0 ? edge_position<DT>(row, tid) : kNoWindow;       // what is not in a whole window: an element each
     float x_edge = edge != kNoWindow ? load_element<DT>(x, edge - row.head) : neg_inf();
     const bool merges = rank == 0 && warp == (TOP ? T / 32 - 1 : 0);      // with alternatives, others look for their bound meanwhile
@@ -411,11 +412,11 @@ __global__ void __launch_bounds__(kThreads, 4) row_stats_kernel(const StatParams
     // ---- the pass ----
     Sums a;
     float mx = neg_inf();
-    uint32_t groups = 0;
-    for (uint32_t i0 = first; i0 < n_whole; i0 += step, groups++) {
+    for (uint32_t g = 0; g < groups; g++) {
+        const uint32_t i0 = first + g * step;
 #pragma unroll
         for (int u = 0; u < kU; u++) v[u] = next[u];
-        if (i0 + step < n_whole) load(next, i0 + step);
+        if (g + 1 < groups) load(next, i0 + step);
         if (KD == 2) {
 #pragma unroll
             for (int u = 0; u < kU; u++) {
@@ -425,7 +426,7 @@ __global__ void __launch_bounds__(kThreads, 4) row_stats_kernel(const StatParams
             }
         }
         const float m = max_windows<DT, kU>(v);
-        if (TOP) keys[groups * T + tid] = m;
+        if (TOP) keys[g * T + tid] = m;
         mx = max_nan(mx, m);
         if (a.prepare(m, p.s2, gap)) add_windows<DT, ENT, kU>(a, v, p.s2);
     }
@@ -613,8 +614,10 @@ template <int DT> __device__ __forceinline__ uint4 load_shifted(const void *x, u
 }
 
 // dx = p (c0 + c1 t) with t the base-2 logarithm of p, plus the given target's share (KD 0, ENT: c1 is not 0);
-// dx = c0 2^t + c2 2^t2, what is listed made again by itself (KD 1; HARD: c2 is not 0).
-template <int DT, bool ENT, bool KD, bool HARD, bool SAME>
+// dx = c0 2^t + c2 2^t2, what is listed made again by itself (KD 1; HARD 1: c2 is not 0).  HARD 2: at temperature 2 the
+// second power, the softmax's at temperature 1, is the first one's square times a constant of the row (which goes to c2), and an
+// exponential per element less: PLACE.
+template <int DT, bool ENT, bool KD, int HARD, bool SAME>
 __global__ void __launch_bounds__(kThreads, 5) row_grad_kernel(const GradParams p)
 {
     __shared__ __align__(16) int32_t l_id[KD ? kMaxList : 4];
@@ -638,14 +641,15 @@ __global__ void __launch_bounds__(kThreads, 5) row_grad_kernel(const GradParams 
     const float *st = p.stats + (KD && p.tail ? 3 : 2) * (size_t)r;
     const float m = st[0];
     const bool zero = m == neg_inf() || (kMaySkip && target < 0);       // no token is left (every probability is 0), or nothing is asked for
-    auto load = [&](uint32_t w) { return SAME ? load_window(row, w) : load_shifted<DT>(x, orow.head, p.vocab, w); };
+    auto load = [&](uint32_t w) { return SAME ? load_window<DT, true>(row, w) : load_shifted<DT>(x, orow.head, p.vocab, w); };
     uint4 v[kG];
     auto load_round = [&](uint32_t w0) {
 #pragma unroll
         for (int u = 0; u < kG; u++)
             if (w0 + u * T < w_end) v[u] = load(w0 + u * T);
     };
-    if (!zero) load_round(w_begin + tid);
+    const uint32_t first_round = w_end > w_begin ? r % ((w_end - w_begin + kG * T - 1) / (kG * T)) : 0;
+    if (!zero) load_round(w_begin + first_round * (kG * T) + tid);
 
     float c0, c1 = 0.f, c2 = 0.f, l2, l2b = 0.f, target_share = 0.f;
     int32_t id = -1;                                          // KD: this thread's entry of the list
@@ -710,8 +714,15 @@ __global__ void __launch_bounds__(kThreads, 5) row_grad_kernel(const GradParams 
 
     const uint32_t w_target = !KD && target >= 0 ? ((uint32_t)target + orow.head) / E : kNoWindow;
     const Pair minus_m = pair(-m, -m), s2 = pair(p.s2, p.s2), minus_l = pair(-l2, -l2), k0 = pair(c0, c0), k1 = pair(c1, c1);
-    const Pair log2e = pair(kLog2e, kLog2e), minus_lb = pair(-l2b, -l2b), k2 = pair(c2, c2);
-    for (uint32_t w0 = w_begin + tid; w0 - tid < w_end; w0 += kG * T) {
+    // HARD 2: 2^t2 = (2^t)^2 * 2^(2 l2 - l2b)
+    const float c2s = HARD == 2 ? c2 * ex2(fmaf(2.f, l2, -l2b)) : c2;
+    const Pair log2e = pair(kLog2e, kLog2e), minus_lb = pair(-l2b, -l2b), k2 = pair(c2s, c2s);
+    // Rows start at different rounds: with all of them at the same column, reads and writes crowded the same memory channels
+    // (8192 rows of 30522 bf16: 195 us so, 158 now).
+    const uint32_t rounds = (w_end - w_begin + kG * T - 1) / (kG * T);
+    for (uint32_t i = 0, round = first_round; i < rounds; i++) {
+        const uint32_t w0 = w_begin + round * (kG * T) + tid;
+        round = round + 1 == rounds ? 0 : round + 1;
 #pragma unroll
         for (int u = 0; u < kG; u++) {
             const uint32_t w = w0 + u * T;
@@ -729,9 +740,11 @@ __global__ void __launch_bounds__(kThreads, 5) row_grad_kernel(const GradParams 
                     halves(t, t0, t1);
                     const Pair e = pair(ex2(t0), ex2(t1));
                     Pair g = mul2(e, ENT ? fma2(k1, pair(fmaxf(t0, kFar), fmaxf(t1, kFar)), k0) : k0);
-                    if (HARD) {
+                    if (HARD == 1) {
                         halves(fma2(log2e, d, minus_lb), t0, t1);
                         g = fma2(k2, pair(ex2(t0), ex2(t1)), g);
+                    } else if (HARD == 2) {
+                        g = fma2(mul2(k2, e), e, g);
                     }
                     halves(g, y[j], y[j + 1]);
                 }
@@ -743,7 +756,7 @@ __global__ void __launch_bounds__(kThreads, 5) row_grad_kernel(const GradParams 
                     if (j == at) y[j] += target_share;
             }
             if (orow.whole(w)) {
-                ((uint4 *)orow.base)[w] = pack<DT>(y);
+                __stcs((uint4 *)orow.base + w, pack<DT>(y));
             } else {
 #pragma unroll
                 for (uint32_t j = 0; j < E; j++) {
@@ -753,7 +766,8 @@ __global__ void __launch_bounds__(kThreads, 5) row_grad_kernel(const GradParams 
             }
         }
         // all of a round's loads after all of the last one's stores: taking turns window by window cost 20 % of the bandwidth
-        if (!zero) load_round(w0 + kG * T);
+        asm volatile("" ::: "memory");
+        if (!zero && i + 1 < rounds) load_round(w_begin + round * (kG * T) + tid);
     }
     if (!KD) return;
     // What is listed, and the target: made again from all the shares it has.  A token that stands in the list twice is
@@ -821,7 +835,7 @@ template <int DT, bool ENT, bool TOP, int KD> static int launch_stats(cudaStream
     return check_launch(who);
 }
 
-template <int DT, bool ENT, bool KD, bool HARD> static int launch_grad(cudaStream_t s, GradParams &p, const char *who)
+template <int DT, bool ENT, bool KD, int HARD> static int launch_grad(cudaStream_t s, GradParams &p, const char *who)
 {
     const int sms = device_sm_count(current_device());
     SFB_REQUIRE(sms > 0, "%s: cannot query the device", who);
@@ -896,7 +910,7 @@ extern "C" int sfb_token_logprobs_grad(sfb_stream_t stream, const void *logits, 
     lg::GradParams p = {logits, out, pitch, out_pitch, rows, vocab, width, 0, 0, scale, scale * lg::kLog2e, targets, stats, dlogp, entropy, dentropy,
                         nullptr, nullptr, nullptr, nullptr, 0, 0};
     cudaStream_t s = as_stream(stream);
-    return dentropy ? BY_TYPE(dtype, lg::launch_grad, true, false, false)(s, p, who) : BY_TYPE(dtype, lg::launch_grad, false, false, false)(s, p, who);
+    return dentropy ? BY_TYPE(dtype, lg::launch_grad, true, false, 0)(s, p, who) : BY_TYPE(dtype, lg::launch_grad, false, false, 0)(s, p, who);
 }
 
 extern "C" int sfb_distill_topk(sfb_stream_t stream, const void *logits, uint64_t pitch, const int32_t *ids, const float *teacher, uint32_t rows,
@@ -929,7 +943,8 @@ extern "C" int sfb_distill_topk_grad(sfb_stream_t stream, const void *logits, ui
     lg::GradParams p = {logits, out, pitch, out_pitch, rows, vocab, width, 0, 0, scale, scale * lg::kLog2e, targets, stats, dlogp, nullptr, nullptr,
                         ids, teacher, dloss, token_stats, k, tail};
     cudaStream_t s = as_stream(stream);
-    return targets ? BY_TYPE(dtype, lg::launch_grad, false, true, true)(s, p, who) : BY_TYPE(dtype, lg::launch_grad, false, true, false)(s, p, who);
+    if (!targets) return BY_TYPE(dtype, lg::launch_grad, false, true, 0)(s, p, who);
+    return scale == 0.5f && !tail ? BY_TYPE(dtype, lg::launch_grad, false, true, 2)(s, p, who) : BY_TYPE(dtype, lg::launch_grad, false, true, 1)(s, p, who);
 }
 
 extern "C" uint64_t sfb_linear_logprobs_workspace(uint32_t m, uint32_t vocab) { return tc_linear_logprobs_workspace(m, vocab); }
