@@ -40,7 +40,8 @@ struct GParams {
     uint32_t band;      // CTA-pair kernel: column tiles per band of the tile order (tile_coords)
     const void *resid;  // split kernel: [m, n] of x's type, added to the product (not out itself), or NULL
     // scores: what is kept of each row's 128 columns in place of the columns themselves
-    float4 *score_parts;       // [ceil(n / 128)][m]: largest, sum of the powers, sum of them times their exponents
+    uint32_t bn;               // columns of a tile (256 where the product itself is wanted)
+    float4 *score_parts;       // [part][m]: largest, sum of the powers, sum of them times their exponents; a part is a tile's 128 columns or less
     float *target_logit;       // [m]
     const int32_t *targets;    // [m]
     float s2;                  // scale * log2(e)
@@ -195,10 +196,11 @@ __device__ __forceinline__ void drain_rows_staged(const GParams &p, const CUtens
 // place.  A thread has a whole row of the tile, so nothing is exchanged.  128 columns cost a thread about 128 x 6
 // instructions and the SM 2048 cycles of exponentials per 256-column tile; the tile's MMAs take 2048 cycles per 256 of k.
 template <bool ENT>
-__device__ __forceinline__ void score_rows(const GParams &p, uint32_t tcol, const float *bias, uint32_t row, uint32_t n0)
+__device__ __forceinline__ void score_rows(const GParams &p, uint32_t tcol, const float *bias, uint32_t row, uint32_t target, uint32_t tile_n, uint32_t chalf)
 {
     const bool row_ok = row < p.M;
-    const uint32_t target = row_ok ? (uint32_t)p.targets[row] : 0xffffffffu;
+    const uint32_t n0 = tile_n * p.bn + chalf * 128, end = min(p.N, (tile_n + 1) * p.bn);      // this thread's columns: [n0, n0 + 128) before end
+    if (n0 >= end) return;
     lg::Sums a;
     float mx = lg::neg_inf();
     const float gap = 40.f / p.s2;
@@ -207,9 +209,10 @@ __device__ __forceinline__ void score_rows(const GParams &p, uint32_t tcol, cons
 #pragma unroll
     for (uint32_t c = 0; c < 4; c++) {
         const uint32_t c0 = c * 32, col = n0 + c0;
+        if (col >= end) break;
         __syncwarp();                        // the lanes parted over targets and references
         tmem_wait_ld();
-        if (c + 1 < 4) TMEM_LD_32((v[(c + 1) & 1]), tcol + c0 + 32);
+        if (c + 1 < 4 && col + 32 < end) TMEM_LD_32((v[(c + 1) & 1]), tcol + c0 + 32);
         uint32_t(&cur)[32] = v[c & 1];
         float x[32];
 #pragma unroll
@@ -218,39 +221,59 @@ __device__ __forceinline__ void score_rows(const GParams &p, uint32_t tcol, cons
 #pragma unroll
             for (int j = 0; j < 8; j++) {
                 const float4 bb = *(const float4 *)(bias + c0 + 4 * j);
-                x[4 * j] += bb.x; x[4 * j + 1] += bb.y; x[4 * j + 2] += bb.z; x[4 * j + 3] += bb.w;
+                lg::halves(lg::add2(lg::pair(x[4 * j], x[4 * j + 1]), lg::pair(bb.x, bb.y)), x[4 * j], x[4 * j + 1]);
+                lg::halves(lg::add2(lg::pair(x[4 * j + 2], x[4 * j + 3]), lg::pair(bb.z, bb.w)), x[4 * j + 2], x[4 * j + 3]);
             }
         }
-        if (col + 32 > p.N) {
+        if (col + 32 > end) {
 #pragma unroll
             for (uint32_t j = 0; j < 32; j++)
-                if (col + j >= p.N) x[j] = lg::neg_inf();
+                if (col + j >= end) x[j] = lg::neg_inf();
         }
-        if (target - col < 32u && target < p.N) {
+        if (target - col < 32u && target < end) {
             float xt = x[0];
 #pragma unroll
             for (uint32_t j = 1; j < 32; j++)
                 if (target - col == j) xt = x[j];
             p.target_logit[row] = xt;
         }
-        float m = x[0];
+        float m4[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
-        for (int j = 1; j < 32; j++) m = lg::max_nan(m, x[j]);
+        for (int j = 4; j < 32; j++) m4[j & 3] = lg::max_nan(m4[j & 3], x[j]);
+        const float m = lg::max_nan(lg::max_nan(m4[0], m4[1]), lg::max_nan(m4[2], m4[3]));
         mx = lg::max_nan(mx, m);
         if (a.prepare(m, p.s2, gap)) {
-            float s[4] = {0.f, 0.f, 0.f, 0.f}, e[4] = {0.f, 0.f, 0.f, 0.f};
+            const lg::Pair minus_r = lg::pair(-a.r, -a.r), factor = lg::pair(p.s2, p.s2);
+            lg::Pair s[2] = {lg::pair(a.s, 0.f), lg::pair(0.f, 0.f)}, e[2] = {lg::pair(a.e, 0.f), lg::pair(0.f, 0.f)};
 #pragma unroll
-            for (int j = 0; j < 32; j++) {
-                const float t = p.s2 * (x[j] - a.r), y = lg::ex2(t);
-                s[j & 3] += y;
-                if (ENT) e[j & 3] = fmaf(y, fmaxf(t, lg::kFar), e[j & 3]);
+            for (int j = 0; j < 32; j += 2) {
+                const lg::Pair t = lg::mul2(factor, lg::add2(lg::pair(x[j], x[j + 1]), minus_r));
+                float t0, t1;
+                lg::halves(t, t0, t1);
+                const lg::Pair y = lg::pair(lg::ex2(t0), lg::ex2(t1));
+                s[j >> 1 & 1] = lg::add2(s[j >> 1 & 1], y);
+                if (ENT) e[j >> 1 & 1] = lg::fma2(y, t, e[j >> 1 & 1]);
             }
-            a.s += (s[0] + s[1]) + (s[2] + s[3]);
-            if (ENT) a.e += (e[0] + e[1]) + (e[2] + e[3]);
+            float f0, f1;
+            if (ENT) {
+                lg::halves(lg::add2(e[0], e[1]), f0, f1);
+                f0 += f1;
+                if (f0 != f0) {              // a logit of -inf (0 times its exponent): once more, with finite exponents
+                    f0 = a.e;
+#pragma unroll
+                    for (int j = 0; j < 32; j++) {
+                        const float t = p.s2 * (x[j] - a.r);
+                        f0 = fmaf(lg::ex2(t), fmaxf(t, lg::kFar), f0);
+                    }
+                }
+                a.e = f0;
+            }
+            lg::halves(lg::add2(s[0], s[1]), f0, f1);
+            a.s = f0 + f1;
         }
     }
     a.move_to(mx, p.s2);
-    if (row_ok && n0 < p.N) p.score_parts[(size_t)(n0 / 128) * p.M + row] = make_float4(mx, a.s, a.e, 0.f);
+    if (row_ok) p.score_parts[(size_t)(p.bn > 128 ? tile_n * 2 + chalf : tile_n) * p.M + row] = make_float4(mx, a.s, a.e, 0.f);
 }
 
 // SCORE: 0 the product itself, 1 scores of its rows, 2 with the sum that the entropy takes
@@ -269,6 +292,7 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant
     const uint32_t fmt = p.is_bf16 ? 1u : 0u;
     const uint32_t n_tiles = p.tiles_m * p.tiles_n;
     const uint32_t kblocks = (p.K + kGBK - 1) / kGBK;
+    const uint32_t bn = SCORE ? p.bn : kGBN;
 
     if (threadIdx.x == 0) {
         prefetch_map(amap);
@@ -296,13 +320,13 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant
         if (elect_one()) {
             uint32_t g = 0;   // k-blocks loaded so far (ring position)
             for (uint32_t t = blockIdx.x; t < n_tiles; t += gridDim.x) {
-                const int32_t m0 = (int32_t)((t % p.tiles_m) * kGBM), n0 = (int32_t)((t / p.tiles_m) * kGBN);
+                const int32_t m0 = (int32_t)((t % p.tiles_m) * kGBM), n0 = (int32_t)((t / p.tiles_m) * bn);
                 bool alive = true;
                 for (uint32_t kb = 0; kb < kblocks; kb++, g++) {
                     const uint32_t s = g % kGStages;
                     if (g >= kGStages && !mbar_wait(&st->empty[s], ((g / kGStages) - 1) & 1, abort_flag, 41)) { alive = false; break; }
                     const uint32_t base = smem_u32(tiles + s * kGStageBytes);
-                    mbar_expect_tx(&st->full[s], kGStageBytes);   // boxes beyond the tensor arrive as zeros and still count
+                    mbar_expect_tx(&st->full[s], SCORE ? kGABytes + bn * (kGBK * 2) : kGStageBytes);   // boxes beyond the tensor arrive as zeros and still count
                     tma_load_2d(base, &amap, &st->full[s], (int32_t)(kb * kGBK), m0);
                     if (p.w_transposed) {
                         // 256 rows of w, 64 of k: one box
@@ -319,7 +343,7 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant
     } else if (warp == 1) {
         // ===== MMA issuer =====
         if (elect_one()) {
-            const uint32_t idesc = instr_desc(fmt, fmt, kGBM, kGBN, p.w_transposed ? 0 : 1);
+            const uint32_t idesc = instr_desc(fmt, fmt, kGBM, bn, p.w_transposed ? 0 : 1);
             const uint32_t b_step = p.w_transposed ? 2u : 128u;   // descriptor units of 16 bytes per 16 of K
             uint32_t g = 0, i = 0;
             for (uint32_t t = blockIdx.x; t < n_tiles; t += gridDim.x, i++) {
@@ -352,17 +376,22 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant
         const uint32_t lane_field = (quarter * 32) << 16;
         uint32_t i = 0;
         auto bias_of = [&](uint32_t n0) { return SCORE ? fetch_bias_any(p, n0, lane) : fetch_bias(p, n0, lane); };
-        float4 next = bias_of((blockIdx.x / p.tiles_m) * kGBN + chalf * 128);
+        auto target_of = [&](uint32_t t) { const uint32_t row = (t % p.tiles_m) * kGBM + r; return SCORE && row < p.M ? (uint32_t)p.targets[row] : 0xffffffffu; };
+        float4 next = bias_of((blockIdx.x / p.tiles_m) * bn + chalf * 128);
+        uint32_t next_target = target_of(blockIdx.x);
         for (uint32_t t = blockIdx.x; t < n_tiles; t += gridDim.x, i++) {
             const uint32_t buf = i % kGBufs;
-            const uint32_t n0 = (t / p.tiles_m) * kGBN + chalf * 128;
+            const uint32_t n0 = (t / p.tiles_m) * bn + chalf * 128, target = next_target;
             float *bias = bias_s + ((i & 1) * 2 + chalf) * 128;
             if (!mbar_wait_warp(&st->acc_full[buf], (i / kGBufs) & 1, abort_flag, 44)) break;
             *(float4 *)(bias + lane * 4) = next;
             __syncwarp();
-            if (t + gridDim.x < n_tiles) next = bias_of(((t + gridDim.x) / p.tiles_m) * kGBN + chalf * 128);
+            if (t + gridDim.x < n_tiles) {
+                next = bias_of(((t + gridDim.x) / p.tiles_m) * bn + chalf * 128);
+                next_target = target_of(t + gridDim.x);
+            }
             tcgen05_fence_after();
-            if (SCORE) score_rows<SCORE == 2>(p, tmem + buf * kGBN + chalf * 128 + lane_field, bias, (t % p.tiles_m) * kGBM + r, n0);
+            if (SCORE) score_rows<SCORE == 2>(p, tmem + buf * kGBN + chalf * 128 + lane_field, bias, (t % p.tiles_m) * kGBM + r, target, t / p.tiles_m, chalf);
             else drain_rows(p, tmem + buf * kGBN + chalf * 128 + lane_field, bias, (t % p.tiles_m) * kGBM + r, n0);
             tcgen05_fence_before();
             mbar_arrive(&st->acc_empty[buf]);
@@ -491,6 +520,7 @@ linear_tc_pair_kernel(const __grid_constant__ CUtensorMap amap, const __grid_con
     const uint32_t fmt = p.is_bf16 ? 1u : 0u;
     const uint32_t n_tiles = p.tiles_m * p.tiles_n;          // tiles of 256 x 256
     const uint32_t kblocks = (p.K + kGBK - 1) / kGBK;
+    const uint32_t bn = SCORE ? p.bn : kGBN;
 
     if (threadIdx.x == 0) {
         prefetch_map(amap);
@@ -523,14 +553,14 @@ linear_tc_pair_kernel(const __grid_constant__ CUtensorMap amap, const __grid_con
                 uint32_t tm, tn;
                 tile_coords(p, t, tm, tn);
                 const int32_t m0 = (int32_t)(tm * 256 + rank * kGBM);
-                const int32_t n0 = (int32_t)(tn * kGBN + rank * (kGBN / 2));
+                const int32_t n0 = (int32_t)(tn * bn + rank * (bn / 2));
                 bool alive = true;
                 for (uint32_t kb = 0; kb < kblocks; kb++, g++) {
                     const uint32_t s = g % kPStages;
                     if (g >= kPStages && !mbar_wait(&st->empty[s], ((g / kPStages) - 1) & 1, abort_flag, 51)) { alive = false; break; }
                     const uint32_t base = smem_u32(tiles + s * kPStageBytes);
                     const uint32_t bar = mapa_rank(smem_u32(&st->full[s]), 0);
-                    if (rank == 0) mbar_expect_tx(&st->full[s], 2 * kPStageBytes);   // both CTAs' bytes; boxes beyond the tensor arrive as zeros and still count
+                    if (rank == 0) mbar_expect_tx(&st->full[s], SCORE ? 2 * (kPABytes + (bn / 2) * (kGBK * 2)) : 2 * kPStageBytes);   // both CTAs' bytes; boxes beyond the tensor arrive as zeros and still count
                     tma_load_2d_pair(base, &amap, bar, (int32_t)(kb * kGBK), m0);
                     if (p.w_transposed) {
                         tma_load_2d_pair(base + kPABytes, &bmap, bar, (int32_t)(kb * kGBK), n0);      // 128 rows of w, 64 of k
@@ -546,7 +576,7 @@ linear_tc_pair_kernel(const __grid_constant__ CUtensorMap amap, const __grid_con
     } else if (warp == 1) {
         // ===== MMA issuer: one thread of the even CTA for the pair =====
         if (rank == 0 && elect_one()) {
-            const uint32_t idesc = instr_desc(fmt, fmt, 256, kGBN, p.w_transposed ? 0 : 1);
+            const uint32_t idesc = instr_desc(fmt, fmt, 256, bn, p.w_transposed ? 0 : 1);
             const uint32_t b_step = p.w_transposed ? 2u : 128u;
             uint32_t g = 0, i = 0;
             for (uint32_t t = pair; t < n_tiles; t += pairs, i++) {
@@ -580,10 +610,13 @@ linear_tc_pair_kernel(const __grid_constant__ CUtensorMap amap, const __grid_con
         uint32_t i = 0, tm, tn;
         tile_coords(p, pair, tm, tn);
         auto bias_of = [&](uint32_t n0) { return SCORE ? fetch_bias_any(p, n0, lane) : fetch_bias(p, n0, lane); };
-        float4 next = bias_of(tn * kGBN + chalf * 128);
+        auto target_of = [&](uint32_t row) { return SCORE && row < p.M ? (uint32_t)p.targets[row] : 0xffffffffu; };
+        const uint32_t r = rank * kGBM + quarter * 32 + lane;
+        float4 next = bias_of(tn * bn + chalf * 128);
+        uint32_t next_target = target_of(tm * 256 + r);
         for (uint32_t t = pair; t < n_tiles; t += pairs, i++) {
             const uint32_t buf = i & 1;
-            const uint32_t n0 = tn * kGBN + chalf * 128;
+            const uint32_t n0 = tn * bn + chalf * 128, tile_n = tn, target = next_target;
             const uint32_t m0 = tm * 256 + rank * kGBM;
             float *bias = bias_s + (buf * 2 + chalf) * 128;
             if (!mbar_wait_warp(&st->acc_full[buf], (i >> 1) & 1, abort_flag, 54)) break;
@@ -591,10 +624,11 @@ linear_tc_pair_kernel(const __grid_constant__ CUtensorMap amap, const __grid_con
             __syncwarp();
             if (t + pairs < n_tiles) {
                 tile_coords(p, t + pairs, tm, tn);
-                next = bias_of(tn * kGBN + chalf * 128);
+                next = bias_of(tn * bn + chalf * 128);
+                next_target = target_of(tm * 256 + r);
             }
             tcgen05_fence_after();
-            if (SCORE) score_rows<SCORE == 2>(p, tmem + buf * kGBN + chalf * 128 + lane_field, bias, m0 + quarter * 32 + lane, n0);
+            if (SCORE) score_rows<SCORE == 2>(p, tmem + buf * kGBN + chalf * 128 + lane_field, bias, m0 + quarter * 32 + lane, target, tile_n, chalf);
             else drain_rows_staged(p, &omap, tmem + buf * kGBN + chalf * 128 + lane_field, staging + (warp - 2) * 4096, bias, m0 + quarter * 32, n0, lane);
             tcgen05_fence_before();
             __syncwarp();
@@ -1045,32 +1079,41 @@ __global__ void __launch_bounds__(256) score_join_kernel(const float4 *parts, co
             mx = top;
         }
     }
-    sh[0][tid] = mx; sh[1][tid] = a.s; sh[2][tid] = a.e;
-    for (uint32_t half = 128; half >= R; half >>= 1) {
-        __syncthreads();
-        if (tid < half) {
-            Sums x, y;
-            x.r = sh[0][tid]; x.s = sh[1][tid]; x.e = sh[2][tid];
-            y.r = sh[0][tid + half]; y.s = sh[1][tid + half]; y.e = sh[2][tid + half];
-            const float top = max_nan(x.r, y.r);
-            x.move_to(top, s2);
-            y.move_to(top, s2);
-            sh[0][tid] = top; sh[1][tid] = x.s + y.s; sh[2][tid] = x.e + y.e;
-        }
+    a.r = mx;
+    // a warp's threads of the same row (32 / R of them), then the warps'
+    for (uint32_t o = 16; o >= R; o >>= 1) {
+        Sums b;
+        b.r = __shfl_xor_sync(0xffffffffu, a.r, o); b.s = __shfl_xor_sync(0xffffffffu, a.s, o); b.e = __shfl_xor_sync(0xffffffffu, a.e, o);
+        const float top = max_nan(a.r, b.r);
+        a.move_to(top, s2);
+        b.move_to(top, s2);
+        a.s += b.s; a.e += b.e;
     }
+    const uint32_t lane = tid & 31;
+    if (lane < R) { sh[0][tid / 32 * R + lane] = a.r; sh[1][tid / 32 * R + lane] = a.s; sh[2][tid / 32 * R + lane] = a.e; }
     __syncthreads();
     if (tid >= R || row >= m) return;
-    const float top = sh[0][tid], s = sh[1][tid];
+    float top = sh[0][tid];
+    for (uint32_t w = 1; w < 8; w++) top = max_nan(top, sh[0][w * R + tid]);
+    a.r = neg_inf(); a.s = a.e = 0.f;
+    for (uint32_t w = 0; w < 8; w++) {
+        Sums b;
+        b.r = sh[0][w * R + tid]; b.s = sh[1][w * R + tid]; b.e = sh[2][w * R + tid];
+        b.move_to(top, s2);
+        a.s += b.s; a.e += b.e;
+    }
+    const float s = a.s;
     const bool empty = top == neg_inf(), inside = (uint32_t)targets[row] < vocab;
     const float l = empty ? neg_inf() : logf(s);
     const bool asked = inside || ENT;
     stats[2 * (size_t)row] = asked ? top : 0.f;
     stats[2 * (size_t)row + 1] = asked ? l : 0.f;
     logp[row] = !inside ? 0.f : empty ? neg_inf() : scale * (target_logit[row] - top) - l;
-    if (ENT) entropy[row] = empty ? 0.f : l - kLn2 * (sh[2][tid] / s);
+    if (ENT) entropy[row] = empty ? 0.f : l - kLn2 * (a.e / s);
 }
 
-uint64_t tc_linear_logprobs_workspace(uint32_t m, uint32_t n) { return ((uint64_t)((n + 127) / 128) * 16 + 4) * m; }
+// parts of a row: at most one per 64 columns (tiles are 64 to 256 wide, those beyond 128 in two parts), and one more
+uint64_t tc_linear_logprobs_workspace(uint32_t m, uint32_t n) { return ((uint64_t)((n + 63) / 64 + 1) * 16 + 4) * m; }
 
 template <bool ENT> static int linear_logprobs(cudaStream_t s, const void *x, const void *table, const float *bias, const int32_t *targets, uint32_t m,
                                                uint32_t n, uint32_t k, int dtype, float scale, float *logp, float *stats, float *entropy,
@@ -1082,10 +1125,20 @@ template <bool ENT> static int linear_logprobs(cudaStream_t s, const void *x, co
     constexpr int kScore = ENT ? 2 : 1;
     const int dev = current_device(), sms = device_sm_count(dev);
     if (sms <= 0) return fail("%s: cannot read the SM count", who);
-    const uint32_t tiles_n = (n + kGBN - 1) / kGBN, n_parts = (n + 127) / 128;
-    float4 *parts = (float4 *)workspace;
-    float *target_logit = (float *)(parts + (size_t)n_parts * m);
-    GParams prm = {nullptr, bias, m, n, k, 0, tiles_n, is_bf16, SFB_ACT_NONE, 1, 1, nullptr, parts, target_logit, targets, scale * lg::kLog2e};
+    GParams prm = {nullptr, bias, m, n, k, 0, 0, is_bf16, SFB_ACT_NONE, 1, 1, nullptr, kGBN, (float4 *)workspace, nullptr, targets, scale * lg::kLog2e};
+    // Tiles as narrow as keeps the number of rounds (one row of 30522 logits: 147 tiles of 208 columns on 148 SMs, not 120 of 256)
+    uint32_t n_parts = 0;
+    auto tile = [&](uint32_t rows, uint32_t slots, uint32_t unit) {
+        prm.tiles_m = (m + rows - 1) / rows;
+        const uint64_t rounds = ((uint64_t)prm.tiles_m * ((n + kGBN - 1) / kGBN) + slots - 1) / slots;
+        uint32_t bn = 64;
+        while (bn < kGBN && (uint64_t)prm.tiles_m * ((n + bn - 1) / bn) > rounds * slots) bn += unit;
+        prm.bn = bn;
+        prm.tiles_n = (n + bn - 1) / bn;
+        n_parts = bn > 128 ? (prm.tiles_n - 1) * 2 + (n - (prm.tiles_n - 1) * bn > 128 ? 2 : 1) : prm.tiles_n;
+        prm.target_logit = (float *)(prm.score_parts + (size_t)n_parts * m);
+        return (uint64_t)prm.tiles_m * prm.tiles_n;
+    };
     CUtensorMap am, bm;
     if (make_map_2d(&am, x, m, k, is_bf16, kGBM)) return 1;
     static DeviceOnce once;
@@ -1097,26 +1150,24 @@ template <bool ENT> static int linear_logprobs(cudaStream_t s, const void *x, co
     }
     bool launched = false;
     if (kUsePairs && sms >= 2 && m > kGBM) {
-        if (make_map_2d(&bm, table, n, k, is_bf16, kGBN / 2)) return 1;
-        prm.tiles_m = (m + 255) / 256;
-        prm.band = tiles_n < kPBand ? tiles_n : kPBand;
-        const uint64_t tiles = (uint64_t)prm.tiles_m * tiles_n;
+        const uint64_t tiles = tile(256, (uint32_t)sms / 2, 32);
+        if (make_map_2d(&bm, table, n, k, is_bf16, prm.bn / 2)) return 1;
+        prm.band = prm.tiles_n < kPBand ? prm.tiles_n : kPBand;
         const uint32_t pairs = tiles < (uint64_t)(sms / 2) ? (uint32_t)tiles : (uint32_t)(sms / 2);
         launched = launch_overlapped(linear_tc_pair_kernel<kScore>, dim3(2 * pairs), dim3(320), kPSmem, s, am, bm, am, prm) == cudaSuccess;
         if (!launched) (void)cudaGetLastError();
     }
     if (!launched) {
-        if (make_map_2d(&bm, table, n, k, is_bf16, kGBN)) return 1;
-        prm.tiles_m = (m + kGBM - 1) / kGBM;
+        const uint64_t tiles = tile(kGBM, (uint32_t)sms, 16);
+        if (make_map_2d(&bm, table, n, k, is_bf16, prm.bn)) return 1;
         prm.band = 1;
-        const uint64_t tiles = (uint64_t)prm.tiles_m * tiles_n;
         launch_overlapped(linear_tc_kernel<kScore>, dim3(tiles < (uint64_t)sms ? (uint32_t)tiles : (uint32_t)sms), dim3(320), kGSmem, s, am, bm, prm);
     }
     if (check_launch(who)) return 1;
     // as many rows per CTA (up to 32, a warp's) as leave a CTA for every SM
     uint32_t R = 1;
     while (R < 32 && m / (2 * R) >= (uint32_t)sms) R *= 2;
-    launch_overlapped(score_join_kernel<ENT>, dim3((m + R - 1) / R + (missed ? 1 : 0)), dim3(256), 0, s, (const float4 *)parts, (const float *)target_logit,
+    launch_overlapped(score_join_kernel<ENT>, dim3((m + R - 1) / R + (missed ? 1 : 0)), dim3(256), 0, s, (const float4 *)prm.score_parts, (const float *)prm.target_logit,
                       targets, n_parts, m, n, R, scale, prm.s2, logp, stats, entropy, missed);
     return check_launch(who);
 }
