@@ -21,6 +21,7 @@ constexpr uint32_t kGBM = 128, kGBN = 256, kGBK = 64;
 constexpr uint32_t kGABytes = kGBM * kGBK * 2;           // 16 KB per 128 rows
 constexpr uint32_t kGBBytes = kGBK * kGBN * 2;           // 32 KB: four 64 x 64 boxes
 constexpr uint32_t kBiasBytes = 2 * 2 * 128 * 4;          // the epilogue's bias: [accumulator][column half][128]
+constexpr uint32_t kScoreBiasBytes = 8 * 128 * 4;        // scores: each epilogue warp's own, which it reads after it has given the accumulator back
 constexpr int kGStages = 4, kGBufs = 2;
 constexpr uint32_t kGStageBytes = kGABytes + kGBBytes;
 constexpr size_t kGSmem = 1024 + kGStages * kGStageBytes + kBiasBytes + 256;
@@ -40,8 +41,9 @@ struct GParams {
     uint32_t band;      // CTA-pair kernel: column tiles per band of the tile order (tile_coords)
     const void *resid;  // split kernel: [m, n] of x's type, added to the product (not out itself), or NULL
     // scores: what is kept of each row's 128 columns in place of the columns themselves
+    uint32_t box_m;            // rows of x that a copy brings
     uint32_t bn;               // columns of a tile (256 where the product itself is wanted)
-    float4 *score_parts;       // [part][m]: largest, sum of the powers, sum of them times their exponents; a part is a tile's 128 columns or less
+    float4 *score_parts;       // [part][m]: largest, sum of the powers, sum of them times their exponents; a part is half a tile's columns
     float *target_logit;       // [m]
     const int32_t *targets;    // [m]
     float s2;                  // scale * log2(e)
@@ -195,25 +197,24 @@ __device__ __forceinline__ void drain_rows_staged(const GParams &p, const CUtens
 // (ENT) the sum of those times their exponents go to the row's part for these 128 columns, the target's logit to its
 // place.  A thread has a whole row of the tile, so nothing is exchanged.  128 columns cost a thread about 128 x 6
 // instructions and the SM 2048 cycles of exponentials per 256-column tile; the tile's MMAs take 2048 cycles per 256 of k.
-template <bool ENT>
-__device__ __forceinline__ void score_rows(const GParams &p, uint32_t tcol, const float *bias, uint32_t row, uint32_t target, uint32_t tile_n, uint32_t chalf)
+template <bool ENT, typename Release>
+__device__ __forceinline__ void score_rows(const GParams &p, uint32_t tcol, const float *bias, uint32_t row, uint32_t target, uint32_t tile_n, uint32_t chalf,
+                                           Release release)
 {
     const bool row_ok = row < p.M;
-    const uint32_t n0 = tile_n * p.bn + chalf * 128, end = min(p.N, (tile_n + 1) * p.bn);      // this thread's columns: [n0, n0 + 128) before end
-    if (n0 >= end) return;
+    const uint32_t half = p.bn / 2, n0 = tile_n * p.bn + chalf * half, end = min(p.N, n0 + half);      // this thread's columns
+    if (n0 >= end || !__any_sync(0xffffffffu, row_ok)) { release(); return; }
     lg::Sums a;
     float mx = lg::neg_inf();
     const float gap = 40.f / p.s2;
-    uint32_t v[2][32];
-    TMEM_LD_32((v[0]), tcol);
-#pragma unroll
-    for (uint32_t c = 0; c < 4; c++) {
-        const uint32_t c0 = c * 32, col = n0 + c0;
-        if (col >= end) break;
+#pragma unroll 1
+    for (uint32_t c0 = 0; n0 + c0 < end; c0 += 32) {
+        const uint32_t col = n0 + c0;
+        uint32_t cur[32];
         __syncwarp();                        // the lanes parted over targets and references
+        TMEM_LD_32(cur, tcol + c0);
         tmem_wait_ld();
-        if (c + 1 < 4 && col + 32 < end) TMEM_LD_32((v[(c + 1) & 1]), tcol + c0 + 32);
-        uint32_t(&cur)[32] = v[c & 1];
+        if (col + 32 >= end) release();
         float x[32];
 #pragma unroll
         for (int j = 0; j < 32; j++) x[j] = __uint_as_float(cur[j]);
@@ -273,7 +274,7 @@ __device__ __forceinline__ void score_rows(const GParams &p, uint32_t tcol, cons
         }
     }
     a.move_to(mx, p.s2);
-    if (row_ok) p.score_parts[(size_t)(p.bn > 128 ? tile_n * 2 + chalf : tile_n) * p.M + row] = make_float4(mx, a.s, a.e, 0.f);
+    if (row_ok) p.score_parts[(size_t)(tile_n * 2 + chalf) * p.M + row] = make_float4(mx, a.s, a.e, 0.f);
 }
 
 // SCORE: 0 the product itself, 1 scores of its rows, 2 with the sum that the entropy takes
@@ -285,14 +286,14 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant
     uint8_t *smem = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     uint8_t *tiles = smem;                                   // stage s: A (16 KB) then B (32 KB)
     float *bias_s = (float *)(tiles + kGStages * kGStageBytes);
-    GShared *st = (GShared *)((uint8_t *)bias_s + kBiasBytes);
+    GShared *st = (GShared *)((uint8_t *)bias_s + (SCORE ? kScoreBiasBytes : kBiasBytes));
 
     const uint32_t warp = uniform_warp(), lane = threadIdx.x & 31;
     volatile uint32_t *abort_flag = &st->abort_flag;
     const uint32_t fmt = p.is_bf16 ? 1u : 0u;
     const uint32_t n_tiles = p.tiles_m * p.tiles_n;
     const uint32_t kblocks = (p.K + kGBK - 1) / kGBK;
-    const uint32_t bn = SCORE ? p.bn : kGBN;
+    const uint32_t bn = SCORE ? p.bn : kGBN, half = SCORE ? p.bn / 2 : 128;      // a tile's columns, an epilogue warp's
 
     if (threadIdx.x == 0) {
         prefetch_map(amap);
@@ -326,7 +327,7 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant
                     const uint32_t s = g % kGStages;
                     if (g >= kGStages && !mbar_wait(&st->empty[s], ((g / kGStages) - 1) & 1, abort_flag, 41)) { alive = false; break; }
                     const uint32_t base = smem_u32(tiles + s * kGStageBytes);
-                    mbar_expect_tx(&st->full[s], SCORE ? kGABytes + bn * (kGBK * 2) : kGStageBytes);   // boxes beyond the tensor arrive as zeros and still count
+                    mbar_expect_tx(&st->full[s], SCORE ? (p.box_m + bn) * (kGBK * 2) : kGStageBytes);   // boxes beyond the tensor arrive as zeros and still count
                     tma_load_2d(base, &amap, &st->full[s], (int32_t)(kb * kGBK), m0);
                     if (p.w_transposed) {
                         // 256 rows of w, 64 of k: one box
@@ -377,24 +378,30 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant
         uint32_t i = 0;
         auto bias_of = [&](uint32_t n0) { return SCORE ? fetch_bias_any(p, n0, lane) : fetch_bias(p, n0, lane); };
         auto target_of = [&](uint32_t t) { const uint32_t row = (t % p.tiles_m) * kGBM + r; return SCORE && row < p.M ? (uint32_t)p.targets[row] : 0xffffffffu; };
-        float4 next = bias_of((blockIdx.x / p.tiles_m) * bn + chalf * 128);
+        float4 next = bias_of((blockIdx.x / p.tiles_m) * bn + chalf * half);
         uint32_t next_target = target_of(blockIdx.x);
         for (uint32_t t = blockIdx.x; t < n_tiles; t += gridDim.x, i++) {
             const uint32_t buf = i % kGBufs;
-            const uint32_t n0 = (t / p.tiles_m) * bn + chalf * 128, target = next_target;
-            float *bias = bias_s + ((i & 1) * 2 + chalf) * 128;
+            const uint32_t n0 = (t / p.tiles_m) * bn + chalf * half, target = next_target;
+            float *bias = bias_s + (SCORE ? warp - 2 : (i & 1) * 2 + chalf) * 128;
             if (!mbar_wait_warp(&st->acc_full[buf], (i / kGBufs) & 1, abort_flag, 44)) break;
             *(float4 *)(bias + lane * 4) = next;
             __syncwarp();
             if (t + gridDim.x < n_tiles) {
-                next = bias_of(((t + gridDim.x) / p.tiles_m) * bn + chalf * 128);
+                next = bias_of(((t + gridDim.x) / p.tiles_m) * bn + chalf * half);
                 next_target = target_of(t + gridDim.x);
             }
             tcgen05_fence_after();
-            if (SCORE) score_rows<SCORE == 2>(p, tmem + buf * kGBN + chalf * 128 + lane_field, bias, (t % p.tiles_m) * kGBM + r, target, t / p.tiles_m, chalf);
-            else drain_rows(p, tmem + buf * kGBN + chalf * 128 + lane_field, bias, (t % p.tiles_m) * kGBM + r, n0);
-            tcgen05_fence_before();
-            mbar_arrive(&st->acc_empty[buf]);
+            auto release = [&]() {
+                tcgen05_fence_before();
+                mbar_arrive(&st->acc_empty[buf]);
+            };
+            if (SCORE) {
+                score_rows<SCORE == 2>(p, tmem + buf * kGBN + chalf * half + lane_field, bias, (t % p.tiles_m) * kGBM + r, target, t / p.tiles_m, chalf, release);
+            } else {
+                drain_rows(p, tmem + buf * kGBN + chalf * 128 + lane_field, bias, (t % p.tiles_m) * kGBM + r, n0);
+                release();
+            }
         }
     }
 
@@ -520,7 +527,7 @@ linear_tc_pair_kernel(const __grid_constant__ CUtensorMap amap, const __grid_con
     const uint32_t fmt = p.is_bf16 ? 1u : 0u;
     const uint32_t n_tiles = p.tiles_m * p.tiles_n;          // tiles of 256 x 256
     const uint32_t kblocks = (p.K + kGBK - 1) / kGBK;
-    const uint32_t bn = SCORE ? p.bn : kGBN;
+    const uint32_t bn = SCORE ? p.bn : kGBN, half = SCORE ? p.bn / 2 : 128;      // a tile's columns, an epilogue warp's
 
     if (threadIdx.x == 0) {
         prefetch_map(amap);
@@ -612,27 +619,33 @@ linear_tc_pair_kernel(const __grid_constant__ CUtensorMap amap, const __grid_con
         auto bias_of = [&](uint32_t n0) { return SCORE ? fetch_bias_any(p, n0, lane) : fetch_bias(p, n0, lane); };
         auto target_of = [&](uint32_t row) { return SCORE && row < p.M ? (uint32_t)p.targets[row] : 0xffffffffu; };
         const uint32_t r = rank * kGBM + quarter * 32 + lane;
-        float4 next = bias_of(tn * bn + chalf * 128);
+        float4 next = bias_of(tn * bn + chalf * half);
         uint32_t next_target = target_of(tm * 256 + r);
         for (uint32_t t = pair; t < n_tiles; t += pairs, i++) {
             const uint32_t buf = i & 1;
-            const uint32_t n0 = tn * bn + chalf * 128, tile_n = tn, target = next_target;
+            const uint32_t n0 = tn * bn + chalf * half, tile_n = tn, target = next_target;
             const uint32_t m0 = tm * 256 + rank * kGBM;
-            float *bias = bias_s + (buf * 2 + chalf) * 128;
+            float *bias = SCORE ? (float *)staging + (warp - 2) * 128 : bias_s + (buf * 2 + chalf) * 128;
             if (!mbar_wait_warp(&st->acc_full[buf], (i >> 1) & 1, abort_flag, 54)) break;
             *(float4 *)(bias + lane * 4) = next;
             __syncwarp();
             if (t + pairs < n_tiles) {
                 tile_coords(p, t + pairs, tm, tn);
-                next = bias_of(tn * bn + chalf * 128);
+                next = bias_of(tn * bn + chalf * half);
                 next_target = target_of(tm * 256 + r);
             }
             tcgen05_fence_after();
-            if (SCORE) score_rows<SCORE == 2>(p, tmem + buf * kGBN + chalf * 128 + lane_field, bias, m0 + quarter * 32 + lane, target, tile_n, chalf);
-            else drain_rows_staged(p, &omap, tmem + buf * kGBN + chalf * 128 + lane_field, staging + (warp - 2) * 4096, bias, m0 + quarter * 32, n0, lane);
-            tcgen05_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive_cluster(buf ? acc_empty0[1] : acc_empty0[0]);
+            auto release = [&]() {
+                tcgen05_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_cluster(buf ? acc_empty0[1] : acc_empty0[0]);
+            };
+            if (SCORE) {
+                score_rows<SCORE == 2>(p, tmem + buf * kGBN + chalf * half + lane_field, bias, m0 + quarter * 32 + lane, target, tile_n, chalf, release);
+            } else {
+                drain_rows_staged(p, &omap, tmem + buf * kGBN + chalf * 128 + lane_field, staging + (warp - 2) * 4096, bias, m0 + quarter * 32, n0, lane);
+                release();
+            }
         }
         if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");   // the last tile has left shared memory
     }
@@ -1068,14 +1081,24 @@ __global__ void __launch_bounds__(256) score_join_kernel(const float4 *parts, co
     Sums a;
     float mx = neg_inf();
     if (row < m) {
-        for (uint32_t i = tid / R; i < n_parts; i += groups) {
-            const float4 q = parts[(size_t)i * m + row];
-            Sums b;
-            b.r = q.x; b.s = q.y; b.e = q.z;
-            const float top = max_nan(mx, q.x);
+        for (uint32_t i0 = tid / R; i0 < n_parts; i0 += 8 * groups) {
+            float4 q[8];
+            float top = mx;
+#pragma unroll
+            for (uint32_t j = 0; j < 8; j++) {
+                const uint32_t i = i0 + j * groups;
+                q[j] = i < n_parts ? parts[(size_t)i * m + row] : make_float4(neg_inf(), 0.f, 0.f, 0.f);
+            }
+#pragma unroll
+            for (uint32_t j = 0; j < 8; j++) top = max_nan(top, q[j].x);
             a.move_to(top, s2);
-            b.move_to(top, s2);
-            a.s += b.s; a.e += b.e;
+#pragma unroll
+            for (uint32_t j = 0; j < 8; j++) {
+                Sums b;
+                b.r = q[j].x; b.s = q[j].y; b.e = q[j].z;
+                b.move_to(top, s2);
+                a.s += b.s; a.e += b.e;
+            }
             mx = top;
         }
     }
@@ -1112,8 +1135,8 @@ __global__ void __launch_bounds__(256) score_join_kernel(const float4 *parts, co
     if (ENT) entropy[row] = empty ? 0.f : l - kLn2 * (a.e / s);
 }
 
-// parts of a row: at most one per 64 columns (tiles are 64 to 256 wide, those beyond 128 in two parts), and one more
-uint64_t tc_linear_logprobs_workspace(uint32_t m, uint32_t n) { return ((uint64_t)((n + 63) / 64 + 1) * 16 + 4) * m; }
+// parts of a row: two per tile of 64 columns or more
+uint64_t tc_linear_logprobs_workspace(uint32_t m, uint32_t n) { return ((uint64_t)((n + 63) / 64) * 32 + 4) * m; }
 
 template <bool ENT> static int linear_logprobs(cudaStream_t s, const void *x, const void *table, const float *bias, const int32_t *targets, uint32_t m,
                                                uint32_t n, uint32_t k, int dtype, float scale, float *logp, float *stats, float *entropy,
@@ -1125,7 +1148,8 @@ template <bool ENT> static int linear_logprobs(cudaStream_t s, const void *x, co
     constexpr int kScore = ENT ? 2 : 1;
     const int dev = current_device(), sms = device_sm_count(dev);
     if (sms <= 0) return fail("%s: cannot read the SM count", who);
-    GParams prm = {nullptr, bias, m, n, k, 0, 0, is_bf16, SFB_ACT_NONE, 1, 1, nullptr, kGBN, (float4 *)workspace, nullptr, targets, scale * lg::kLog2e};
+    const uint32_t box_m = m < kGBM ? (m + 7) / 8 * 8 : kGBM;       // few rows: no more of a tile is copied than there is (the rest of it is never looked at)
+    GParams prm = {nullptr, bias, m, n, k, 0, 0, is_bf16, SFB_ACT_NONE, 1, 1, nullptr, box_m, kGBN, (float4 *)workspace, nullptr, targets, scale * lg::kLog2e};
     // Tiles as narrow as keeps the number of rounds (one row of 30522 logits: 147 tiles of 208 columns on 148 SMs, not 120 of 256)
     uint32_t n_parts = 0;
     auto tile = [&](uint32_t rows, uint32_t slots, uint32_t unit) {
@@ -1135,16 +1159,16 @@ template <bool ENT> static int linear_logprobs(cudaStream_t s, const void *x, co
         while (bn < kGBN && (uint64_t)prm.tiles_m * ((n + bn - 1) / bn) > rounds * slots) bn += unit;
         prm.bn = bn;
         prm.tiles_n = (n + bn - 1) / bn;
-        n_parts = bn > 128 ? (prm.tiles_n - 1) * 2 + (n - (prm.tiles_n - 1) * bn > 128 ? 2 : 1) : prm.tiles_n;
+        n_parts = (prm.tiles_n - 1) * 2 + (n - (prm.tiles_n - 1) * bn > bn / 2 ? 2 : 1);
         prm.target_logit = (float *)(prm.score_parts + (size_t)n_parts * m);
         return (uint64_t)prm.tiles_m * prm.tiles_n;
     };
     CUtensorMap am, bm;
-    if (make_map_2d(&am, x, m, k, is_bf16, kGBM)) return 1;
+    if (make_map_2d(&am, x, m, k, is_bf16, box_m)) return 1;
     static DeviceOnce once;
     if (!once.done(dev)) {
         if (cudaFuncSetAttribute(linear_tc_pair_kernel<kScore>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kPSmem) != cudaSuccess ||
-            cudaFuncSetAttribute(linear_tc_kernel<kScore>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kGSmem) != cudaSuccess)
+            cudaFuncSetAttribute(linear_tc_kernel<kScore>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(kGSmem + kScoreBiasBytes)) != cudaSuccess)
             return fail("%s: cannot reserve %zu bytes of shared memory", who, kPSmem);
         once.mark(dev);
     }
@@ -1161,12 +1185,12 @@ template <bool ENT> static int linear_logprobs(cudaStream_t s, const void *x, co
         const uint64_t tiles = tile(kGBM, (uint32_t)sms, 16);
         if (make_map_2d(&bm, table, n, k, is_bf16, prm.bn)) return 1;
         prm.band = 1;
-        launch_overlapped(linear_tc_kernel<kScore>, dim3(tiles < (uint64_t)sms ? (uint32_t)tiles : (uint32_t)sms), dim3(320), kGSmem, s, am, bm, prm);
+        launch_overlapped(linear_tc_kernel<kScore>, dim3(tiles < (uint64_t)sms ? (uint32_t)tiles : (uint32_t)sms), dim3(320), kGSmem + kScoreBiasBytes, s, am, bm, prm);
     }
     if (check_launch(who)) return 1;
-    // as many rows per CTA (up to 32, a warp's) as leave a CTA for every SM
+    // as many rows per CTA as leave a thread at most eight parts, which it asks for at once
     uint32_t R = 1;
-    while (R < 32 && m / (2 * R) >= (uint32_t)sms) R *= 2;
+    while (R < 32 && 2 * R < m && 2 * R * n_parts <= 2048) R *= 2;
     launch_overlapped(score_join_kernel<ENT>, dim3((m + R - 1) / R + (missed ? 1 : 0)), dim3(256), 0, s, (const float4 *)prm.score_parts, (const float *)prm.target_logit,
                       targets, n_parts, m, n, R, scale, prm.s2, logp, stats, entropy, missed);
     return check_launch(who);
