@@ -584,12 +584,33 @@ inline int64_t vocab_or_width(PyObject *o, const LogitRows &x)
 inline void require_cuda(const at::Tensor &t) { require(t.is_cuda(), "expected a tensor on a CUDA device"); }
 // The calls below run on the device of their tensors, on its current stream, whichever device is the current one.
 inline sfb_stream_t stream_of(const at::Tensor &t) { return (sfb_stream_t)c10::cuda::getCurrentCUDAStream(t.device().index()).stream(); }
-inline at::Tensor rows_like(const LogitRows &x, int64_t last, at::ScalarType type)
-{
-    std::vector<int64_t> size(x.lead().begin(), x.lead().end());
-    if (last) size.push_back(last);
-    return empty(size, type, x.t);
-}
+// The results of a call, [...] or [..., last] of four-byte elements.  An allocation takes about a microsecond of host time, and a
+// call for one row has six results: together at most 64 KB they share one, each at 64 bytes of its own.
+struct Results {
+    const LogitRows &x;
+    int64_t room, used = 0;
+    at::Tensor shared;
+    Results(const LogitRows &rows, std::initializer_list<int64_t> elements) : x(rows), room(0)
+    {
+        for (int64_t n : elements) room += (n * 4 + 63) / 64 * 64;
+        if (room && room <= (64 << 10)) shared = empty({room}, at::kByte, x.t);
+    }
+    at::Tensor take(at::IntArrayRef size, at::ScalarType type)
+    {
+        if (!shared.defined()) return empty(size, type, x.t);
+        at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(shared.storage()), shared.key_set(), c10::scalarTypeToTypeMeta(type));
+        t.unsafeGetTensorImpl()->set_storage_offset(used / 4);
+        t.unsafeGetTensorImpl()->set_sizes_contiguous(size);
+        used += (t.numel() * 4 + 63) / 64 * 64;
+        return t;
+    }
+    at::Tensor rows(int64_t last, at::ScalarType type)
+    {
+        std::vector<int64_t> size(x.lead().begin(), x.lead().end());
+        if (last) size.push_back(last);
+        return take(size, type);
+    }
+};
 // the gradient's tensor: laid out as the logits, or the caller's
 at::Tensor grad_out(PyObject *out, const LogitRows &x)
 {
@@ -626,10 +647,11 @@ FUNCTION(py_token_logprobs, 6)
     const int32_t *targets = ptr_of<int32_t>(a[1], x, at::kInt, 0, bad_targets);
     require_cuda(x.t);
     const c10::cuda::CUDAGuard on(x.t.device());
-    at::Tensor stats = rows_like(x, 2, at::kFloat), missed = empty({1}, at::kInt, x.t), logp, entropy, top_logp, top_ids;
-    if (a[1] != Py_None) logp = rows_like(x, 0, at::kFloat);
-    if (ent) entropy = rows_like(x, 0, at::kFloat);
-    if (k) { top_logp = rows_like(x, k, at::kFloat); top_ids = rows_like(x, k, at::kInt); }
+    Results res(x, {x.rows, 2 * x.rows, x.rows, k * x.rows, k * x.rows, 1});
+    at::Tensor stats = res.rows(2, at::kFloat), missed = res.take({1}, at::kInt), logp, entropy, top_logp, top_ids;
+    if (a[1] != Py_None) logp = res.rows(0, at::kFloat);
+    if (ent) entropy = res.rows(0, at::kFloat);
+    if (k) { top_logp = res.rows(k, at::kFloat); top_ids = res.rows(k, at::kInt); }
     auto p = [](const at::Tensor &o) { return o.defined() ? (float *)ptr(o) : nullptr; };
     call(L.sfb_token_logprobs, stream_of(x.t), ptr(x.t), (uint64_t)x.pitch, targets, (uint32_t)x.rows, (uint32_t)vocab, t, scale, p(logp), p(stats),
          p(entropy), p(top_logp), k ? (int32_t *)ptr(top_ids) : nullptr, (uint32_t)k, (uint32_t *)ptr(missed));
@@ -681,7 +703,8 @@ FUNCTION(py_distill_topk, 6)
     const float *teacher = (float *)ptr(beside(a[2], x, at::kFloat, k, bad_lists));
     require_cuda(x.t);
     const c10::cuda::CUDAGuard on(x.t.device());
-    at::Tensor loss = rows_like(x, 0, at::kFloat), stats = rows_like(x, tail ? 3 : 2, at::kFloat), missed = empty({1}, at::kInt, x.t);
+    Results res(x, {x.rows, 3 * x.rows, 1});
+    at::Tensor loss = res.rows(0, at::kFloat), stats = res.rows(tail ? 3 : 2, at::kFloat), missed = res.take({1}, at::kInt);
     call(L.sfb_distill_topk, stream_of(x.t), ptr(x.t), (uint64_t)x.pitch, ids, teacher, (uint32_t)x.rows, (uint32_t)vocab, (uint32_t)k, t, scale,
          (int)tail, (float *)ptr(loss), (float *)ptr(stats), (uint32_t *)ptr(missed));
     Ref l(wrap(loss)), s(wrap(stats)), n(wrap(missed));
@@ -731,8 +754,9 @@ FUNCTION(py_linear_logprobs, 7)
     }
     require_cuda(x.t);
     const c10::cuda::CUDAGuard on(x.t.device());
-    at::Tensor logp = rows_like(x, 0, at::kFloat), stats = rows_like(x, 2, at::kFloat), missed = empty({1}, at::kInt, x.t), entropy;
-    if (ent) entropy = rows_like(x, 0, at::kFloat);
+    Results res(x, {x.rows, 2 * x.rows, x.rows, 1});
+    at::Tensor logp = res.rows(0, at::kFloat), stats = res.rows(2, at::kFloat), missed = res.take({1}, at::kInt), entropy;
+    if (ent) entropy = res.rows(0, at::kFloat);
     at::Tensor ws = empty({(int64_t)L.sfb_linear_logprobs_workspace((uint32_t)x.rows, (uint32_t)vocab)}, at::kByte, x.t);
     call(L.sfb_linear_logprobs, stream_of(x.t), ptr(x.t), ptr(table), bias, targets, (uint32_t)x.rows, (uint32_t)vocab, (uint32_t)x.width, t, scale,
          (float *)ptr(logp), (float *)ptr(stats), ent ? (float *)ptr(entropy) : nullptr, (uint32_t *)ptr(missed), ptr(ws));
