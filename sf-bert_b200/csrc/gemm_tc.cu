@@ -1060,7 +1060,7 @@ int tc_linear(cudaStream_t s, void *out, const void *x, const void *w, const flo
 // A row's parts joined: R rows per CTA, its other threads spread over the parts.
 template <bool ENT>
 __global__ void __launch_bounds__(256) score_join_kernel(const float4 *parts, const float *target_logit, const int32_t *targets, uint32_t n_parts,
-                                                         uint32_t m, uint32_t vocab, uint32_t R, float scale, float s2, float *logp, float *stats,
+                                                         uint32_t m, uint32_t n_targets, uint32_t vocab, uint32_t R, float scale, float s2, float *logp, float *stats,
                                                          float *entropy, uint32_t *missed)
 {
     using namespace lg;
@@ -1070,7 +1070,7 @@ __global__ void __launch_bounds__(256) score_join_kernel(const float4 *parts, co
     grid_launch_dependents();
     if (blockIdx.x * R >= m) {                   // the CTA behind the rows' counts the targets that are none
         uint32_t bad = 0;
-        for (uint32_t i = tid; i < m; i += 256) bad += (uint32_t)targets[i] >= vocab;
+        for (uint32_t i = tid; i < n_targets; i += 256) bad += (uint32_t)targets[i] >= vocab;
         bad = __reduce_add_sync(0xffffffffu, bad);
         if (tid % 32 == 0) ((uint32_t *)sh)[tid / 32] = bad;
         __syncthreads();
@@ -1135,11 +1135,18 @@ __global__ void __launch_bounds__(256) score_join_kernel(const float4 *parts, co
     if (ENT) entropy[row] = empty ? 0.f : l - kLn2 * (a.e / s);
 }
 
-// parts of a row: two per tile of 64 columns or more
-uint64_t tc_linear_logprobs_workspace(uint32_t m, uint32_t n) { return ((uint64_t)((n + 63) / 64) * 32 + 4) * m; }
+// Rows go through the workspace kScoreRows at a time; a row takes two parts per tile, of 256 columns beyond kNarrowRows rows and of
+// 64 at least up to there.
+constexpr uint32_t kScoreRows = 32768, kNarrowRows = 1024;
+uint64_t tc_linear_logprobs_workspace(uint32_t m, uint32_t n)
+{
+    const uint32_t narrow = m < kNarrowRows ? m : kNarrowRows, wide = m < kScoreRows ? m : kScoreRows;
+    const uint64_t a = ((uint64_t)((n + 63) / 64) * 32 + 4) * narrow, b = ((uint64_t)((n + 255) / 256) * 32 + 4) * wide;
+    return a > b ? a : b;
+}
 
 template <bool ENT> static int linear_logprobs(cudaStream_t s, const void *x, const void *table, const float *bias, const int32_t *targets, uint32_t m,
-                                               uint32_t n, uint32_t k, int dtype, float scale, float *logp, float *stats, float *entropy,
+                                               uint32_t n_targets, uint32_t n, uint32_t k, int dtype, float scale, float *logp, float *stats, float *entropy,
                                                uint32_t *missed, void *workspace)
 {
     using namespace tc;
@@ -1155,7 +1162,7 @@ template <bool ENT> static int linear_logprobs(cudaStream_t s, const void *x, co
     auto tile = [&](uint32_t rows, uint32_t slots, uint32_t unit) {
         prm.tiles_m = (m + rows - 1) / rows;
         const uint64_t rounds = ((uint64_t)prm.tiles_m * ((n + kGBN - 1) / kGBN) + slots - 1) / slots;
-        uint32_t bn = 64;
+        uint32_t bn = m <= kNarrowRows ? 64 : kGBN;
         while (bn < kGBN && (uint64_t)prm.tiles_m * ((n + bn - 1) / bn) > rounds * slots) bn += unit;
         prm.bn = bn;
         prm.tiles_n = (n + bn - 1) / bn;
@@ -1192,15 +1199,22 @@ template <bool ENT> static int linear_logprobs(cudaStream_t s, const void *x, co
     uint32_t R = 1;
     while (R < 32 && 2 * R < m && 2 * R * n_parts <= 2048) R *= 2;
     launch_overlapped(score_join_kernel<ENT>, dim3((m + R - 1) / R + (missed ? 1 : 0)), dim3(256), 0, s, (const float4 *)prm.score_parts, (const float *)prm.target_logit,
-                      targets, n_parts, m, n, R, scale, prm.s2, logp, stats, entropy, missed);
+                      targets, n_parts, m, n_targets, n, R, scale, prm.s2, logp, stats, entropy, missed);
     return check_launch(who);
 }
 
 int tc_linear_logprobs(cudaStream_t s, const void *x, const void *table, const float *bias, const int32_t *targets, uint32_t m, uint32_t n,
                        uint32_t k, int dtype, float scale, float *logp, float *stats, float *entropy, uint32_t *missed, void *workspace)
 {
-    return entropy ? linear_logprobs<true>(s, x, table, bias, targets, m, n, k, dtype, scale, logp, stats, entropy, missed, workspace)
-                   : linear_logprobs<false>(s, x, table, bias, targets, m, n, k, dtype, scale, logp, stats, entropy, missed, workspace);
+    for (uint32_t r = 0; r < m; r += kScoreRows) {
+        const uint32_t rows = m - r < kScoreRows ? m - r : kScoreRows;
+        const void *xr = (const char *)x + (size_t)r * k * 2;
+        uint32_t *count = r ? nullptr : missed;              // the first rows' call counts all targets
+        const int rc = entropy ? linear_logprobs<true>(s, xr, table, bias, targets + r, rows, m, n, k, dtype, scale, logp + r, stats + 2 * (size_t)r, entropy + r, count, workspace)
+                               : linear_logprobs<false>(s, xr, table, bias, targets + r, rows, m, n, k, dtype, scale, logp + r, stats + 2 * (size_t)r, nullptr, count, workspace);
+        if (rc) return rc;
+    }
+    return 0;
 }
 
 int tc_status_clear_gemm()

@@ -173,9 +173,64 @@ __device__ __forceinline__ uint32_t block_sum(uint32_t v, uint32_t *part)
     return v;
 }
 
-// The candidates when too many values reach the bound (values tie, or most of the large ones went to a few threads): the bound is
-// bisected over the values and their indices, a pass over the row (by now in L2) for each step.  One CTA, the whole row; the
-// candidates are then sh->cnt from the first place on.
+// The candidates when too many values reach the bound, by one CTA from the whole row (by now in L2); they are then sh->cnt from the
+// first place on.
+// Mostly it is one value that many have: a constant row, or one whose banned tokens hold the type's lowest value and too few
+// others are left.  Then what is above it is collected, and of the ties the first ones, which are the ones that count: a pass or two.
+__device__ __forceinline__ void push_candidate(TopShared *sh, float v, uint32_t index)
+{
+    const uint32_t at = atomicAdd(&sh->cnt, 1u);
+    if (at < kCap) sh->cand[at] = rank_key(v, index);
+}
+template <int DT> __device__ __noinline__ bool collect_ties(const Row<DT> row, uint32_t k, TopShared *sh)
+{
+    constexpr uint32_t E = Win<DT>::kElems;
+    const uint32_t windows = row.windows(), tau = sh->tau, top = tau | 0xffu;       // the bound is 24 bits of a value
+    uint32_t above = 0, least = 0xffffffffu, most = 0;
+    for (uint32_t w = threadIdx.x; w < windows; w += blockDim.x) {
+        float v[E];
+        unpack<DT>(load_window(row, w), v);
+#pragma unroll
+        for (uint32_t j = 0; j < E; j++) {
+            const uint32_t o = ordered(v[j]);
+            if (!(v[j] > neg_inf()) || o < tau) continue;
+            above += o > top;
+            if (o <= top) { least = min(least, o); most = max(most, o); }
+        }
+    }
+    above = block_sum(above, sh->part);
+    __syncthreads();
+    if (threadIdx.x == 0) { sh->cnt = 0; sh->part[0] = 0xffffffffu; sh->part[1] = 0; }
+    __syncthreads();
+    atomicMin(&sh->part[0], least);
+    atomicMax(&sh->part[1], most);
+    __syncthreads();
+    least = sh->part[0];
+    if (above >= k || least != sh->part[1]) return false;
+    for (uint32_t w = threadIdx.x; w < windows && above; w += blockDim.x) {
+        float v[E];
+        unpack<DT>(load_window(row, w), v);
+#pragma unroll
+        for (uint32_t j = 0; j < E; j++)
+            if (v[j] > neg_inf() && ordered(v[j]) > top) push_candidate(sh, v[j], w * E + j - row.head);
+    }
+    for (uint32_t w0 = 0; w0 < windows; w0 += 64) {                // at most 64 windows' ties beyond those that are needed
+        if (threadIdx.x < 64 && w0 + threadIdx.x < windows) {
+            float v[E];
+            unpack<DT>(load_window(row, w0 + threadIdx.x), v);
+#pragma unroll
+            for (uint32_t j = 0; j < E; j++)
+                if (v[j] > neg_inf() && ordered(v[j]) == least) push_candidate(sh, v[j], (w0 + threadIdx.x) * E + j - row.head);
+        }
+        __syncthreads();
+        const bool enough = sh->cnt >= k;
+        __syncthreads();
+        if (enough) break;
+    }
+    return true;
+}
+// Otherwise (most of the large values went to a few threads) the bound is bisected over the values and their indices, a pass for each
+// step.
 template <int DT> __device__ __noinline__ void bisect_candidates(const Row<DT> row, uint32_t k, TopShared *sh)
 {
     unsigned long long lo = (unsigned long long)sh->tau << 32, hi = ~0ull, x = lo;      // at least k reach lo (or all there are), fewer than k hi
@@ -558,7 +613,7 @@ __global__ void __launch_bounds__(kThreads, 4) row_stats_kernel(const StatParams
     } else {
         __syncthreads();
     }
-    if (top_s->cnt > kCap) bisect_candidates<DT>(row, p.k, top_s);
+    if (top_s->cnt > kCap && !collect_ties<DT>(row, p.k, top_s)) bisect_candidates<DT>(row, p.k, top_s);
     const uint32_t total = top_s->cnt;
     int32_t *out_ids = p.top_ids + (size_t)r * p.k;
     for (uint32_t i = tid; i < total; i += T) {
@@ -804,9 +859,10 @@ template <int DT, bool ENT, bool TOP, int KD> static int launch_stats(cudaStream
     const int dev = current_device(), sms = device_sm_count(dev);
     SFB_REQUIRE(sms > 0, "%s: cannot query the device", who);
     const uint32_t windows = p.vocab / Win<DT>::kElems + 2;      // at most, wherever a row starts
-    // What a row's end costs is paid by each of its warps, so many rows have four of them each (4096 rows of 30522 bf16: 47 us,
-    // with eight 50), few rows eight (257 of 50021 fp32: 19 us, with four 25).
-    const uint32_t T = windows > 512 && (p.rows < (uint32_t)sms * 8 || (TOP && p.k > 32)) ? 256 : windows > 256 || TOP || KD ? 128 : 64;
+    // What a row's end costs is paid by each of its warps, so many rows have four of them each (4096 rows of 30522 bf16: 44 us, with
+    // eight 50), few rows eight (257 of 50021 fp32: 19 us, with four 25), and so have long rows with alternatives, whose bound is the
+    // tighter the more threads it comes from (4096 rows of 100003 bf16, 20 alternatives: 162 us, with four 180).
+    const uint32_t T = windows > 512 && (p.rows < (uint32_t)sms * 8 || (TOP && (p.k > 32 || windows > 8192))) ? 256 : windows > 256 || TOP || KD ? 128 : 64;
     uint32_t C = 1;
     // CTAs per row: as many as there are SMs without one, and a few for every SM as long as each has two groups of windows
     while (C < kMaxCluster && windows > C * T * 2 && (!TOP || C * p.k <= 80)) {

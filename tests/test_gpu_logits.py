@@ -119,6 +119,25 @@ def test_values_that_are_not_ordinary(sfb, dtype, rows):
             assert bool(top_logp[r].isnan().all()) == bad and bool((top_ids[r] == -1).all()) == bad
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("rows", [1, 30, 1500])
+def test_ties_at_the_bound(sfb, rows, dtype):
+    """More equal values than there are places for candidates, with more, fewer and no larger ones above them."""
+    vocab = 20001
+    for n, (value, larger) in enumerate([(0.0, 0), (1.5, 5), (-2.0, 19), (-2.0, 20), (torch.finfo(TYPES[dtype]).min, 3)]):
+        x = torch.full((rows, vocab + 7), value, device="cuda", dtype=TYPES[dtype])
+        at = torch.randint(0, vocab, (rows, max(larger, 1)), device="cuda", generator=gen(n))
+        if larger:
+            x.scatter_(1, at, 3.0 + torch.arange(larger, device="cuda").to(x.dtype).expand(rows, -1))
+        x[0, :500] = -INF
+        x[-1, vocab - 30:] = -INF
+        some = [0, rows // 2, rows - 1]
+        _, stats, _, top_logp, top_ids, _ = sfb.token_logprobs(x, vocab=vocab, top_k=20)
+        want = R.token_logprobs(x[some], None, vocab, 1.0, 20)
+        assert torch.equal(top_ids[some].long(), want["top_ids"])
+        same(top_logp[some], want["top_logp"], R.bounds(vocab) + 2.0 ** -22 * want["top_logp"].abs(), "top_logp")
+
+
 @pytest.mark.parametrize("rows", [2, 500])
 def test_alternatives_that_sit_with_few_threads(sfb, rows):
     """Large values at one place of every 2048 elements: a thread or two hold most of them, and its neighbours' bound is far below."""
@@ -440,6 +459,20 @@ def test_linear_logprobs(sfb, m, vocab, rows, k, dtype):
             assert ent is None
         again = sfb.linear_logprobs(x, table, t, bias=bias, vocab=vocab, scale=scale, entropy=entropy)
         assert torch.equal(logp, again[0]) and torch.equal(stats, again[1])
+
+
+def test_linear_logprobs_of_many_rows(sfb):
+    """More rows than go through the workspace at a time."""
+    m, vocab, k = 70001, 300, 16
+    g = gen(5)
+    x = torch.randn(m, k, device="cuda", generator=g).to(torch.bfloat16)
+    table = torch.randn(vocab, k, device="cuda", generator=g).to(torch.bfloat16)
+    t = torch.randint(-1, vocab, (m,), device="cuda", generator=g, dtype=torch.int32)
+    logp, stats, ent, missed = sfb.linear_logprobs(x, table, t, entropy=True)
+    want = R.token_logprobs(x.double() @ table.double().t(), t, vocab, 1.0)
+    same(logp, want["logp"], 5e-5, "logp")                               # 16 products of at most 20: off by 2^-22 * 5 * 200 at most in a logit
+    same(ent, want["entropy"], 5e-4, "entropy")
+    assert int(missed) == want["missed"]
 
 
 def test_linear_logprobs_of_what_is_not_finite(sfb):
