@@ -194,9 +194,11 @@ __device__ __forceinline__ void drain_rows_staged(const GParams &p, const CUtens
 }
 
 // The same share of an accumulator as logits that are never stored: the largest, the sum of 2^(s2 (x - r)) beside it and
-// (ENT) the sum of those times their exponents go to the row's part for these 128 columns, the target's logit to its
-// place.  A thread has a whole row of the tile, so nothing is exchanged.  128 columns cost a thread about 128 x 6
-// instructions and the SM 2048 cycles of exponentials per 256-column tile; the tile's MMAs take 2048 cycles per 256 of k.
+// (ENT) the sum of those times their exponents go to the row's part for this half of the tile's columns, the target's logit to its
+// place.  A thread has a whole row of the tile, so nothing is exchanged.  The loop is short on purpose: unrolled, with the next 32
+// columns on their way, it ran out of the instruction cache (a tile of 256 columns 5900 cycles, now 5400; its MMAs take 6100 at
+// k = 768, so the scores are bound by the product from there on, by this loop below).  4096 x 30522 x 768: 121 us by itself with the
+// tensor pipe 79 % busy, 150 under the power cap, and 5 for the join.
 template <bool ENT, typename Release>
 __device__ __forceinline__ void score_rows(const GParams &p, uint32_t tcol, const float *bias, uint32_t row, uint32_t target, uint32_t tile_n, uint32_t chalf,
                                            Release release)

@@ -355,6 +355,13 @@ template <int KD> __device__ __forceinline__ void finish_lists(const StatParams 
 
 // A row's statistics, and what is made of them.  One CTA per row, or a cluster of CTAs where there are few rows: each
 // takes every C-th piece, and CTA 0 joins the parts.  KD: 0 tokens, 1 lists, 2 lists with the remainder as one more class.
+// Many rows are bound by the pass: 9 instructions and an exponential per element with entropy and alternatives, the issue slots
+// 72 % and the exponential unit 66 % busy beside 5.2 TB/s from memory (2048 rows of 131072 bf16, 103 us).  8192 such rows take 385 us,
+// 4096 of 30522 (without entropy) 44, 86 % of what a copy's rate allows both.  Fewer rows are bound by what comes one after another:
+// launch, the first loads, the join of a cluster's CTAs over their barrier (about 1000 cycles), and for alternatives their bound, the
+// second look and the ranks: one row of 30522 bf16 takes 3.1 us, with 20 alternatives 5.5, 64 rows of 100003 fp16 8.2.
+// Rows streamed through a ring of bulk copies by CTAs that stay were built, too: the loads then never pause, but
+// the warps that add up waited at every row's end for the one that finishes it, and the same rows took 59 us instead of 44.
 template <int DT, bool ENT, bool TOP, int KD>
 __global__ void __launch_bounds__(kThreads, 4) row_stats_kernel(const StatParams p)
 {
@@ -668,6 +675,9 @@ template <int DT> __device__ __forceinline__ uint4 load_shifted(const void *x, u
     return make_uint4(v[0], v[1], v[2], v[3]);
 }
 
+// A row (or a part of it) per CTA, a round of kG windows per thread at a time: loaded, turned into the gradient and stored.  Bound by
+// memory: 8192 rows of 30522 bf16 158 us, 97 % of a copy's rate; lists and hard labels add a prologue to each row (4096 rows:
+// 100 us, 77 %).
 // dx = p (c0 + c1 t) with t the base-2 logarithm of p, plus the given target's share (KD 0, ENT: c1 is not 0);
 // dx = c0 2^t + c2 2^t2, what is listed made again by itself (KD 1; HARD 1: c2 is not 0).  HARD 2: at temperature 2 the
 // second power, the softmax's at temperature 1, is the first one's square times a constant of the row (which goes to c2), and an
