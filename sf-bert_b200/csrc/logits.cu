@@ -676,14 +676,14 @@ template <int DT> __device__ __forceinline__ uint4 load_shifted(const void *x, u
 }
 
 // A row (or a part of it) per CTA, a round of kG windows per thread at a time: loaded, turned into the gradient and stored.  Bound by
-// memory: 8192 rows of 30522 bf16 158 us, 97 % of a copy's rate; lists and hard labels add a prologue to each row (4096 rows:
-// 100 us, 77 %).
+// memory: 8192 rows of 30522 bf16 157 us, 97 % of a copy's rate; lists and hard labels add a prologue to each row (4096 rows:
+// 93 us, 82 %).
 // dx = p (c0 + c1 t) with t the base-2 logarithm of p, plus the given target's share (KD 0, ENT: c1 is not 0);
 // dx = c0 2^t + c2 2^t2, what is listed made again by itself (KD 1; HARD 1: c2 is not 0).  HARD 2: at temperature 2 the
 // second power, the softmax's at temperature 1, is the first one's square times a constant of the row (which goes to c2), and an
 // exponential per element less: 4096 rows of 30522 bf16 with lists of 64, 107 -> 100 us.
 template <int DT, bool ENT, bool KD, int HARD, bool SAME>
-__global__ void __launch_bounds__(kThreads, 5) row_grad_kernel(const GradParams p)
+__global__ void __launch_bounds__(kThreads, KD ? 5 : 6) row_grad_kernel(const GradParams p)
 {
     __shared__ __align__(16) int32_t l_id[KD ? kMaxList : 4];
     __shared__ __align__(16) float l_q[KD ? kMaxList : 4];
@@ -706,15 +706,17 @@ __global__ void __launch_bounds__(kThreads, 5) row_grad_kernel(const GradParams 
     const float *st = p.stats + (KD && p.tail ? 3 : 2) * (size_t)r;
     const float m = st[0];
     const bool zero = m == neg_inf() || (kMaySkip && target < 0);       // no token is left (every probability is 0), or nothing is asked for
-    auto load = [&](uint32_t w) { return SAME ? load_window<DT, true>(row, w) : load_shifted<DT>(x, orow.head, p.vocab, w); };
+    // the windows [a_begin, a_end) are whole ones of x and out (none if theirs start at different places); the few others come after them
+    const uint32_t a_begin = SAME ? max(w_begin, row.first_whole()) : w_begin, a_end = SAME ? max(a_begin, min(w_end, row.first_whole() + row.whole_count())) : w_begin;
+    const uint32_t rounds = (a_end - a_begin + kG * T - 1) / (kG * T), first_round = rounds ? r % rounds : 0;
     uint4 v[kG];
-    auto load_round = [&](uint32_t w0) {
+    auto load_round = [&](uint32_t round) {
+        const uint32_t w0 = a_begin + round * (kG * T) + tid;
 #pragma unroll
         for (int u = 0; u < kG; u++)
-            if (w0 + u * T < w_end) v[u] = load(w0 + u * T);
+            if (w0 + u * T < a_end) v[u] = __ldcs(row.base + w0 + u * T);
     };
-    const uint32_t first_round = w_end > w_begin ? r % ((w_end - w_begin + kG * T - 1) / (kG * T)) : 0;
-    if (!zero) load_round(w_begin + first_round * (kG * T) + tid);
+    if (!zero && rounds) load_round(first_round);
 
     float c0, c1 = 0.f, c2 = 0.f, l2, l2b = 0.f, target_share = 0.f;
     int32_t id = -1;                                          // KD: this thread's entry of the list
@@ -782,57 +784,74 @@ __global__ void __launch_bounds__(kThreads, 5) row_grad_kernel(const GradParams 
     // HARD 2: 2^t2 = (2^t)^2 * 2^(2 l2 - l2b)
     const float c2s = HARD == 2 ? c2 * ex2(fmaf(2.f, l2, -l2b)) : c2;
     const Pair log2e = pair(kLog2e, kLog2e), minus_lb = pair(-l2b, -l2b), k2 = pair(c2s, c2s);
-    // Rows start at different rounds: with all of them at the same column, reads and writes crowded the same memory channels
-    // (8192 rows of 30522 bf16: 195 us so, 158 now).
-    const uint32_t rounds = (w_end - w_begin + kG * T - 1) / (kG * T);
-    for (uint32_t i = 0, round = first_round; i < rounds; i++) {
-        const uint32_t w0 = w_begin + round * (kG * T) + tid;
-        round = round + 1 == rounds ? 0 : round + 1;
+    auto turn = [&](float (&y)[E]) {
 #pragma unroll
-        for (int u = 0; u < kG; u++) {
-            const uint32_t w = w0 + u * T;
-            if (w >= w_end) break;
-            float y[E];
-            if (zero) {
-#pragma unroll
-                for (uint32_t j = 0; j < E; j++) y[j] = 0.f;
-            } else {
-                unpack<DT>(v[u], y);
-#pragma unroll
-                for (uint32_t j = 0; j < E; j += 2) {
-                    const Pair d = add2(pair(y[j], y[j + 1]), minus_m), t = fma2(s2, d, minus_l);
-                    float t0, t1;
-                    halves(t, t0, t1);
-                    const Pair e = pair(ex2(t0), ex2(t1));
-                    Pair g = mul2(e, ENT ? fma2(k1, pair(fmaxf(t0, kFar), fmaxf(t1, kFar)), k0) : k0);
-                    if (HARD == 1) {
-                        halves(fma2(log2e, d, minus_lb), t0, t1);
-                        g = fma2(k2, pair(ex2(t0), ex2(t1)), g);
-                    } else if (HARD == 2) {
-                        g = fma2(mul2(k2, e), e, g);
-                    }
-                    halves(g, y[j], y[j + 1]);
-                }
+        for (uint32_t j = 0; j < E; j += 2) {
+            const Pair d = add2(pair(y[j], y[j + 1]), minus_m), t = fma2(s2, d, minus_l);
+            float t0, t1;
+            halves(t, t0, t1);
+            const Pair e = pair(ex2(t0), ex2(t1));
+            Pair g = mul2(e, ENT ? fma2(k1, pair(fmaxf(t0, kFar), fmaxf(t1, kFar)), k0) : k0);
+            if (HARD == 1) {
+                halves(fma2(log2e, d, minus_lb), t0, t1);
+                g = fma2(k2, pair(ex2(t0), ex2(t1)), g);
+            } else if (HARD == 2) {
+                g = fma2(mul2(k2, e), e, g);
             }
-            if (w == w_target) {
-                const uint32_t at = ((uint32_t)target + orow.head) % E;
-#pragma unroll
-                for (uint32_t j = 0; j < E; j++)
-                    if (j == at) y[j] += target_share;
-            }
-            if (orow.whole(w)) {
-                __stcs((uint4 *)orow.base + w, pack<DT>(y));
-            } else {
-#pragma unroll
-                for (uint32_t j = 0; j < E; j++) {
-                    const uint32_t pos = w * E + j;
-                    if (pos >= orow.head && pos < orow.end) store_element<DT>(out, pos - orow.head, y[j]);
-                }
-            }
+            halves(g, y[j], y[j + 1]);
         }
-        // all of a round's loads after all of the last one's stores: taking turns window by window cost 20 % of the bandwidth
-        asm volatile("" ::: "memory");
-        if (!zero && i + 1 < rounds) load_round(w_begin + round * (kG * T) + tid);
+    };
+    auto add_target = [&](float (&y)[E]) {
+        const uint32_t at = ((uint32_t)target + orow.head) % E;
+#pragma unroll
+        for (uint32_t j = 0; j < E; j++)
+            if (j == at) y[j] += target_share;
+    };
+    if (zero) {
+        for (uint32_t w = a_begin + tid; w < a_end; w += T) {
+            float y[E] = {};
+            if (w == w_target) add_target(y);
+            __stcs((uint4 *)orow.base + w, pack<DT>(y));
+        }
+    } else {
+        // Rows start at different rounds: with all of them at the same column, reads and writes crowded the same memory channels
+        // (8192 rows of 30522 bf16: 195 us so, 158 now).
+        for (uint32_t i = 0, round = first_round; i < rounds; i++) {
+            const uint32_t w0 = a_begin + round * (kG * T) + tid;
+            round = round + 1 == rounds ? 0 : round + 1;
+#pragma unroll
+            for (int u = 0; u < kG; u++) {
+                const uint32_t w = w0 + u * T;
+                if (w >= a_end) break;
+                float y[E];
+                unpack<DT>(v[u], y);
+                turn(y);
+                if (w == w_target) add_target(y);
+                __stcs((uint4 *)orow.base + w, pack<DT>(y));
+            }
+            // all of a round's loads after all of the last one's stores: taking turns window by window cost 20 % of the bandwidth
+            asm volatile("" ::: "memory");
+            if (i + 1 < rounds) load_round(round);
+        }
+    }
+    // the windows before and behind those, element by element where they are not whole
+    for (uint32_t n = tid;; n += T) {
+        const uint32_t before = a_begin - w_begin, w = n < before ? w_begin + n : max(a_end, w_begin) + (n - before);
+        if (w >= w_end) break;
+        float y[E];
+        unpack<DT>(SAME ? load_window(row, w) : load_shifted<DT>(x, orow.head, p.vocab, w), y);
+        if (zero) {
+#pragma unroll
+            for (uint32_t j = 0; j < E; j++) y[j] = 0.f;
+        } else {
+            turn(y);
+        }
+        if (w == w_target) add_target(y);
+#pragma unroll
+        for (uint32_t j = 0; j < E; j++) {
+            const uint32_t pos = w * E + j;
+            if (pos >= orow.head && pos < orow.end) store_element<DT>(out, pos - orow.head, y[j]);
+        }
     }
     if (!KD) return;
     // What is listed, and the target: made again from all the shares it has.  A token that stands in the list twice is

@@ -118,10 +118,9 @@ template <int DT> __device__ __forceinline__ uint4 no_elements()
     const uint32_t none = DT == SFB_F32 ? Win<DT>::kInf : Win<DT>::kInf << 16 | Win<DT>::kInf;
     return make_uint4(none, none, none, none);
 }
-// ONCE: what nobody reads again, first to leave the cache
-template <int DT, bool ONCE = false> __device__ __forceinline__ uint4 load_window(const Row<DT> &r, uint32_t w)
+template <int DT> __device__ __forceinline__ uint4 load_window(const Row<DT> &r, uint32_t w)
 {
-    if (r.whole(w)) return ONCE ? __ldcs(r.base + w) : load16(r.base + w);
+    if (r.whole(w)) return load16(r.base + w);
     if (w * Win<DT>::kElems >= r.end) return no_elements<DT>();
     return edge_window<DT>(r.base, r.head, r.end, w);
 }
