@@ -893,8 +893,9 @@ template <int DT, bool ENT, bool TOP, int KD> static int launch_stats(cudaStream
     // tighter the more threads it comes from (4096 rows of 100003 bf16, 20 alternatives: 162 us, with four 180).
     const uint32_t T = windows > 512 && (p.rows < (uint32_t)sms * 8 || (TOP && (p.k > 32 || windows > 8192))) ? 256 : windows > 256 || TOP || KD ? 128 : 64;
     uint32_t C = 1;
-    // CTAs per row: as many as there are SMs without one, and a few for every SM as long as each has two groups of windows
-    while (C < kMaxCluster && windows > C * T * 2 && (!TOP || C * p.k <= 80)) {
+    // CTAs per row, while each has more than a group of windows: as many as there are SMs without one, and a few for every SM where
+    // each has two groups.  (Alternatives: CTA 0 ranks what all of them find.)
+    while (C < kMaxCluster && windows > C * kU * T && (!TOP || C * p.k <= 40)) {
         const uint64_t ctas = (uint64_t)p.rows * C * 2;
         if (ctas > (uint64_t)sms && (2 * ctas > 7 * (uint64_t)sms || windows < 2 * C * 2 * kU * T)) break;
         C *= 2;
