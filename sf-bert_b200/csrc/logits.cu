@@ -14,12 +14,17 @@
 namespace cg = cooperative_groups;
 
 namespace sfb {
+// A counter is cleared by a kernel and not by a memset, which nothing overlaps: the launch behind it sets itself up meanwhile.
+__global__ void zero_kernel(uint32_t *counter)
+{
+    grid_dependency_wait();
+    grid_launch_dependents();
+    *counter = 0;
+}
 static int set_zero(const char *who, uint32_t *counter, cudaStream_t s)
 {
-    const cudaError_t e = counter ? cudaMemsetAsync(counter, 0, sizeof(uint32_t), s) : cudaSuccess;
-    SFB_REQUIRE(e == cudaSuccess, "%s: %s", who, cudaGetErrorString(e));
-    clear_error();
-    return 0;
+    if (counter) launch_overlapped(zero_kernel, dim3(1), dim3(1), 0, s, counter);
+    return check_launch(who);
 }
 
 namespace lg {
@@ -305,7 +310,7 @@ template <bool ENT> __device__ __forceinline__ void finish_tokens(const StatPara
 // What a warp's entries of a row's list come to before the row's sums are known.  With q_k = e^(lq_k - mq) / Z and x_r the
 // largest listed logit, loss = sum_k q_k (ln q_k - s (x_k - m) + l) is linear in s (x_r - m) and l.
 struct ListPart {
-    float mq, z, u, v, x_r, listed;       // max lq, sum e = e^(lq - mq), sum e lq, sum e (x - x_r), max x, sum over distinct of 2^(s2 (x - x_r))
+    float mq, z, u, v, x_r, listed;       // max lq, sum e = e^(lq - mq), sum e (lq - mq), sum e (x - x_r), max x, sum over distinct of 2^(s2 (x - x_r))
 };
 
 // One warp: its entries, one per lane.  again: the lane's token stands earlier in the list.
@@ -313,7 +318,7 @@ template <int KD> __device__ __forceinline__ void sum_entries(float lq, float x,
 {
     const float mq = KD == 1 ? warp_max_nan(lq) : 0.f, x_r = warp_max_nan(x), base = x_r == neg_inf() ? 0.f : x_r;
     const float e = lq == neg_inf() ? 0.f : ex2(kLog2e * (lq - mq));
-    const float z = warp_sum(e), u = warp_sum(e > 0.f || e != e ? e * lq : 0.f), v = warp_sum(e > 0.f ? e * (x - base) : 0.f);
+    const float z = warp_sum(e), u = warp_sum(e > 0.f || e != e ? e * (lq - mq) : 0.f), v = warp_sum(e > 0.f ? e * (x - base) : 0.f);
     const float listed = KD == 2 ? warp_sum(again ? 0.f : ex2(s2 * (x - base))) : 0.f;
     if ((threadIdx.x & 31) == 0) *out = {mq, z, u, v, x_r, x_r == neg_inf() ? 0.f : listed};
 }
@@ -330,7 +335,7 @@ template <int KD> __device__ __forceinline__ void finish_lists(const StatParams 
         const ListPart g = part[w];
         const float f = KD == 2 ? 1.f : g.mq == neg_inf() ? 0.f : ex2(kLog2e * (g.mq - mq)), base = g.x_r == neg_inf() ? 0.f : g.x_r;
         z += f * g.z;
-        u += f * g.u;
+        if (f > 0.f || f != f) u += f * (KD == 2 ? g.u : g.u + g.z * (g.mq - mq));      // sum of e (lq - mq)
         if (f * g.z > 0.f) v += f * (g.v + g.z * (base - m));        // sum of e (x - m)
         if (KD == 2 && g.x_r != neg_inf()) listed += g.listed * ex2(p.s2 * (base - m));
     }
@@ -339,7 +344,7 @@ template <int KD> __device__ __forceinline__ void finish_lists(const StatParams 
     const float l = empty ? neg_inf() : logf(s);
     float loss = 0.f;
     if (!(z <= 0.f)) {
-        if (KD == 1) loss = empty ? -neg_inf() : (u - p.scale * v) / z - (mq + logf(z)) + l;
+        if (KD == 1) loss = empty ? -neg_inf() : (u - p.scale * v) / z - logf(z) + l;
         else loss = empty ? -neg_inf() : u - p.scale * v + z * l;
     }
     float *st = p.stats + (KD == 2 ? 3 : 2) * (size_t)r;

@@ -312,6 +312,17 @@ def test_distill(sfb, rows, vocab, width, k, tail, dtype):
         assert torch.equal(apart, got)
 
 
+def test_weights_far_from_probabilities(sfb):
+    """The renormalised list may be any log weights: their common offset does not matter, and costs nothing of the loss."""
+    x = make(9, 3000, 3000, "f32", 1)
+    ids, teacher = make_lists(x, 3000, 100, 7, False)
+    for shift in (1024.0, -4096.0):                                     # exact sums: the list's values have 2^-11 to spare below
+        moved = ((teacher * 2048).round() / 2048).contiguous()
+        a, _, _ = sfb.distill_topk(x, ids, moved)
+        b, _, _ = sfb.distill_topk(x, ids, moved + shift)
+        same(b, a.double(), 2.0 ** -20 * (1 + a.double().abs()), "loss")
+
+
 def test_remainder_that_is_small(sfb):
     """Nearly all of the student's mass is on the list: what it leaves is summed by itself, not as a difference from 1."""
     x = make(4, 20000, 20000, "f32", 1, spread=1.0)
