@@ -35,6 +35,7 @@ constexpr int kG = 4;                     // the same for gradients
 constexpr uint32_t kCap = 1024;           // candidates for a row's alternatives
 constexpr uint32_t kMaxList = 128;        // alternatives, entries of a teacher's list
 constexpr uint32_t kMaxCluster = 8;
+constexpr uint32_t kShort = 1024;         // windows of a row that a warp takes by itself where there are many
 
 struct StatParams {
     const void *x;
@@ -647,6 +648,80 @@ __global__ void __launch_bounds__(kThreads, 4) row_stats_kernel(const StatParams
     }
 }
 
+// Many rows: a warp each, eight to a CTA, with nothing to wait for.  Four warps that share a row wait for its end, and the SM for
+// their successors: 8192 rows of 4000 bf16 with entropy take 14 us so, 24 with a CTA per row; of 30522 83 and 91.  KD 0 or 1.
+template <int DT, bool ENT, int KD>
+__global__ void __launch_bounds__(kThreads, 4) short_rows_kernel(const StatParams p)
+{
+    constexpr uint32_t kWarps = kThreads / 32, T = 32;
+    constexpr bool kMaySkip = KD == 0 && !ENT;
+    __shared__ ListPart list[kWarps][kMaxList / 32];
+    __shared__ uint32_t part[kWarps];
+    const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32, r = blockIdx.x * kWarps + warp;
+    grid_dependency_wait();
+    grid_launch_dependents();
+    if (blockIdx.x * kWarps >= p.rows) {
+        count_missed(KD ? p.ids : p.targets, p.count_here, p.vocab, p.missed, part);
+        return;
+    }
+    if (r >= p.rows) return;
+    const void *x = (const char *)p.x + (size_t)r * p.pitch * Win<DT>::kSize;
+    int32_t target = KD == 0 && p.targets ? p.targets[r] : -1;
+    if (KD == 0 && p.targets && (uint32_t)target >= p.vocab) {
+        target = -1;
+        if (lane == 0 && p.missed && !p.count_here) atomicAdd(p.missed, 1u);
+        if (kMaySkip) {
+            if (lane == 0) { p.logp[r] = 0.f; p.stats[2 * (size_t)r] = p.stats[2 * (size_t)r + 1] = 0.f; }
+            return;
+        }
+    }
+    const Row<DT> row(x, p.vocab);
+    const float gap = 40.f / p.s2;
+    const uint32_t n_whole = row.whole_count();
+    const uint4 *src = row.base + row.first_whole() + lane;
+    auto load = [&](uint4 (&v)[kU], uint32_t i0) {
+#pragma unroll
+        for (int u = 0; u < kU; u++) v[u] = i0 + u * T + lane < n_whole ? load16(src + i0 + u * T) : no_elements<DT>();
+    };
+    uint4 v[kU], next[kU];
+    if (n_whole) load(next, 0);
+    const uint32_t edge = edge_position<DT>(row, lane);
+    const float x_edge = edge != kNoWindow ? load_element<DT>(x, edge - row.head) : neg_inf();
+    const float x_target = KD == 0 && target >= 0 ? load_element<DT>(x, (uint32_t)target) : 0.f;
+    if (KD) {
+        uint32_t bad = 0;
+        for (uint32_t i0 = 0; i0 < p.k; i0 += 32) {
+            const uint32_t i = i0 + lane;
+            const int32_t id = i < p.k ? p.ids[(size_t)r * p.k + i] : -1;
+            const bool ok = (uint32_t)id < p.vocab;
+            bad += __popc(__ballot_sync(0xffffffffu, i < p.k && !ok));
+            const float lq = ok ? p.teacher[(size_t)r * p.k + i] : neg_inf(), xl = ok ? load_element<DT>(x, (uint32_t)id) : neg_inf();
+            sum_entries<KD>(lq, xl, false, p.s2, &list[warp][i0 / 32]);
+        }
+        if (lane == 0 && bad && p.missed && !p.count_here) atomicAdd(p.missed, bad);
+    }
+    Sums a;
+    float mx = neg_inf();
+    for (uint32_t i0 = 0; i0 < n_whole; i0 += kU * T) {
+#pragma unroll
+        for (int u = 0; u < kU; u++) v[u] = next[u];
+        if (i0 + kU * T < n_whole) load(next, i0 + kU * T);
+        const float m = max_windows<DT, kU>(v);
+        mx = max_nan(mx, m);
+        if (a.prepare(m, p.s2, gap)) add_windows<DT, ENT, kU>(a, v, p.s2);
+    }
+    if (edge != kNoWindow) {
+        mx = max_nan(mx, x_edge);
+        add_element<ENT>(a, x_edge, p.s2, gap);
+    }
+    __syncwarp();
+    warp_sums<ENT>(a, mx, p.s2);
+    if (lane == 0) {
+        if (KD) finish_lists<KD>(p, r, list[warp], mx, a.s);
+        else finish_tokens<ENT>(p, r, target, x_target, mx, a.s, a.e);
+    }
+}
+
 // ---- gradients --------------------------------------------------------------------------------------------------------
 struct GradParams {
     const void *x;
@@ -893,6 +968,19 @@ template <int DT, bool ENT, bool TOP, int KD> static int launch_stats(cudaStream
     const int dev = current_device(), sms = device_sm_count(dev);
     SFB_REQUIRE(sms > 0, "%s: cannot query the device", who);
     const uint32_t windows = p.vocab / Win<DT>::kElems + 2;      // at most, wherever a row starts
+    const uint64_t entries = p.missed ? KD ? (uint64_t)p.rows * p.k : p.targets ? p.rows : 0 : 0;
+    if constexpr (!TOP && KD != 2) {
+        constexpr bool kMaySkip = KD == 0 && !ENT;
+        // A warp per row: short rows, and rows up to four times as long where there is one for every warp that the SMs hold, unless they may
+        // have nothing to do.  (Of longer ones the last to be dealt take too long by themselves: 5000 rows of 50021 fp32 190 us, 153 else.)
+        if (p.rows >= (uint32_t)sms * 8 && (windows <= kShort || (windows <= 4 * kShort && p.rows >= (uint32_t)sms * 32 && !(kMaySkip && p.targets)))) {
+            p.count_here = entries <= kThreads * 32 ? (uint32_t)entries : 0;
+            if (!p.count_here && set_zero(who, p.missed, s)) return 1;
+            const uint32_t rows_per = kThreads / 32;
+            launch_overlapped(short_rows_kernel<DT, ENT, KD>, dim3((p.rows + rows_per - 1) / rows_per + (p.count_here ? 1 : 0)), dim3(kThreads), 0, s, p);
+            return check_launch(who);
+        }
+    }
     // What a row's end costs is paid by each of its warps, so many rows have four of them each (4096 rows of 30522 bf16: 44 us, with
     // eight 50), few rows eight (257 of 50021 fp32: 19 us, with four 25), and so have long rows with alternatives, whose bound is the
     // tighter the more threads it comes from (4096 rows of 100003 bf16, 20 alternatives: 162 us, with four 180).
@@ -905,7 +993,6 @@ template <int DT, bool ENT, bool TOP, int KD> static int launch_stats(cudaStream
         if (ctas > (uint64_t)sms && (2 * ctas > 7 * (uint64_t)sms || windows < 2 * C * 2 * kU * T)) break;
         C *= 2;
     }
-    const uint64_t entries = p.missed ? KD ? (uint64_t)p.rows * p.k : p.targets ? p.rows : 0 : 0;
     p.count_here = entries <= T * 32u ? (uint32_t)entries : 0;
     if (!p.count_here && set_zero(who, p.missed, s)) return 1;
     for (;; C = 1) {

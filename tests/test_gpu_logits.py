@@ -67,7 +67,7 @@ def check_forward(sfb, x, targets, vocab, scale, entropy, top_k):
 
 
 SIZES = [(1, 1, 1), (3, 2, 2), (2, 7, 9), (1, 8, 8), (5, 33, 33), (2, 129, 144), (37, 1000, 1000), (3, 2049, 2050), (1, 30522, 30528), (2, 30522, 30522),
-         (300, 5003, 5003), (9, 100003, 100003), (700, 3000, 3008), (20, 131072, 131072)]
+         (300, 5003, 5003), (9, 100003, 100003), (700, 3000, 3008), (20, 131072, 131072), (1300, 517, 520), (6000, 1203, 1203)]
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
@@ -94,7 +94,7 @@ def test_rows_that_start_anywhere(sfb, dtype, offset):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
-@pytest.mark.parametrize("rows", [1, 400])
+@pytest.mark.parametrize("rows", [1, 400, 5000])
 def test_values_that_are_not_ordinary(sfb, dtype, rows):
     vocab = 9000
     low = torch.finfo(TYPES[dtype]).min
@@ -110,13 +110,16 @@ def test_values_that_are_not_ordinary(sfb, dtype, rows):
         t[0] = 7
         if n < 12:
             check_forward(sfb, x, t, vocab, 1.0, True, 20)
+            check_forward(sfb, x, t, vocab, 1.0, True, 0)
             check_forward(sfb, x, t, vocab, 1.0, False, 0)
             continue
-        logp, stats, ent, top_logp, top_ids, _ = sfb.token_logprobs(x, t, entropy=True, top_k=20)
-        for r in range(rows):
-            bad = r in {0, rows // 2, rows - 1}
-            assert bool(logp[r].isnan()) == bad and bool(ent[r].isnan()) == bad and bool(stats[r, 1].isnan()) == bad
-            assert bool(top_logp[r].isnan().all()) == bad and bool((top_ids[r] == -1).all()) == bad
+        bad = torch.zeros(rows, dtype=torch.bool, device="cuda")
+        bad[[0, rows // 2, rows - 1]] = True
+        for k in (20, 0):
+            logp, stats, ent, top_logp, top_ids, _ = sfb.token_logprobs(x, t, entropy=True, top_k=k)
+            assert torch.equal(logp.isnan(), bad) and torch.equal(ent.isnan(), bad) and torch.equal(stats[:, 1].isnan(), bad)
+            if k:
+                assert torch.equal(top_logp.isnan().all(1), bad) and torch.equal((top_ids == -1).all(1), bad)
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
@@ -273,7 +276,7 @@ def make_lists(x, vocab, k, seed, tail):
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("tail", [False, True])
-@pytest.mark.parametrize("rows,vocab,width,k", [(1, 1, 1, 1), (3, 5, 8, 7), (5, 33, 33, 4), (37, 1000, 1000, 128), (6, 4099, 4101, 20), (1, 30522, 30528, 64), (400, 5003, 5003, 17),
+@pytest.mark.parametrize("rows,vocab,width,k", [(1, 1, 1, 1), (3, 5, 8, 7), (5, 33, 33, 4), (37, 1000, 1000, 128), (6, 4099, 4101, 20), (1, 30522, 30528, 64), (400, 5003, 5003, 17), (1500, 1003, 1003, 40), (5000, 9001, 9008, 3),
                                                (9, 100003, 100003, 100)])
 def test_distill(sfb, rows, vocab, width, k, tail, dtype):
     x = make(rows, vocab, width, dtype, rows + k)
