@@ -154,6 +154,18 @@ def test_alternatives_that_sit_with_few_threads(sfb, rows):
     check_forward(sfb, y[:4], None, None, 1.0, False, 100)
 
 
+@pytest.mark.parametrize("rows", [2, 1300])
+@pytest.mark.parametrize("vocab,k", [(65, 1), (300, 32), (1000, 33), (4100, 5), (8200, 32)])
+def test_alternatives_of_short_rows(sfb, rows, vocab, k):
+    """From two to eight warps per row, by their length, their number and the alternatives'."""
+    for dtype in ("f32", "bf16"):
+        x = make(rows, vocab, vocab, dtype, vocab).round_(decimals=1)      # with ties
+        t = torch.randint(-1, vocab, (rows,), device="cuda", generator=gen(5), dtype=torch.int32)
+        check_forward(sfb, x, t, None, 1.0, True, k)
+        x[1:] = 2.0
+        check_forward(sfb, x, t, None, 1.0, False, k)
+
+
 def test_rows_without_a_target_are_not_read(sfb):
     x = make(50, 3001, 3001, "f32", 1)
     t = torch.randint(0, 3001, (50,), device="cuda", generator=gen(1), dtype=torch.int32)
