@@ -308,52 +308,51 @@ template <bool ENT> __device__ __forceinline__ void finish_tokens(const StatPara
     if (ENT) p.entropy[r] = empty ? 0.f : l - kLn2 * (e / s);
 }
 
-// What a warp's entries of a row's list come to before the row's sums are known.  With q_k = e^(lq_k - mq) / Z and x_r the
-// largest listed logit, loss = sum_k q_k (ln q_k - s (x_k - m) + l) is linear in s (x_r - m) and l.
+// What a warp's entries of a row's list come to before the row's sums are known.  A divergence is small beside the logarithms that it
+// is made of, so those are subtracted entry by entry, d_k = (lq_k - mq) - s (x_k - x_r) with x_r the largest listed logit, and what
+// is left of the sums' logarithms is taken from their quotient: with q_k = e^(lq_k - mq) / Z
+//   loss = sum_k q_k d_k - s (x_r - m) + ln (S / Z).
 struct ListPart {
-    float mq, z, u, v, x_r, listed;       // max lq, sum e = e^(lq - mq), sum e (lq - mq), sum e (x - x_r), max x, sum over distinct of 2^(s2 (x - x_r))
+    float mq, z, w, x_r, listed;          // max lq, sum e = e^(lq - mq), sum e d, max x, sum over distinct of 2^(s2 (x - x_r))
 };
 
 // One warp: its entries, one per lane.  again: the lane's token stands earlier in the list.
-template <int KD> __device__ __forceinline__ void sum_entries(float lq, float x, bool again, float s2, ListPart *out)
+template <int KD> __device__ __forceinline__ void sum_entries(float lq, float x, bool again, float scale, float s2, ListPart *out)
 {
     const float mq = KD == 1 ? warp_max_nan(lq) : 0.f, x_r = warp_max_nan(x), base = x_r == neg_inf() ? 0.f : x_r;
     const float e = lq == neg_inf() ? 0.f : ex2(kLog2e * (lq - mq));
-    const float z = warp_sum(e), u = warp_sum(e > 0.f || e != e ? e * (lq - mq) : 0.f), v = warp_sum(e > 0.f ? e * (x - base) : 0.f);
+    const float z = warp_sum(e), w = warp_sum(e > 0.f || e != e ? e * fmaf(-scale, x - base, lq - mq) : 0.f);
     const float listed = KD == 2 ? warp_sum(again ? 0.f : ex2(s2 * (x - base))) : 0.f;
-    if ((threadIdx.x & 31) == 0) *out = {mq, z, u, v, x_r, x_r == neg_inf() ? 0.f : listed};
+    if ((threadIdx.x & 31) == 0) *out = {mq, z, w, x_r, x_r == neg_inf() ? 0.f : listed};
 }
 
 // One thread: the row's results, m and s (KD 2: without the listed tokens) known.
 template <int KD> __device__ __forceinline__ void finish_lists(const StatParams &p, uint32_t r, const ListPart *part, float m, float s)
 {
     const uint32_t n = (p.k + 31) / 32;
-    float mq = KD == 1 ? neg_inf() : 0.f, z = 0.f, u = 0.f, v = 0.f, listed = 0.f;
+    float mq = KD == 1 ? neg_inf() : 0.f, z = 0.f, w = 0.f, listed = 0.f;
     const bool empty = m == neg_inf();
     if (KD == 1)
-        for (uint32_t w = 0; w < n; w++) mq = max_nan(mq, part[w].mq);
-    for (uint32_t w = 0; w < n; w++) {
-        const ListPart g = part[w];
+        for (uint32_t i = 0; i < n; i++) mq = max_nan(mq, part[i].mq);
+    for (uint32_t i = 0; i < n; i++) {
+        const ListPart g = part[i];
         const float f = KD == 2 ? 1.f : g.mq == neg_inf() ? 0.f : ex2(kLog2e * (g.mq - mq)), base = g.x_r == neg_inf() ? 0.f : g.x_r;
         z += f * g.z;
-        if (f > 0.f || f != f) u += f * (KD == 2 ? g.u : g.u + g.z * (g.mq - mq));      // sum of e (lq - mq)
-        if (f * g.z > 0.f) v += f * (g.v + g.z * (base - m));        // sum of e (x - m)
+        if (!(f * g.z <= 0.f)) w += f * (g.w + g.z * fmaf(-p.scale, base - m, KD == 2 ? 0.f : g.mq - mq));     // sum of e ((lq - mq) - s (x - m))
         if (KD == 2 && g.x_r != neg_inf()) listed += g.listed * ex2(p.s2 * (base - m));
     }
     const float rest = s;
     if (KD == 2) s += listed;
     const float l = empty ? neg_inf() : logf(s);
     float loss = 0.f;
-    if (!(z <= 0.f)) {
-        if (KD == 1) loss = empty ? -neg_inf() : (u - p.scale * v) / z - logf(z) + l;
-        else loss = empty ? -neg_inf() : u - p.scale * v + z * l;
-    }
+    if (!(z <= 0.f)) loss = empty ? -neg_inf() : KD == 1 ? w / z + logf(s / z) : fmaf(z, l, w);
     float *st = p.stats + (KD == 2 ? 3 : 2) * (size_t)r;
     st[0] = m;
     st[1] = l;
     if (KD == 2) {
         const float lr = rest == 0.f ? neg_inf() : logf(rest), left = fmaxf(0.f, 1.f - z);
-        if (left > 0.f && !(lr == neg_inf())) loss += left * (logf(left) - (lr - l));
+        // ln p_r and ln q_r, which are small where most is left, without the sums' own logarithms
+        if (left > 0.f && !(lr == neg_inf())) loss += left * (log1pf(-z) - (rest > listed ? log1pf(-listed / s) : lr - l));
         st[2] = lr;
     }
     p.loss[r] = loss;
@@ -473,7 +472,7 @@ __global__ void __launch_bounds__(kThreads, 4) row_stats_kernel(const StatParams
                 const uint32_t bad = __popc(__ballot_sync(0xffffffffu, tid < p.k && !ok));
                 if (lane == 0 && bad) atomicAdd(p.missed, bad);
             }
-            sum_entries<KD>(lq, xl, again, p.s2, &list[warp]);
+            sum_entries<KD>(lq, xl, again, p.scale, p.s2, &list[warp]);
         }
     }
 
@@ -696,7 +695,7 @@ __global__ void __launch_bounds__(kThreads, 4) short_rows_kernel(const StatParam
             const bool ok = (uint32_t)id < p.vocab;
             bad += __popc(__ballot_sync(0xffffffffu, i < p.k && !ok));
             const float lq = ok ? p.teacher[(size_t)r * p.k + i] : neg_inf(), xl = ok ? load_element<DT>(x, (uint32_t)id) : neg_inf();
-            sum_entries<KD>(lq, xl, false, p.s2, &list[warp][i0 / 32]);
+            sum_entries<KD>(lq, xl, false, p.scale, p.s2, &list[warp][i0 / 32]);
         }
         if (lane == 0 && bad && p.missed && !p.count_here) atomicAdd(p.missed, bad);
     }

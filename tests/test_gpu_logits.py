@@ -327,6 +327,28 @@ def test_distill(sfb, rows, vocab, width, k, tail, dtype):
         assert torch.equal(apart, got)
 
 
+@pytest.mark.parametrize("tail", [False, True])
+@pytest.mark.parametrize("rows", [3, 2000])
+def test_divergences_that_are_small(sfb, rows, tail):
+    """A student next to its teacher, most of the mass outside the list (tail) or on it: the divergence is a thousandth of the
+    logarithms it is made of.  Each of those, at most 16, rounds by 2^-21; they come weighted by the list's mass, at most 0.1 here
+    with the tail, where the two remainders' logarithms are below 0.1 and round by 2^-27; sums of the list and the row are
+    off by their bounds, once for each side: in all at most (2^-20 + 2 D) times that mass, D = bounds(vocab)."""
+    vocab, k = (10413, 73) if tail else (400, 128)
+    x = make(rows, vocab, vocab, "f32", 1, spread=2.0)
+    if not tail:
+        x[:, 128:] -= 12.0
+    noisy = x + 0.1 * torch.randn(rows, vocab, device="cuda", generator=gen(2))
+    lp, ids = torch.log_softmax(0.25 * noisy if tail else noisy, 1).topk(k, 1)
+    ids, lp = ids.to(torch.int32).contiguous(), lp.contiguous()
+    scale = 0.25 if tail else 1.0
+    loss, _, _ = sfb.distill_topk(x, ids, lp, scale=scale, tail=tail)
+    want = R.distill(x, ids, lp, vocab, scale, tail)
+    mass = lp.double().exp().sum(1)
+    assert float(mass.max()) < 0.1 if tail else float(mass.min()) > 0.9
+    same(loss, want["loss"], (2.0 ** -20 + 2 * R.bounds(vocab)) * mass, "loss")
+
+
 def test_weights_far_from_probabilities(sfb):
     """The renormalised list may be any log weights: their common offset does not matter, and costs nothing of the loss."""
     x = make(9, 3000, 3000, "f32", 1)
