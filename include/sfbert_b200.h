@@ -287,7 +287,7 @@ int sfb_embedding(sfb_stream_t stream, void *out, const void *table, const int32
  * all fp32 (ids int32).  A target outside [0, vocab) -- a row without one -- gives a logp of 0; it is counted in *missed
  * (device uint32, may be NULL), and unless entropy or alternatives are asked for its row is not read and its stats are 0.  A NaN
  * or +inf among a row's logits makes its results NaN (its alternatives' ids -1).  Sums are fp32.  vocab is at most 2^30, with
- * alternatives 2^19. */
+ * alternatives 2^19; scale at most 1e6. */
 int sfb_token_logprobs(sfb_stream_t stream, const void *logits, uint64_t pitch, const int32_t *targets, uint32_t rows,
                        uint32_t vocab, int dtype, float scale, float *logp, float *stats, float *entropy,
                        float *top_logp, int32_t *top_ids, uint32_t top_k, uint32_t *missed);
@@ -307,7 +307,8 @@ int sfb_token_logprobs_grad(sfb_stream_t stream, const void *logits, uint64_t pi
  * with p_r what the student leaves to the tokens that are not listed (summed over them; where that is nothing the term is
  * left out).  An id outside [0, vocab) is no entry: its weight is 0, it is counted in *missed (may be NULL).  The same id
  * twice is two entries of one token.  stats [rows][2 + tail] = m, l and with tail the log of the unlisted tokens' sum beside m.
- * The loss carries no factor for the temperature.  vocab is at most 2^30, with tail 2^20. */
+ * Without tail the list may be log weights of any offset.  The loss carries no factor for the temperature.  vocab is at most 2^30, with
+ * tail 2^20. */
 int sfb_distill_topk(sfb_stream_t stream, const void *logits, uint64_t pitch, const int32_t *ids, const float *teacher,
                      uint32_t rows, uint32_t vocab, uint32_t k, int dtype, float scale, int tail, float *loss, float *stats,
                      uint32_t *missed);
