@@ -983,10 +983,11 @@ template <int DT, bool ENT, bool TOP, int KD> static int launch_stats(cudaStream
     // What a row's end costs is paid by each of its warps, so many rows have four of them each (4096 rows of 30522 bf16: 44 us, with
     // eight 50), few rows eight (257 of 50021 fp32: 19 us, with four 25), and so have long rows with alternatives, whose bound is the
     // tighter the more threads it comes from (4096 rows of 100003 bf16, 20 alternatives: 162 us, with four 180).  Many short rows
-    // with few alternatives have two (8192 of 1000 fp32: 20 us, with four 32).
+    // with few alternatives, or short lists and their remainder, have two (8192 of 1000 fp32, one alternative: 20 us, with four 32; 8192
+    // of 1000 bf16, lists of 64: 22 and 32).
     uint32_t T = windows > 256 || TOP || KD ? 128 : 64;
     if (windows > 512 && (p.rows < (uint32_t)sms * 8 || (TOP && (p.k > 32 || windows > 8192)))) T = 256;
-    if (TOP && p.k <= 32 && windows <= 1024 && p.rows >= (uint32_t)sms * 8) T = 64;
+    if (((TOP && p.k <= 32) || (KD == 2 && p.k <= 64)) && windows <= 1024 && p.rows >= (uint32_t)sms * 8) T = 64;
     uint32_t C = 1;
     // CTAs per row, while each has more than a group of windows: as many as there are SMs without one, and a few for every SM where
     // each has two groups.  (Alternatives: CTA 0 ranks what all of them find.)
