@@ -382,8 +382,13 @@ __global__ void __launch_bounds__(kThreads, 4) row_stats_kernel(const StatParams
     const uint32_t T = blockDim.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t C = cluster_size(), rank = cluster_rank();
     const uint32_t r = blockIdx.x / C;
-    if (C > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");    // waited for before the first word into another CTA
+    // Every CTA of the cluster waits for this arrival before its first word into another CTA.  CTA 0 has to be there by then, and, with
+    // alternatives, its counter of candidates, to which all of them add, has to be 0: the arrival releases that store, the wait acquires it.
     if (TOP && tid == 0) { top_s->cnt = 0; top_s->n_hits = 0; }
+    if (C > 1) {
+        if (TOP) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+        else asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+    }
     if (KD == 2)
         for (uint32_t i = tid; i < (p.vocab + 2 * Win<DT>::kElems + 31) / 32; i += T) ((uint32_t *)dyn)[i] = 0;
     grid_dependency_wait();
@@ -406,7 +411,7 @@ __global__ void __launch_bounds__(kThreads, 4) row_stats_kernel(const StatParams
     }
     if (skip) {
         __syncwarp();
-        if (C > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+        if (C > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
         return;
     }
 
@@ -516,7 +521,7 @@ __global__ void __launch_bounds__(kThreads, 4) row_stats_kernel(const StatParams
     }
     warp_sums<ENT>(a, mx, p.s2);
     if (C > 1) {
-        asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
         if (lane == 0) cg::this_cluster().map_shared_rank(parts, 0)[rank * 8 + warp] = Part{mx, a.s, a.e};
         if (!TOP) {
             cg::this_cluster().sync();

@@ -2,6 +2,7 @@
 all of them on CPU tensors is refused for being there), and so do those of the C ABI."""
 import ctypes as C
 import math
+import os
 import re
 
 import pytest
@@ -124,3 +125,17 @@ def test_workspace_of_the_scores(sfb):
     assert f(1, 1) >= 36 and f(0, 30522) == 0
     assert f(4096, 30522) >= 4096 * (120 * 32 + 4)
     assert f(1 << 20, 30522) == f(32768, 30522) < 1 << 28
+
+
+def test_order_of_the_candidates_counter():
+    """CTAs of a cluster add to CTA 0's counter once they have waited for its arrival: the counter has to be cleared before that arrival,
+    which has to release the store, and the wait has to acquire it.  Nothing but the order in the source can show a missing one: a whole
+    pass over the row lies between, so results are right all the same, nearly always."""
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "sf-bert_b200", "csrc", "logits.cu")
+    with open(path) as f:
+        text = re.sub(r"//[^\n]*", "", f.read())
+    body = text[text.index("row_stats_kernel(const StatParams p)"):]
+    clear, arrive, wait, add = (body.index(x) for x in ("top_s->cnt = 0", "barrier.cluster.arrive.", "barrier.cluster.wait.", "atomicAdd(&join->cnt"))
+    assert clear < arrive < wait < add
+    assert "if (TOP) asm volatile(\"barrier.cluster.arrive.release.aligned" in body[arrive - 60:arrive + 80]
+    assert not re.search(r"barrier\.cluster\.wait\.(?!acquire)", body[:add])
