@@ -304,9 +304,10 @@ int sfb_token_logprobs_grad(sfb_stream_t stream, const void *logits, uint64_t pi
  * probabilities at the temperature (what sfb_token_logprobs gives as alternatives); logits are the student's, p their softmax:
  *   tail 0: q = softmax(teacher) over the list,            loss = sum_k q_k (log q_k - log p_k)
  *   tail 1: q = exp(teacher), q_r = max(0, 1 - sum_k q_k),  loss = sum_k q_k (log q_k - log p_k) + q_r (log q_r - log p_r)
- * with p_r what the student leaves to the tokens that are not listed (summed over them; where that is nothing the term is
- * left out).  An id outside [0, vocab) is no entry: its weight is 0, it is counted in *missed (may be NULL).  The same id
- * twice is two entries of one token.  stats [rows][2 + tail] = m, l and with tail the log of the unlisted tokens' sum beside m.
+ * with p_r what the student leaves to the tokens that are not listed: summed over them beside their own largest, however far below the row's
+ * that is; where all of them are at -inf the term is left out (a token at the type's lowest value counts).  An id outside [0, vocab) is no entry: its weight is 0, it is counted in *missed (may be NULL).  The same id
+ * twice is two entries of one token.  stats [rows][2 + tail] = m, l and with tail the log of the unlisted tokens' sum beside m (-inf
+ * only where the term is left out).
  * Without tail the list may be log weights of any offset.  The loss carries no factor for the temperature.  vocab is at most 2^30, with
  * tail 2^20. */
 int sfb_distill_topk(sfb_stream_t stream, const void *logits, uint64_t pitch, const int32_t *ids, const float *teacher,

@@ -10,6 +10,7 @@
 // each element is read once, whole windows of 16 bytes at a time, several on their way per thread.
 #include "logits.cuh"
 #include <cooperative_groups.h>
+#include <cfloat>
 
 namespace cg = cooperative_groups;
 
@@ -33,8 +34,11 @@ constexpr uint32_t kThreads = 256;
 constexpr int kU = 4;                     // windows that a thread has on their way at a time
 constexpr int kG = 4;                     // the same for gradients
 constexpr uint32_t kCap = 1024;           // candidates for a row's alternatives
-constexpr uint32_t kMaxList = 128;        // alternatives, entries of a teacher's list
+constexpr uint32_t kMaxList = 128;        // alternatives, entries of a teacher's list (four per lane)
 constexpr uint32_t kMaxCluster = 8;
+// A remainder whose logarithm is below this is summed again for the gradient (sum_unlisted): an unlisted token's share of it is the power of a
+// difference from that logarithm, of which fp32 loses 2^-24 of its size -- 2^-17 of the share here, all of it at ten million.
+constexpr float kFarRest = -64.f;
 constexpr uint32_t kShort = 1024;         // windows of a row that a warp takes by itself where there are many
 
 struct StatParams {
@@ -326,11 +330,15 @@ template <int KD> __device__ __forceinline__ void sum_entries(float lq, float x,
     if ((threadIdx.x & 31) == 0) *out = {mq, z, w, x_r, x_r == neg_inf() ? 0.f : listed};
 }
 
-// One thread: the row's results, m and s (KD 2: without the listed tokens) known.
+// One thread: the row's results, m and s known.  KD 2: those of the tokens that are not listed.  Their sum stands beside their own
+// largest logit: beside the row's, which a list that holds nearly all of the mass leaves far behind, it would be lost.
 template <int KD> __device__ __forceinline__ void finish_lists(const StatParams &p, uint32_t r, const ListPart *part, float m, float s)
 {
     const uint32_t n = (p.k + 31) / 32;
     float mq = KD == 1 ? neg_inf() : 0.f, z = 0.f, w = 0.f, listed = 0.f;
+    const float m_rest = m, s_rest = s;
+    if (KD == 2)
+        for (uint32_t i = 0; i < n; i++) m = max_nan(m, part[i].x_r);
     const bool empty = m == neg_inf();
     if (KD == 1)
         for (uint32_t i = 0; i < n; i++) mq = max_nan(mq, part[i].mq);
@@ -341,8 +349,8 @@ template <int KD> __device__ __forceinline__ void finish_lists(const StatParams 
         if (!(f * g.z <= 0.f)) w += f * (g.w + g.z * fmaf(-p.scale, base - m, KD == 2 ? 0.f : g.mq - mq));     // sum of e ((lq - mq) - s (x - m))
         if (KD == 2 && g.x_r != neg_inf()) listed += g.listed * ex2(p.s2 * (base - m));
     }
-    const float rest = s;
-    if (KD == 2) s += listed;
+    const float rest = KD == 2 && !(m_rest == neg_inf()) ? s_rest * ex2(fmaxf(p.s2 * (m_rest - m), kFar)) : 0.f;
+    if (KD == 2) s = rest + listed;
     const float l = empty ? neg_inf() : logf(s);
     float loss = 0.f;
     if (!(z <= 0.f)) loss = empty ? -neg_inf() : KD == 1 ? w / z + logf(s / z) : fmaf(z, l, w);
@@ -350,9 +358,15 @@ template <int KD> __device__ __forceinline__ void finish_lists(const StatParams 
     st[0] = m;
     st[1] = l;
     if (KD == 2) {
-        const float lr = rest == 0.f ? neg_inf() : logf(rest), left = fmaxf(0.f, 1.f - z);
-        // ln p_r and ln q_r, which are small where most is left, without the sums' own logarithms
-        if (left > 0.f && !(lr == neg_inf())) loss += left * (log1pf(-z) - (rest > listed ? log1pf(-listed / s) : lr - l));
+        const float left = fmaxf(0.f, 1.f - z);
+        float lr = neg_inf();
+        if (!(m_rest == neg_inf())) {
+            // ln p_r and ln q_r, which are small where most is left, without the sums' own logarithms; a product with the distance to the
+            // largest logit stays finite where the distance times the scale may not
+            const float ls = logf(s_rest);
+            if (left > 0.f) loss += rest > listed ? left * (log1pf(-z) - log1pf(-listed / s)) : fmaf(left * p.scale, m - m_rest, left * (log1pf(-z) + (l - ls)));
+            lr = l != l ? l : fmaxf(fmaf(p.scale, m_rest - m, ls), -FLT_MAX);      // -inf is what has no token left
+        }
         st[2] = lr;
     }
     p.loss[r] = loss;
@@ -546,7 +560,6 @@ __global__ void __launch_bounds__(kThreads, 4) row_stats_kernel(const StatParams
             b.s += c.s; b.e += c.e;
             bm = m2;
         }
-        if (KD == 2 && lane < (p.k + 31) / 32) bm = max_nan(bm, list[lane].x_r);
         warp_sums<ENT>(b, bm, p.s2);
         if (lane == 0) {
             if (KD) finish_lists<KD>(p, r, list, bm, b.s);
@@ -739,7 +752,6 @@ struct GradParams {
     const int32_t *ids;
     const float *teacher, *dloss, *token_stats;
     uint32_t k;
-    int tail;
 };
 
 // windows of x that start where those of out do not
@@ -759,18 +771,56 @@ template <int DT> __device__ __forceinline__ uint4 load_shifted(const void *x, u
     return make_uint4(v[0], v[1], v[2], v[3]);
 }
 
+// One CTA: the tokens of a row that are not listed, the largest and the base-2 logarithm of their sum beside it.  ids: kMaxList of them, -1
+// for none.  seen: a bit for each remainder modulo kSeen that a window with a listed token has; a warp looks at such a window together,
+// four entries of the list per lane.  part: one per warp.
+// 257 rows of 50021 fp32 whose remainders are all far away, lists of 128: the gradient takes 70 us, 29 otherwise; 4096 of 30522 bf16, lists of 64, 180 and 102.
+constexpr uint32_t kSeen = 8192;
+template <int DT> __device__ __noinline__ float2 sum_unlisted(const Row<DT> row, float s2, const int32_t *ids, const uint32_t *seen, Part *part)
+{
+    constexpr uint32_t E = Win<DT>::kElems;
+    const uint32_t windows = row.windows(), T = blockDim.x, lane = threadIdx.x % 32;
+    const float gap = 40.f / s2;
+    const int4 o = ((const int4 *)ids)[lane];
+    Sums a;
+    float mx = neg_inf();
+    for (uint32_t w0 = threadIdx.x - lane; w0 < windows; w0 += T) {
+        uint4 v[1] = {load_window(row, w0 + lane)};
+        for (uint32_t hits = __ballot_sync(0xffffffffu, seen[(w0 + lane) % kSeen / 32] >> ((w0 + lane) % 32) & 1); hits; hits &= hits - 1) {
+            const uint32_t at = __ffs(hits) - 1, first = (w0 + at) * E - row.head;     // (-1 is a position in front of the row, which holds -inf)
+            auto bit = [&](int32_t id) { return (uint32_t)id - first < E ? 1u << ((uint32_t)id - first) : 0u; };
+            const uint32_t bits = __reduce_or_sync(0xffffffffu, bit(o.x) | bit(o.y) | bit(o.z) | bit(o.w));
+            if (lane == at) drop_listed<DT>(v[0], bits);
+        }
+        const float m = max_windows<DT, 1>(v);
+        mx = max_nan(mx, m);
+        if (a.prepare(m, s2, gap)) add_windows<DT, false, 1>(a, v, s2);
+        __syncwarp();
+    }
+    warp_sums<false>(a, mx, s2);
+    if (lane == 0) part[threadIdx.x / 32] = {mx, a.s, 0.f};
+    __syncthreads();
+    mx = neg_inf();
+    for (uint32_t w = 0; w < T / 32; w++) mx = max_nan(mx, part[w].m);
+    float s = 0.f;
+    for (uint32_t w = 0; w < T / 32; w++) s += part[w].s * ex2(fmaxf(s2 * (part[w].m - mx), kFar));
+    return make_float2(mx, log2f(s));
+}
+
 // A row (or a part of it) per CTA, a round of kG windows per thread at a time: loaded, turned into the gradient and stored.  Bound by
 // memory: 8192 rows of 30522 bf16 157 us, 97 % of a copy's rate; lists and hard labels add a prologue to each row (4096 rows:
 // 93 us, 82 %).
 // dx = p (c0 + c1 t) with t the base-2 logarithm of p, plus the given target's share (KD 0, ENT: c1 is not 0);
-// dx = c0 2^t + c2 2^t2, what is listed made again by itself (KD 1; HARD 1: c2 is not 0).  HARD 2: at temperature 2 the
+// dx = c0 2^t + c2 2^t2, what is listed made again by itself (KD 1, and 2 with the remainder; HARD 1: c2 is not 0).  HARD 2: at temperature 2 the
 // second power, the softmax's at temperature 1, is the first one's square times a constant of the row (which goes to c2), and an
 // exponential per element less: 4096 rows of 30522 bf16 with lists of 64, 107 -> 100 us.
-template <int DT, bool ENT, bool KD, int HARD, bool SAME>
+template <int DT, bool ENT, int KD, int HARD, bool SAME>
 __global__ void __launch_bounds__(kThreads, KD ? 5 : 6) row_grad_kernel(const GradParams p)
 {
     __shared__ __align__(16) int32_t l_id[KD ? kMaxList : 4];
     __shared__ __align__(16) float l_q[KD ? kMaxList : 4];
+    __shared__ uint32_t l_seen[KD == 2 ? kSeen / 32 : 1];
+    __shared__ Part l_sum[KD == 2 ? kThreads / 32 : 1];
     __shared__ float2 l_part[kMaxList / 32];                  // a warp's entries: the largest teacher value, the sum of the powers beside it
     constexpr uint32_t E = Win<DT>::kElems;
     constexpr bool kMaySkip = !KD && !ENT;                    // a row without a target is zeros
@@ -782,17 +832,23 @@ __global__ void __launch_bounds__(kThreads, KD ? 5 : 6) row_grad_kernel(const Gr
     const void *x = (const char *)p.x + (size_t)r * p.pitch * Win<DT>::kSize;
     void *out = (char *)p.out + (size_t)r * p.out_pitch * Win<DT>::kSize;
     const Row<DT> orow(out, p.width), row(x, p.vocab);        // SAME: both start at the same place of their windows
-    const uint32_t w_begin = part * p.per, w_end = min(orow.windows(), w_begin + p.per);
-    const int32_t i_begin = (int32_t)(w_begin * E) - (int32_t)orow.head, i_end = (int32_t)(w_end * E) - (int32_t)orow.head;
+    uint32_t w_begin = part * p.per, w_end = min(orow.windows(), w_begin + p.per);
+    int32_t i_begin = (int32_t)(w_begin * E) - (int32_t)orow.head, i_end = (int32_t)(w_end * E) - (int32_t)orow.head;
 
     int32_t target = p.targets ? p.targets[r] : -1;
     if ((uint32_t)target >= p.vocab) target = -1;
-    const float *st = p.stats + (KD && p.tail ? 3 : 2) * (size_t)r;
+    const float *st = p.stats + (KD == 2 ? 3 : 2) * (size_t)r;
     const float m = st[0];
     const bool zero = m == neg_inf() || (kMaySkip && target < 0);       // no token is left (every probability is 0), or nothing is asked for
     // the windows [a_begin, a_end) are whole ones of x and out (none if theirs start at different places); the few others come after them
-    const uint32_t a_begin = SAME ? max(w_begin, row.first_whole()) : w_begin, a_end = SAME ? max(a_begin, min(w_end, row.first_whole() + row.whole_count())) : w_begin;
-    const uint32_t rounds = (a_end - a_begin + kG * T - 1) / (kG * T), first_round = rounds ? r % rounds : 0;
+    uint32_t a_begin, a_end, rounds, first_round;
+    auto set_rounds = [&]() {
+        a_begin = SAME ? max(w_begin, row.first_whole()) : w_begin;
+        a_end = SAME ? max(a_begin, min(w_end, row.first_whole() + row.whole_count())) : w_begin;
+        rounds = (a_end - a_begin + kG * T - 1) / (kG * T);
+        first_round = rounds ? r % rounds : 0;
+    };
+    set_rounds();
     uint4 v[kG];
     auto load_round = [&](uint32_t round) {
         const uint32_t w0 = a_begin + round * (kG * T) + tid;
@@ -803,6 +859,7 @@ __global__ void __launch_bounds__(kThreads, KD ? 5 : 6) row_grad_kernel(const Gr
     if (!zero && rounds) load_round(first_round);
 
     float c0, c1 = 0.f, c2 = 0.f, l2, l2b = 0.f, target_share = 0.f;
+    float ref = m;                                            // what the exponents of the pass are taken beside
     int32_t id = -1;                                          // KD: this thread's entry of the list
     float x_listed = 0.f, x_target = 0.f, listed_w = 0.f, listed_c = 0.f;
     if (!KD) {
@@ -827,13 +884,16 @@ __global__ void __launch_bounds__(kThreads, KD ? 5 : 6) row_grad_kernel(const Gr
         }
         const uint32_t n = (p.k + 31) / 32;
         if (tid / 32 < n) {
-            const float mq = p.tail ? 0.f : warp_max_nan(lq), z = warp_sum(lq == neg_inf() ? 0.f : ex2(kLog2e * (lq - mq)));
+            const float mq = KD == 2 ? 0.f : warp_max_nan(lq), z = warp_sum(lq == neg_inf() ? 0.f : ex2(kLog2e * (lq - mq)));
             if (lane == 0) l_part[tid / 32] = make_float2(mq, z);
         }
         // out may be x: what is listed (and the target) is read before anything is written
-        if (id >= i_begin && id < i_end && id >= 0) x_listed = load_element<DT>(x, (uint32_t)id);
-        if (HARD && tid == 0 && target >= 0 && target >= i_begin && target < i_end) x_target = load_element<DT>(x, (uint32_t)target);
-        const float sw = p.scale * p.dloss[r], l = st[1], lr = p.tail ? st[2] : 0.f;
+        auto load_listed = [&]() {
+            if (id >= i_begin && id < i_end && id >= 0) x_listed = load_element<DT>(x, (uint32_t)id);
+            if (HARD && tid == 0 && target >= 0 && target >= i_begin && target < i_end) x_target = load_element<DT>(x, (uint32_t)target);
+        };
+        load_listed();
+        const float sw = p.scale * p.dloss[r], l = st[1], lr = KD == 2 ? st[2] : 0.f;
         if (HARD) {
             const float g = target >= 0 ? p.dlogp[r] : 0.f;
             c2 = -g;
@@ -841,18 +901,18 @@ __global__ void __launch_bounds__(kThreads, KD ? 5 : 6) row_grad_kernel(const Gr
             target_share = g;
         }
         __syncthreads();
-        float mq = p.tail ? 0.f : neg_inf(), z = 0.f;
-        if (!p.tail)
+        float mq = KD == 2 ? 0.f : neg_inf(), z = 0.f;
+        if (KD == 1)
             for (uint32_t w = 0; w < n; w++) mq = max_nan(mq, l_part[w].x);
-        for (uint32_t w = 0; w < n; w++) z += l_part[w].x == neg_inf() ? 0.f : l_part[w].y * (p.tail ? 1.f : ex2(kLog2e * (l_part[w].x - mq)));
+        for (uint32_t w = 0; w < n; w++) z += l_part[w].x == neg_inf() ? 0.f : l_part[w].y * (KD == 2 ? 1.f : ex2(kLog2e * (l_part[w].x - mq)));
         const bool none = mq == neg_inf();
-        if (tid < kMaxList) l_q[tid] = lq == neg_inf() || none ? 0.f : ex2(kLog2e * (lq - mq)) * (p.tail ? 1.f : 1.f / z);
-        const float left = p.tail ? fmaxf(0.f, 1.f - z) : 0.f, all = p.tail ? z + left : none ? 0.f : 1.f;
+        if (tid < kMaxList) l_q[tid] = lq == neg_inf() || none ? 0.f : ex2(kLog2e * (lq - mq)) * (KD == 2 ? 1.f : 1.f / z);
+        const float left = KD == 2 ? fmaxf(0.f, 1.f - z) : 0.f, all = KD == 2 ? z + left : none ? 0.f : 1.f;
         listed_w = sw;
         listed_c = sw * all;
         l2 = l * kLog2e;
         c0 = sw * all;
-        if (p.tail) {
+        if (KD == 2) {
             // unlisted tokens: all * p - left * p / p_rest, as a multiple of their share of the remainder
             if (lr == neg_inf()) {
                 c0 = 0.f;                                     // every unlisted one has a probability of 0
@@ -860,18 +920,38 @@ __global__ void __launch_bounds__(kThreads, KD ? 5 : 6) row_grad_kernel(const Gr
                 c0 = sw * (all * expf(lr - l) - left);
                 l2 = lr * kLog2e;
             }
+            if (lr < kFarRest && lr > neg_inf() && left > 0.f) {
+                // One CTA for the whole row, the others are done: out may be x, and the row is read before any of it is written.
+                if (part) return;
+                w_end = orow.windows();
+                i_end = (int32_t)(w_end * E) - (int32_t)orow.head;
+                set_rounds();
+                load_listed();
+                for (uint32_t i = tid; i < kSeen / 32; i += T) l_seen[i] = 0;
+                __syncthreads();
+                const uint32_t w_id = ((uint32_t)id + row.head) / E;
+                if (id >= 0) atomicOr(&l_seen[w_id % kSeen / 32], 1u << (w_id % 32));
+                __syncthreads();
+                const float2 rest = sum_unlisted<DT>(row, p.s2, l_id, l_seen, l_sum);
+                ref = rest.x;
+                l2 = rest.y;
+#pragma unroll
+                for (int u = 0; u < kG; u++) v[u] = no_elements<DT>();
+                if (!zero && rounds) load_round(first_round);
+            }
         }
     }
 
     const uint32_t w_target = !KD && target >= 0 ? ((uint32_t)target + orow.head) / E : kNoWindow;
-    const Pair minus_m = pair(-m, -m), s2 = pair(p.s2, p.s2), minus_l = pair(-l2, -l2), k0 = pair(c0, c0), k1 = pair(c1, c1);
+    const Pair minus_r = pair(-ref, -ref), s2 = pair(p.s2, p.s2), minus_l = pair(-l2, -l2), k0 = pair(c0, c0), k1 = pair(c1, c1);
     // HARD 2: 2^t2 = (2^t)^2 * 2^(2 l2 - l2b)
     const float c2s = HARD == 2 ? c2 * ex2(fmaf(2.f, l2, -l2b)) : c2;
-    const Pair log2e = pair(kLog2e, kLog2e), minus_lb = pair(-l2b, -l2b), k2 = pair(c2s, c2s);
+    const float l2r = HARD == 1 ? fmaf(kLog2e, m - ref, l2b) : l2b;
+    const Pair log2e = pair(kLog2e, kLog2e), minus_lb = pair(-l2r, -l2r), k2 = pair(c2s, c2s);
     auto turn = [&](float (&y)[E]) {
 #pragma unroll
         for (uint32_t j = 0; j < E; j += 2) {
-            const Pair d = add2(pair(y[j], y[j + 1]), minus_m), t = fma2(s2, d, minus_l);
+            const Pair d = add2(pair(y[j], y[j + 1]), minus_r), t = fma2(s2, d, minus_l);
             float t0, t1;
             halves(t, t0, t1);
             const Pair e = pair(ex2(t0), ex2(t1));
@@ -954,7 +1034,7 @@ __global__ void __launch_bounds__(kThreads, KD ? 5 : 6) row_grad_kernel(const Gr
         }
         const float d = xl - m;
         float y = 0.f;
-        if (!zero) y = listed ? listed_c * ex2(fmaf(p.s2, d, -st[1] * kLog2e)) : c0 * ex2(fmaf(p.s2, d, -l2));
+        if (!zero) y = listed ? listed_c * ex2(fmaf(p.s2, d, -st[1] * kLog2e)) : c0 * ex2(fmaf(p.s2, xl - ref, -l2));
         y -= listed_w * q;
         if (HARD) {
             if (!zero) y = fmaf(c2, ex2(fmaf(kLog2e, d, -l2b)), y);
@@ -1021,7 +1101,7 @@ template <int DT, bool ENT, bool TOP, int KD> static int launch_stats(cudaStream
     return check_launch(who);
 }
 
-template <int DT, bool ENT, bool KD, int HARD> static int launch_grad(cudaStream_t s, GradParams &p, const char *who)
+template <int DT, bool ENT, int KD, int HARD> static int launch_grad(cudaStream_t s, GradParams &p, const char *who)
 {
     const int sms = device_sm_count(current_device());
     SFB_REQUIRE(sms > 0, "%s: cannot query the device", who);
@@ -1094,9 +1174,9 @@ extern "C" int sfb_token_logprobs_grad(sfb_stream_t stream, const void *logits, 
     SFB_REQUIRE(!entropy == !dentropy, "%s: entropy and dentropy go together", who);
     SFB_REQUIRE(((uintptr_t)out & (elem_size(dtype) - 1)) == 0 && (out_pitch >= width || rows <= 1), "%s: out is misaligned or its rows overlap", who);
     lg::GradParams p = {logits, out, pitch, out_pitch, rows, vocab, width, 0, 0, scale, scale * lg::kLog2e, targets, stats, dlogp, entropy, dentropy,
-                        nullptr, nullptr, nullptr, nullptr, 0, 0};
+                        nullptr, nullptr, nullptr, nullptr, 0};
     cudaStream_t s = as_stream(stream);
-    return dentropy ? BY_TYPE(dtype, lg::launch_grad, true, false, 0)(s, p, who) : BY_TYPE(dtype, lg::launch_grad, false, false, 0)(s, p, who);
+    return dentropy ? BY_TYPE(dtype, lg::launch_grad, true, 0, 0)(s, p, who) : BY_TYPE(dtype, lg::launch_grad, false, 0, 0)(s, p, who);
 }
 
 extern "C" int sfb_distill_topk(sfb_stream_t stream, const void *logits, uint64_t pitch, const int32_t *ids, const float *teacher, uint32_t rows,
@@ -1127,10 +1207,11 @@ extern "C" int sfb_distill_topk_grad(sfb_stream_t stream, const void *logits, ui
     SFB_REQUIRE(k >= 1 && k <= lg::kMaxList, "%s: %u entries per list (1 to %u)", who, k, lg::kMaxList);
     SFB_REQUIRE(((uintptr_t)out & (elem_size(dtype) - 1)) == 0 && (out_pitch >= width || rows <= 1), "%s: out is misaligned or its rows overlap", who);
     lg::GradParams p = {logits, out, pitch, out_pitch, rows, vocab, width, 0, 0, scale, scale * lg::kLog2e, targets, stats, dlogp, nullptr, nullptr,
-                        ids, teacher, dloss, token_stats, k, tail};
+                        ids, teacher, dloss, token_stats, k};
     cudaStream_t s = as_stream(stream);
-    if (!targets) return BY_TYPE(dtype, lg::launch_grad, false, true, 0)(s, p, who);
-    return scale == 0.5f && !tail ? BY_TYPE(dtype, lg::launch_grad, false, true, 2)(s, p, who) : BY_TYPE(dtype, lg::launch_grad, false, true, 1)(s, p, who);
+    if (tail) return targets ? BY_TYPE(dtype, lg::launch_grad, false, 2, 1)(s, p, who) : BY_TYPE(dtype, lg::launch_grad, false, 2, 0)(s, p, who);
+    if (!targets) return BY_TYPE(dtype, lg::launch_grad, false, 1, 0)(s, p, who);
+    return scale == 0.5f ? BY_TYPE(dtype, lg::launch_grad, false, 1, 2)(s, p, who) : BY_TYPE(dtype, lg::launch_grad, false, 1, 1)(s, p, who);
 }
 
 extern "C" uint64_t sfb_linear_logprobs_workspace(uint32_t m, uint32_t vocab) { return tc_linear_logprobs_workspace(m, vocab); }

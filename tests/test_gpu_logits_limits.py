@@ -30,3 +30,159 @@ def test_shared_rows_one_after_another(sfb, rows, vocab, k):
     for n, g in enumerate(got):
         assert torch.equal(g[4].long(), want[n % 4]["top_ids"]), n
         assert torch.equal(g[3], got[n % 4][3]), n
+
+
+# ---- distillation whose remainder is far below the row's largest logit -------------------------------------------------------
+def divergence(x, ids, teacher, vocab, scale, tail):
+    """The loss of each row in 64 bits from its definition, as something to differentiate: x double [rows, >= vocab].  Sums stand beside their
+    largest logit: the logarithm of a sum, which a logit of -3.4e38 would swallow, is a value by itself."""
+    x = x[:, :vocab]
+
+    def beside_largest(x):
+        top = x.detach().amax(1)
+        return top, torch.where(x > -INF, scale * (x - top[:, None]), -INF)
+    ids, w = ids.long(), teacher.double()
+    ok = (ids >= 0) & (ids < vocab)
+    w = torch.where(ok, w, -INF)
+    lq = w if tail else torch.log_softmax(w, 1)
+    q = lq.exp()
+    m, z = beside_largest(x)
+    l = z.exp().sum(1).log()
+    lp = z.gather(1, torch.where(ok, ids, 0)) - l[:, None]
+    loss = torch.where(q > 0, q * (torch.where(q > 0, lq, 0.0) - lp), 0.0).sum(1)
+    out = {"q": q, "ok": ok, "m": m, "l": l.detach(), "lp": lp.detach(), "z": z.detach()}
+    if tail:
+        there = torch.zeros(x.shape[0], vocab + 1, dtype=torch.bool, device=x.device).scatter_(1, torch.where(ok, ids, vocab), True)[:, :vocab]
+        left = (1 - q.sum(1)).clamp_min(0.0)
+        some = (~there & (x > -INF)).any(1) & (left > 0)
+        mu, zu = beside_largest(torch.where(some[:, None], x.masked_fill(there, -INF), torch.zeros_like(x)))
+        lu = zu.exp().sum(1).log()
+        lr = torch.where(some, scale * (mu - m) + lu, -INF)
+        loss = loss + torch.where(some, left * (left.clamp_min(1e-300).log() - lr + l), 0.0)
+        out.update(left=torch.where(some, left, 0.0), lr=lr.detach(), there=there, some=some, log_share=(zu - lu[:, None]).detach())
+    return loss, out
+
+
+def check_remainder(sfb, x, ids, teacher, vocab, scale, hard=False, seed=3):
+    """Loss, statistics and gradient of lists with the remainder.  With u = 2^-24: the teacher's q, a power each and sums of them in
+    at most 14 additions, are off by 2^-20, and so is what they leave, q_r; the loss gets that much of log p_r, and 2^-22 of each of its
+    terms, and D for either sum (bounds).  A token's p is off by 2^-22 of its exponent, by D, and by what the sum's logarithm is;
+    an unlisted token's share of the remainder by 2^-22 of the base-2 exponent it is made from: the distance to the largest unlisted token, and
+    where the remainder's logarithm is at least -64, the distances of both to the row's largest.  Then a rounding to the type."""
+    rows = x.shape[0]
+    dtype = {v: k for k, v in TYPES.items()}[x.dtype]
+    loss, stats, missed = sfb.distill_topk(x, ids, teacher, vocab=vocab, scale=scale, tail=True)
+    y = x.double().requires_grad_(True)
+    want, more = divergence(y, ids, teacher, vocab, scale, True)
+    d = R.bounds(vocab)
+    l, lr, lp = more["l"], more["lr"], more["lp"]
+    q, left = more["q"], more["left"]
+    size = torch.where(q > 0, q * (lp.abs() + 20), 0.0).sum(1) + torch.where(left > 0, left * (lr.abs() + l + 20), 0.0)
+    lim = (d + 2.0 ** -20) * (1 + size) + 2.0 ** -20 * torch.where(left > 0, lr.abs(), 0.0)
+    assert bool(loss.isfinite().all()) and int(missed) == int((~more["ok"]).sum())
+    assert bool(((loss.double() - want.detach()).abs() <= lim).all()), float(((loss.double() - want.detach()).abs() / lim).max())
+    assert bool(((stats[:, 1].double() - l).abs() <= d + 2.0 ** -22 * l).all())
+    some = more["some"]
+    assert bool(((stats[:, 2].double() - lr)[some].abs() <= d + 2.0 ** -22 * lr[some].abs()).all())
+
+    g = torch.randn(rows, device="cuda", generator=gen(seed))
+    total, args = (g.double() * want).sum(), {}
+    if hard:
+        t = torch.randint(-1, vocab, (rows,), device="cuda", generator=gen(seed + 1), dtype=torch.int32)
+        t[0] = ids[0, 0]
+        b = torch.randn(rows, device="cuda", generator=gen(seed + 2))
+        _, ts, _, _, _, _ = sfb.token_logprobs(x, t, vocab=vocab, entropy=True)
+        args = dict(targets=t, token_stats=ts, dlogp=b)
+        lp1 = torch.log_softmax(y[:, :vocab], 1)
+        total = total + torch.where(t >= 0, b.double() * lp1.gather(1, t.clamp_min(0).long()[:, None])[:, 0], 0.0).sum()
+    total.backward()
+    dx = y.grad[:, :vocab]
+    p, near = (more["z"] - l[:, None]).exp(), lr >= -64
+    share = more["log_share"].exp().masked_fill(more["there"], 0.0)
+    at_share = torch.where(share > 0, more["log_share"].abs(), 0.0) + math.log(vocab) + torch.where(near, 2 * lr.abs(), 0.0)[:, None]
+    at_p = torch.where(p > 0, more["z"].abs(), 0.0) + l[:, None] + torch.where(near, lr.abs(), 0.0)[:, None]
+    w = scale * g.double().abs()[:, None]
+    rel = lambda e: 2.0 ** -22 * (e / math.log(2) + 2) + 2 * d + 2.0 ** -20
+    push = torch.zeros(rows, vocab + 1, dtype=torch.float64, device="cuda").scatter_add_(1, torch.where(more["ok"], ids.long(), vocab), q)[:, :vocab]
+    lim = w * (p * rel(at_p) + left[:, None] * share * rel(at_share) + 2.0 ** -20 * (push + share))
+    if hard:
+        p1, m1 = lp1.detach().exp(), y.detach()[:, :vocab].amax(1, keepdim=True)
+        far = (y.detach()[:, :vocab] - m1).abs().clamp_max(1e4)
+        lim = lim + b.double().abs()[:, None] * (p1 * rel(3 * far + 20) + 2.0 ** -22)
+    lim = lim + R.EPS[x.dtype] * 1.001 * dx.abs() + (2.0 ** -25 if dtype == "f16" else 0) + 2.0 ** -126 * (1 + w)
+    got = sfb.distill_topk_grad(x, ids, teacher, stats, g, vocab=vocab, scale=scale, tail=True, **args)
+    # beyond the type's range a gradient rounds to an infinity (fp16: 0.5 * 10^6 * |g| against 65504 at the largest scale below)
+    beyond = (dx.to(x.dtype).isinf()) & (got[:, :vocab] == dx.to(x.dtype))
+    off = torch.where(beyond, 0.0, (got[:, :vocab].double() - dx).abs())
+    assert bool((off <= lim).all()), "off by %g, %g times the bound" % (float(off.max()), float((off / lim).max()))
+    assert not bool(got[:, vocab:].any())
+    again = x.clone()
+    assert torch.equal(sfb.distill_topk_grad(again, ids, teacher, stats, g, vocab=vocab, scale=scale, tail=True, out=again, **args), got)
+    apart = torch.empty(x.numel() + 1, device="cuda", dtype=x.dtype)[1:].view(x.shape)
+    sfb.distill_topk_grad(x, ids, teacher, stats, g, vocab=vocab, scale=scale, tail=True, out=apart, **args)
+    assert torch.equal(apart, got)
+
+
+def far_lists(rows, vocab, k, seed):
+    """k tokens per row, some of them twice, some no entries, half of the mass or less in the list."""
+    g = gen(seed)
+    ids = torch.rand(rows, vocab, device="cuda", generator=g).topk(k, 1).indices.to(torch.int32)
+    teacher = (torch.log_softmax(torch.randn(rows, k, device="cuda", generator=g), 1) + math.log(0.5)).contiguous()
+    if k > 3:
+        ids[:, 2] = ids[:, 0]
+        ids[-1, 1] = -1
+    return ids.contiguous(), teacher
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("rows,vocab,width,k", [(5, 700, 704, 9), (1, 100003, 100003, 100), (1500, 1003, 1008, 5), (40, 30522, 30528, 64)])
+def test_remainder_far_below(sfb, rows, vocab, width, k, dtype):
+    """Listed logits stand 30 to 3000 above the rest, and some of the rest stand out of it."""
+    ids, teacher = far_lists(rows, vocab, k, rows + k)
+    at = torch.where(ids < 0, ids[:, :1], ids).long()
+    for scale, gap in [(1.0, 30.0), (1.0, 62.0), (1.0, 80.0), (1.0, 88.0), (1.0, 104.0), (1.0, 300.0), (10.0, 9.0), (0.5, 3000.0), (64.0, 20.0)]:
+        x = make(rows, width, dtype, int(gap), spread=0.5)
+        x.scatter_(1, at, make(rows, k, dtype, 1, spread=0.5) + torch.tensor(gap, dtype=x.dtype, device="cuda"))
+        check_remainder(sfb, x, ids, teacher, vocab, scale, hard=scale != 0.5)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_remainder_of_the_lowest_values(sfb, dtype):
+    """Everything that is not listed holds the type's lowest value, or all but one token does; one row has nothing in its list."""
+    rows, vocab, k = 6, 5003, 12
+    ids, teacher = far_lists(rows, vocab, k, 4)
+    x = torch.full((rows, vocab), torch.finfo(TYPES[dtype]).min, device="cuda", dtype=TYPES[dtype])
+    x.scatter_(1, torch.where(ids < 0, ids[:, :1], ids).long(), make(rows, k, dtype, 1))
+    x[1, 77] = -200.0
+    x[2, 78] = 3.0
+    ids[3] = -1
+    for scale in (1.0, 0.5, 0.25):
+        check_remainder(sfb, x, ids, teacher, vocab, scale, hard=scale == 1.0)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+def test_remainder_at_a_large_scale(sfb, dtype):
+    """Products with the scale that reach 10^7: powers are of one token, or of ties."""
+    rows, vocab, k = 9, 3001, 4
+    ids, teacher = far_lists(rows, vocab, k, 4)
+    x = make(rows, vocab, dtype, 2).round_()
+    for scale in (1000.0, 1.0e6):
+        check_remainder(sfb, x, ids, teacher, vocab, scale)
+
+
+def test_remainder_against_differences(sfb):
+    """Central differences of the 64-bit loss (step 1e-5: off by 1e-10 times its third derivative, and by 2^-52 of its value over the step)
+    against the gradient's product with the direction, off by 2e-5 of the sum of absolute products: 2^-22 of exponents up to 92, sums."""
+    rows, vocab, k = 4, 900, 7
+    ids, teacher = far_lists(rows, vocab, k, 9)
+    way = make(rows, vocab, "f32", 5).double()
+    ones = torch.ones(rows, device="cuda")
+    for gap, scale in [(50.0, 1.0), (88.0, 1.0), (150.0, 1.0), (300.0, 1.0), (12.0, 10.0)]:
+        x = make(rows, vocab, "f32", 2, spread=1.0)
+        x[torch.arange(rows, device="cuda")[:, None], torch.where(ids < 0, ids[:, :1], ids).long()] += gap
+        _, stats, _ = sfb.distill_topk(x, ids, teacher, scale=scale, tail=True)
+        got = sfb.distill_topk_grad(x, ids, teacher, stats, ones, scale=scale, tail=True).double()
+        loss = [divergence(x.double() + s * way, ids, teacher, vocab, scale, True)[0] for s in (1e-5, -1e-5)]
+        want = (loss[0] - loss[1]) / 2e-5
+        assert bool((((got * way).sum(1) - want).abs() <= 2e-5 * (got * way).abs().sum(1) + 1e-7).all())
+        assert bool((got.sum(1).abs() <= 2e-5 * got.abs().sum(1)).all())
