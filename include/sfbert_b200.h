@@ -305,8 +305,8 @@ int sfb_token_logprobs_grad(sfb_stream_t stream, const void *logits, uint64_t pi
  *   tail 0: q = softmax(teacher) over the list,            loss = sum_k q_k (log q_k - log p_k)
  *   tail 1: q = exp(teacher), q_r = max(0, 1 - sum_k q_k),  loss = sum_k q_k (log q_k - log p_k) + q_r (log q_r - log p_r)
  * with p_r what the student leaves to the tokens that are not listed: summed over them beside their own largest, however far below the row's
- * that is; where all of them are at -inf the term is left out (a token at the type's lowest value counts).  An id outside [0, vocab) is no entry: its weight is 0, it is counted in *missed (may be NULL).  The same id
- * twice is two entries of one token.  stats [rows][2 + tail] = m, l and with tail the log of the unlisted tokens' sum beside m (-inf
+ * that is; where all of them are at -inf the term is left out (a token at the type's lowest value counts).  An id outside
+ * [0, vocab) is no entry: its weight is 0, it is counted in *missed (may be NULL).  The same id twice is two entries of one token.  stats [rows][2 + tail] = m, l and with tail the log of the unlisted tokens' sum beside m (-inf
  * only where the term is left out).
  * Without tail the list may be log weights of any offset.  The loss carries no factor for the temperature.  vocab is at most 2^30, with
  * tail 2^20. */
@@ -315,9 +315,10 @@ int sfb_distill_topk(sfb_stream_t stream, const void *logits, uint64_t pitch, co
                      uint32_t *missed);
 
 /* Its gradient: out = scale dloss (Q p_j - q_j), Q the sum of the q; with tail, for tokens that are not listed, scale dloss
- * p_j (Q - q_r / p_r).  targets, token_stats and dlogp (all or none): + dlogp (d_jt - p1_j), the hard label's share with p1 the
- * softmax at scale 1 and token_stats its stats [rows][2] from sfb_token_logprobs.  Columns from vocab to width: 0.  out may be
- * logits itself. */
+ * p_j (Q - q_r / p_r); where the remainder's term is left out there is no q_r, neither by itself nor in Q
+ * (a list that holds the whole vocabulary keeps it in Q).  targets, token_stats and dlogp (all or none): + dlogp (d_jt - p1_j),
+ * the hard label's share with p1 the softmax at scale 1 and token_stats its stats [rows][2] from sfb_token_logprobs.  Columns
+ * from vocab to width: 0.  out may be logits itself. */
 int sfb_distill_topk_grad(sfb_stream_t stream, const void *logits, uint64_t pitch, const int32_t *ids, const float *teacher,
                           const float *stats, const float *dloss, const int32_t *targets, const float *token_stats,
                           const float *dlogp, void *out, uint64_t out_pitch, uint32_t rows, uint32_t vocab, uint32_t width,

@@ -771,6 +771,13 @@ template <int DT> __device__ __forceinline__ uint4 load_shifted(const void *x, u
     return make_uint4(v[0], v[1], v[2], v[3]);
 }
 
+// One CTA of at least kMaxList threads: the list names every token of the vocabulary.
+__device__ __noinline__ bool lists_all(const int32_t *ids, uint32_t vocab)
+{
+    bool first = threadIdx.x < kMaxList && ids[threadIdx.x] >= 0;
+    for (uint32_t j = 0; j < threadIdx.x && first; j++) first = ids[j] != ids[threadIdx.x];
+    return (uint32_t)__syncthreads_count(first) == vocab;
+}
 // One CTA: the tokens of a row that are not listed, the largest and the base-2 logarithm of their sum beside it.  ids: kMaxList of them, -1
 // for none.  seen: a bit for each remainder modulo kSeen that a window with a listed token has; a warp looks at such a window together,
 // four entries of the list per lane.  part: one per warp.
@@ -819,6 +826,7 @@ __global__ void __launch_bounds__(kThreads, KD ? 5 : 6) row_grad_kernel(const Gr
 {
     __shared__ __align__(16) int32_t l_id[KD ? kMaxList : 4];
     __shared__ __align__(16) float l_q[KD ? kMaxList : 4];
+    __shared__ float l_x[KD ? kMaxList + 1 : 1];              // the logits of the list's tokens, and of the target; each is its thread's own
     __shared__ uint32_t l_seen[KD == 2 ? kSeen / 32 : 1];
     __shared__ Part l_sum[KD == 2 ? kThreads / 32 : 1];
     __shared__ float2 l_part[kMaxList / 32];                  // a warp's entries: the largest teacher value, the sum of the powers beside it
@@ -860,8 +868,7 @@ __global__ void __launch_bounds__(kThreads, KD ? 5 : 6) row_grad_kernel(const Gr
 
     float c0, c1 = 0.f, c2 = 0.f, l2, l2b = 0.f, target_share = 0.f;
     float ref = m;                                            // what the exponents of the pass are taken beside
-    int32_t id = -1;                                          // KD: this thread's entry of the list
-    float x_listed = 0.f, x_target = 0.f, listed_w = 0.f, listed_c = 0.f;
+    float listed_c = 0.f;
     if (!KD) {
         const float g = target >= 0 ? p.dlogp[r] : 0.f;
         l2 = st[1] * kLog2e;
@@ -873,6 +880,7 @@ __global__ void __launch_bounds__(kThreads, KD ? 5 : 6) row_grad_kernel(const Gr
         }
         target_share = p.scale * g;
     } else {
+        int32_t id = -1;                                      // this thread's entry of the list
         float lq = neg_inf();
         if (tid < p.k) {
             id = p.ids[(size_t)r * p.k + tid];
@@ -889,8 +897,8 @@ __global__ void __launch_bounds__(kThreads, KD ? 5 : 6) row_grad_kernel(const Gr
         }
         // out may be x: what is listed (and the target) is read before anything is written
         auto load_listed = [&]() {
-            if (id >= i_begin && id < i_end && id >= 0) x_listed = load_element<DT>(x, (uint32_t)id);
-            if (HARD && tid == 0 && target >= 0 && target >= i_begin && target < i_end) x_target = load_element<DT>(x, (uint32_t)target);
+            if (id >= i_begin && id < i_end && id >= 0) l_x[tid] = load_element<DT>(x, (uint32_t)id);
+            if (HARD && tid == 0 && target >= 0 && target >= i_begin && target < i_end) l_x[kMaxList] = load_element<DT>(x, (uint32_t)target);
         };
         load_listed();
         const float sw = p.scale * p.dloss[r], l = st[1], lr = KD == 2 ? st[2] : 0.f;
@@ -898,7 +906,6 @@ __global__ void __launch_bounds__(kThreads, KD ? 5 : 6) row_grad_kernel(const Gr
             const float g = target >= 0 ? p.dlogp[r] : 0.f;
             c2 = -g;
             l2b = p.token_stats[2 * (size_t)r + 1] * kLog2e;
-            target_share = g;
         }
         __syncthreads();
         float mq = KD == 2 ? 0.f : neg_inf(), z = 0.f;
@@ -908,14 +915,16 @@ __global__ void __launch_bounds__(kThreads, KD ? 5 : 6) row_grad_kernel(const Gr
         const bool none = mq == neg_inf();
         if (tid < kMaxList) l_q[tid] = lq == neg_inf() || none ? 0.f : ex2(kLog2e * (lq - mq)) * (KD == 2 ? 1.f : 1.f / z);
         const float left = KD == 2 ? fmaxf(0.f, 1.f - z) : 0.f, all = KD == 2 ? z + left : none ? 0.f : 1.f;
-        listed_w = sw;
         listed_c = sw * all;
         l2 = l * kLog2e;
         c0 = sw * all;
         if (KD == 2) {
             // unlisted tokens: all * p - left * p / p_rest, as a multiple of their share of the remainder
             if (lr == neg_inf()) {
-                c0 = 0.f;                                     // every unlisted one has a probability of 0
+                // Every unlisted one has a probability of 0, the loss has no term for the remainder, and neither has its gradient.  (A list that
+                // holds the whole vocabulary keeps q_r in Q: no token is there to take it, and nothing goes to one.)
+                if (!(p.k >= p.vocab && lists_all(l_id, p.vocab))) listed_c = sw * z;
+                c0 = 0.f;
             } else {
                 c0 = sw * (all * expf(lr - l) - left);
                 l2 = lr * kLog2e;
@@ -1021,6 +1030,7 @@ __global__ void __launch_bounds__(kThreads, KD ? 5 : 6) row_grad_kernel(const Gr
     // What is listed, and the target: made again from all the shares it has.  A token that stands in the list twice is
     // written twice, with the same value.
     __syncthreads();
+    const float listed_w = p.scale * p.dloss[r], l2_listed = st[1] * kLog2e, l2_hard = HARD ? p.token_stats[2 * (size_t)r + 1] * kLog2e : 0.f;
     auto again = [&](int32_t token, float xl) {
         float q = 0.f;
         bool listed = false;
@@ -1034,16 +1044,17 @@ __global__ void __launch_bounds__(kThreads, KD ? 5 : 6) row_grad_kernel(const Gr
         }
         const float d = xl - m;
         float y = 0.f;
-        if (!zero) y = listed ? listed_c * ex2(fmaf(p.s2, d, -st[1] * kLog2e)) : c0 * ex2(fmaf(p.s2, xl - ref, -l2));
+        if (!zero) y = listed ? listed_c * ex2(fmaf(p.s2, d, -l2_listed)) : c0 * ex2(fmaf(p.s2, xl - ref, -l2));
         y -= listed_w * q;
         if (HARD) {
-            if (!zero) y = fmaf(c2, ex2(fmaf(kLog2e, d, -l2b)), y);
-            if (token == target) y += target_share;
+            if (!zero) y = fmaf(c2, ex2(fmaf(kLog2e, d, -l2_hard)), y);
+            if (token == target) y -= c2;
         }
         store_element<DT>(out, (uint32_t)token, y);
     };
-    if (id >= 0 && id >= i_begin && id < i_end) again(id, x_listed);
-    if (HARD && tid == 0 && target >= 0 && target >= i_begin && target < i_end) again(target, x_target);
+    const int32_t id = tid < kMaxList ? l_id[tid] : -1;
+    if (id >= 0 && id >= i_begin && id < i_end) again(id, l_x[tid]);
+    if (HARD && tid == 0 && target >= 0 && target >= i_begin && target < i_end) again(target, l_x[kMaxList]);
 }
 
 // ---- launches -----------------------------------------------------------------------------------------------------------

@@ -98,7 +98,7 @@ def check_remainder(sfb, x, ids, teacher, vocab, scale, hard=False, seed=3):
     total.backward()
     dx = y.grad[:, :vocab]
     p, near = (more["z"] - l[:, None]).exp(), lr >= -64
-    share = more["log_share"].exp().masked_fill(more["there"], 0.0)
+    share = more["log_share"].exp().masked_fill(more["there"] | ~more["some"][:, None], 0.0)
     at_share = torch.where(share > 0, more["log_share"].abs(), 0.0) + math.log(vocab) + torch.where(near, 2 * lr.abs(), 0.0)[:, None]
     at_p = torch.where(p > 0, more["z"].abs(), 0.0) + l[:, None] + torch.where(near, lr.abs(), 0.0)[:, None]
     w = scale * g.double().abs()[:, None]
@@ -158,6 +158,25 @@ def test_remainder_of_the_lowest_values(sfb, dtype):
     ids[3] = -1
     for scale in (1.0, 0.5, 0.25):
         check_remainder(sfb, x, ids, teacher, vocab, scale, hard=scale == 1.0)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("rows,vocab,width,k", [(5, 700, 704, 9), (300, 20011, 20011, 40)])
+def test_remainder_of_nothing(sfb, rows, vocab, width, k, dtype):
+    """Every token that is not listed is banned: the loss has no term for the remainder, and its gradient, whose sum over a row is 0, neither.
+    One row has a token besides, and one a listed token that is banned, of weight 0."""
+    ids, teacher = far_lists(rows, vocab, k, 5)
+    x = torch.full((rows, width), -INF, device="cuda", dtype=TYPES[dtype])
+    x.scatter_(1, torch.where(ids < 0, ids[:, :1], ids).long(), make(rows, k, dtype, 1))
+    x[1, :vocab][torch.ones(vocab, dtype=torch.bool, device="cuda").scatter_(0, ids[1].long(), False).nonzero()[7]] = 1.0
+    x[2, ids[2, 4].long()], teacher[2, 4] = -INF, -INF
+    for scale in (1.0, 0.5):
+        check_remainder(sfb, x, ids, teacher, vocab, scale, hard=scale == 1.0)
+        _, stats, _ = sfb.distill_topk(x, ids, teacher, vocab=vocab, scale=scale, tail=True)
+        assert torch.equal(stats[:, 2] == -INF, torch.arange(rows, device="cuda") != 1)
+        got = sfb.distill_topk_grad(x, ids, teacher, stats, torch.ones(rows, device="cuda"), vocab=vocab, scale=scale, tail=True).double()
+        # k entries, each rounded to the type, and the shares' own 2^-18
+        assert bool((got.sum(1).abs() <= (R.EPS[x.dtype] + 2.0 ** -18) * got.abs().sum(1) + 1e-7).all())
 
 
 @pytest.mark.parametrize("dtype", ["f32", "f16"])
