@@ -1023,7 +1023,8 @@ __global__ void __launch_bounds__(kThreads, KD ? 5 : 6) row_grad_kernel(const Gr
 #pragma unroll
         for (uint32_t j = 0; j < E; j++) {
             const uint32_t pos = w * E + j;
-            if (pos >= orow.head && pos < orow.end) store_element<DT>(out, pos - orow.head, y[j]);
+            // behind the vocabulary it is 0 whatever the row's factors are (times which a probability of 0 may be NaN)
+            if (pos >= orow.head && pos < orow.end) store_element<DT>(out, pos - orow.head, pos - orow.head < p.vocab ? y[j] : 0.f);
         }
     }
     if (!KD) return;

@@ -205,3 +205,41 @@ def test_remainder_against_differences(sfb):
         want = (loss[0] - loss[1]) / 2e-5
         assert bool((((got * way).sum(1) - want).abs() <= 2e-5 * (got * way).abs().sum(1) + 1e-7).all())
         assert bool((got.sum(1).abs() <= 2e-5 * got.abs().sum(1)).all())
+
+
+# ---- rows whose gradient is not finite ---------------------------------------------------------------------------------------
+def gradients(sfb, x, vocab, scale, targets, ids, teacher, g):
+    """All of the gradients of some logits, by name: g is every factor that comes from behind."""
+    _, stats, ent, _, _, _ = sfb.token_logprobs(x, targets, vocab=vocab, scale=scale, entropy=True)
+    _, ts, _, _, _, _ = sfb.token_logprobs(x, targets, vocab=vocab, entropy=True)
+    out = {"tokens": sfb.token_logprobs_grad(x, targets, stats, g, vocab=vocab, scale=scale),
+           "entropy": sfb.token_logprobs_grad(x, targets, stats, g, ent, g, vocab=vocab, scale=scale)}
+    for tail in (False, True):
+        _, st, _ = sfb.distill_topk(x, ids, teacher, vocab=vocab, scale=scale, tail=tail)
+        out["list", tail] = sfb.distill_topk_grad(x, ids, teacher, st, g, vocab=vocab, scale=scale, tail=tail)
+        out["hard", tail] = sfb.distill_topk_grad(x, ids, teacher, st, g, vocab=vocab, scale=scale, tail=tail, targets=targets, token_stats=ts, dlogp=g)
+    return out
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("rows,vocab,width", [(8, 997, 1008), (8, 30522, 30528), (600, 1003, 1003 + 37), (8, 4, 40)])
+def test_padding_of_rows_that_are_not_finite(sfb, rows, vocab, width, dtype):
+    """Columns behind the vocabulary get 0 whatever a row holds or is given; the other rows' gradients are what they are without it."""
+    x = make(rows, width, dtype, 1)
+    x[:, vocab:] = INF
+    k = min(4, vocab - 1)
+    ids, teacher = far_lists(rows, vocab, k, 3)
+    t = torch.randint(0, vocab, (rows,), device="cuda", generator=gen(2), dtype=torch.int32)
+    g = torch.randn(rows, device="cuda", generator=gen(4))
+    for scale in (1.0, 0.5):
+        plain = gradients(sfb, x, vocab, scale, t, ids, teacher, g)
+        y, h = x.clone(), g.clone()
+        y[0, 1], y[1, vocab - 1], y[2, :vocab], y[3, 1] = math.nan, INF, -INF, -INF
+        h[4], h[5], h[6] = INF, -INF, math.nan
+        bad = torch.arange(rows, device="cuda") < 7
+        for name, got in gradients(sfb, y, vocab, scale, t, ids, teacher, h).items():
+            assert not bool(got[:, vocab:].any()), name
+            assert torch.equal(got[~bad], plain[name][~bad]), name
+            assert bool(got[[0, 1, 6], :vocab].isnan().all()), name
+            assert bool((~got[4:6, :vocab].isfinite()).any(1).all()), name
+            assert bool(got[2:4, :vocab].isfinite().all()), name
