@@ -5,6 +5,7 @@ import pytest
 
 torch = pytest.importorskip("torch")
 import logits_reference as R  # noqa: E402
+import test_gpu_logits as G  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 TYPES = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
@@ -243,3 +244,83 @@ def test_padding_of_rows_that_are_not_finite(sfb, rows, vocab, width, dtype):
             assert bool(got[[0, 1, 6], :vocab].isnan().all()), name
             assert bool((~got[4:6, :vocab].isfinite()).any(1).all()), name
             assert bool(got[2:4, :vocab].isfinite().all()), name
+
+
+# ---- banned tokens, and factors of both softmaxes ----------------------------------------------------------------------------
+def bounds_of(x, t, vocab, size, share, want):
+    r = dict(R.token_logprobs(x, t, vocab, 1.0))
+    r["l"] = r["l"].clamp_min(0.0)                                       # a row without a token has no sum, and no probability either
+    return G.grad_bound(size, share, want, r, vocab, {v: k for k, v in TYPES.items()}[x.dtype])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("rows,vocab,width", [(9, 700, 704), (9, 30522, 30528), (1400, 1003, 1003)])
+def test_gradients_of_banned_tokens(sfb, rows, vocab, width, dtype):
+    """-inf and the type's lowest value in a third of the columns each, among them a target; one row has nothing but -inf, one a single token."""
+    x = make(rows, width, dtype, vocab)
+    for r, value in ((0, -INF), (1, torch.finfo(TYPES[dtype]).min), (rows - 1, -INF)):
+        x[r, ::3] = value
+    x[2:4] = -INF
+    x[3, 5] = 1.0
+    x[4:, 1::3] = torch.finfo(TYPES[dtype]).min
+    x[4:, 2::3] = -INF
+    t = torch.randint(-1, vocab, (rows,), device="cuda", generator=gen(5), dtype=torch.int32)
+    t[:5] = torch.tensor([3, 6, 7, 5, 2], device="cuda")
+    a, b = torch.randn(rows, device="cuda", generator=gen(8)), torch.randn(rows, device="cuda", generator=gen(9))
+    for scale, h in [(1.0, None), (1.0, b), (0.25, b)]:
+        _, stats, ent, _, _, _ = sfb.token_logprobs(x, t, vocab=vocab, scale=scale, entropy=True)
+        got = sfb.token_logprobs_grad(x, t, stats, a, ent if h is not None else None, h, vocab=vocab, scale=scale)
+        want, size, _, share = R.token_grad(x, t, a, h, vocab, scale)
+        G.same(got[:, :vocab], want, bounds_of(x, t, vocab, size, share, want), "gradient")
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("tail", [False, True])
+@pytest.mark.parametrize("rows,vocab,width,k", [(9, 700, 704, 12), (9, 30522, 30528, 64), (1400, 1003, 1003, 5)])
+def test_distillation_with_banned_tokens(sfb, rows, vocab, width, k, tail, dtype):
+    """The student's banned tokens beside the list's (rows 0 and 1), among them (2: a loss of +inf), and everywhere (3), at the temperatures
+    where the hard label's softmax is a power of the student's and at one where it is not."""
+    x = make(rows, width, dtype, k)
+    ids, teacher = far_lists(rows, vocab, k, 6)
+    listed = torch.zeros(rows, vocab + 1, dtype=torch.bool, device="cuda").scatter_(1, torch.where(ids < 0, vocab, ids).long(), True)[:, :vocab]
+    third = torch.arange(vocab, device="cuda") % 3 == 0
+    for r, value in ((0, -INF), (1, torch.finfo(TYPES[dtype]).min)):
+        x[r, :vocab][third & ~listed[r]] = value
+    x[2, ids[2, 3].long()] = -INF
+    x[3] = -INF
+    t = torch.randint(-1, vocab, (rows,), device="cuda", generator=gen(5), dtype=torch.int32)
+    t[0], t[4], t[5] = 3, ids[4, 1], ids[5, 0]
+    a, b = torch.randn(rows, device="cuda", generator=gen(8)), torch.randn(rows, device="cuda", generator=gen(9))
+    _, ts, _, _, _, _ = sfb.token_logprobs(x, t, vocab=vocab)
+    d = R.bounds(vocab)
+    for scale in (1.0, 0.5, 0.25, 0.375):
+        loss, stats, missed = sfb.distill_topk(x, ids, teacher, vocab=vocab, scale=scale, tail=tail)
+        want = R.distill(x, ids, teacher, vocab, scale, tail)
+        want["loss"][3] = INF                                            # no token has a probability
+        assert int(missed) == want["missed"] and bool(want["loss"][2:4].isinf().all())
+        G.same(loss, want["loss"], (d + 2.0 ** -20) * (1 + want["size"].nan_to_num(0, 0, 0)), "loss")
+        G.same(stats[:, 1], want["l"], d, "l")
+        for hard in (False, True):
+            more = dict(targets=t, token_stats=ts, dlogp=a) if hard else {}
+            got = sfb.distill_topk_grad(x, ids, teacher, stats, b, vocab=vocab, scale=scale, tail=tail, **more)
+            ref, size, share = R.distill_grad(x, ids, teacher, b, vocab, scale, tail, t if hard else None, a if hard else None)
+            # beside the gradients' bounds: the list's probabilities are off by 2^-20 of themselves, the remainder by 2^-22 of 1
+            tol = bounds_of(x, t, vocab, size, share, ref) + 2.0 ** -20 * size + (scale * b.double().abs()[:, None]) * 2.0 ** -22 * tail
+            G.same(got[:, :vocab], ref, tol, "gradient")
+            assert not bool(got[:, vocab:].any())
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("rows", [4, 1400])
+def test_distillation_of_rows_that_are_not_finite(sfb, rows, dtype):
+    vocab, k = 5001, 10
+    ids, teacher = far_lists(rows, vocab, k, 6)
+    x = make(rows, vocab, dtype, 2)
+    for at in (ids[1, 1].item(), (ids[1].amax().item() + 1) % vocab):    # a listed token, and (the odds are) another one
+        for value in (math.nan, INF):
+            y = x.clone()
+            y[1, at] = value
+            for tail in (False, True):
+                loss, stats, _ = sfb.distill_topk(y, ids, teacher, tail=tail)
+                bad = torch.arange(rows, device="cuda") == 1
+                assert torch.equal(loss.isnan(), bad) and torch.equal(stats[:, 1:].isnan().all(1), bad) and torch.equal(stats[:, 1:].isnan().any(1), bad)
