@@ -304,12 +304,12 @@ int sfb_token_logprobs_grad(sfb_stream_t stream, const void *logits, uint64_t pi
  * probabilities at the temperature (what sfb_token_logprobs gives as alternatives); logits are the student's, p their softmax:
  *   tail 0: q = softmax(teacher) over the list,            loss = sum_k q_k (log q_k - log p_k)
  *   tail 1: q = exp(teacher), q_r = max(0, 1 - sum_k q_k),  loss = sum_k q_k (log q_k - log p_k) + q_r (log q_r - log p_r)
- * with p_r what the student leaves to the tokens that are not listed: summed over them beside their own largest, however far below the row's
- * that is; where all of them are at -inf the term is left out (a token at the type's lowest value counts).  An id outside
- * [0, vocab) is no entry: its weight is 0, it is counted in *missed (may be NULL).  The same id twice is two entries of one token.  stats [rows][2 + tail] = m, l and with tail the log of the unlisted tokens' sum beside m (-inf
- * only where the term is left out).
- * Without tail the list may be log weights of any offset.  The loss carries no factor for the temperature.  vocab is at most 2^30, with
- * tail 2^20. */
+ * with p_r what the student leaves to the tokens that are not listed: summed over them beside their own largest, however far
+ * below the row's that is; where all of them are at -inf the term is left out (a token at the type's lowest value counts).  An id outside
+ * [0, vocab) is no entry: its weight is 0, it is counted in *missed (may be NULL).  The same id twice is two entries of one
+ * token.  A listed token of weight that the student bans (-inf) makes the loss +inf.  stats [rows][2 + tail] = m, l and with tail
+ * the log of the unlisted tokens' sum beside m (-inf only where all of them are at -inf, or there are none).  Without tail the list
+ * may be log weights of any offset.  The loss carries no factor for the temperature.  vocab is at most 2^30, with tail 2^20. */
 int sfb_distill_topk(sfb_stream_t stream, const void *logits, uint64_t pitch, const int32_t *ids, const float *teacher,
                      uint32_t rows, uint32_t vocab, uint32_t k, int dtype, float scale, int tail, float *loss, float *stats,
                      uint32_t *missed);
@@ -326,7 +326,8 @@ int sfb_distill_topk_grad(sfb_stream_t stream, const void *logits, uint64_t pitc
 
 /* sfb_token_logprobs of logits = x . table^T + bias that are never written (nor rounded to 16 bits): x [m, k] and table [vocab, k] of
  * type dtype (SFB_BF16 or SFB_F16), row-major, 16-byte aligned, k a multiple of 8; bias fp32 [vocab] or NULL; any vocab of at least 1.
- * logp, stats, entropy (or NULL) and *missed (or NULL) as there, without alternatives.  workspace: device memory of
+ * logp, stats, entropy (or NULL) and *missed (or NULL) as there, without alternatives.  The logits are the tensor cores' fp32 sums, which
+ * drop what their additions shift out: 1.2e-6 of their norm from 64 bits at k = 1024 (a plain fp32 product: 0.6e-6).  workspace: device memory of
  * sfb_linear_logprobs_workspace(m, vocab) bytes, 16-byte aligned, for this call alone. */
 uint64_t sfb_linear_logprobs_workspace(uint32_t m, uint32_t vocab);
 int sfb_linear_logprobs(sfb_stream_t stream, const void *x, const void *table, const float *bias, const int32_t *targets,

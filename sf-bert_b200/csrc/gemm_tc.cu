@@ -198,7 +198,7 @@ __device__ __forceinline__ void drain_rows_staged(const GParams &p, const CUtens
 // place.  A thread has a whole row of the tile, so nothing is exchanged.  The loop is short on purpose: unrolled, with the next 32
 // columns on their way, it ran out of the instruction cache (a tile of 256 columns 5900 cycles, now 5400; its MMAs take 6100 at
 // k = 768, so the scores are bound by the product from there on, by this loop below).  4096 x 30522 x 768: 121 us by itself with the
-// tensor pipe 79 % busy, 150 under the power cap, and 5 for the join.  The accumulators are fp32 but drop what their additions
+// tensor pipe 79 % busy, and 5 for the join; a call 137 us in a short burst, 165 under the power cap.  The accumulators are fp32 but drop what their additions
 // shift out: logits end up 1.2e-6 of their norm from 64 bits at k = 1024, those of an fp32 product 0.5e-6.
 template <bool ENT, typename Release>
 __device__ __forceinline__ void score_rows(const GParams &p, uint32_t tcol, const float *bias, uint32_t row, uint32_t target, uint32_t tile_n, uint32_t chalf,

@@ -375,10 +375,11 @@ template <int KD> __device__ __forceinline__ void finish_lists(const StatParams 
 // A row's statistics, and what is made of them.  One CTA per row, or a cluster of CTAs where there are few rows: each
 // takes every C-th piece, and CTA 0 joins the parts.  KD: 0 tokens, 1 lists, 2 lists with the remainder as one more class.
 // Many rows are bound by the pass: 9 instructions and an exponential per element with entropy and alternatives, the issue slots
-// 72 % and the exponential unit 66 % busy beside 5.2 TB/s from memory (2048 rows of 131072 bf16, 103 us).  8192 such rows take 385 us,
-// 4096 of 30522 (without entropy) 44, 86 % of what a copy's rate allows both.  Fewer rows are bound by what comes one after another:
+// 72 % and the exponential unit 66 % busy beside 5.2 TB/s from memory (2048 rows of 131072 bf16, 103 us).  8192 such rows take 355 us in a short
+// burst and 421 under the power cap, when passes follow each other: 93 and 78 % of what a copy's rate allows; 4096 of 30522 (without entropy) 46, 83 %.  Fewer rows are bound by what comes one after another:
 // launch, the first loads, the join of a cluster's CTAs over their barrier (about 1000 cycles), and for alternatives their bound, the
-// second look and the ranks: one row of 30522 bf16 takes 3.1 us, with 20 alternatives 5.5, 64 rows of 100003 fp16 8.2.
+// second look and the ranks: one row of 30522 bf16 takes 2.6 us, with entropy and 20 alternatives 5.3, 64 rows of 100003 fp16 with 5 8.1; a
+// call from the host 6.7 and 10.1 of the last two.
 // Rows streamed through a ring of bulk copies by CTAs that stay were built, too: the loads then never pause, but
 // the warps that add up waited at every row's end for the one that finishes it, and the same rows took 59 us instead of 44.
 template <int DT, bool ENT, bool TOP, int KD>
@@ -781,7 +782,7 @@ __device__ __noinline__ bool lists_all(const int32_t *ids, uint32_t vocab)
 // One CTA: the tokens of a row that are not listed, the largest and the base-2 logarithm of their sum beside it.  ids: kMaxList of them, -1
 // for none.  seen: a bit for each remainder modulo kSeen that a window with a listed token has; a warp looks at such a window together,
 // four entries of the list per lane.  part: one per warp.
-// 257 rows of 50021 fp32 whose remainders are all far away, lists of 128: the gradient takes 70 us, 29 otherwise; 4096 of 30522 bf16, lists of 64, 180 and 102.
+// 257 rows of 50021 fp32 whose remainders are all far away, lists of 128: the gradient takes 70 us, 29 otherwise; 4096 of 30522 bf16, lists of 64, 182 and 102 (L2 flushed).
 constexpr uint32_t kSeen = 8192;
 template <int DT> __device__ __noinline__ float2 sum_unlisted(const Row<DT> row, float s2, const int32_t *ids, const uint32_t *seen, Part *part)
 {
@@ -815,12 +816,12 @@ template <int DT> __device__ __noinline__ float2 sum_unlisted(const Row<DT> row,
 }
 
 // A row (or a part of it) per CTA, a round of kG windows per thread at a time: loaded, turned into the gradient and stored.  Bound by
-// memory: 8192 rows of 30522 bf16 157 us, 97 % of a copy's rate; lists and hard labels add a prologue to each row (4096 rows:
-// 93 us, 82 %).
+// memory: 8192 rows of 30522 bf16 156 us in a short burst, 162 when passes follow each other, 98 and 95 % of a copy's rate; lists and hard
+// labels add a prologue to each row (4096 rows: 94 and 100 us, 82 and 77 %).
 // dx = p (c0 + c1 t) with t the base-2 logarithm of p, plus the given target's share (KD 0, ENT: c1 is not 0);
 // dx = c0 2^t + c2 2^t2, what is listed made again by itself (KD 1, and 2 with the remainder; HARD 1: c2 is not 0).  HARD 2: at temperature 2 the
 // second power, the softmax's at temperature 1, is the first one's square times a constant of the row (which goes to c2), and an
-// exponential per element less: 4096 rows of 30522 bf16 with lists of 64, 107 -> 100 us.
+// exponential per element less: 4096 rows of 30522 bf16 with lists of 64 take 104.5 us at scale 0.5, 108.5 at any other (L2 flushed).
 template <int DT, bool ENT, int KD, int HARD, bool SAME>
 __global__ void __launch_bounds__(kThreads, KD ? 5 : 6) row_grad_kernel(const GradParams p)
 {
@@ -988,7 +989,7 @@ __global__ void __launch_bounds__(kThreads, KD ? 5 : 6) row_grad_kernel(const Gr
         }
     } else {
         // Rows start at different rounds: with all of them at the same column, reads and writes crowded the same memory channels
-        // (8192 rows of 30522 bf16: 195 us so, 158 now).
+        // (8192 rows of 30522 bf16: 195 us so, 158 with it).
         for (uint32_t i = 0, round = first_round; i < rounds; i++) {
             const uint32_t w0 = a_begin + round * (kG * T) + tid;
             round = round + 1 == rounds ? 0 : round + 1;
@@ -1087,7 +1088,9 @@ template <int DT, bool ENT, bool TOP, int KD> static int launch_stats(cudaStream
     if (((TOP && p.k <= 32) || (KD == 2 && p.k <= 64)) && windows <= 1024 && p.rows >= (uint32_t)sms * 8) T = 64;
     uint32_t C = 1;
     // CTAs per row, while each has more than a group of windows: as many as there are SMs without one, and a few for every SM where
-    // each has two groups.  (Alternatives: CTA 0 ranks what all of them find.)
+    // each has two groups.  With alternatives CTA 0 ranks what all of them find, at least k from each, in time that grows as the square: from
+    // 40 on that costs more than a shorter pass gives (rows of 131072: one row with 20 in four CTAs 7.8 us, in eight 7.7; 40 in two 10.5, in eight
+    // 12.9; 64 in one 14.1, in eight 25.3; 64 rows with 20 in four 9.6, in eight 12.8).
     while (C < kMaxCluster && windows > C * kU * T && (!TOP || C * p.k <= 40)) {
         const uint64_t ctas = (uint64_t)p.rows * C * 2;
         if (ctas > (uint64_t)sms && (2 * ctas > 7 * (uint64_t)sms || windows < 2 * C * 2 * kU * T)) break;
