@@ -327,16 +327,17 @@ def token_logprobs(logits, targets=None, vocab=None, scale=1.0, entropy=False, t
     read (stats 0) unless entropy or alternatives are asked for.  To score each token by the logits before it, shift the targets and give
     each sequence's last row the target -1: logits[:, :-1] has no single pitch.
 
-    The results of a call that has less than 64 KB of them, here and below, are views of one allocation: keeping (or saving) one keeps them
-    all; clone() what is kept for long."""
+    The results of a call that has at most 64 KB of them, here and in the forward calls below, are views of one allocation: keeping
+    (or saving) one keeps them all; clone() what is kept for long."""
     return _host.token_logprobs(logits, targets, vocab, scale, entropy, top_k)
 
 
 def token_logprobs_grad(logits, targets, stats, dlogp, entropy=None, dentropy=None, vocab=None, scale=1.0, out=None):
     """The gradient of token_logprobs' logp and entropy with respect to the logits (in their type and layout; out may be logits):
     scale * (dlogp * (onehot - p) - dentropy * p * (log p + entropy)).  dlogp and dentropy are fp32 [...]; columns from vocab on
-    get 0.  The alternatives' log probabilities have no gradient.  An out that starts elsewhere in its 16 bytes than the logits' rows do (a
-    fresh one for logits[1:] of an odd width) is written element by element: up to four times as long in 16 bits."""
+    get 0.  The alternatives' log probabilities have no gradient.  An out whose rows start elsewhere in
+    their 16 bytes than the logits' do (a fresh one for logits[1:] of an odd width) is written element by element, which takes up to
+    four times as long in 16 bits."""
     return _host.token_logprobs_grad(logits, targets, stats, dlogp, entropy, dentropy, vocab, scale, out)
 
 
@@ -344,8 +345,9 @@ def distill_topk(logits, ids, teacher, vocab=None, scale=1.0, tail=False):
     """KL divergence of the student's softmax(scale * logits) from a teacher's list of at most 128 tokens: ids int32 [..., k] and
     teacher fp32 [..., k], their log probabilities at the temperature (token_logprobs(teacher_logits, scale=scale, top_k=k)).
     The list is renormalised, or with tail=True what it leaves is one more class beside what the student leaves to unlisted
-    tokens (left out of loss and gradient where all of those are at -inf).  Ids outside [0, vocab) are no entries (lists of uneven length) and are counted.  Returns (loss [...],
-    stats [..., 2] or with tail [..., 3], missed).  The loss has no factor for the temperature."""
+    tokens (left out of loss and gradient where all of those are at -inf).  Ids outside [0, vocab) are no entries (lists of uneven
+    length) and are counted.  Returns (loss [...], stats [..., 2] or with tail [..., 3], missed).  The loss has no factor for the
+    temperature."""
     return _host.distill_topk(logits, ids, teacher, vocab, scale, tail)
 
 
@@ -359,9 +361,9 @@ def distill_topk_grad(logits, ids, teacher, stats, dloss, vocab=None, scale=1.0,
 def linear_logprobs(x, table, targets, bias=None, vocab=None, scale=1.0, entropy=False):
     """token_logprobs(linear_nt(x, table, bias), targets) without the logits: scores of given tokens straight from hidden states
     x [..., k] over the (tied) table [n, k], 16-bit, k a multiple of 8.  Only the first vocab rows of the table are tokens (None: all;
-    any number).  The logits are the tensor cores' fp32 sums, neither rounded nor stored: they drop what their additions shift out, 1.2e-6 of
-    their norm from 64 bits at k = 1024 (a plain fp32 product: 0.6e-6).  There is no gradient; training goes through linear_nt's logits.  Returns (logp, stats, entropy or
-    None, missed) as token_logprobs does."""
+    any number).  The logits are the tensor cores' fp32 sums, neither rounded nor stored: they drop what their additions
+    shift out, 1.2e-6 of their norm from 64 bits at k = 1024 (a plain fp32 product: 0.6e-6).  There is no gradient; training goes
+    through linear_nt's logits.  Returns (logp, stats, entropy or None, missed) as token_logprobs does."""
     return _host.linear_logprobs(x, table, targets, bias, vocab, scale, entropy)
 
 

@@ -376,7 +376,8 @@ template <int KD> __device__ __forceinline__ void finish_lists(const StatParams 
 // takes every C-th piece, and CTA 0 joins the parts.  KD: 0 tokens, 1 lists, 2 lists with the remainder as one more class.
 // Many rows are bound by the pass: 9 instructions and an exponential per element with entropy and alternatives, the issue slots
 // 72 % and the exponential unit 66 % busy beside 5.2 TB/s from memory (2048 rows of 131072 bf16, 103 us).  8192 such rows take 355 us in a short
-// burst and 421 under the power cap, when passes follow each other: 93 and 78 % of what a copy's rate allows; 4096 of 30522 (without entropy) 46, 83 %.  Fewer rows are bound by what comes one after another:
+// burst and 421 under the power cap, when passes follow each other: 93 and 78 % of what a copy's rate allows; 4096 of 30522
+// (without entropy) 46, 83 %.  Fewer rows are bound by what comes one after another:
 // launch, the first loads, the join of a cluster's CTAs over their barrier (about 1000 cycles), and for alternatives their bound, the
 // second look and the ranks: one row of 30522 bf16 takes 2.6 us, with entropy and 20 alternatives 5.3, 64 rows of 100003 fp16 with 5 8.1; a
 // call from the host 6.7 and 10.1 of the last two.
@@ -782,7 +783,8 @@ __device__ __noinline__ bool lists_all(const int32_t *ids, uint32_t vocab)
 // One CTA: the tokens of a row that are not listed, the largest and the base-2 logarithm of their sum beside it.  ids: kMaxList of them, -1
 // for none.  seen: a bit for each remainder modulo kSeen that a window with a listed token has; a warp looks at such a window together,
 // four entries of the list per lane.  part: one per warp.
-// 257 rows of 50021 fp32 whose remainders are all far away, lists of 128: the gradient takes 70 us, 29 otherwise; 4096 of 30522 bf16, lists of 64, 182 and 102 (L2 flushed).
+// With L2 flushed, 257 rows of 50021 fp32 and lists of 128 take 70 us where all remainders are far away, 29 where none is; 4096 of 30522 bf16 and
+// lists of 64 182 and 102.
 constexpr uint32_t kSeen = 8192;
 template <int DT> __device__ __noinline__ float2 sum_unlisted(const Row<DT> row, float s2, const int32_t *ids, const uint32_t *seen, Part *part)
 {
