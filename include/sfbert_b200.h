@@ -327,7 +327,8 @@ int sfb_distill_topk_grad(sfb_stream_t stream, const void *logits, uint64_t pitc
 /* sfb_token_logprobs of logits = x . table^T + bias that are never written (nor rounded to 16 bits): x [m, k] and table [vocab, k] of
  * type dtype (SFB_BF16 or SFB_F16), row-major, 16-byte aligned, k a multiple of 8; bias fp32 [vocab] or NULL; any vocab of at least 1.
  * logp, stats, entropy (or NULL) and *missed (or NULL) as there, without alternatives.  The logits are the tensor cores' fp32 sums, which
- * drop what their additions shift out: 1.2e-6 of their norm from 64 bits at k = 1024 (a plain fp32 product: 0.6e-6).  workspace: device memory of
+ * drop what their additions shift out: 7e-7 of their norm from 64 bits at k = 768, 2e-6 at 2048 (a plain fp32 product: 2 to 5e-7).  Up
+ * to 128 rows sums of more than 512 products are put together from pieces of 512: 5e-7.  workspace: device memory of
  * sfb_linear_logprobs_workspace(m, vocab) bytes, 16-byte aligned, for this call alone. */
 uint64_t sfb_linear_logprobs_workspace(uint32_t m, uint32_t vocab);
 int sfb_linear_logprobs(sfb_stream_t stream, const void *x, const void *table, const float *bias, const int32_t *targets,

@@ -362,8 +362,8 @@ def linear_logprobs(x, table, targets, bias=None, vocab=None, scale=1.0, entropy
     """token_logprobs(linear_nt(x, table, bias), targets) without the logits: scores of given tokens straight from hidden states
     x [..., k] over the (tied) table [n, k], 16-bit, k a multiple of 8.  Only the first vocab rows of the table are tokens (None: all;
     any number).  The logits are the tensor cores' fp32 sums, neither rounded nor stored: they drop what their additions
-    shift out, 1.2e-6 of their norm from 64 bits at k = 1024 (a plain fp32 product: 0.6e-6).  There is no gradient; training goes
-    through linear_nt's logits.  Returns (logp, stats, entropy or None, missed) as token_logprobs does."""
+    shift out, 7e-7 of their norm from 64 bits at k = 768 and 2e-6 at 2048 (a plain fp32 product: 2 to 5e-7); for up to 128 rows and k
+    above 512, 5e-7.  There is no gradient; training goes through linear_nt's logits.  Returns (logp, stats, entropy or None, missed) as token_logprobs does."""
     return _host.linear_logprobs(x, table, targets, bias, vocab, scale, entropy)
 
 

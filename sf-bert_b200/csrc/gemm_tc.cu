@@ -23,6 +23,7 @@ constexpr uint32_t kGBBytes = kGBK * kGBN * 2;           // 32 KB: four 64 x 64 
 constexpr uint32_t kBiasBytes = 2 * 2 * 128 * 4;          // the epilogue's bias: [accumulator][column half][128]
 constexpr uint32_t kScoreBiasBytes = 8 * 128 * 4;        // scores: each epilogue warp's own, which it reads after it has given the accumulator back
 constexpr int kGStages = 4, kGBufs = 2;
+constexpr uint32_t kChunk = 8;                           // k-blocks that are summed in one accumulator where a sum is put together from pieces
 constexpr uint32_t kGStageBytes = kGABytes + kGBBytes;
 constexpr size_t kGSmem = 1024 + kGStages * kGStageBytes + kBiasBytes + 256;
 
@@ -198,9 +199,10 @@ __device__ __forceinline__ void drain_rows_staged(const GParams &p, const CUtens
 // place.  A thread has a whole row of the tile, so nothing is exchanged.  The loop is short on purpose: unrolled, with the next 32
 // columns on their way, it ran out of the instruction cache (a tile of 256 columns 5900 cycles, now 5400; its MMAs take 6100 at
 // k = 768, so the scores are bound by the product from there on, by this loop below).  4096 x 30522 x 768: 121 us by itself with the
-// tensor pipe 79 % busy, and 5 for the join; a call 137 us in a short burst, 165 under the power cap.  The accumulators are fp32 but drop what their additions
-// shift out: logits end up 1.2e-6 of their norm from 64 bits at k = 1024, those of an fp32 product 0.5e-6.
-template <bool ENT, typename Release>
+// tensor pipe 79 % busy, and 5 for the join; a call 137 us in a short burst, 165 under the power cap.  The accumulators are fp32 but
+// drop what their additions shift out: logits end up 7.4e-7 of their norm from 64 bits at k = 768 and 2e-6 at 2048 (those of an fp32 product 2 to 5e-7).
+// CHUNKS: the accumulator holds the last kChunk k-blocks' sum at most, and what comes before them stands 256 columns further: 5e-7 at any k.
+template <bool ENT, bool CHUNKS, typename Release>
 __device__ __forceinline__ void score_rows(const GParams &p, uint32_t tcol, const float *bias, uint32_t row, uint32_t target, uint32_t tile_n, uint32_t chalf,
                                            Release release)
 {
@@ -216,11 +218,19 @@ __device__ __forceinline__ void score_rows(const GParams &p, uint32_t tcol, cons
         uint32_t cur[32];
         __syncwarp();                        // the lanes parted over targets and references
         TMEM_LD_32(cur, tcol + c0);
-        tmem_wait_ld();
-        if (col + 32 >= end) release();
         float x[32];
+        if (CHUNKS) {
+            uint32_t sum[32];
+            TMEM_LD_32(sum, tcol + kGBN + c0);
+            tmem_wait_ld();
 #pragma unroll
-        for (int j = 0; j < 32; j++) x[j] = __uint_as_float(cur[j]);
+            for (int j = 0; j < 32; j++) x[j] = __uint_as_float(sum[j]) + __uint_as_float(cur[j]);
+        } else {
+            tmem_wait_ld();
+#pragma unroll
+            for (int j = 0; j < 32; j++) x[j] = __uint_as_float(cur[j]);
+        }
+        if (col + 32 >= end) release();
         if (p.bias) {
 #pragma unroll
             for (int j = 0; j < 8; j++) {
@@ -280,8 +290,26 @@ __device__ __forceinline__ void score_rows(const GParams &p, uint32_t tcol, cons
     if (row_ok) p.score_parts[(size_t)(tile_n * 2 + chalf) * p.M + row] = make_float4(mx, a.s, a.e, 0.f);
 }
 
+// A warp's share of an accumulator added to the sum 256 columns further, for its rows and half of the tile's columns in whole steps of 32: what lies
+// behind the tile's columns is never looked at, and what another warp reads in the end it reads after products that waited for this.
+__device__ __forceinline__ void add_chunk(uint32_t tmem, uint32_t bn, uint32_t chalf)
+{
+    const uint32_t middle = (bn / 2 + 31) / 32 * 32;
+#pragma unroll 1
+    for (uint32_t c0 = chalf ? middle : 0; c0 < (chalf ? bn : middle); c0 += 32) {
+        uint32_t cur[32], sum[32];
+        TMEM_LD_32(cur, tmem + c0);
+        TMEM_LD_32(sum, tmem + kGBN + c0);
+        tmem_wait_ld();
+#pragma unroll
+        for (int j = 0; j < 32; j++) sum[j] = __float_as_uint(__uint_as_float(sum[j]) + __uint_as_float(cur[j]));
+        TMEM_ST_32(tmem + kGBN + c0, sum);
+    }
+    tmem_wait_st();
+}
+
 // SCORE: 0 the product itself, 1 scores of its rows, 2 with the sum that the entropy takes
-template <int SCORE>
+template <int SCORE, bool CHUNKS = false>
 __global__ void __launch_bounds__(320, 1)
 linear_tc_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap bmap, const GParams p)
 {
@@ -349,14 +377,19 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant
         if (elect_one()) {
             const uint32_t idesc = instr_desc(fmt, fmt, kGBM, bn, p.w_transposed ? 0 : 1);
             const uint32_t b_step = p.w_transposed ? 2u : 128u;   // descriptor units of 16 bytes per 16 of K
-            uint32_t g = 0, i = 0;
+            uint32_t g = 0, i = 0, handed = 0;                    // handed: accumulators given to the epilogue (chunks)
             for (uint32_t t = blockIdx.x; t < n_tiles; t += gridDim.x, i++) {
-                const uint32_t buf = i % kGBufs;
+                const uint32_t buf = CHUNKS ? 0 : i % kGBufs;
                 bool alive = true;
-                if (i >= (uint32_t)kGBufs && !mbar_wait(&st->acc_empty[buf], ((i / kGBufs) - 1) & 1, abort_flag, 42)) break;
+                if (!CHUNKS && i >= (uint32_t)kGBufs && !mbar_wait(&st->acc_empty[buf], ((i / kGBufs) - 1) & 1, abort_flag, 42)) break;
                 tcgen05_fence_after();
                 for (uint32_t kb = 0; kb < kblocks; kb++, g++) {
-                    const uint32_t s = g % kGStages;
+                    const uint32_t s = g % kGStages, at = CHUNKS ? kb % kChunk : kb;       // at: k-blocks in this accumulator so far
+                    // a tile's first chunk is the sum itself; it and the accumulator are free once what was handed over last has been read
+                    if (CHUNKS && at == 0 && kb != kChunk && handed) {
+                        if (!mbar_wait(&st->acc_empty[0], (handed - 1) & 1, abort_flag, 42)) { alive = false; break; }
+                        tcgen05_fence_after();
+                    }
                     if (!mbar_wait(&st->full[s], (g / kGStages) & 1, abort_flag, 43)) { alive = false; break; }
                     tcgen05_fence_after();
                     const uint32_t base = smem_u32(tiles + s * kGStageBytes);
@@ -365,11 +398,16 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant
                     const uint64_t a_desc = smem_desc_sw128(base);
 #pragma unroll
                     for (uint32_t kk = 0; kk < 4; kk++)   // 16 of K per MMA: +32 bytes in A's swizzled rows, +16 rows (2048 bytes) in B
-                        umma_f16(tmem + buf * kGBN, a_desc + 2 * kk, b_desc + b_step * kk, idesc, (kb | kk) ? 1u : 0u);
+                        umma_f16(tmem + (CHUNKS ? (kb < kChunk ? kGBN : 0) : buf * kGBN), a_desc + 2 * kk, b_desc + b_step * kk, idesc, (at | kk) ? 1u : 0u);
                     umma_commit(&st->empty[s]);
+                    if (CHUNKS && at == kChunk - 1 && kb >= kChunk && kb + 1 < kblocks) {
+                        umma_commit(&st->acc_full[0]);
+                        handed++;
+                    }
                 }
                 if (!alive) break;
                 umma_commit(&st->acc_full[buf]);
+                handed++;
             }
         }
     } else {
@@ -378,16 +416,32 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant
         const uint32_t chalf = (warp - 2) >> 2;            // which 128 columns
         const uint32_t r = quarter * 32 + lane;
         const uint32_t lane_field = (quarter * 32) << 16;
-        uint32_t i = 0;
+        uint32_t i = 0, taken = 0;                         // taken: accumulators read (chunks)
         auto bias_of = [&](uint32_t n0) { return SCORE ? fetch_bias_any(p, n0, lane) : fetch_bias(p, n0, lane); };
         auto target_of = [&](uint32_t t) { const uint32_t row = (t % p.tiles_m) * kGBM + r; return SCORE && row < p.M ? (uint32_t)p.targets[row] : 0xffffffffu; };
         float4 next = bias_of((blockIdx.x / p.tiles_m) * bn + chalf * half);
         uint32_t next_target = target_of(blockIdx.x);
         for (uint32_t t = blockIdx.x; t < n_tiles; t += gridDim.x, i++) {
-            const uint32_t buf = i % kGBufs;
+            const uint32_t buf = CHUNKS ? 0 : i % kGBufs;
             const uint32_t n0 = (t / p.tiles_m) * bn + chalf * half, target = next_target;
             float *bias = bias_s + (SCORE ? warp - 2 : (i & 1) * 2 + chalf) * 128;
-            if (!mbar_wait_warp(&st->acc_full[buf], (i / kGBufs) & 1, abort_flag, 44)) break;
+            if (CHUNKS) {
+                // all chunks but the first, which is the sum, and the last
+                const bool some_rows = __any_sync(0xffffffffu, (t % p.tiles_m) * kGBM + r < p.M);
+                bool alive = true;
+                for (uint32_t kb = 2 * kChunk; kb < kblocks; kb += kChunk) {
+                    alive = mbar_wait_warp(&st->acc_full[0], taken & 1, abort_flag, 44);
+                    if (!alive) break;
+                    taken++;
+                    tcgen05_fence_after();
+                    if (some_rows) add_chunk(tmem + lane_field, bn, chalf);
+                    tcgen05_fence_before();
+                    mbar_arrive(&st->acc_empty[0]);
+                }
+                if (!alive) break;
+            }
+            if (!mbar_wait_warp(&st->acc_full[buf], (CHUNKS ? taken : i / kGBufs) & 1, abort_flag, 44)) break;
+            taken++;
             *(float4 *)(bias + lane * 4) = next;
             __syncwarp();
             if (t + gridDim.x < n_tiles) {
@@ -400,7 +454,7 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant
                 mbar_arrive(&st->acc_empty[buf]);
             };
             if (SCORE) {
-                score_rows<SCORE == 2>(p, tmem + buf * kGBN + chalf * half + lane_field, bias, (t % p.tiles_m) * kGBM + r, target, t / p.tiles_m, chalf, release);
+                score_rows<SCORE == 2, CHUNKS>(p, tmem + buf * kGBN + chalf * half + lane_field, bias, (t % p.tiles_m) * kGBM + r, target, t / p.tiles_m, chalf, release);
             } else {
                 drain_rows(p, tmem + buf * kGBN + chalf * 128 + lane_field, bias, (t % p.tiles_m) * kGBM + r, n0);
                 release();
@@ -644,7 +698,7 @@ linear_tc_pair_kernel(const __grid_constant__ CUtensorMap amap, const __grid_con
                 if (lane == 0) mbar_arrive_cluster(buf ? acc_empty0[1] : acc_empty0[0]);
             };
             if (SCORE) {
-                score_rows<SCORE == 2>(p, tmem + buf * kGBN + chalf * half + lane_field, bias, m0 + quarter * 32 + lane, target, tile_n, chalf, release);
+                score_rows<SCORE == 2, false>(p, tmem + buf * kGBN + chalf * half + lane_field, bias, m0 + quarter * 32 + lane, target, tile_n, chalf, release);
             } else {
                 drain_rows_staged(p, &omap, tmem + buf * kGBN + chalf * 128 + lane_field, staging + (warp - 2) * 4096, bias, m0 + quarter * 32, n0, lane);
                 release();
@@ -1178,7 +1232,8 @@ template <bool ENT> static int linear_logprobs(cudaStream_t s, const void *x, co
     static DeviceOnce once;
     if (!once.done(dev)) {
         if (cudaFuncSetAttribute(linear_tc_pair_kernel<kScore>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kPSmem) != cudaSuccess ||
-            cudaFuncSetAttribute(linear_tc_kernel<kScore>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(kGSmem + kScoreBiasBytes)) != cudaSuccess)
+            cudaFuncSetAttribute(linear_tc_kernel<kScore>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(kGSmem + kScoreBiasBytes)) != cudaSuccess ||
+            cudaFuncSetAttribute(linear_tc_kernel<kScore, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(kGSmem + kScoreBiasBytes)) != cudaSuccess)
             return fail("%s: cannot reserve %zu bytes of shared memory", who, kPSmem);
         once.mark(dev);
     }
@@ -1195,7 +1250,12 @@ template <bool ENT> static int linear_logprobs(cudaStream_t s, const void *x, co
         const uint64_t tiles = tile(kGBM, (uint32_t)sms, 16);
         if (make_map_2d(&bm, table, n, k, is_bf16, prm.bn)) return 1;
         prm.band = 1;
-        launch_overlapped(linear_tc_kernel<kScore>, dim3(tiles < (uint64_t)sms ? (uint32_t)tiles : (uint32_t)sms), dim3(320), kGSmem + kScoreBiasBytes, s, am, bm, prm);
+        // Few rows: a CTA waits for the table from memory, and its warps can add pieces of a sum meanwhile (linear_tc_kernel's CHUNKS).  Both
+        // accumulators belong to one tile then, so the next one's products wait for its epilogue: 7 rows of k = 1024 over 30522 tokens 17.7 us and 5e-7
+        // from 64 bits, 17.1 and 1e-6 in one piece; 128 rows over 131072 tokens 52.6 and 50.6.  Pieces of 256 take 17.8 and 53.0 for 2.3e-7.
+        const dim3 grid(tiles < (uint64_t)sms ? (uint32_t)tiles : (uint32_t)sms);
+        if (m <= kGBM && k > kChunk * kGBK) launch_overlapped(linear_tc_kernel<kScore, true>, grid, dim3(320), kGSmem + kScoreBiasBytes, s, am, bm, prm);
+        else launch_overlapped(linear_tc_kernel<kScore>, grid, dim3(320), kGSmem + kScoreBiasBytes, s, am, bm, prm);
     }
     if (check_launch(who)) return 1;
     // as many rows per CTA as leave a thread at most eight parts, which it asks for at once

@@ -324,3 +324,34 @@ def test_distillation_of_rows_that_are_not_finite(sfb, rows, dtype):
                 loss, stats, _ = sfb.distill_topk(y, ids, teacher, tail=tail)
                 bad = torch.arange(rows, device="cuda") == 1
                 assert torch.equal(loss.isnan(), bad) and torch.equal(stats[:, 1:].isnan().all(1), bad) and torch.equal(stats[:, 1:].isnan().any(1), bad)
+
+
+# ---- scores of few rows: how exact their logits are ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("m,vocab,k", [(1, 30522, 264), (7, 30522, 512), (7, 30522, 1024), (33, 5003, 520), (128, 2049, 1000), (100, 70001, 776), (5, 100003, 2048),
+                                       (16, 37889, 1544)])
+def test_logits_of_few_rows(sfb, m, vocab, k, dtype):
+    """Products summed 512 of k at a time, from one tile per CTA to several.  A piece takes 32 additions, each of which drops up to a unit in the last
+    place of what has been summed so far, half of one on average: at most 2^-24 of it.  Towards a row's largest logit a sum grows evenly, so it is half of
+    its end on average: 32 * 2^-24 / 2 = 2^-20 of the logit in all, to which the additions of the pieces add 2^-24 of half the logit each.  In the
+    2-norm over the rows' largest logits."""
+    g = gen(m + k)
+    x = torch.randn(m, k, device="cuda", generator=g).to(TYPES[dtype])
+    table = (2.0 / math.sqrt(k) * torch.randn(vocab, k, device="cuda", generator=g)).to(TYPES[dtype])
+    t = torch.randint(-1, vocab, (m,), device="cuda", generator=g, dtype=torch.int32)
+    t[0] = vocab - 1
+    bias = torch.randn(vocab, device="cuda", generator=g)
+    for scale, b in [(1.0, None), (0.5, bias)]:
+        logp, stats, ent, missed = sfb.linear_logprobs(x, table, t, bias=b, scale=scale, entropy=True)
+        assert sfb.device_status() == 0
+        z = x.double() @ table.double().t() + (0 if b is None else b.double())
+        want = R.token_logprobs(z, t, vocab, scale)
+        off = (stats[:, 0].double() - want["m"]).norm() / want["m"].norm()
+        assert float(off) <= 2.0 ** -20 + 2.0 ** -25 * (k / 256 + 1), float(off)
+        # a token's probability is off by its logit's error, and that of a sum of logits by no more: 2^-20 of the largest |x| |w| of a token, which bounds
+        # every partial sum, and D
+        d = R.bounds(vocab) + 2.0 ** -24 * 128 + 2 * scale * 2.0 ** -20 * float((x.double().abs() @ table.double().abs().t()).amax() + 4)
+        G.same(logp, want["logp"], d + 2.0 ** -22 * want["logp"].abs(), "logp")
+        G.same(ent, want["entropy"], 2 * d * (1 + 2 * want["entropy"].abs()), "entropy")
+        again = sfb.linear_logprobs(x, table, t, bias=b, scale=scale, entropy=True)
+        assert torch.equal(logp, again[0]) and torch.equal(stats, again[1])
