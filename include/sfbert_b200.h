@@ -211,6 +211,38 @@ int sfb_fused_attention_slice(sfb_stream_t stream, const void *nn_lut, const voi
                               uint32_t lut_heads, uint32_t lut_dim, uint32_t mask_heads,
                               float scale, uint32_t max_lut, uint64_t in_pitch, uint64_t out_pitch);
 
+/* sfb_fused_attention_slice that also writes lse [batch_dim, head_dim, L] (fp32): the natural logarithm of the sum of exp(scale * score)
+ * over what a row keeps, -inf where it keeps nothing.  It is all that the backward pass below needs of the probabilities.  o is bit for
+ * bit what sfb_fused_attention_slice writes.  No counterpart in the reference. */
+int sfb_fused_attention_stats(sfb_stream_t stream, const void *nn_lut, const void *q, const void *k, const void *v, void *o,
+                              float *lse, const void *mask, int dtype, uint32_t block_size, uint32_t blocks, uint32_t batch_dim,
+                              uint32_t ctx_blks, uint32_t head_dim, uint32_t state_dim, uint32_t lut_heads, uint32_t lut_dim,
+                              uint32_t mask_heads, float scale, uint32_t max_lut, uint64_t in_pitch, uint64_t out_pitch);
+
+/* The backward pass of sfb_fused_attention_stats, with the probabilities made again from q, k and lse:
+ *   P = exp(scale * Q.K^T - lse) on the kept elements, dS = P * (dO.V^T - rowsum(dO * O)) * scale,
+ *   dQ = dS.K, dK = dS^T.Q, dV = P^T.dO.
+ * All types, block sizes and head sizes (at most 128) of the forward call; mask, mask_heads and scale as there.  nt_lut, nn_lut and tn_lut
+ * are the layout's three tables, lut_dim the nt_lut's stride (`blocks`; the others': blocks + ctx_blks), nn_max and tn_max the longest row
+ * and column (0: unknown).  Rows (columns) that keep nothing get zeros.  P and dS are operands of the products in the type of q: with
+ * 16-bit types each entry is rounded once.  Every sum has a fixed order: the same inputs give the same bits.
+ * q, k, v (in_pitch), o (o_pitch), dout (dout_pitch) and dq, dk, dv (grad_pitch) may be head slices of wider tensors, as in
+ * sfb_fused_attention_slice (0: packed); dq, dk and dv share no memory with the operands.
+ * Operands are finite: an infinity or NaN in a row of q, k, v or dout makes the gradients of all positions NaN that share its blocks or a
+ * pair of block-rows (columns) with one that does, masked or not.
+ * workspace: device memory of sfb_attention_backward_workspace() bytes, 16-byte aligned, for this call alone; aligned is 1 where
+ * q, k, v, dout, dq, dk and dv are 16-byte aligned and their pitches multiples of 8 elements, 0 otherwise or where that is unknown
+ * (which 16-bit operands with blocks and heads of 64 need more workspace for).  No counterpart in the reference. */
+uint64_t sfb_attention_backward_workspace(int dtype, uint32_t block_size, uint32_t blocks, uint32_t batch_dim, uint32_t ctx_blks,
+                                          uint32_t head_dim, uint32_t state_dim, uint32_t nn_max, uint32_t tn_max, int aligned);
+int sfb_attention_backward_recompute(sfb_stream_t stream, const void *nt_lut, const void *nn_lut, const void *tn_lut, const void *q,
+                                     const void *k, const void *v, const void *o, const void *dout, const float *lse,
+                                     const void *mask, void *dq, void *dk, void *dv, int dtype, uint32_t block_size,
+                                     uint32_t blocks, uint32_t batch_dim, uint32_t ctx_blks, uint32_t head_dim,
+                                     uint32_t state_dim, uint32_t lut_heads, uint32_t lut_dim, uint32_t mask_heads, float scale,
+                                     uint32_t nn_max, uint32_t tn_max, uint64_t in_pitch, uint64_t o_pitch, uint64_t dout_pitch,
+                                     uint64_t grad_pitch, void *workspace, uint64_t workspace_bytes);
+
 /* Synchronises with the device and reads the library's status word into *status (HOST pointer):
  * 0 while no kernel has given up on a bounded wait, otherwise (code << 24 | CTA index) of the
  * first one that did.  Code 9 is not a wait: a row pair of sfb_fused_attention touched more key blocks than the
@@ -274,6 +306,39 @@ int sfb_linear_residual(sfb_stream_t stream, void *out, const void *x, const voi
  * (embedding.h:5-12) and tensor_add_matrix (ewops.h:276-282); call site transformer_inference_part.cpp:201-209. */
 int sfb_embedding(sfb_stream_t stream, void *out, const void *table, const int32_t *ids, const void *pos,
                   uint32_t batch, uint32_t seq_len, uint32_t hidden, uint32_t vocab, int dtype, uint32_t *bad_ids);
+
+/* The same with the table's rows multiplied by scale: out[b, l, :] = scale * table[ids[b, l], :] + pos[l, :], rounded once.  No
+ * counterpart in the reference. */
+int sfb_embedding_scaled(sfb_stream_t stream, void *out, const void *table, const int32_t *ids, const void *pos,
+                         uint32_t batch, uint32_t seq_len, uint32_t hidden, uint32_t vocab, int dtype, float scale, uint32_t *bad_ids);
+
+/* The gradients of the above from dout [batch, seq_len, hidden] (type dtype):
+ *   dtable [vocab, hidden]: row v = scale * the sum of dout over the positions whose id is v; rows of ids that do not occur are zeros
+ *   dpos [seq_len, hidden] (NULL: not asked for) = the sum of dout over the batch
+ * of type grad_dtype (SFB_F32 or dtype); accumulate != 0 adds them to what is there (a tied table's gradient).  Sums are fp32, in a fixed
+ * order, rounded once.  Ids outside [0, vocab) have no row; they are counted in *bad_ids (device uint32, may be NULL).  hidden is a
+ * multiple of 8, vocab at most 2^27; dtable, dpos, dout 16-byte aligned.  workspace: device memory of
+ * sfb_embedding_grad_workspace() bytes, 16-byte aligned, for this call alone.  No counterpart in the reference. */
+uint64_t sfb_embedding_grad_workspace(uint32_t batch, uint32_t seq_len, uint32_t hidden, uint32_t vocab);
+int sfb_embedding_grad(sfb_stream_t stream, void *dtable, void *dpos, const void *dout, const int32_t *ids, uint32_t batch,
+                       uint32_t seq_len, uint32_t hidden, uint32_t vocab, int dtype, int grad_dtype, float scale, int accumulate,
+                       uint32_t *bad_ids, void *workspace);
+
+/* ---- a list of gradients ---------------------------------------------------------------------------------- */
+
+/* The norm of scale * g over all elements g of `count` tensors: *norm (device, fp32) = scale * sqrt(sum of g^2), the sum in fp64 and in
+ * a fixed order.  grads, numel and dtypes are HOST arrays (read before the call returns): device pointers, aligned to their elements,
+ * numbers of elements and types, which may differ from tensor to tensor.  scale > 0: 1 / the loss scale, or 1.  workspace: device memory
+ * of sfb_clip_grad_norm_workspace(count) bytes, 8-byte aligned, for this call alone.  No counterpart in the reference. */
+uint64_t sfb_clip_grad_norm_workspace(uint32_t count);
+int sfb_grad_norm(sfb_stream_t stream, uint32_t count, const void *const *grads, const uint64_t *numel, const int32_t *dtypes, float scale,
+                  float *norm, void *workspace);
+
+/* The same, and out = g * scale * min(1, max_norm / (*norm + 1e-6)): in place (out and out_dtypes NULL) or into out, HOST arrays of device
+ * pointers and types (SFB_F32 or the gradient's own).  out[i] is grads[i], in its type, or shares memory with none of the tensors.  Where the norm is
+ * infinite or NaN, or beyond fp32, nothing is written: the caller sees it in *norm. */
+int sfb_clip_grad_norm(sfb_stream_t stream, uint32_t count, const void *const *grads, void *const *out, const uint64_t *numel,
+                       const int32_t *dtypes, const int32_t *out_dtypes, float max_norm, float scale, float *norm, void *workspace);
 
 /* ---- what logits are turned into: scores, losses, answers ---------------------------------------------- */
 

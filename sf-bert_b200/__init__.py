@@ -29,7 +29,9 @@ SYMBOLS = [
     "sfb_csr_attention", "sfb_rowdot", "sfb_fused_sddmm_softmax_grad", "sfb_fused_attention_slice", "sfb_device_status_clear",
     "sfb_linear_residual", "sfb_attention_backward", "sfb_csr_workspace",
     "sfb_csr_attention_planned", "sfb_token_logprobs", "sfb_token_logprobs_grad", "sfb_distill_topk", "sfb_distill_topk_grad",
-    "sfb_linear_logprobs", "sfb_linear_logprobs_workspace",
+    "sfb_linear_logprobs", "sfb_linear_logprobs_workspace", "sfb_fused_attention_stats", "sfb_attention_backward_recompute",
+    "sfb_attention_backward_workspace", "sfb_embedding_scaled", "sfb_embedding_grad", "sfb_embedding_grad_workspace", "sfb_grad_norm",
+    "sfb_clip_grad_norm", "sfb_clip_grad_norm_workspace",
 ]
 
 if not os.path.exists(LIB_PATH):
@@ -86,6 +88,19 @@ lib.sfb_distill_topk_grad.argtypes = [_vp, _vp, _u64] + [_vp] * 8 + [_u64, _u32,
 lib.sfb_linear_logprobs_workspace.argtypes = [_u32, _u32]
 lib.sfb_linear_logprobs_workspace.restype = _u64
 lib.sfb_linear_logprobs.argtypes = [_vp] * 5 + [_u32, _u32, _u32, _i32, _f32] + [_vp] * 5
+
+lib.sfb_fused_attention_stats.argtypes = [_vp] * 8 + [_i32] + [_u32] * 9 + [_f32, _u32, _u64, _u64]
+lib.sfb_attention_backward_recompute.argtypes = [_vp] * 14 + [_i32] + [_u32] * 9 + [_f32, _u32, _u32] + [_u64] * 4 + [_vp, _u64]
+lib.sfb_attention_backward_workspace.argtypes = [_i32] + [_u32] * 8 + [_i32]
+lib.sfb_attention_backward_workspace.restype = _u64
+lib.sfb_embedding_scaled.argtypes = [_vp] * 5 + [_u32] * 4 + [_i32, _f32, _vp]
+lib.sfb_embedding_grad.argtypes = [_vp] * 5 + [_u32] * 4 + [_i32, _i32, _f32, _i32, _vp, _vp]
+lib.sfb_embedding_grad_workspace.argtypes = [_u32] * 4
+lib.sfb_embedding_grad_workspace.restype = _u64
+lib.sfb_grad_norm.argtypes = [_vp, _u32, _vp, _vp, _vp, _f32, _vp, _vp]
+lib.sfb_clip_grad_norm.argtypes = [_vp, _u32] + [_vp] * 5 + [_f32, _f32, _vp, _vp]
+lib.sfb_clip_grad_norm_workspace.argtypes = [_u32]
+lib.sfb_clip_grad_norm_workspace.restype = _u64
 
 
 def device_status():
@@ -231,10 +246,19 @@ def linear_nt(x, wt, bias=None, act=ACT_NONE, out=None):
     return _host.linear(x, wt, bias, act, out, True)
 
 
-def embedding(table, ids, pos=None):
-    """out[b, l, :] = table[ids[b, l], :] + pos[l, :] (embedding_lookup + tensor_add_matrix, embedding.h:5-12,
+def embedding(table, ids, pos=None, scale=1.0):
+    """out[b, l, :] = scale * table[ids[b, l], :] + pos[l, :] (embedding_lookup + tensor_add_matrix, embedding.h:5-12,
     ewops.h:276-282).  Returns (out, number of ids that were outside the table)."""
-    return _host.embedding(table, ids, pos)
+    return _host.embedding(table, ids, pos, scale)
+
+
+def embedding_grad(dout, ids, vocab, scale=1.0, positions=False, dtype=torch.float32, out=None):
+    """The gradients of embedding's tables from dout [B, L, hidden] and the same ids: dtable [vocab, hidden], scale times the sum of
+    dout over the tokens of each id, and with positions dpos [L, hidden], its sum over the batch.  dtype: fp32 or dout's type (sums
+    are fp32 either way, in a fixed order).  out: tensors (dtable, or with positions the pair) that the gradients are added to, such
+    as a tied table's from the logits; None: new ones, zeros where an id does not occur.  Ids outside [0, vocab) have no row and are
+    counted.  Returns (dtable, dpos or None, that count)."""
+    return _host.embedding_grad(dout, ids, vocab, scale, positions, _DT[dtype], out)
 
 
 def csr_from_layout(lay, head=0):
@@ -302,6 +326,34 @@ def fused_attention_slice(q, k, v, lay, scale=None, use_mask=False, out=None):
     """fused_attention on views that select some heads (and batch elements) of wider [B, L, H_total, d] tensors, in
     place (sfb_fused_attention_slice): what one rank of a multi-GPU run calls on its share of the (batch, head) pairs."""
     return _host.fused_attention_slice(q, k, v, lay, scale, use_mask, out)
+
+
+def fused_attention_stats(q, k, v, lay, scale=None, use_mask=False, out=None):
+    """fused_attention for a training step: returns (o, lse), lse [B, H, L] the natural log of each row's sum of exp(scale * score) (fp32;
+    -inf where a row keeps nothing), which is all that attention_backward_recompute needs of the probabilities.  q, k, v (and out)
+    may be views that select some heads of wider [B, L, H_total, d] tensors, as in fused_attention_slice."""
+    return _host.fused_attention_stats(q, k, v, lay, scale, use_mask, out)
+
+
+def attention_backward_recompute(q, k, v, o, do, lse, lay, scale=None, use_mask=False, out=None):
+    """The gradients (dq, dk, dv) of fused_attention_stats' output, with the probabilities made again from lse: nothing of the size
+    of the scores was kept.  Any type, block and head size of the forward call; scale and use_mask as there.  q, k, v share a pitch, o and do
+    have their own; out: three views to write to, of one pitch (such as the three parts of a packed [B, L, 3, H, d] gradient).  The same
+    inputs give the same bits.  With 16-bit operands P and dS are rounded to their type as operands of the products."""
+    return _host.attention_backward_recompute(q, k, v, o, do, lse, lay, scale, use_mask, out)
+
+
+def grad_norm(grads, scale=1.0):
+    """scale times the 2-norm over all elements of a list of tensors (fp32, bf16 and fp16 together; any dense layout), as a tensor of
+    one fp32 element on their device.  The squares are summed in fp64, in a fixed order."""
+    return _host.clip_grad_norm(grads, float("inf"), scale, None, False)
+
+
+def clip_grad_norm(grads, max_norm, scale=1.0, out=None):
+    """Multiplies every gradient by scale * min(1, max_norm / (norm + 1e-6)), norm = grad_norm(grads, scale): in place, or into the
+    tensors of out (of the gradients' types or fp32: gradients of a scaled loss go, unscaled and clipped, into master gradients).
+    Returns the norm; where it is infinite or NaN nothing is written.  Nothing is read back: the call can be captured in a graph."""
+    return _host.clip_grad_norm(grads, max_norm, scale, out, True)
 
 
 def bias_residual_layernorm(x, bias, resid, gain, beta, want_sum=False, out=None):

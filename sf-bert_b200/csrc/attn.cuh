@@ -8,8 +8,8 @@ struct AttnDims {
     uint32_t B, H, d, nb_a, nb_b, blocks;
     uint32_t lut_stride;   // uint2 per head in the LUT handed to the kernel (0 = shared by all heads)
     uint32_t mask_stride;  // words per head in the mask (0 = shared)
-    uint64_t in_pitch;     // elements between consecutive rows of q, k, v (0 = H * d: the tensors hold these heads only)
-    uint64_t out_pitch;    // the same for o
+    uint64_t in_pitch;     // elements between consecutive rows of q, k, v, or of a product's second operand (0 = H * d: the tensors hold these heads only)
+    uint64_t out_pitch;    // the same for o, or the product's result
 };
 
 // fp32 operands and the shapes that the tcgen05 kernels do not take (attn_simt.cu)
@@ -23,12 +23,12 @@ int simt_softmax_grad(cudaStream_t s, const void *lut, const void *dy, const voi
                       const AttnDims &p, float scale, uint32_t max_lut);
 int simt_fused_sddmm_softmax(cudaStream_t s, const void *nn_lut, const void *a, const void *b, const void *mask, void *y,
                              int ab_dtype, int y_dtype, uint32_t bs, const AttnDims &p, float scale);
-int simt_fused_attention(cudaStream_t s, const void *nn_lut, const void *q, const void *k, const void *v, void *o,
+int simt_fused_attention(cudaStream_t s, const void *nn_lut, const void *q, const void *k, const void *v, void *o, float *lse,
                          const void *mask, int dtype, uint32_t bs, const AttnDims &p, float scale);
 
 // tcgen05 kernels (attn_tc.cu)
 bool tc_fused_attention_supported(int dtype, uint32_t bs, const AttnDims &p, float scale, uint32_t max_lut);
-int tc_fused_attention(cudaStream_t s, const void *nn_lut, const void *q, const void *k, const void *v, void *o,
+int tc_fused_attention(cudaStream_t s, const void *nn_lut, const void *q, const void *k, const void *v, void *o, float *lse,
                        const void *mask, int dtype, const AttnDims &p, float scale, uint32_t max_lut);
 int tc_status_fused(uint32_t *out);
 int tc_status_clear_fused();
@@ -55,7 +55,7 @@ int tc_status_clear_unfused();
 int tc_linear(cudaStream_t s, void *out, const void *x, const void *w, const float *bias, uint32_t m, uint32_t n, uint32_t k,
               int dtype, int act, bool w_transposed, const void *resid);
 int embedding_lookup(cudaStream_t s, void *out, const void *table, const int32_t *ids, const void *pos, uint32_t batch,
-                     uint32_t seq_len, uint32_t hidden, uint32_t vocab, int dtype, uint32_t *bad_ids);
+                     uint32_t seq_len, uint32_t hidden, uint32_t vocab, int dtype, float scale, uint32_t *bad_ids);
 uint64_t tc_linear_logprobs_workspace(uint32_t m, uint32_t n);
 int tc_linear_logprobs(cudaStream_t s, const void *x, const void *table, const float *bias, const int32_t *targets, uint32_t m, uint32_t n,
                        uint32_t k, int dtype, float scale, float *logp, float *stats, float *entropy, uint32_t *missed, void *workspace);

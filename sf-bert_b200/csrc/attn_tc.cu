@@ -90,6 +90,7 @@ struct Params {
     const uint2 *nn_lut;
     const uint64_t *mask;
     void *O;
+    float *lse;            // [B, H, L] log-sums of the rows (STATS)
     uint32_t B, H, nb, npairs, n_items, lut_stride, mask_stride;
     uint32_t o_pitch;      // elements between consecutive rows of O
     uint32_t deal;         // how items are dealt to the CTAs' streams (item_id): kDealNear, kDealSpread, kDealSplit
@@ -276,7 +277,7 @@ __device__ __forceinline__ void tma_producer(uint32_t s, uint8_t *smem, SharedSt
 
 // ---- the kernel ---------------------------------------------------------------------------------
 // SPLIT: the streams of a CTA share its items (a kernel of its own: the merge in the epilogue cost the others 3 %)
-template <bool HAS_MASK, bool BF16, bool SPLIT>
+template <bool HAS_MASK, bool BF16, bool SPLIT, bool STATS>
 __global__ void __launch_bounds__(kThreads, 1)
 fused_attention_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
                           const __grid_constant__ CUtensorMap vmap, const __grid_constant__ CUtensorMap omap, const Params p)
@@ -483,8 +484,8 @@ fused_attention_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid
                 tcgen05_fence_before();
                 mbar_arrive_warp(&st->part_ready, lane);
             } else {
+                float M = m_used;
                 if (SPLIT) {
-                    float M = m_used;
                     float2 part[kStreams];
 #pragma unroll
                     for (int j = 1; j < kStreams; j++) {
@@ -505,6 +506,9 @@ fused_attention_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid
                 const float inv = lsum > 0.f ? 1.f / lsum : 0.f;
 #pragma unroll
                 for (int j = 0; j < kStreams; j++) fac[j] *= inv;
+                // a row's sum is relative to the reference maximum that its powers were taken beside; M: the shares' common one
+                if (STATS && (half == 0 || has_row1))
+                    p.lse[((size_t)e_b * p.H + e_h) * L + (size_t)e_pair * 128 + r] = lsum == 0.f ? -INFINITY : (M + log2f(lsum)) * 0.69314718055994531f;
             }
             // the previous store out of the staging tile has been read out of shared memory
             if (n_epi >= 1 && !mbar_wait_warp(&st->stage_free, (n_epi - 1) & 1, abort_flag, 13)) return false;
@@ -711,18 +715,18 @@ bool tc_fused_attention_supported(int dtype, uint32_t bs, const AttnDims &p, flo
            longest <= (uint64_t)tc::kMaxU && (uint64_t)p.B * p.nb_a * 64 < (1ull << 31) && p.nb_a < (1u << 30);
 }
 
-template <bool HAS_MASK, bool BF16, bool SPLIT>
+template <bool HAS_MASK, bool BF16, bool SPLIT, bool STATS>
 static int launch_fused(cudaStream_t s, dim3 grid, const CUtensorMap &qm, const CUtensorMap &km, const CUtensorMap &vm, const CUtensorMap &om,
                         const tc::Params &prm, int dev)
 {
     using namespace tc;
     static DeviceOnce once;
     if (!once.done(dev)) {
-        if (cudaFuncSetAttribute(fused_attention_tc_kernel<HAS_MASK, BF16, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemBytes) != cudaSuccess)
+        if (cudaFuncSetAttribute(fused_attention_tc_kernel<HAS_MASK, BF16, SPLIT, STATS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemBytes) != cudaSuccess)
             return fail("sfb_fused_attention: cannot reserve %zu bytes of shared memory", kSmemBytes);
         once.mark(dev);
     }
-    launch_overlapped(fused_attention_tc_kernel<HAS_MASK, BF16, SPLIT>, grid, dim3(kThreads), kSmemBytes, s, qm, km, vm, om, prm);
+    launch_overlapped(fused_attention_tc_kernel<HAS_MASK, BF16, SPLIT, STATS>, grid, dim3(kThreads), kSmemBytes, s, qm, km, vm, om, prm);
     return check_launch("sfb_fused_attention");
 }
 
@@ -744,7 +748,7 @@ static uint32_t choose_deal(uint32_t n_items, double mean, uint32_t longest, uin
     return split < spread ? kDealSplit : kDealSpread;
 }
 
-int tc_fused_attention(cudaStream_t s, const void *nn_lut, const void *q, const void *k, const void *v, void *o,
+int tc_fused_attention(cudaStream_t s, const void *nn_lut, const void *q, const void *k, const void *v, void *o, float *lse,
                        const void *mask, int dtype, const AttnDims &p, float scale, uint32_t max_lut)
 {
     using namespace tc;
@@ -757,7 +761,7 @@ int tc_fused_attention(cudaStream_t s, const void *nn_lut, const void *q, const 
     const uint32_t npairs = (p.nb_a + 1) / 2;
     const uint64_t n_items = (uint64_t)npairs * p.B * p.H;
     SFB_REQUIRE(n_items < (1ull << 31), "sfb_fused_attention: too many row pairs for one launch");
-    Params prm = {(const uint2 *)nn_lut, (const uint64_t *)mask, o, p.B, p.H, p.nb_a, npairs, (uint32_t)n_items, p.lut_stride,
+    Params prm = {(const uint2 *)nn_lut, (const uint64_t *)mask, o, lse, p.B, p.H, p.nb_a, npairs, (uint32_t)n_items, p.lut_stride,
                   p.mask_stride, (uint32_t)(p.out_pitch ? p.out_pitch : (uint64_t)p.H * 64), 0u, scale * 1.4426950408889634f};
     const int dev = current_device();
     const int sms = device_sm_count(dev);
@@ -766,12 +770,18 @@ int tc_fused_attention(cudaStream_t s, const void *nn_lut, const void *q, const 
     // one CTA per SM, three streams each; fewer CTAs only when there are fewer items than SMs (few rounds) or than streams
     const uint64_t want = prm.deal != kDealNear ? n_items : (n_items + kStreams - 1) / kStreams;
     const dim3 grid((unsigned)(want < (uint64_t)sms ? want : (uint64_t)sms));
-    const int variant = (mask ? 4 : 0) | (is_bf16 ? 2 : 0) | (prm.deal == kDealSplit ? 1 : 0);
-#define FA_CASE(V, M, BF, SP) case V: return launch_fused<M, BF, SP>(s, grid, qm, km, vm, om, prm, dev)
+    const int variant = (lse ? 8 : 0) | (mask ? 4 : 0) | (is_bf16 ? 2 : 0) | (prm.deal == kDealSplit ? 1 : 0);
+#define FA_CASE(V, M, BF, SP, ST) case V: return launch_fused<M, BF, SP, ST>(s, grid, qm, km, vm, om, prm, dev)
+#define FA_CASES(V, ST)                                                                                                  \
+    FA_CASE(V + 0, false, false, false, ST); FA_CASE(V + 1, false, false, true, ST); FA_CASE(V + 2, false, true, false, ST); \
+    FA_CASE(V + 3, false, true, true, ST); FA_CASE(V + 4, true, false, false, ST); FA_CASE(V + 5, true, false, true, ST);    \
+    FA_CASE(V + 6, true, true, false, ST); FA_CASE(V + 7, true, true, true, ST)
     switch (variant) {
-        FA_CASE(0, false, false, false); FA_CASE(1, false, false, true); FA_CASE(2, false, true, false); FA_CASE(3, false, true, true);
-        FA_CASE(4, true, false, false); FA_CASE(5, true, false, true); FA_CASE(6, true, true, false); default: FA_CASE(7, true, true, true);
+        FA_CASES(0, false);
+        FA_CASES(8, true);
     }
+    return fail("sfb_fused_attention: no such variant");
+#undef FA_CASES
 #undef FA_CASE
 }
 

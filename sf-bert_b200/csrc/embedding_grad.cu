@@ -1,0 +1,439 @@
+// Gradients of the embedding lookup out[b, l] = scale table[ids[b, l]] + pos[l]:
+//   dtable[v] = scale sum over the tokens with id v of dout,     dpos[l] = sum over the batch of dout[., l].
+// No atomics on floating-point numbers: every sum has a fixed order, so that the same inputs give the same bits.
+//
+// Four launches.  (1) sort_ids_kernel brings the tokens into the order of their ids, equal ids by position.  (2) pos_grad_kernel adds
+// up the batch, reading dout in order.  (3) table_grad_kernel walks the sorted tokens in pieces of equal length, so that a word that
+// is a tenth of the text does not hang on one CTA; a run of equal ids that lies in one piece is written at once, the parts of
+// one that does not go to the workspace.  The rows of tokens that do not occur are written as zeros by the same launch.
+// (4) join_kernel adds up the parts.  Bound by memory: dout is read by (2) and gathered by (3), from L2 where it fits, and the table's
+// gradient is written once.
+#include "common.cuh"
+
+namespace sfb {
+namespace emb {
+
+constexpr uint32_t kSortThreads = 512, kSortWarps = kSortThreads / 32;
+constexpr uint32_t kMaxRange = 1024;                 // ids that one CTA sorts
+
+struct GradArgs {
+    const void *dout;
+    const int32_t *ids;
+    void *dtable, *dpos;
+    uint32_t n, batch, len, hidden, vocab, range, piece, pieces;
+    float scale;
+    int accumulate;
+    uint32_t *bad;
+    // workspace
+    int2 *sorted, *unsorted;                         // (position, id), in the order of the ids; one CTA's in the order of the positions
+    uint32_t *starts;                                // [vocab + 1]
+    float *parts;                                    // [pieces][2][hidden]
+};
+
+__device__ __forceinline__ uint32_t warp_scan(uint32_t v, uint32_t lane)      // inclusive
+{
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t u = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= (uint32_t)o) v += u;
+    }
+    return v;
+}
+
+// A CTA owns `range` consecutive ids and looks at all tokens: it counts those below its range, which is where its part of the sorted
+// list begins, and collects its own in order, a share of the tokens per warp.  These are then sorted by counting, per warp and id, so
+// that equal ids stay in order.  No CTA waits for another.  The ids come from L2 (4 bytes per token and CTA).
+__global__ void __launch_bounds__(kSortThreads) sort_ids_kernel(const GradArgs a)
+{
+    extern __shared__ uint32_t count[];              // [range][kSortWarps]
+    __shared__ uint32_t s_below[kSortWarps], s_mine[kSortWarps], s_bad[kSortWarps], s_sum[kSortWarps];
+    grid_dependency_wait();
+    grid_launch_dependents();
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t lo = blockIdx.x * a.range, width = min(a.range, a.vocab - lo);
+    const uint32_t share = ((a.n + kSortWarps - 1) / kSortWarps + 31) / 32 * 32, t0 = min(a.n, warp * share), t1 = min(a.n, t0 + share);
+    uint32_t below = 0, mine = 0, bad = 0;
+#pragma unroll 8
+    for (uint32_t t = t0 + lane; t < t1; t += 32) {
+        const uint32_t id = (uint32_t)__ldg(a.ids + t);        // a negative id is a large one
+        below += id < lo;
+        mine += id - lo < width;
+        bad += id >= a.vocab;
+    }
+    below = __reduce_add_sync(0xffffffffu, below);
+    mine = __reduce_add_sync(0xffffffffu, mine);
+    bad = __reduce_add_sync(0xffffffffu, bad);
+    if (lane == 0) {
+        s_below[warp] = below;
+        s_mine[warp] = mine;
+        s_bad[warp] = bad;
+    }
+    for (uint32_t i = threadIdx.x; i < width * kSortWarps; i += kSortThreads) count[i] = 0;
+    __syncthreads();
+    uint32_t base = 0, total = 0, before = 0, bad_all = 0;
+#pragma unroll
+    for (uint32_t w = 0; w < kSortWarps; w++) {
+        base += s_below[w];
+        if (w < warp) before += s_mine[w];
+        total += s_mine[w];
+        bad_all += s_bad[w];
+    }
+    if (blockIdx.x == 0 && threadIdx.x == 0 && a.bad) *a.bad = bad_all;
+    // own tokens, in order of position
+    int2 *list = a.unsorted + base;
+    if (total) {
+        uint32_t at = before;
+        for (uint32_t t = t0; t < t1; t += 32) {               // whole warps: t0 and share are multiples of 32, t1 need not be
+            const uint32_t id = t + lane < t1 ? (uint32_t)__ldg(a.ids + t + lane) : 0xffffffffu;
+            const bool in = id - lo < width;
+            const uint32_t votes = __ballot_sync(0xffffffffu, in);
+            if (in) list[at + __popc(votes & ((1u << lane) - 1u))] = make_int2((int)(t + lane), (int)id);
+            at += __popc(votes);
+        }
+    }
+    __syncthreads();
+    // how often each warp's share of them has each id
+    const uint32_t part = ((total + kSortWarps - 1) / kSortWarps + 31) / 32 * 32, i0 = min(total, warp * part), i1 = min(total, i0 + part);
+    for (uint32_t i = i0 + lane; i < i1; i += 32) atomicAdd(&count[((uint32_t)list[i].y - lo) * kSortWarps + warp], 1u);
+    __syncthreads();
+    // where each (id, warp) begins: an exclusive scan, ids outermost; a thread takes neighbouring ids
+    const uint32_t per = (width + kSortThreads - 1) / kSortThreads, v0 = min(width, threadIdx.x * per), v1 = min(width, v0 + per);
+    uint32_t sum = 0;
+    for (uint32_t i = v0 * kSortWarps; i < v1 * kSortWarps; i++) sum += count[i];
+    const uint32_t upto = warp_scan(sum, lane);
+    if (lane == 31) s_sum[warp] = upto;
+    __syncthreads();
+    uint32_t off = upto - sum;
+#pragma unroll
+    for (uint32_t w = 0; w < kSortWarps; w++)
+        if (w < warp) off += s_sum[w];
+    for (uint32_t v = v0; v < v1; v++) {
+        a.starts[lo + v] = base + off;
+        for (uint32_t w = 0; w < kSortWarps; w++) {
+            const uint32_t c = count[v * kSortWarps + w];
+            count[v * kSortWarps + w] = off;
+            off += c;
+        }
+    }
+    if (lo + width == a.vocab && threadIdx.x == 0) a.starts[a.vocab] = base + total;
+    __syncthreads();
+    for (uint32_t i = i0; i < i1; i += 32) {
+        const bool in = i + lane < i1;
+        const int2 e = in ? list[i + lane] : make_int2(0, -1);
+        const uint32_t same = __match_any_sync(0xffffffffu, e.y), rank = __popc(same & ((1u << lane) - 1u));
+        uint32_t *c = &count[(in ? (uint32_t)e.y - lo : 0u) * kSortWarps + warp];
+        const uint32_t at = in ? *c + rank : 0u;
+        __syncwarp();
+        if (in && rank == 0) *c += __popc(same);
+        __syncwarp();
+        if (in) a.sorted[base + at] = e;
+    }
+}
+
+// ---- sums of rows --------------------------------------------------------------------------------------------------------------
+template <int DT> struct Piece;                      // what a lane has of a row: 16 bytes
+template <> struct Piece<SFB_F32> {
+    static constexpr int N = 4;
+    static __device__ __forceinline__ void add(float (&s)[N], const uint4 &u)
+    {
+        s[0] += __uint_as_float(u.x); s[1] += __uint_as_float(u.y); s[2] += __uint_as_float(u.z); s[3] += __uint_as_float(u.w);
+    }
+};
+template <> struct Piece<SFB_BF16> {
+    static constexpr int N = 8;
+    static __device__ __forceinline__ void add(float (&s)[N], const uint4 &u)
+    {
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            s[2 * i] += __uint_as_float(w[i] << 16);
+            s[2 * i + 1] += __uint_as_float(w[i] & 0xffff0000u);
+        }
+    }
+};
+template <> struct Piece<SFB_F16> {
+    static constexpr int N = 8;
+    static __device__ __forceinline__ void add(float (&s)[N], const uint4 &u)
+    {
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
+            s[2 * i] += f.x;
+            s[2 * i + 1] += f.y;
+        }
+    }
+};
+template <int N> struct Words { typedef uint4 type; };
+template <> struct Words<2> { typedef uint2 type; };
+// N neighbouring results, times scale, rounded once; add: onto what is there
+template <int GT, int N>
+__device__ __forceinline__ void write_sums(void *out, size_t at, const float (&s)[N], float scale, bool add)
+{
+    float v[N];
+#pragma unroll
+    for (int i = 0; i < N; i++) v[i] = s[i] * scale;
+    if constexpr (GT == SFB_F32) {
+#pragma unroll
+        for (int i = 0; i < N; i += 4) {
+            float4 *p = (float4 *)((float *)out + at + i);
+            float4 o = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+            if (add) {
+                const float4 u = *p;
+                o.x += u.x; o.y += u.y; o.z += u.z; o.w += u.w;
+            }
+            __stcs(p, o);
+        }
+    } else {
+        typedef typename Words<N / 2>::type W;
+        W *p = (W *)((uint16_t *)out + at);
+        __align__(16) uint32_t w[N / 2];
+        if (add) *(W *)w = *p;
+#pragma unroll
+        for (int i = 0; i < N / 2; i++) {
+            float x = v[2 * i], y = v[2 * i + 1];
+            if constexpr (GT == SFB_BF16) {
+                if (add) {
+                    x += __uint_as_float(w[i] << 16);
+                    y += __uint_as_float(w[i] & 0xffff0000u);
+                }
+                const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+                w[i] = *reinterpret_cast<const uint32_t *>(&h);
+            } else {
+                if (add) {
+                    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
+                    x += f.x;
+                    y += f.y;
+                }
+                const __half2 h = __floats2half2_rn(x, y);
+                w[i] = *reinterpret_cast<const uint32_t *>(&h);
+            }
+        }
+        __stcs(p, *(const W *)w);
+    }
+}
+
+// A warp takes `piece` sorted tokens and 32 lanes' columns.  The first CTAs do this, the others write the rows of tokens that do
+// not occur.
+template <int DT, int GT>
+__global__ void __launch_bounds__(256) table_grad_kernel(const GradArgs a)
+{
+    constexpr int N = Piece<DT>::N, U = 8;
+    grid_dependency_wait();
+    grid_launch_dependents();
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t groups = (a.hidden / N + 31) / 32, y = blockIdx.x / groups, col = ((blockIdx.x - y * groups) * 32 + lane) * N;
+    const bool live = col < a.hidden;
+    const uint32_t piece_ctas = (a.pieces + 7) / 8;
+    if (y >= piece_ctas) {
+        if (a.accumulate) return;
+        const uint32_t v0 = ((y - piece_ctas) * 8 + warp) * 32;
+        const bool empty = v0 + lane < a.vocab && a.starts[v0 + lane] == a.starts[v0 + lane + 1];
+        uint32_t todo = __ballot_sync(0xffffffffu, empty);
+        const float none[N] = {};
+        for (; todo; todo &= todo - 1)
+            if (live) write_sums<GT, N>(a.dtable, (size_t)(v0 + __ffs(todo) - 1) * a.hidden + col, none, 1.f, false);
+        return;
+    }
+    const uint32_t c = y * 8 + warp, total = a.starts[a.vocab];
+    const uint32_t i0 = c * a.piece, i1 = min(total, i0 + a.piece);
+    if (i0 >= total) return;
+    const int before = i0 ? a.sorted[i0 - 1].y : -1, after = i1 < total ? a.sorted[i1].y : -1;
+    float s[N] = {};
+    int cur = -1;
+    bool opened = false;                             // the current run began before this piece
+    auto flush = [&](bool goes_on) {
+        if (cur < 0 || !live) return;
+        if (!opened && !goes_on) {
+            write_sums<GT, N>(a.dtable, (size_t)cur * a.hidden + col, s, a.scale, a.accumulate);
+        } else {
+            float *p = a.parts + ((size_t)c * 2 + (opened ? 0 : 1)) * a.hidden + col;
+#pragma unroll
+            for (int i = 0; i < N; i += 4) *(float4 *)(p + i) = make_float4(s[i], s[i + 1], s[i + 2], s[i + 3]);
+        }
+    };
+    for (uint32_t g = i0; g < i1; g += 32) {
+        const int2 e = g + lane < i1 ? a.sorted[g + lane] : make_int2(0, -1);
+        const uint32_t here = min(32u, i1 - g);
+        for (uint32_t j = 0; j < here; j += U) {
+            uint4 u[U];
+#pragma unroll
+            for (int k = 0; k < U; k++) {
+                const uint32_t pos = (uint32_t)__shfl_sync(0xffffffffu, e.x, (j + k) & 31);
+                u[k] = make_uint4(0u, 0u, 0u, 0u);
+                if (live && j + k < here) u[k] = __ldg((const uint4 *)((const typename Elem<DT>::type *)a.dout + (size_t)pos * a.hidden + col));
+            }
+#pragma unroll
+            for (int k = 0; k < U; k++) {
+                const int id = __shfl_sync(0xffffffffu, e.y, (j + k) & 31);
+                if (j + k < here) {
+                    if (id != cur) {
+                        flush(false);
+                        opened = cur < 0 && id == before;
+                        cur = id;
+#pragma unroll
+                        for (int i = 0; i < N; i++) s[i] = 0.f;
+                    }
+                    Piece<DT>::add(s, u[k]);
+                }
+            }
+        }
+    }
+    flush(cur == after);
+}
+
+// The runs that more than one piece has.  A CTA per piece in which such a run begins; its warps take shares of the parts.
+template <int GT>
+__global__ void __launch_bounds__(256) join_kernel(const GradArgs a)
+{
+    __shared__ float4 share[8][32];
+    grid_dependency_wait();
+    grid_launch_dependents();
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t groups = (a.hidden / 4 + 31) / 32, c = blockIdx.x / groups, total = a.starts[a.vocab], end = (c + 1) * a.piece;
+    if (end >= total) return;
+    const int id = a.sorted[end - 1].y;
+    if (a.sorted[end].y != id || a.starts[id] < c * a.piece) return;
+    const uint32_t col = ((blockIdx.x - c * groups) * 32 + lane) * 4;
+    const bool live = col < a.hidden;
+    // part 0 is this piece's second slot, part k the first slot of piece c + k
+    const uint32_t parts = 1 + (a.starts[id + 1] - end + a.piece - 1) / a.piece, per = (parts + 7) / 8;
+    const uint32_t k0 = min(parts, warp * per), k1 = min(parts, k0 + per);
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (live) {
+#pragma unroll 8
+        for (uint32_t k = k0; k < k1; k++) {
+            const float4 u = *(const float4 *)(a.parts + ((size_t)(c + k) * 2 + (k ? 0 : 1)) * a.hidden + col);
+            s.x += u.x; s.y += u.y; s.z += u.z; s.w += u.w;
+        }
+    }
+    share[warp][lane] = s;
+    __syncthreads();
+    if (warp || !live) return;
+#pragma unroll
+    for (int w = 1; w < 8; w++) {
+        const float4 u = share[w][lane];
+        s.x += u.x; s.y += u.y; s.z += u.z; s.w += u.w;
+    }
+    const float v[4] = {s.x, s.y, s.z, s.w};
+    write_sums<GT, 4>(a.dtable, (size_t)id * a.hidden + col, v, a.scale, a.accumulate);
+}
+
+// dpos: a warp has 32 lanes' columns of one position and a share of the batch (WAYS warps per position).
+template <int DT, int GT, int WAYS>
+__global__ void __launch_bounds__(256) pos_grad_kernel(const GradArgs a)
+{
+    constexpr int N = Piece<DT>::N, PER = 8 / WAYS;
+    __shared__ float share[WAYS > 1 ? 8 : 1][N][33];
+    grid_dependency_wait();
+    grid_launch_dependents();
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t groups = (a.hidden / N + 31) / 32, y = blockIdx.x / groups, col = ((blockIdx.x - y * groups) * 32 + lane) * N, l = y * PER + warp / WAYS;
+    const bool live = col < a.hidden && l < a.len;
+    const uint32_t per = (a.batch + WAYS - 1) / WAYS, b0 = min(a.batch, warp % WAYS * per), b1 = min(a.batch, b0 + per);
+    float s[N] = {};
+    if (live) {
+        const typename Elem<DT>::type *src = (const typename Elem<DT>::type *)a.dout + (size_t)l * a.hidden + col;
+#pragma unroll 8
+        for (uint32_t b = b0; b < b1; b++) Piece<DT>::add(s, __ldg((const uint4 *)(src + (size_t)b * a.len * a.hidden)));
+    }
+    if (WAYS > 1) {
+#pragma unroll
+        for (int i = 0; i < N; i++) share[warp][i][lane] = s[i];
+        __syncthreads();
+        if (warp % WAYS) return;
+#pragma unroll
+        for (int w = 1; w < WAYS; w++)
+#pragma unroll
+            for (int i = 0; i < N; i++) s[i] += share[warp + w][i][lane];
+    }
+    if (live) write_sums<GT, N>(a.dpos, (size_t)l * a.hidden + col, s, 1.f, a.accumulate);
+}
+
+// sorted tokens per piece: short enough for a long run to spread, long enough for its parts to be few
+static uint32_t piece_length(uint32_t n) { return n <= (1u << 16) ? 32u : 128u; }
+static uint64_t padded(uint64_t bytes) { return (bytes + 63) / 64 * 64; }
+static uint32_t piece_count(uint32_t n) { return (uint32_t)(((uint64_t)n + piece_length(n) - 1) / piece_length(n)); }
+
+template <int DT, int GT>
+static int launch(cudaStream_t s, const GradArgs &a)
+{
+    const int dev = current_device(), sms = device_sm_count(dev);
+    if (sms <= 0) return fail("sfb_embedding_grad: cannot query the device");
+    constexpr uint32_t N = Piece<DT>::N;
+    const uint64_t groups = (a.hidden / N + 31) / 32, rows = (a.pieces + 7) / 8 + ((uint64_t)a.vocab + 255) / 256;
+    SFB_REQUIRE(groups * a.len < (1ull << 31) && groups * rows < (1ull << 31) && (uint64_t)((a.hidden / 4 + 31) / 32) * a.pieces < (1ull << 31),
+                "sfb_embedding_grad: too many rows for one launch");
+    if (a.dpos) {
+        // positions enough to fill the SMs: a warp each; otherwise several share the batch of one
+        const uint64_t warps = groups * a.len, want = 16ull * sms;
+        const uint32_t ways = warps >= want || a.batch < 16 ? 1 : warps * 2 >= want ? 2 : 8, per = 8 / ways;
+        const dim3 grid((unsigned)(groups * ((a.len + per - 1) / per)));
+        if (ways == 1) launch_overlapped(pos_grad_kernel<DT, GT, 1>, grid, dim3(256), 0, s, a);
+        else if (ways == 2) launch_overlapped(pos_grad_kernel<DT, GT, 2>, grid, dim3(256), 0, s, a);
+        else launch_overlapped(pos_grad_kernel<DT, GT, 8>, grid, dim3(256), 0, s, a);
+    }
+    const uint32_t ctas = (a.vocab + a.range - 1) / a.range;
+    static DeviceOnce once;
+    if (!once.done(dev)) {
+        if (cudaFuncSetAttribute(sort_ids_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(kMaxRange * kSortWarps * 4)) != cudaSuccess)
+            return fail("sfb_embedding_grad: cannot reserve shared memory");
+        once.mark(dev);
+    }
+    launch_overlapped(sort_ids_kernel, dim3(ctas), dim3(kSortThreads), (size_t)a.range * kSortWarps * 4, s, a);
+    launch_overlapped(table_grad_kernel<DT, GT>, dim3((unsigned)(groups * rows)), dim3(256), 0, s, a);
+    if (a.pieces > 1) launch_overlapped(join_kernel<GT>, dim3((a.hidden / 4 + 31) / 32 * (a.pieces - 1)), dim3(256), 0, s, a);
+    return check_launch("sfb_embedding_grad");
+}
+
+}  // namespace emb
+}  // namespace sfb
+
+using namespace sfb;
+
+extern "C" uint64_t sfb_embedding_grad_workspace(uint32_t batch, uint32_t seq_len, uint32_t hidden, uint32_t vocab)
+{
+    using namespace emb;
+    const uint64_t n = (uint64_t)batch * seq_len;
+    if (n >= (1ull << 31)) return 0;
+    return 2 * padded(n * 8) + padded(((uint64_t)vocab + 1) * 4) + (uint64_t)piece_count((uint32_t)n) * 2 * hidden * 4;
+}
+
+extern "C" int sfb_embedding_grad(sfb_stream_t stream, void *dtable, void *dpos, const void *dout, const int32_t *ids, uint32_t batch,
+                                  uint32_t seq_len, uint32_t hidden, uint32_t vocab, int dtype, int grad_dtype, float scale, int accumulate,
+                                  uint32_t *bad_ids, void *workspace)
+{
+    using namespace emb;
+    const char *who = "sfb_embedding_grad";
+    SFB_REQUIRE(dtable, "%s: NULL pointer", who);
+    SFB_REQUIRE(valid_dtype(dtype) && (grad_dtype == dtype || grad_dtype == SFB_F32), "%s: unknown dtype, or gradients neither fp32 nor of dout's type", who);
+    SFB_REQUIRE(hidden >= 8 && hidden % 8 == 0, "%s: hidden=%u must be a multiple of 8", who, hidden);
+    SFB_REQUIRE(vocab >= 1 && vocab <= (1u << 27), "%s: vocab=%u must be 1 to 2^27", who, vocab);
+    SFB_REQUIRE((((uintptr_t)dtable | (uintptr_t)dpos | (uintptr_t)dout | (uintptr_t)workspace) & 15) == 0, "%s: dtable, dpos, dout and workspace must be 16-byte aligned", who);
+    const uint64_t n = (uint64_t)batch * seq_len;
+    SFB_REQUIRE(n < (1ull << 31), "%s: too many tokens", who);
+    SFB_REQUIRE(n == 0 || (dout && ids && workspace), "%s: NULL pointer", who);
+    cudaStream_t s = as_stream(stream);
+    if (n == 0) {
+        const size_t row = (size_t)hidden * elem_size(grad_dtype);
+        cudaError_t e = bad_ids ? cudaMemsetAsync(bad_ids, 0, 4, s) : cudaSuccess;
+        if (e == cudaSuccess && !accumulate) e = cudaMemsetAsync(dtable, 0, vocab * row, s);
+        if (e == cudaSuccess && !accumulate && dpos && seq_len) e = cudaMemsetAsync(dpos, 0, seq_len * row, s);
+        if (e != cudaSuccess) return fail("%s: %s", who, cudaGetErrorString(e));
+        clear_error();
+        return 0;
+    }
+    GradArgs a = {dout, ids, dtable, dpos, (uint32_t)n, batch, seq_len, hidden, vocab, 0, piece_length((uint32_t)n), piece_count((uint32_t)n), scale, accumulate, bad_ids};
+    // a CTA per SM sorts, more where its counters would not fit
+    const int sms = device_sm_count(current_device());
+    const uint32_t ctas = max((uint32_t)(sms > 0 ? sms : 1), (vocab + kMaxRange - 1) / kMaxRange);
+    a.range = (vocab + ctas - 1) / ctas;
+    char *w = (char *)workspace;
+    a.sorted = (int2 *)w;
+    a.unsorted = (int2 *)(w += padded(n * 8));
+    a.starts = (uint32_t *)(w += padded(n * 8));
+    a.parts = (float *)(w + padded(((uint64_t)vocab + 1) * 4));
+    if (dtype == SFB_F32) return launch<SFB_F32, SFB_F32>(s, a);
+    if (dtype == SFB_BF16) return grad_dtype == SFB_F32 ? launch<SFB_BF16, SFB_F32>(s, a) : launch<SFB_BF16, SFB_BF16>(s, a);
+    return grad_dtype == SFB_F32 ? launch<SFB_F16, SFB_F32>(s, a) : launch<SFB_F16, SFB_F16>(s, a);
+}

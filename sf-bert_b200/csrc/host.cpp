@@ -9,8 +9,10 @@
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <algorithm>
 #include <cmath>
 #include <string>
+#include <vector>
 #include "../../include/sfbert_b200.h"
 
 namespace {
@@ -21,7 +23,9 @@ namespace {
     X(sfb_linear_nt) X(sfb_linear_residual) X(sfb_embedding) X(sfb_csr_attention) X(sfb_csr_attention_planned) X(sfb_csr_workspace) X(sfb_rowdot) X(sfb_fused_sddmm_softmax_grad)                  \
     X(sfb_fused_sddmm_softmax) X(sfb_fused_attention) X(sfb_fused_attention_slice) X(sfb_bias_residual_layernorm)         \
     X(sfb_bias_gelu) X(sfb_attention_backward) X(sfb_token_logprobs) X(sfb_token_logprobs_grad) X(sfb_distill_topk)      \
-    X(sfb_distill_topk_grad) X(sfb_linear_logprobs) X(sfb_linear_logprobs_workspace)
+    X(sfb_distill_topk_grad) X(sfb_linear_logprobs) X(sfb_linear_logprobs_workspace) X(sfb_fused_attention_stats)          \
+    X(sfb_attention_backward_recompute) X(sfb_attention_backward_workspace) X(sfb_embedding_scaled) X(sfb_embedding_grad)   \
+    X(sfb_embedding_grad_workspace) X(sfb_grad_norm) X(sfb_clip_grad_norm) X(sfb_clip_grad_norm_workspace)
 struct Lib {
 #define DECL(f) decltype(&::f) f = nullptr;
     SFB_FUNCTIONS(DECL)
@@ -317,16 +321,17 @@ FUNCTION(py_linear, 6)
     Py_INCREF(a[4]);
     return a[4];
 }
-// (table, ids, pos)
-FUNCTION(py_embedding, 3)
+// (table, ids, pos, scale)
+FUNCTION(py_embedding, 4)
 {
     const at::Tensor &table = tensor(a[0]), &ids = tensor(a[1]);
     require(ids.dim() == 2 && table.dim() == 2, "ids must be [B, L] and the table [vocab, hidden]");
     require(ids.scalar_type() == at::kInt && ids.is_contiguous() && table.is_contiguous(), "ids must be int32 and contiguous, like the table");
     const int64_t B = ids.size(0), len = ids.size(1), vocab = table.size(0), hidden = table.size(1);
+    const float scale = (float)number(a[3]);
     at::Tensor out = empty({B, len, hidden}, table.scalar_type(), table), bad = empty({1}, at::kInt, table);
-    call(L.sfb_embedding, stream(), ptr(out), ptr(table), (const int32_t *)ptr(ids), ptr_or_null(a[2]), (uint32_t)B, (uint32_t)len,
-                          (uint32_t)hidden, (uint32_t)vocab, tag(table), (uint32_t *)ptr(bad));
+    call(L.sfb_embedding_scaled, stream(), ptr(out), ptr(table), (const int32_t *)ptr(ids), ptr_or_null(a[2]), (uint32_t)B, (uint32_t)len,
+                                 (uint32_t)hidden, (uint32_t)vocab, tag(table), scale, (uint32_t *)ptr(bad));
     Ref o(wrap(out)), n(wrap(bad));
     return PyTuple_Pack(2, o.o, n.o);
 }
@@ -766,6 +771,255 @@ FUNCTION(py_linear_logprobs, 7)
     return PyTuple_Pack(4, l.o, s.o, e.o, n.o);
 }
 
+// ---- a training step around the attention ------------------------------------------------------------------------------------------
+// one of a layout's tables, on the device of the operands
+void *table_on(const Lay &lay, Name n, int64_t numel, const at::Tensor &like, const char *text)
+{
+    Ref v(PyObject_GetAttr(lay.o, names[n]));
+    if (v.o == Py_None) raise(PyExc_AssertionError, text);
+    const at::Tensor &t = tensor(v.o);
+    require(t.device() == like.device() && t.is_contiguous() && t.numel() == numel, text);
+    return ptr(t);
+}
+const char *const bad_layout = "the layout's tables are not on the operands' device";
+const char *const bad_mask = "use_mask needs the layout's mask_np (pack_mask) on the operands' device: a word per kept block and row";
+inline void *mask_on(const Lay &lay, bool use_mask, const at::Tensor &like)
+{
+    if (!use_mask) return nullptr;
+    Ref v(PyObject_GetAttr(lay.o, names[n_mask_np]));
+    require(v.o == Py_None || tensor(v.o).scalar_type() == (lay.bs == 32 ? at::kInt : at::kLong), bad_mask);
+    return table_on(lay, n_mask_np, (int64_t)lay.heads * lay.blocks * lay.bs, like, bad_mask);
+}
+// q, k, v: views of one type, size, device and pitch
+uint64_t operand_pitch(const at::Tensor &q, const at::Tensor &k, const at::Tensor &v)
+{
+    tag(q);
+    require(k.sizes() == q.sizes() && v.sizes() == q.sizes() && k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type() &&
+                k.device() == q.device() && v.device() == q.device(),
+            "q, k and v must be alike");
+    const uint64_t pitch = row_pitch(q);
+    require(row_pitch(k) == pitch && row_pitch(v) == pitch, "q, k and v have different row pitches");
+    return pitch;
+}
+struct Bytes {
+    const char *begin, *end;
+    bool meets(const Bytes &o) const { return begin < o.end && o.begin < end; }
+};
+// the bytes from the first to the last element of a [B, L, H, d] view
+inline Bytes bytes_of(const at::Tensor &t)
+{
+    const char *p = (const char *)ptr(t);
+    const int64_t rows = t.size(0) * t.size(1);
+    return {p, rows ? p + ((rows - 1) * t.stride(1) + t.size(2) * t.size(3)) * t.element_size() : p};
+}
+inline at::Tensor like_operand(PyObject *out, const at::Tensor &q, const char *text)
+{
+    if (out == Py_None) return empty(q.sizes(), q.scalar_type(), q);
+    const at::Tensor &o = tensor(out);
+    require(o.sizes() == q.sizes() && o.scalar_type() == q.scalar_type() && o.device() == q.device(), text);
+    return o;
+}
+// (q, k, v, lay, scale, use_mask, out) -> (o, lse)
+FUNCTION(py_fused_attention_stats, 7)
+{
+    const at::Tensor &q = tensor(a[0]), &k = tensor(a[1]), &v = tensor(a[2]);
+    const Lay lay(a[3]);
+    const Dims n(q, lay);
+    const uint64_t pitch = operand_pitch(q, k, v);
+    const float scale = scale_or(a[4], n.d);
+    require(n.d >= 1 && n.d <= 128, "heads must be 1 to 128 wide");
+    require_cuda(q);
+    const c10::cuda::CUDAGuard on(q.device());
+    void *nn = table_on(lay, n_nn_lut, 2ll * lay.heads * (lay.nb + lay.blocks), q, bad_layout), *mask = mask_on(lay, truth(a[5]), q);
+    at::Tensor o = like_operand(a[6], q, "out must be like q");
+    const uint64_t out_pitch = row_pitch(o);
+    const Bytes r = bytes_of(o);
+    require(!r.meets(bytes_of(q)) && !r.meets(bytes_of(k)) && !r.meets(bytes_of(v)), "out must not share memory with the operands");
+    at::Tensor lse = empty({n.B, n.H, n.L}, at::kFloat, q);
+    if (n.B && n.H)
+        call(L.sfb_fused_attention_stats, stream_of(q), nn, ptr(q), ptr(k), ptr(v), ptr(o), (float *)ptr(lse), mask, tag(q), lay.bs, lay.blocks, n.B, lay.nb, n.H,
+             n.d, lay.heads, lay.blocks, lay.heads, scale, lay.nn_max, pitch, out_pitch);
+    Ref x(wrap(o)), y(wrap(lse));
+    return PyTuple_Pack(2, x.o, y.o);
+}
+// (q, k, v, o, do, lse, lay, scale, use_mask, out) -> (dq, dk, dv)
+FUNCTION(py_attention_backward_recompute, 10)
+{
+    const at::Tensor &q = tensor(a[0]), &k = tensor(a[1]), &v = tensor(a[2]), &o = tensor(a[3]), &dout = tensor(a[4]), &lse = tensor(a[5]);
+    const Lay lay(a[6]);
+    const Dims n(q, lay);
+    const uint64_t pitch = operand_pitch(q, k, v);
+    const float scale = scale_or(a[7], n.d);
+    require(n.d >= 1 && n.d <= 128, "heads must be 1 to 128 wide");
+    for (const at::Tensor *t : {&o, &dout})
+        require(t->sizes() == q.sizes() && t->scalar_type() == q.scalar_type() && t->device() == q.device(), "o and dO must be like q");
+    const uint64_t o_pitch = row_pitch(o), do_pitch = row_pitch(dout);
+    require(lse.scalar_type() == at::kFloat && lse.is_contiguous() && lse.device() == q.device() && lse.dim() == 3 && lse.size(0) == n.B && lse.size(1) == n.H &&
+                lse.size(2) == n.L,
+            "lse must be the contiguous fp32 [B, H, L] tensor that the forward call gave");
+    require_cuda(q);
+    const c10::cuda::CUDAGuard on(q.device());
+    at::Tensor grad[3];
+    if (a[9] == Py_None) {
+        for (at::Tensor &g : grad) g = empty(q.sizes(), q.scalar_type(), q);
+    } else {
+        Ref list(PySequence_Fast(a[9], "out must be a sequence of three tensors"));
+        require(PySequence_Fast_GET_SIZE(list.o) == 3, "out must be a sequence of three tensors");
+        for (int i = 0; i < 3; i++) grad[i] = like_operand(PySequence_Fast_GET_ITEM(list.o, i), q, "out's tensors must be like q");
+    }
+    const uint64_t grad_pitch = row_pitch(grad[0]);
+    require(row_pitch(grad[1]) == grad_pitch && row_pitch(grad[2]) == grad_pitch, "out's tensors have different row pitches");
+    const Bytes in[6] = {bytes_of(q), bytes_of(k), bytes_of(v), bytes_of(o), bytes_of(dout), {(const char *)ptr(lse), (const char *)ptr(lse) + lse.numel() * 4}};
+    for (int i = 0; i < 3; i++) {
+        const Bytes r = bytes_of(grad[i]);
+        for (const Bytes &x : in) require(!r.meets(x), "out must not share memory with the operands");
+        for (int j = 0; j < i; j++) {
+            // apart, or side by side in the rows of one wider tensor
+            const Bytes r2 = bytes_of(grad[j]);
+            const int64_t off = (r.begin < r2.begin ? r2.begin - r.begin : r.begin - r2.begin) / q.element_size() % (int64_t)grad_pitch, width = (int64_t)n.H * n.d;
+            require(!r.meets(r2) || (off >= width && off + width <= (int64_t)grad_pitch), "out's tensors must not share memory");
+        }
+    }
+    const bool use_mask = truth(a[8]);
+    if (n.B && n.H && n.L) {
+        const uint32_t tn_max = attr_u32(lay.o, n_tn_max);
+        void *nt = table_on(lay, n_nt_lut, 2ll * lay.heads * lay.blocks, q, bad_layout), *nn = table_on(lay, n_nn_lut, 2ll * lay.heads * (lay.nb + lay.blocks), q, bad_layout);
+        void *tn = table_on(lay, n_tn_lut, 2ll * lay.heads * (lay.nb + lay.blocks), q, bad_layout), *mask = mask_on(lay, use_mask, q);
+        uintptr_t all = 0;
+        for (const at::Tensor &t : {q, k, v, dout, grad[0], grad[1], grad[2]}) all |= (uintptr_t)ptr(t);
+        const int aligned = (all & 15) == 0 && ((pitch | do_pitch | grad_pitch) & 7) == 0;
+        const uint64_t bytes = L.sfb_attention_backward_workspace(tag(q), lay.bs, lay.blocks, n.B, lay.nb, n.H, n.d, lay.nn_max, tn_max, aligned);
+        at::Tensor ws = empty({(int64_t)bytes}, at::kByte, q);
+        // a layout without blocks has tables of no elements
+        if (!nt) nt = nn;
+        call(L.sfb_attention_backward_recompute, stream_of(q), nt, nn, tn, ptr(q), ptr(k), ptr(v), ptr(o), ptr(dout), (const float *)ptr(lse), mask, ptr(grad[0]),
+             ptr(grad[1]), ptr(grad[2]), tag(q), lay.bs, lay.blocks, n.B, lay.nb, n.H, n.d, lay.heads, lay.blocks, lay.heads, scale, lay.nn_max, tn_max, pitch,
+             o_pitch, do_pitch, grad_pitch, ptr(ws), bytes);
+    }
+    Ref x(wrap(grad[0])), y(wrap(grad[1])), z(wrap(grad[2]));
+    return PyTuple_Pack(3, x.o, y.o, z.o);
+}
+// (dout, ids, vocab, scale, positions, grad_tag, out) -> (dtable, dpos or None, bad)
+FUNCTION(py_embedding_grad, 7)
+{
+    const at::Tensor &dout = tensor(a[0]), &ids = tensor(a[1]);
+    require(dout.dim() == 3 && ids.dim() == 2 && dout.size(0) == ids.size(0) && dout.size(1) == ids.size(1), "dout must be [B, L, hidden] and ids [B, L]");
+    require(ids.scalar_type() == at::kInt && ids.is_contiguous() && dout.is_contiguous() && ids.device() == dout.device(),
+            "ids must be int32 and contiguous, like dout, on its device");
+    const int64_t B = dout.size(0), len = dout.size(1), hidden = dout.size(2), vocab = (int64_t)integer(a[2]);
+    const float scale = (float)number(a[3]);
+    const bool positions = truth(a[4]);
+    const int t = tag(dout), g = (int)integer(a[5]);
+    require(g == SFB_F32 || g == t, "gradients are fp32 or of dout's type");
+    require(vocab >= 1 && vocab <= (1 << 27), "vocab must be 1 to 2^27");
+    require(hidden >= 8 && hidden % 8 == 0 && hidden < (1ll << 31), "hidden must be a multiple of 8");
+    require(B * len < (1ll << 31) && B < (1ll << 31) && len < (1ll << 31), "too many tokens");
+    require_cuda(dout);
+    const c10::cuda::CUDAGuard on(dout.device());
+    at::Tensor dtable, dpos;
+    if (a[6] == Py_None) {
+        dtable = empty({vocab, hidden}, scalar_type(g), dout);
+        if (positions) dpos = empty({len, hidden}, scalar_type(g), dout);
+    } else {
+        const char *text = "out must be the table's gradient, or with positions a pair: contiguous, of the gradients' type and the tables' sizes, on dout's device";
+        auto fits = [&](PyObject *o, int64_t rows) {
+            const at::Tensor &x = tensor(o);
+            require(x.dim() == 2 && x.size(0) == rows && x.size(1) == hidden && x.scalar_type() == scalar_type(g) && x.is_contiguous() && x.device() == dout.device(), text);
+            return x;
+        };
+        if (positions) {
+            require(PyTuple_Check(a[6]) || PyList_Check(a[6]), text);
+            Ref list(PySequence_Fast(a[6], text));
+            require(PySequence_Fast_GET_SIZE(list.o) == 2, text);
+            dtable = fits(PySequence_Fast_GET_ITEM(list.o, 0), vocab);
+            dpos = fits(PySequence_Fast_GET_ITEM(list.o, 1), len);
+        } else {
+            dtable = fits(a[6], vocab);
+        }
+        auto span = [](const at::Tensor &x) { return Bytes{(const char *)ptr(x), (const char *)ptr(x) + x.numel() * x.element_size()}; };
+        const Bytes table = span(dtable);
+        require(!table.meets(span(dout)) && !table.meets(span(ids)) && (!positions || (!span(dpos).meets(table) && !span(dpos).meets(span(dout)) && !span(dpos).meets(span(ids)))),
+                "out must not share memory with the operands");
+    }
+    at::Tensor bad = empty({1}, at::kInt, dout);
+    at::Tensor ws = empty({(int64_t)L.sfb_embedding_grad_workspace((uint32_t)B, (uint32_t)len, (uint32_t)hidden, (uint32_t)vocab)}, at::kByte, dout);
+    call(L.sfb_embedding_grad, stream_of(dout), ptr(dtable), positions ? ptr(dpos) : nullptr, ptr(dout), (const int32_t *)ptr(ids), (uint32_t)B, (uint32_t)len,
+         (uint32_t)hidden, (uint32_t)vocab, t, g, scale, (int)(a[6] != Py_None), (uint32_t *)ptr(bad), ptr(ws));
+    Ref x(wrap(dtable)), n(wrap(bad));
+    if (!positions) return PyTuple_Pack(3, x.o, Py_None, n.o);
+    Ref y(wrap(dpos));
+    return PyTuple_Pack(3, x.o, y.o, n.o);
+}
+// (grads, max_norm, scale, out, write) -> norm
+FUNCTION(py_clip_grad_norm, 5)
+{
+    Ref list(PySequence_Fast(a[0], "grads must be a sequence of tensors"));
+    const Py_ssize_t count = PySequence_Fast_GET_SIZE(list.o);
+    require(count >= 1 && count < (1 << 24), "grads must hold at least one tensor");
+    const float max_norm = (float)number(a[1]), scale = (float)number(a[2]);
+    require(max_norm >= 0.f, "max_norm must not be negative or NaN");
+    require(scale > 0.f && scale <= 3.402823466e38f, "scale must be positive and finite");
+    const bool write = truth(a[4]), other = a[3] != Py_None;
+    std::vector<const void *> in(count);
+    std::vector<void *> out(other ? count : 0);
+    std::vector<uint64_t> numel(count);
+    std::vector<int32_t> types(2 * count);
+    const at::Tensor &first = tensor(PySequence_Fast_GET_ITEM(list.o, 0));
+    for (Py_ssize_t i = 0; i < count; i++) {
+        const at::Tensor &t = tensor(PySequence_Fast_GET_ITEM(list.o, i));
+        types[i] = tag(t);
+        require(t.device() == first.device(), "the gradients must be on one device");
+        require(t.is_non_overlapping_and_dense(), "a gradient must be dense: its elements next to each other");
+        in[i] = ptr(t);
+        numel[i] = (uint64_t)t.numel();
+    }
+    if (other) {
+        Ref into(PySequence_Fast(a[3], "out must be a sequence of tensors"));
+        require(PySequence_Fast_GET_SIZE(into.o) == count, "out must hold a tensor per gradient");
+        for (Py_ssize_t i = 0; i < count; i++) {
+            const at::Tensor &t = tensor(PySequence_Fast_GET_ITEM(list.o, i)), &o = tensor(PySequence_Fast_GET_ITEM(into.o, i));
+            types[count + i] = tag(o);
+            require(o.sizes() == t.sizes() && (o.strides() == t.strides() || (o.is_contiguous() && t.is_contiguous())) && o.device() == t.device() &&
+                        (types[count + i] == SFB_F32 || types[count + i] == types[i]),
+                    "out's tensors must be laid out as the gradients, in their types or fp32, on their device");
+            out[i] = ptr(o);
+        }
+    }
+    require_cuda(first);
+    if (write) {
+        // what is written shares memory with nothing else, but for a gradient that stays where it is
+        struct Span {
+            uintptr_t begin, end;
+            bool written;
+        };
+        std::vector<Span> spans;
+        spans.reserve(2 * count);
+        for (Py_ssize_t i = 0; i < count; i++) {
+            if (!numel[i]) continue;
+            const uintptr_t p = (uintptr_t)in[i], e = types[i] == SFB_F32 ? 4 : 2;
+            const bool stays = !other || ((uintptr_t)out[i] == p && types[count + i] == types[i]);
+            spans.push_back({p, p + numel[i] * e, stays});
+            if (!stays) spans.push_back({(uintptr_t)out[i], (uintptr_t)out[i] + numel[i] * (types[count + i] == SFB_F32 ? 4 : 2), true});
+        }
+        std::sort(spans.begin(), spans.end(), [](const Span &x, const Span &y) { return x.begin < y.begin; });
+        uintptr_t end = 0, written_end = 0;
+        for (const Span &x : spans) {
+            require(x.begin >= (x.written ? end : written_end), "a tensor that is written shares memory with another one");
+            end = std::max(end, x.end);
+            if (x.written) written_end = std::max(written_end, x.end);
+        }
+    }
+    const c10::cuda::CUDAGuard on(first.device());
+    at::Tensor norm = empty({1}, at::kFloat, first), ws = empty({(int64_t)L.sfb_clip_grad_norm_workspace((uint32_t)count)}, at::kByte, first);
+    if (write)
+        call(L.sfb_clip_grad_norm, stream_of(first), (uint32_t)count, (const void *const *)in.data(), other ? (void *const *)out.data() : nullptr, (const uint64_t *)numel.data(),
+             (const int32_t *)types.data(), other ? (const int32_t *)types.data() + count : nullptr, max_norm, scale, (float *)ptr(norm), ptr(ws));
+    else
+        call(L.sfb_grad_norm, stream_of(first), (uint32_t)count, (const void *const *)in.data(), (const uint64_t *)numel.data(), (const int32_t *)types.data(), scale,
+             (float *)ptr(norm), ptr(ws));
+    return wrap(norm);
+}
+
 // bind(addresses by name): which build of the library the functions call
 PyObject *py_bind(PyObject *, PyObject *args)
 {
@@ -797,6 +1051,7 @@ PyMethodDef methods[] = {
     ENTRY(fused_sddmm_softmax), ENTRY(linear), ENTRY(embedding), ENTRY(csr_attention), ENTRY(fused_attention), ENTRY(fused_attention_slice),
     ENTRY(bias_residual_layernorm), ENTRY(bias_gelu), ENTRY(encoder_layer), ENTRY(attention_backward_fused), ENTRY(attention_backward),
     ENTRY(token_logprobs), ENTRY(token_logprobs_grad), ENTRY(distill_topk), ENTRY(distill_topk_grad), ENTRY(linear_logprobs),
+    ENTRY(fused_attention_stats), ENTRY(attention_backward_recompute), ENTRY(embedding_grad), ENTRY(clip_grad_norm),
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -466,7 +466,7 @@ template <int DT>
 __global__ void __launch_bounds__(256) embedding_kernel(void *__restrict__ out, const void *__restrict__ table,
                                                        const int32_t *__restrict__ ids, const void *__restrict__ pos, uint32_t batch,
                                                        uint32_t per_cta_y, uint32_t seq_len, uint32_t hidden, uint32_t vocab,
-                                                       uint32_t *bad_ids, uint32_t count_column)
+                                                       float scale, uint32_t *bad_ids, uint32_t count_column)
 {
     grid_dependency_wait();
     grid_launch_dependents();
@@ -529,7 +529,7 @@ __global__ void __launch_bounds__(256) embedding_kernel(void *__restrict__ out, 
                 float v[N];
                 Vec8<DT>::decode(v, tv[u]);
 #pragma unroll
-                for (int t = 0; t < N; t++) v[t] += q[t];
+                for (int t = 0; t < N; t++) v[t] = fmaf(v[t], scale, q[t]);      // scale 1: the sum, rounded once
                 st_stream16((uint8_t *)out + (((size_t)(b0 + u) * seq_len + l) * hidden + col) * ESZ, Vec8<DT>::encode(v));
             }
             id[u] = id_next[u];
@@ -573,7 +573,7 @@ int rowdot(cudaStream_t s, float *out, const void *a, const void *b, size_t rows
 }
 
 int embedding_lookup(cudaStream_t s, void *out, const void *table, const int32_t *ids, const void *pos, uint32_t batch,
-                     uint32_t seq_len, uint32_t hidden, uint32_t vocab, int dtype, uint32_t *bad_ids)
+                     uint32_t seq_len, uint32_t hidden, uint32_t vocab, int dtype, float scale, uint32_t *bad_ids)
 {
     const int per = dtype == SFB_F32 ? 4 : 8;
     if (hidden % per) return fail("sfb_embedding: hidden=%u must be a multiple of %d for this type", hidden, per);
@@ -595,9 +595,9 @@ int embedding_lookup(cudaStream_t s, void *out, const void *table, const int32_t
         if (e != cudaSuccess) return fail("sfb_embedding: %s", cudaGetErrorString(e));
     }
     const dim3 grid((unsigned)ctas_x + one_cta, (batch + per_y - 1) / per_y);
-    if (dtype == SFB_F32) launch_overlapped(embedding_kernel<SFB_F32>, grid, dim3(256), 0, s, out, table, ids, pos, batch, per_y, seq_len, hidden, vocab, bad_ids, column);
-    else if (dtype == SFB_BF16) launch_overlapped(embedding_kernel<SFB_BF16>, grid, dim3(256), 0, s, out, table, ids, pos, batch, per_y, seq_len, hidden, vocab, bad_ids, column);
-    else launch_overlapped(embedding_kernel<SFB_F16>, grid, dim3(256), 0, s, out, table, ids, pos, batch, per_y, seq_len, hidden, vocab, bad_ids, column);
+    if (dtype == SFB_F32) launch_overlapped(embedding_kernel<SFB_F32>, grid, dim3(256), 0, s, out, table, ids, pos, batch, per_y, seq_len, hidden, vocab, scale, bad_ids, column);
+    else if (dtype == SFB_BF16) launch_overlapped(embedding_kernel<SFB_BF16>, grid, dim3(256), 0, s, out, table, ids, pos, batch, per_y, seq_len, hidden, vocab, scale, bad_ids, column);
+    else launch_overlapped(embedding_kernel<SFB_F16>, grid, dim3(256), 0, s, out, table, ids, pos, batch, per_y, seq_len, hidden, vocab, scale, bad_ids, column);
     return check_launch("sfb_embedding");
 }
 

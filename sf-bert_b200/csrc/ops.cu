@@ -1,6 +1,7 @@
 // C ABI of the attention operators: argument checks and the choice between the tensor-core
 // (tcgen05) kernels and the kernels of attn_simt.cu.  No path leaves the GPU.
 #include "attn.cuh"
+#include "recompute.cuh"
 
 using namespace sfb;
 
@@ -108,7 +109,7 @@ extern "C" int sfb_fused_sddmm_softmax(sfb_stream_t stream, const void *nn_lut, 
 static int fused_attention_common(const char *who, sfb_stream_t stream, const void *nn_lut, const void *q, const void *k, const void *v,
                                   void *o, const void *mask, int dtype, uint32_t block_size, uint32_t blocks, uint32_t batch_dim,
                                   uint32_t ctx_blks, uint32_t head_dim, uint32_t state_dim, uint32_t lut_heads, uint32_t lut_dim,
-                                  uint32_t mask_heads, float scale, uint32_t max_lut, uint64_t in_pitch, uint64_t out_pitch)
+                                  uint32_t mask_heads, float scale, uint32_t max_lut, uint64_t in_pitch, uint64_t out_pitch, float *lse)
 {
     SFB_REQUIRE(nn_lut && q && k && v && o, "%s: NULL pointer", who);
     SFB_REQUIRE(valid_dtype(dtype), "%s: unknown dtype %d", who, dtype);
@@ -126,8 +127,8 @@ static int fused_attention_common(const char *who, sfb_stream_t stream, const vo
     // (16-byte aligned bases and row pitches); everything else goes to attn_simt.cu
     const bool tma_ok = ((((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)o) & 15) == 0) && in_pitch % 8 == 0 && out_pitch % 8 == 0;
     if (tma_ok && tc_fused_attention_supported(dtype, block_size, p, scale, max_lut))
-        return tc_fused_attention(as_stream(stream), nn_lut, q, k, v, o, mask, dtype, p, scale, max_lut);
-    return simt_fused_attention(as_stream(stream), nn_lut, q, k, v, o, mask, dtype, block_size, p, scale);
+        return tc_fused_attention(as_stream(stream), nn_lut, q, k, v, o, lse, mask, dtype, p, scale, max_lut);
+    return simt_fused_attention(as_stream(stream), nn_lut, q, k, v, o, lse, mask, dtype, block_size, p, scale);
 }
 
 extern "C" int sfb_fused_attention(sfb_stream_t stream, const void *nn_lut, const void *q, const void *k, const void *v, void *o,
@@ -136,7 +137,7 @@ extern "C" int sfb_fused_attention(sfb_stream_t stream, const void *nn_lut, cons
                                    uint32_t mask_heads, float scale, uint32_t max_lut)
 {
     return fused_attention_common("sfb_fused_attention", stream, nn_lut, q, k, v, o, mask, dtype, block_size, blocks, batch_dim, ctx_blks,
-                                  head_dim, state_dim, lut_heads, lut_dim, mask_heads, scale, max_lut, 0, 0);
+                                  head_dim, state_dim, lut_heads, lut_dim, mask_heads, scale, max_lut, 0, 0, nullptr);
 }
 
 extern "C" int sfb_fused_attention_slice(sfb_stream_t stream, const void *nn_lut, const void *q, const void *k, const void *v, void *o,
@@ -146,7 +147,70 @@ extern "C" int sfb_fused_attention_slice(sfb_stream_t stream, const void *nn_lut
                                          uint64_t out_pitch)
 {
     return fused_attention_common("sfb_fused_attention_slice", stream, nn_lut, q, k, v, o, mask, dtype, block_size, blocks, batch_dim,
-                                  ctx_blks, head_dim, state_dim, lut_heads, lut_dim, mask_heads, scale, max_lut, in_pitch, out_pitch);
+                                  ctx_blks, head_dim, state_dim, lut_heads, lut_dim, mask_heads, scale, max_lut, in_pitch, out_pitch, nullptr);
+}
+
+extern "C" int sfb_fused_attention_stats(sfb_stream_t stream, const void *nn_lut, const void *q, const void *k, const void *v, void *o,
+                                         float *lse, const void *mask, int dtype, uint32_t block_size, uint32_t blocks, uint32_t batch_dim,
+                                         uint32_t ctx_blks, uint32_t head_dim, uint32_t state_dim, uint32_t lut_heads, uint32_t lut_dim,
+                                         uint32_t mask_heads, float scale, uint32_t max_lut, uint64_t in_pitch, uint64_t out_pitch)
+{
+    SFB_REQUIRE(lse, "sfb_fused_attention_stats: NULL pointer");
+    return fused_attention_common("sfb_fused_attention_stats", stream, nn_lut, q, k, v, o, mask, dtype, block_size, blocks, batch_dim,
+                                  ctx_blks, head_dim, state_dim, lut_heads, lut_dim, mask_heads, scale, max_lut, in_pitch, out_pitch, lse);
+}
+
+// bytes of the rows' constants, [B, H, L] each
+static uint64_t constants_bytes(uint32_t B, uint32_t L, uint32_t H) { return ((uint64_t)B * H * L * 4 + 255) / 256 * 256; }
+
+extern "C" uint64_t sfb_attention_backward_workspace(int dtype, uint32_t block_size, uint32_t blocks, uint32_t batch_dim, uint32_t ctx_blks,
+                                                     uint32_t head_dim, uint32_t state_dim, uint32_t nn_max, uint32_t tn_max, int aligned)
+{
+    if (!valid_dtype(dtype) || (block_size != 32 && block_size != 64) || !batch_dim || !head_dim) return 0;
+    const uint64_t rows = 2 * constants_bytes(batch_dim, ctx_blks * block_size, head_dim);
+    const AttnDims p = {batch_dim, head_dim, state_dim, ctx_blks, ctx_blks, blocks, 0, 0};
+    if (aligned && tc_backward_recompute_supported(dtype, block_size, p, nn_max, tn_max)) return rows;
+    return rows + simt_backward_workspace(dtype, block_size, blocks, batch_dim, head_dim);
+}
+
+extern "C" int sfb_attention_backward_recompute(sfb_stream_t stream, const void *nt_lut, const void *nn_lut, const void *tn_lut, const void *q,
+                                                const void *k, const void *v, const void *o, const void *dout, const float *lse,
+                                                const void *mask, void *dq, void *dk, void *dv, int dtype, uint32_t block_size,
+                                                uint32_t blocks, uint32_t batch_dim, uint32_t ctx_blks, uint32_t head_dim,
+                                                uint32_t state_dim, uint32_t lut_heads, uint32_t lut_dim, uint32_t mask_heads, float scale,
+                                                uint32_t nn_max, uint32_t tn_max, uint64_t in_pitch, uint64_t o_pitch, uint64_t dout_pitch,
+                                                uint64_t grad_pitch, void *workspace, uint64_t workspace_bytes)
+{
+    const char *who = "sfb_attention_backward_recompute";
+    SFB_REQUIRE(nt_lut && nn_lut && tn_lut && q && k && v && o && dout && lse && dq && dk && dv, "%s: NULL pointer", who);
+    SFB_REQUIRE(valid_dtype(dtype), "%s: unknown dtype %d", who, dtype);
+    if (check_common(who, block_size, batch_dim, head_dim, state_dim, lut_heads)) return 1;
+    SFB_REQUIRE(state_dim <= 128, "%s: state_dim %u > 128 not supported", who, state_dim);
+    SFB_REQUIRE(mask_heads == 1 || mask_heads == head_dim, "%s: mask_heads=%u must be 1 or head_dim", who, mask_heads);
+    SFB_REQUIRE(lut_heads == 1 || lut_dim >= blocks, "%s: lut_dim %u smaller than blocks %u", who, lut_dim, blocks);
+    const uint64_t width = (uint64_t)head_dim * state_dim;
+    uint64_t *pitches[4] = {&in_pitch, &o_pitch, &dout_pitch, &grad_pitch};
+    for (uint64_t *x : pitches) {
+        if (*x == 0) *x = width;
+        SFB_REQUIRE(*x >= width && *x < (1ull << 31), "%s: a row pitch smaller than head_dim * state_dim = %llu elements, or too large", who, (unsigned long long)width);
+    }
+    SFB_REQUIRE((uint64_t)ctx_blks * block_size < (1ull << 31), "%s: sequence too long", who);
+    if (ctx_blks == 0) { clear_error(); return 0; }
+    AttnDims p = {batch_dim, head_dim, state_dim, ctx_blks, ctx_blks, blocks, lut_heads > 1 ? lut_dim + ctx_blks : 0,
+                  mask_heads > 1 ? blocks * block_size : 0, in_pitch, 0};
+    // what the TMA and 16-byte stores can address
+    const uintptr_t all = (uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)dout | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv;
+    const bool tc = (all & 15) == 0 && ((in_pitch | dout_pitch | grad_pitch) & 7) == 0 && tc_backward_recompute_supported(dtype, block_size, p, nn_max, tn_max);
+    const uint64_t rows = constants_bytes(batch_dim, ctx_blks * block_size, head_dim);
+    const uint64_t need = 2 * rows + (tc ? 0 : simt_backward_workspace(dtype, block_size, blocks, batch_dim, head_dim));
+    SFB_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= need, "%s: needs a 16-byte aligned workspace of %llu bytes", who, (unsigned long long)need);
+    const BackwardArgs a = {nt_lut, nn_lut, tn_lut, q, k, v, o, dout, mask, dq, dk, dv, dtype, block_size, lut_heads > 1 ? lut_dim : 0, nn_max, tn_max,
+                            in_pitch, o_pitch, dout_pitch, grad_pitch, scale, p};
+    float *neg_lse = (float *)workspace, *neg_delta = (float *)((char *)workspace + rows);
+    const uint32_t L = ctx_blks * block_size;
+    if (attention_row_constants(as_stream(stream), o, dout, lse, neg_lse, neg_delta, dtype, batch_dim, L, head_dim, state_dim, o_pitch, dout_pitch, scale)) return 1;
+    if (tc) return tc_backward_recompute(as_stream(stream), a, neg_lse, neg_delta);
+    return simt_backward_recompute(as_stream(stream), a, neg_lse, neg_delta, (char *)workspace + 2 * rows);
 }
 
 static int linear_common(const char *who, sfb_stream_t stream, void *out, const void *x, const void *w, const float *bias, uint32_t m,
@@ -171,17 +235,28 @@ extern "C" int sfb_linear_residual(sfb_stream_t stream, void *out, const void *x
     return linear_common("sfb_linear_residual", stream, out, x, w, bias, m, n, k, dtype, SFB_ACT_NONE, false, resid);
 }
 
-extern "C" int sfb_embedding(sfb_stream_t stream, void *out, const void *table, const int32_t *ids, const void *pos, uint32_t batch,
-                             uint32_t seq_len, uint32_t hidden, uint32_t vocab, int dtype, uint32_t *bad_ids)
+static int embedding_common(const char *who, sfb_stream_t stream, void *out, const void *table, const int32_t *ids, const void *pos, uint32_t batch,
+                            uint32_t seq_len, uint32_t hidden, uint32_t vocab, int dtype, float scale, uint32_t *bad_ids)
 {
-    const char *who = "sfb_embedding";
     SFB_REQUIRE(out && table && ids, "%s: NULL pointer", who);
     SFB_REQUIRE(valid_dtype(dtype), "%s: unknown dtype", who);
     SFB_REQUIRE(hidden % 8 == 0, "%s: hidden=%u must be a multiple of 8", who, hidden);
     SFB_REQUIRE(aligned16(out) && aligned16(table) && (!pos || aligned16(pos)), "%s: out, table and pos must be 16-byte aligned", who);
     SFB_REQUIRE((uint64_t)batch * seq_len < (1ull << 31), "%s: too many tokens", who);
     if (batch == 0 || seq_len == 0 || hidden == 0) { clear_error(); return 0; }
-    return embedding_lookup(as_stream(stream), out, table, ids, pos, batch, seq_len, hidden, vocab, dtype, bad_ids);
+    return embedding_lookup(as_stream(stream), out, table, ids, pos, batch, seq_len, hidden, vocab, dtype, scale, bad_ids);
+}
+
+extern "C" int sfb_embedding(sfb_stream_t stream, void *out, const void *table, const int32_t *ids, const void *pos, uint32_t batch,
+                             uint32_t seq_len, uint32_t hidden, uint32_t vocab, int dtype, uint32_t *bad_ids)
+{
+    return embedding_common("sfb_embedding", stream, out, table, ids, pos, batch, seq_len, hidden, vocab, dtype, 1.f, bad_ids);
+}
+
+extern "C" int sfb_embedding_scaled(sfb_stream_t stream, void *out, const void *table, const int32_t *ids, const void *pos, uint32_t batch,
+                                    uint32_t seq_len, uint32_t hidden, uint32_t vocab, int dtype, float scale, uint32_t *bad_ids)
+{
+    return embedding_common("sfb_embedding_scaled", stream, out, table, ids, pos, batch, seq_len, hidden, vocab, dtype, scale, bad_ids);
 }
 
 static int linear_common(const char *who, sfb_stream_t stream, void *out, const void *x, const void *w, const float *bias, uint32_t m,
