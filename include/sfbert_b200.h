@@ -231,7 +231,7 @@ int sfb_fused_attention_stats(sfb_stream_t stream, const void *nn_lut, const voi
  * Operands are finite: an infinity or NaN in a row of q, k, v or dout makes the gradients of all positions NaN that share its blocks or a
  * pair of block-rows (columns) with one that does, masked or not.
  * workspace: device memory of sfb_attention_backward_workspace() bytes, 16-byte aligned, for this call alone; aligned is 1 where
- * q, k, v, dout, dq, dk and dv are 16-byte aligned and their pitches multiples of 8 elements, 0 otherwise or where that is unknown
+ * q, k, v, dout, dq, dk, dv and mask are 16-byte aligned and the pitches multiples of 8 elements, 0 otherwise or where that is unknown
  * (which 16-bit operands with blocks and heads of 64 need more workspace for).  No counterpart in the reference. */
 uint64_t sfb_attention_backward_workspace(int dtype, uint32_t block_size, uint32_t blocks, uint32_t batch_dim, uint32_t ctx_blks,
                                           uint32_t head_dim, uint32_t state_dim, uint32_t nn_max, uint32_t tn_max, int aligned);

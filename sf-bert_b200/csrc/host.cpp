@@ -885,7 +885,7 @@ FUNCTION(py_attention_backward_recompute, 10)
         const uint32_t tn_max = attr_u32(lay.o, n_tn_max);
         void *nt = table_on(lay, n_nt_lut, 2ll * lay.heads * lay.blocks, q, bad_layout), *nn = table_on(lay, n_nn_lut, 2ll * lay.heads * (lay.nb + lay.blocks), q, bad_layout);
         void *tn = table_on(lay, n_tn_lut, 2ll * lay.heads * (lay.nb + lay.blocks), q, bad_layout), *mask = mask_on(lay, use_mask, q);
-        uintptr_t all = 0;
+        uintptr_t all = (uintptr_t)mask;
         for (const at::Tensor &t : {q, k, v, dout, grad[0], grad[1], grad[2]}) all |= (uintptr_t)ptr(t);
         const int aligned = (all & 15) == 0 && ((pitch | do_pitch | grad_pitch) & 7) == 0;
         const uint64_t bytes = L.sfb_attention_backward_workspace(tag(q), lay.bs, lay.blocks, n.B, lay.nb, n.H, n.d, lay.nn_max, tn_max, aligned);

@@ -198,8 +198,8 @@ extern "C" int sfb_attention_backward_recompute(sfb_stream_t stream, const void 
     if (ctx_blks == 0) { clear_error(); return 0; }
     AttnDims p = {batch_dim, head_dim, state_dim, ctx_blks, ctx_blks, blocks, lut_heads > 1 ? lut_dim + ctx_blks : 0,
                   mask_heads > 1 ? blocks * block_size : 0, in_pitch, 0};
-    // what the TMA and 16-byte stores can address
-    const uintptr_t all = (uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)dout | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv;
+    // what the TMA, bulk copies (of mask words) and 16-byte stores can address
+    const uintptr_t all = (uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)dout | (uintptr_t)mask | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv;
     const bool tc = (all & 15) == 0 && ((in_pitch | dout_pitch | grad_pitch) & 7) == 0 && tc_backward_recompute_supported(dtype, block_size, p, nn_max, tn_max);
     const uint64_t rows = constants_bytes(batch_dim, ctx_blks * block_size, head_dim);
     const uint64_t need = 2 * rows + (tc ? 0 : simt_backward_workspace(dtype, block_size, blocks, batch_dim, head_dim));
@@ -324,7 +324,7 @@ extern "C" int sfb_attention_backward(sfb_stream_t stream, const void *nn_lut, c
 
 extern "C" int sfb_device_status_clear(void)
 {
-    if (tc_status_clear_backward() || tc_status_clear_fused() || tc_status_clear_unfused() || tc_status_clear_gemm()) return 1;
+    if (tc_status_clear_backward() || tc_status_clear_fused() || tc_status_clear_unfused() || tc_status_clear_gemm() || tc_status_clear_recompute()) return 1;
     clear_error();
     return 0;
 }
@@ -332,9 +332,9 @@ extern "C" int sfb_device_status_clear(void)
 extern "C" int sfb_device_status(uint32_t *status)
 {
     SFB_REQUIRE(status, "sfb_device_status: NULL pointer");
-    uint32_t a = 0, b = 0, c = 0, d = 0;
-    if (tc_status_fused(&a) || tc_status_unfused(&b) || tc_status_gemm(&c) || tc_status_backward(&d)) return 1;
-    *status = a ? a : b ? b : c ? c : d;
+    uint32_t a = 0, b = 0, c = 0, d = 0, e = 0;
+    if (tc_status_fused(&a) || tc_status_unfused(&b) || tc_status_gemm(&c) || tc_status_backward(&d) || tc_status_recompute(&e)) return 1;
+    *status = a ? a : b ? b : c ? c : d ? d : e;
     clear_error();
     return 0;
 }

@@ -24,5 +24,7 @@ int simt_backward_recompute(cudaStream_t s, const BackwardArgs &a, float *neg_ls
 // tcgen05 (attn_tc_recompute.cu): 16-bit operands, 64x64 blocks, 64-wide heads
 bool tc_backward_recompute_supported(int dtype, uint32_t bs, const AttnDims &p, uint32_t nn_max, uint32_t tn_max);
 int tc_backward_recompute(cudaStream_t s, const BackwardArgs &a, const float *neg_lse, const float *neg_delta);
+int tc_status_recompute(uint32_t *out);
+int tc_status_clear_recompute();
 
 }  // namespace sfb
