@@ -314,6 +314,27 @@ def test_long_rows_of_many_blocks(sfb):
     assert sfb.device_status() == 0
 
 
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("kind", ["diagonal", "two", "three", "mixed", "empty rows"])
+def test_many_short_rows(sfb, dtype, kind):
+    """Dozens of row pairs (column pairs) per CTA, most of them with one to three steps: against the fp32 path."""
+    bs, nb, B, H = 64, 64, 3, 12
+    i, j = np.arange(nb)[:, None], np.arange(nb)[None, :]
+    blocks = {"diagonal": i == j, "two": (i == j) | (j == (i ^ 1)), "three": (j >= i) & (j <= i + 1), "mixed": (j >= i) & (j <= i + i % 5) | (i == 40),
+              "empty rows": (i == j) & (i % 7 < 3)}[kind][None].astype(np.uint8)
+    lay = plan(sfb, blocks, bs)
+    q, k, v, do = (x.cuda() for x in operands(B, nb * bs, H, 64, dtype, 12))
+    o, lse = sfb.fused_attention_stats(q, k, v, lay)
+    want = sfb.attention_backward_recompute(q.float(), k.float(), v.float(), o.float(), do.float(), lse, lay)
+    for _ in range(3):
+        got = sfb.attention_backward_recompute(q, k, v, o, do, lse, lay)
+        assert sfb.device_status() == 0
+        for a, b in zip(got, want):
+            # half a step each of P, dS and the result, block by block of 64 positions and a head
+            off, size = ((x.view(B, nb, bs, H, 64).square().sum((2, 4)).sqrt()) for x in (a.float() - b, b))
+            assert (off <= 3 * half_step(DTYPES[dtype]) * size).all(), float((off / size).max())
+
+
 # ---- embedding ------------------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("B,L,hidden,scale,pos", [(1, 1, 8, 32.0, False), (3, 77, 768, 27.7, True), (5, 9, 264, -0.5, True), (64, 1, 1024, 32.0, False)])
