@@ -2,12 +2,12 @@
 //   dtable[v] = scale sum over the tokens with id v of dout,     dpos[l] = sum over the batch of dout[., l].
 // No atomics on floating-point numbers: every sum has a fixed order, so that the same inputs give the same bits.
 //
-// Four launches.  (1) sort_ids_kernel brings the tokens into the order of their ids, equal ids by position.  (2) pos_grad_kernel adds
-// up the batch, reading dout in order.  (3) table_grad_kernel walks the sorted tokens in pieces of equal length, so that a word that
+// Three launches.  (1) sort_and_positions_kernel: some CTAs bring the tokens into the order of their ids, equal ids by position, while the others
+// add up the batch, reading dout in order.  (2) table_grad_kernel walks the sorted tokens in pieces of equal length, so that a word that
 // is a tenth of the text does not hang on one CTA; a run of equal ids that lies in one piece is written at once, the parts of
 // one that does not go to the workspace.  The rows of tokens that do not occur are written as zeros by the same launch.
-// (4) join_kernel adds up the parts.  Bound by memory: dout is read by (2) and gathered by (3), from L2 where it fits, and the table's
-// gradient is written once.
+// (3) join_kernel adds up the parts.  Bound by memory: dout is read by (1) and gathered by (2), from L2 where it fits, and the table's
+// gradient is written once (a fill runs at 3.8 TB/s on this part, where a copy runs at 6.5).
 #include "common.cuh"
 
 namespace sfb {
@@ -20,7 +20,7 @@ struct GradArgs {
     const void *dout;
     const int32_t *ids;
     void *dtable, *dpos;
-    uint32_t n, batch, len, hidden, vocab, range, piece, pieces;
+    uint32_t n, batch, len, hidden, vocab, range, sorters, ways, piece, pieces;
     float scale;
     int accumulate;
     uint32_t *bad;
@@ -43,22 +43,36 @@ __device__ __forceinline__ uint32_t warp_scan(uint32_t v, uint32_t lane)      //
 // A CTA owns `range` consecutive ids and looks at all tokens: it counts those below its range, which is where its part of the sorted
 // list begins, and collects its own in order, a share of the tokens per warp.  These are then sorted by counting, per warp and id, so
 // that equal ids stay in order.  No CTA waits for another.  The ids come from L2 (4 bytes per token and CTA).
-__global__ void __launch_bounds__(kSortThreads) sort_ids_kernel(const GradArgs a)
+__device__ __forceinline__ void sort_ids(const GradArgs &a, uint32_t *count)      // count: [range][kSortWarps]
 {
-    extern __shared__ uint32_t count[];              // [range][kSortWarps]
     __shared__ uint32_t s_below[kSortWarps], s_mine[kSortWarps], s_bad[kSortWarps], s_sum[kSortWarps];
-    grid_dependency_wait();
-    grid_launch_dependents();
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t lo = blockIdx.x * a.range, width = min(a.range, a.vocab - lo);
-    const uint32_t share = ((a.n + kSortWarps - 1) / kSortWarps + 31) / 32 * 32, t0 = min(a.n, warp * share), t1 = min(a.n, t0 + share);
+    // a warp's share of the tokens, 128 at a time: four neighbours per lane, four such loads on their way
+    const uint32_t share = ((a.n + kSortWarps - 1) / kSortWarps + 127) / 128 * 128, t0 = min(a.n, warp * share), t1 = min(a.n, t0 + share);
+    const bool wide = ((uintptr_t)a.ids & 15) == 0;
+    auto fetch = [&](uint32_t t, uint32_t (&id)[4]) {          // tokens t to t + 3; beyond the share: no id
+        if (wide && t + 4 <= t1) {
+            const uint4 u = __ldg((const uint4 *)(a.ids + t));
+            id[0] = u.x; id[1] = u.y; id[2] = u.z; id[3] = u.w;
+        } else {
+#pragma unroll
+            for (uint32_t j = 0; j < 4; j++) id[j] = t + j < t1 ? (uint32_t)__ldg(a.ids + t + j) : 0xffffffffu;
+        }
+    };
     uint32_t below = 0, mine = 0, bad = 0;
-#pragma unroll 8
-    for (uint32_t t = t0 + lane; t < t1; t += 32) {
-        const uint32_t id = (uint32_t)__ldg(a.ids + t);        // a negative id is a large one
-        below += id < lo;
-        mine += id - lo < width;
-        bad += id >= a.vocab;
+    for (uint32_t t = t0; t < t1; t += 512) {
+        uint32_t id[4][4];
+#pragma unroll
+        for (uint32_t k = 0; k < 4; k++) fetch(t + 128 * k + 4 * lane, id[k]);
+#pragma unroll
+        for (uint32_t k = 0; k < 4; k++)
+#pragma unroll
+            for (uint32_t j = 0; j < 4; j++) {                 // a negative id is a large one
+                below += id[k][j] < lo;
+                mine += id[k][j] - lo < width;
+                bad += t + 128 * k + 4 * lane + j < t1 && id[k][j] >= a.vocab;
+            }
     }
     below = __reduce_add_sync(0xffffffffu, below);
     mine = __reduce_add_sync(0xffffffffu, mine);
@@ -83,12 +97,24 @@ __global__ void __launch_bounds__(kSortThreads) sort_ids_kernel(const GradArgs a
     int2 *list = a.unsorted + base;
     if (total) {
         uint32_t at = before;
-        for (uint32_t t = t0; t < t1; t += 32) {               // whole warps: t0 and share are multiples of 32, t1 need not be
-            const uint32_t id = t + lane < t1 ? (uint32_t)__ldg(a.ids + t + lane) : 0xffffffffu;
-            const bool in = id - lo < width;
-            const uint32_t votes = __ballot_sync(0xffffffffu, in);
-            if (in) list[at + __popc(votes & ((1u << lane) - 1u))] = make_int2((int)(t + lane), (int)id);
-            at += __popc(votes);
+        for (uint32_t t = t0; t < t1; t += 512) {
+            uint32_t id[4][4];
+#pragma unroll
+            for (uint32_t k = 0; k < 4; k++) fetch(t + 128 * k + 4 * lane, id[k]);
+#pragma unroll
+            for (uint32_t k = 0; k < 4; k++) {
+                uint32_t lower = 0, all = 0;                   // of the lanes below; of all
+#pragma unroll
+                for (uint32_t j = 0; j < 4; j++) {
+                    const uint32_t votes = __ballot_sync(0xffffffffu, id[k][j] - lo < width);
+                    lower += __popc(votes & ((1u << lane) - 1u));
+                    all += __popc(votes);
+                }
+#pragma unroll
+                for (uint32_t j = 0; j < 4; j++)
+                    if (id[k][j] - lo < width) list[at + lower++] = make_int2((int)(t + 128 * k + 4 * lane + j), (int)id[k][j]);
+                at += all;
+            }
         }
     }
     __syncthreads();
@@ -213,8 +239,8 @@ __device__ __forceinline__ void write_sums(void *out, size_t at, const float (&s
     }
 }
 
-// A warp takes `piece` sorted tokens and 32 lanes' columns.  The first CTAs do this, the others write the rows of tokens that do
-// not occur.
+// A warp takes `piece` sorted tokens and 32 lanes' columns.  The first CTAs do this, the others write the rows of
+// tokens that do not occur (in turn, one of each kind: 70 -> 72 us).
 template <int DT, int GT>
 __global__ void __launch_bounds__(256) table_grad_kernel(const GradArgs a)
 {
@@ -225,9 +251,11 @@ __global__ void __launch_bounds__(256) table_grad_kernel(const GradArgs a)
     const uint32_t groups = (a.hidden / N + 31) / 32, y = blockIdx.x / groups, col = ((blockIdx.x - y * groups) * 32 + lane) * N;
     const bool live = col < a.hidden;
     const uint32_t piece_ctas = (a.pieces + 7) / 8;
-    if (y >= piece_ctas) {
+    const bool zeros = y >= piece_ctas;
+    const uint32_t at = zeros ? y - piece_ctas : y;
+    if (zeros) {
         if (a.accumulate) return;
-        const uint32_t v0 = ((y - piece_ctas) * 8 + warp) * 32;
+        const uint32_t v0 = (at * 8 + warp) * 32;
         const bool empty = v0 + lane < a.vocab && a.starts[v0 + lane] == a.starts[v0 + lane + 1];
         uint32_t todo = __ballot_sync(0xffffffffu, empty);
         const float none[N] = {};
@@ -235,7 +263,7 @@ __global__ void __launch_bounds__(256) table_grad_kernel(const GradArgs a)
             if (live) write_sums<GT, N>(a.dtable, (size_t)(v0 + __ffs(todo) - 1) * a.hidden + col, none, 1.f, false);
         return;
     }
-    const uint32_t c = y * 8 + warp, total = a.starts[a.vocab];
+    const uint32_t c = at * 8 + warp, total = a.starts[a.vocab];
     const uint32_t i0 = c * a.piece, i1 = min(total, i0 + a.piece);
     if (i0 >= total) return;
     const int before = i0 ? a.sorted[i0 - 1].y : -1, after = i1 < total ? a.sorted[i1].y : -1;
@@ -282,72 +310,112 @@ __global__ void __launch_bounds__(256) table_grad_kernel(const GradArgs a)
     flush(cur == after);
 }
 
-// The runs that more than one piece has.  A CTA per piece in which such a run begins; its warps take shares of the parts.
+// The runs that more than one piece has.  A warp looks at the end of a piece for a run that begins in it and goes on, and adds up its parts; those
+// of a long one are shared by the CTA's warps.
+constexpr uint32_t kAlone = 16;                      // parts that a warp adds up by itself
 template <int GT>
 __global__ void __launch_bounds__(256) join_kernel(const GradArgs a)
 {
     __shared__ float4 share[8][32];
+    __shared__ uint32_t long_id[8], long_parts[8];
     grid_dependency_wait();
     grid_launch_dependents();
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t groups = (a.hidden / 4 + 31) / 32, c = blockIdx.x / groups, total = a.starts[a.vocab], end = (c + 1) * a.piece;
-    if (end >= total) return;
-    const int id = a.sorted[end - 1].y;
-    if (a.sorted[end].y != id || a.starts[id] < c * a.piece) return;
-    const uint32_t col = ((blockIdx.x - c * groups) * 32 + lane) * 4;
+    const uint32_t groups = (a.hidden / 4 + 31) / 32, y = blockIdx.x / groups, col = ((blockIdx.x - y * groups) * 32 + lane) * 4;
     const bool live = col < a.hidden;
+    const uint32_t c = y * 8 + warp, total = a.starts[a.vocab];
+    const uint64_t end = (uint64_t)(c + 1) * a.piece;
     // part 0 is this piece's second slot, part k the first slot of piece c + k
-    const uint32_t parts = 1 + (a.starts[id + 1] - end + a.piece - 1) / a.piece, per = (parts + 7) / 8;
-    const uint32_t k0 = min(parts, warp * per), k1 = min(parts, k0 + per);
-    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (live) {
+    auto sum = [&](uint32_t c0, uint32_t k0, uint32_t k1) {
+        float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (live) {
 #pragma unroll 8
-        for (uint32_t k = k0; k < k1; k++) {
-            const float4 u = *(const float4 *)(a.parts + ((size_t)(c + k) * 2 + (k ? 0 : 1)) * a.hidden + col);
-            s.x += u.x; s.y += u.y; s.z += u.z; s.w += u.w;
+            for (uint32_t k = k0; k < k1; k++) {
+                const float4 u = *(const float4 *)(a.parts + ((size_t)(c0 + k) * 2 + (k ? 0 : 1)) * a.hidden + col);
+                s.x += u.x; s.y += u.y; s.z += u.z; s.w += u.w;
+            }
         }
+        return s;
+    };
+    auto write = [&](uint32_t id, const float4 &s) {
+        const float v[4] = {s.x, s.y, s.z, s.w};
+        if (live) write_sums<GT, 4>(a.dtable, (size_t)id * a.hidden + col, v, a.scale, a.accumulate);
+    };
+    uint32_t parts = 0, id = 0;
+    if (end < total) {
+        id = (uint32_t)a.sorted[end - 1].y;
+        const uint32_t next = (uint32_t)a.sorted[end].y, first = a.starts[id], last = a.starts[id + 1];
+        if (next == id && first >= c * a.piece) parts = 1 + (uint32_t)((last - end + a.piece - 1) / a.piece);
     }
-    share[warp][lane] = s;
+    if (parts && parts <= kAlone) write(id, sum(c, 0, parts));
+    if (lane == 0) {
+        long_id[warp] = id;
+        long_parts[warp] = parts > kAlone ? parts : 0;
+    }
     __syncthreads();
-    if (warp || !live) return;
+    for (uint32_t w = 0; w < 8; w++) {
+        const uint32_t n = long_parts[w];
+        if (!n) continue;
+        const uint32_t per = (n + 7) / 8, k0 = min(n, warp * per);
+        float4 s = sum(y * 8 + w, k0, min(n, k0 + per));
+        share[warp][lane] = s;
+        __syncthreads();
+        if (warp == 0) {
 #pragma unroll
-    for (int w = 1; w < 8; w++) {
-        const float4 u = share[w][lane];
-        s.x += u.x; s.y += u.y; s.z += u.z; s.w += u.w;
+            for (int k = 1; k < 8; k++) {
+                const float4 u = share[k][lane];
+                s.x += u.x; s.y += u.y; s.z += u.z; s.w += u.w;
+            }
+            write(long_id[w], s);
+        }
+        __syncthreads();
     }
-    const float v[4] = {s.x, s.y, s.z, s.w};
-    write_sums<GT, 4>(a.dtable, (size_t)id * a.hidden + col, v, a.scale, a.accumulate);
 }
 
-// dpos: a warp has 32 lanes' columns of one position and a share of the batch (WAYS warps per position).
-template <int DT, int GT, int WAYS>
-__global__ void __launch_bounds__(256) pos_grad_kernel(const GradArgs a)
+// dpos: a warp has 32 lanes' columns of one position and a share of the batch (`ways` warps per position, whose shares meet in shared memory)
+template <int DT, int GT>
+__device__ __forceinline__ void add_positions(const GradArgs &a, uint32_t cta, float *share)      // share: [kSortWarps][N][33]
 {
-    constexpr int N = Piece<DT>::N, PER = 8 / WAYS;
-    __shared__ float share[WAYS > 1 ? 8 : 1][N][33];
-    grid_dependency_wait();
-    grid_launch_dependents();
-    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t groups = (a.hidden / N + 31) / 32, y = blockIdx.x / groups, col = ((blockIdx.x - y * groups) * 32 + lane) * N, l = y * PER + warp / WAYS;
+    constexpr int N = Piece<DT>::N;
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, ways = a.ways, part = warp % ways;
+    const uint32_t groups = (a.hidden / N + 31) / 32, y = cta / groups, col = ((cta - y * groups) * 32 + lane) * N, l = y * (kSortWarps / ways) + warp / ways;
     const bool live = col < a.hidden && l < a.len;
-    const uint32_t per = (a.batch + WAYS - 1) / WAYS, b0 = min(a.batch, warp % WAYS * per), b1 = min(a.batch, b0 + per);
+    const uint32_t per = (a.batch + ways - 1) / ways, b0 = min(a.batch, part * per), b1 = min(a.batch, b0 + per);
     float s[N] = {};
     if (live) {
         const typename Elem<DT>::type *src = (const typename Elem<DT>::type *)a.dout + (size_t)l * a.hidden + col;
-#pragma unroll 8
-        for (uint32_t b = b0; b < b1; b++) Piece<DT>::add(s, __ldg((const uint4 *)(src + (size_t)b * a.len * a.hidden)));
+        const size_t step = (size_t)a.len * a.hidden;
+        uint32_t b = b0;
+        for (; b + 8 <= b1; b += 8) {
+            uint4 u[8];
+#pragma unroll
+            for (int k = 0; k < 8; k++) u[k] = __ldg((const uint4 *)(src + (b + k) * step));
+#pragma unroll
+            for (int k = 0; k < 8; k++) Piece<DT>::add(s, u[k]);
+        }
+        for (; b < b1; b++) Piece<DT>::add(s, __ldg((const uint4 *)(src + b * step)));
     }
-    if (WAYS > 1) {
+    if (ways > 1) {
 #pragma unroll
-        for (int i = 0; i < N; i++) share[warp][i][lane] = s[i];
+        for (int i = 0; i < N; i++) share[(warp * N + i) * 33 + lane] = s[i];
         __syncthreads();
-        if (warp % WAYS) return;
+        if (part) return;
+        for (uint32_t w = 1; w < ways; w++)
 #pragma unroll
-        for (int w = 1; w < WAYS; w++)
-#pragma unroll
-            for (int i = 0; i < N; i++) s[i] += share[warp + w][i][lane];
+            for (int i = 0; i < N; i++) s[i] += share[((warp + w) * N + i) * 33 + lane];
     }
     if (live) write_sums<GT, N>(a.dpos, (size_t)l * a.hidden + col, s, 1.f, a.accumulate);
+}
+
+// The first CTAs sort, the others add up positions: one waits for latencies while the other moves data.
+template <int DT, int GT>
+__global__ void __launch_bounds__(kSortThreads) sort_and_positions_kernel(const GradArgs a)
+{
+    extern __shared__ __align__(16) uint32_t dynamic[];
+    grid_dependency_wait();
+    grid_launch_dependents();
+    if (blockIdx.x < a.sorters) sort_ids(a, dynamic);
+    else add_positions<DT, GT>(a, blockIdx.x - a.sorters, (float *)dynamic);
 }
 
 // sorted tokens per piece: short enough for a long run to spread, long enough for its parts to be few
@@ -356,7 +424,7 @@ static uint64_t padded(uint64_t bytes) { return (bytes + 63) / 64 * 64; }
 static uint32_t piece_count(uint32_t n) { return (uint32_t)(((uint64_t)n + piece_length(n) - 1) / piece_length(n)); }
 
 template <int DT, int GT>
-static int launch(cudaStream_t s, const GradArgs &a)
+static int launch(cudaStream_t s, GradArgs a)
 {
     const int dev = current_device(), sms = device_sm_count(dev);
     if (sms <= 0) return fail("sfb_embedding_grad: cannot query the device");
@@ -364,25 +432,25 @@ static int launch(cudaStream_t s, const GradArgs &a)
     const uint64_t groups = (a.hidden / N + 31) / 32, rows = (a.pieces + 7) / 8 + ((uint64_t)a.vocab + 255) / 256;
     SFB_REQUIRE(groups * a.len < (1ull << 31) && groups * rows < (1ull << 31) && (uint64_t)((a.hidden / 4 + 31) / 32) * a.pieces < (1ull << 31),
                 "sfb_embedding_grad: too many rows for one launch");
+    // positions enough to fill the SMs: a warp each; otherwise several share the batch of one
+    uint64_t pos_ctas = 0;
     if (a.dpos) {
-        // positions enough to fill the SMs: a warp each; otherwise several share the batch of one
         const uint64_t warps = groups * a.len, want = 16ull * sms;
-        const uint32_t ways = warps >= want || a.batch < 16 ? 1 : warps * 2 >= want ? 2 : 8, per = 8 / ways;
-        const dim3 grid((unsigned)(groups * ((a.len + per - 1) / per)));
-        if (ways == 1) launch_overlapped(pos_grad_kernel<DT, GT, 1>, grid, dim3(256), 0, s, a);
-        else if (ways == 2) launch_overlapped(pos_grad_kernel<DT, GT, 2>, grid, dim3(256), 0, s, a);
-        else launch_overlapped(pos_grad_kernel<DT, GT, 8>, grid, dim3(256), 0, s, a);
+        a.ways = 1;
+        while (a.ways < kSortWarps && warps * a.ways < want && a.batch >= 16 * a.ways) a.ways *= 2;
+        pos_ctas = groups * ((a.len + kSortWarps / a.ways - 1) / (kSortWarps / a.ways));
     }
-    const uint32_t ctas = (a.vocab + a.range - 1) / a.range;
+    size_t smem = (size_t)a.range * kSortWarps * 4;
+    if (a.dpos && a.ways > 1 && smem < sizeof(float) * kSortWarps * N * 33) smem = sizeof(float) * kSortWarps * N * 33;
     static DeviceOnce once;
     if (!once.done(dev)) {
-        if (cudaFuncSetAttribute(sort_ids_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(kMaxRange * kSortWarps * 4)) != cudaSuccess)
+        if (cudaFuncSetAttribute(sort_and_positions_kernel<DT, GT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(kMaxRange * kSortWarps * 4)) != cudaSuccess)
             return fail("sfb_embedding_grad: cannot reserve shared memory");
         once.mark(dev);
     }
-    launch_overlapped(sort_ids_kernel, dim3(ctas), dim3(kSortThreads), (size_t)a.range * kSortWarps * 4, s, a);
+    launch_overlapped(sort_and_positions_kernel<DT, GT>, dim3((unsigned)(a.sorters + pos_ctas)), dim3(kSortThreads), smem, s, a);
     launch_overlapped(table_grad_kernel<DT, GT>, dim3((unsigned)(groups * rows)), dim3(256), 0, s, a);
-    if (a.pieces > 1) launch_overlapped(join_kernel<GT>, dim3((a.hidden / 4 + 31) / 32 * (a.pieces - 1)), dim3(256), 0, s, a);
+    if (a.pieces > 1) launch_overlapped(join_kernel<GT>, dim3((a.hidden / 4 + 31) / 32 * ((a.pieces - 1 + 7) / 8)), dim3(256), 0, s, a);
     return check_launch("sfb_embedding_grad");
 }
 
@@ -423,11 +491,12 @@ extern "C" int sfb_embedding_grad(sfb_stream_t stream, void *dtable, void *dpos,
         clear_error();
         return 0;
     }
-    GradArgs a = {dout, ids, dtable, dpos, (uint32_t)n, batch, seq_len, hidden, vocab, 0, piece_length((uint32_t)n), piece_count((uint32_t)n), scale, accumulate, bad_ids};
+    GradArgs a = {dout, ids, dtable, dpos, (uint32_t)n, batch, seq_len, hidden, vocab, 0, 0, 1, piece_length((uint32_t)n), piece_count((uint32_t)n), scale, accumulate, bad_ids};
     // a CTA per SM sorts, more where its counters would not fit
     const int sms = device_sm_count(current_device());
     const uint32_t ctas = max((uint32_t)(sms > 0 ? sms : 1), (vocab + kMaxRange - 1) / kMaxRange);
     a.range = (vocab + ctas - 1) / ctas;
+    a.sorters = (vocab + a.range - 1) / a.range;
     char *w = (char *)workspace;
     a.sorted = (int2 *)w;
     a.unsorted = (int2 *)(w += padded(n * 8));

@@ -15,9 +15,13 @@ namespace sfb {
 namespace gn {
 
 constexpr uint32_t kThreads = 256;
-constexpr uint32_t kChunk = 16384;                   // elements
+constexpr uint32_t kMostChunk = 16384, kLeastChunk = 2048;      // elements: a CTA's unit, shorter where the list is
 constexpr uint32_t kMost = 768;                      // tensors per launch (kernel parameters: 32764 bytes)
 constexpr uint32_t kCtasPerSm = 4;
+// Shared memory that a CTA asks for and does not use: no SM then takes more than four.  Launched behind each other's back, the second launch's CTAs
+// went eight at a time to the first SMs that had room, and half of the SMs had none (clipping 334 M elements 468 -> 834 us).
+constexpr size_t kRoom = 46 * 1024;
+static_assert(kCtasPerSm * (kRoom + 1024) <= 228 * 1024 && (kCtasPerSm + 1) * (kRoom + 1024) > 228 * 1024, "four CTAs per SM, not five");
 
 struct Entry {
     const void *in;
@@ -28,7 +32,7 @@ template <uint32_t M> struct List {
     Entry t[M];
     uint32_t first[M + 1];                           // chunk at which tensor i begins; first[count]: all chunks
     uint8_t types[M];                                // in | out << 4
-    uint32_t count;
+    uint32_t count, chunk;
 };
 
 template <int DT> __device__ __forceinline__ float widen(const typename Elem<DT>::type &v)
@@ -69,28 +73,57 @@ template <uint32_t M> __device__ __forceinline__ uint32_t find(const List<M> &l,
     return lo;
 }
 
+// Sum of the squares of a piece.  fp32: each in fp64.  16 bits: a product of two is exact in fp32 and four of them are added there (three
+// roundings, 2^-24 each of at most the sum), which leaves a quarter of the conversions and fp64 additions: all in fp64, 334 M fp16
+// elements took 182 us.  bf16 squares that leave fp32's range, or come near its end, are made in fp64.
+template <int DT> __device__ __forceinline__ void add_squares(double &s0, double &s1, const uint4 &u)
+{
+    float v[Vec<DT>::N];
+    Vec<DT>::decode(v, u);
+    if constexpr (DT == SFB_F32) {
+        s0 = fma((double)v[0], (double)v[0], s0);
+        s1 = fma((double)v[1], (double)v[1], s1);
+        s0 = fma((double)v[2], (double)v[2], s0);
+        s1 = fma((double)v[3], (double)v[3], s1);
+    } else {
+        const uint32_t any[2] = {(u.x | u.y) & 0x7fff7fffu, (u.z | u.w) & 0x7fff7fffu};
+        double *s[2] = {&s0, &s1};
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const float *x = v + 4 * h;
+            const float p = fmaf(x[0], x[0], x[1] * x[1]) + fmaf(x[2], x[2], x[3] * x[3]);
+            if (DT == SFB_F16 || (p > 1e-30f && p < 1e37f)) {
+                *s[h] += (double)p;
+            } else if (any[h]) {
+#pragma unroll
+                for (int j = 0; j < 4; j++) *s[h] = fma((double)x[j], (double)x[j], *s[h]);
+            }
+        }
+    }
+}
+constexpr int kAhead = 8;                            // 16-byte loads of a thread on their way
 template <int DT> __device__ __forceinline__ double chunk_squares(const void *in, uint64_t begin, uint64_t end)
 {
     constexpr int N = Vec<DT>::N;
     const typename Elem<DT>::type *p = (const typename Elem<DT>::type *)in;
     double s0 = 0.0, s1 = 0.0;
     // up to the first 16-byte boundary, whole pieces, the rest
-    const uint64_t lead = ((16 - ((uintptr_t)(p + begin) & 15)) & 15) / sizeof(*p), body = min(end, begin + lead), pieces = (end - body) / N, tail = body + pieces * N;
+    const uint64_t lead = ((16 - ((uintptr_t)(p + begin) & 15)) & 15) / sizeof(*p), body = min(end, begin + lead), tail = body + (end - body) / N * N;
+    const uint32_t pieces = (uint32_t)((tail - body) / N);
     if (begin + threadIdx.x < body) {
         const double v = widen<DT>(p[begin + threadIdx.x]);
         s0 = v * v;
     }
     const uint4 *q = (const uint4 *)(p + body);
-#pragma unroll 4
-    for (uint32_t i = threadIdx.x; i < pieces; i += kThreads) {
-        float v[N];
-        Vec<DT>::decode(v, __ldg(q + i));
+    uint32_t i = threadIdx.x;
+    for (; i + (kAhead - 1) * kThreads < pieces; i += kAhead * kThreads) {
+        uint4 u[kAhead];
 #pragma unroll
-        for (int j = 0; j < N; j += 2) {
-            s0 = fma((double)v[j], (double)v[j], s0);
-            s1 = fma((double)v[j + 1], (double)v[j + 1], s1);
-        }
+        for (int k = 0; k < kAhead; k++) u[k] = __ldg(q + i + k * kThreads);
+#pragma unroll
+        for (int k = 0; k < kAhead; k++) add_squares<DT>(s0, s1, u[k]);
     }
+    for (; i < pieces; i += kThreads) add_squares<DT>(s0, s1, __ldg(q + i));
     if (tail + threadIdx.x < end) {
         const double v = widen<DT>(p[tail + threadIdx.x]);
         s1 = fma(v, v, s1);
@@ -120,7 +153,7 @@ __global__ void __launch_bounds__(kThreads) square_sums_kernel(const __grid_cons
     double s = 0.0;
     for (uint32_t c = blockIdx.x; c < chunks; c += gridDim.x) {
         const uint32_t i = find(l, c);
-        const uint64_t begin = (uint64_t)(c - l.first[i]) * kChunk, end = min(l.t[i].n, begin + kChunk);
+        const uint64_t begin = (uint64_t)(c - l.first[i]) * l.chunk, end = min(l.t[i].n, begin + l.chunk);
         const int t = l.types[i] & 15;
         s += t == SFB_F32 ? chunk_squares<SFB_F32>(l.t[i].in, begin, end) : t == SFB_BF16 ? chunk_squares<SFB_BF16>(l.t[i].in, begin, end) : chunk_squares<SFB_F16>(l.t[i].in, begin, end);
     }
@@ -163,21 +196,30 @@ __device__ __forceinline__ void chunk_scale(const void *in, void *out, uint64_t 
     // whole pieces of 16 bytes where both sides have their boundaries at the same elements
     const uint64_t lead = ((16 - ((uintptr_t)(p + begin) & 15)) & 15) / S;
     const bool vec = (((uintptr_t)out + (begin + lead) * G) & 15) == 0;
-    const uint64_t body = vec ? min(end, begin + lead) : end, pieces = (end - body) / N, tail = body + pieces * N;
     if (vec) {
+        const uint64_t body = min(end, begin + lead), tail = body + (end - body) / N * N;
+        const uint32_t pieces = (uint32_t)((tail - body) / N);
         if (begin + threadIdx.x < body) put<GT>(out, begin + threadIdx.x, widen<DT>(p[begin + threadIdx.x]) * factor);
         if (tail + threadIdx.x < end) put<GT>(out, tail + threadIdx.x, widen<DT>(p[tail + threadIdx.x]) * factor);
+        const uint4 *q = (const uint4 *)(p + body);
 #pragma unroll 4
         for (uint32_t i = threadIdx.x; i < pieces; i += kThreads) {
             float v[N];
-            Vec<DT>::decode(v, *((const uint4 *)(p + body) + i));
+            Vec<DT>::decode(v, q[i]);
 #pragma unroll
             for (int j = 0; j < N; j++) v[j] *= factor;
             put_vec<GT>(out, body + (uint64_t)i * N, v);
         }
     } else {
-#pragma unroll 8
-        for (uint64_t i = begin + threadIdx.x; i < end; i += kThreads) put<GT>(out, i, widen<DT>(p[i]) * factor);
+        uint64_t i = begin + threadIdx.x;
+        for (; i + (kAhead - 1) * kThreads < end; i += kAhead * kThreads) {
+            float v[kAhead];
+#pragma unroll
+            for (int k = 0; k < kAhead; k++) v[k] = widen<DT>(p[i + k * kThreads]) * factor;
+#pragma unroll
+            for (int k = 0; k < kAhead; k++) put<GT>(out, i + k * kThreads, v[k]);
+        }
+        for (; i < end; i += kThreads) put<GT>(out, i, widen<DT>(p[i]) * factor);
     }
 }
 
@@ -200,7 +242,7 @@ __global__ void __launch_bounds__(kThreads) clip_kernel(const __grid_constant__ 
     const uint32_t chunks = l.first[l.count];
     for (uint32_t k = blockIdx.x; k < chunks; k += gridDim.x) {
         const uint32_t c = chunks - 1 - k, i = find(l, c);
-        const uint64_t begin = (uint64_t)(c - l.first[i]) * kChunk, end = min(l.t[i].n, begin + kChunk);
+        const uint64_t begin = (uint64_t)(c - l.first[i]) * l.chunk, end = min(l.t[i].n, begin + l.chunk);
         const void *in = l.t[i].in;
         void *out = l.t[i].out;
         switch (l.types[i]) {
@@ -224,7 +266,7 @@ static void fill(List<M> &l, uint32_t from, uint32_t count, const void *const *g
         l.t[i] = {grads[k], out ? out[k] : (void *)grads[k], numel[k]};
         l.first[i] = chunks;
         l.types[i] = (uint8_t)(dtypes[k] | (out ? out_dtypes[k] : dtypes[k]) << 4);
-        chunks += (uint32_t)((numel[k] + kChunk - 1) / kChunk);
+        chunks += (uint32_t)((numel[k] + l.chunk - 1) / l.chunk);
     }
     l.first[count] = chunks;
     l.count = count;
@@ -238,17 +280,21 @@ static int run(cudaStream_t s, uint32_t count, const void *const *grads, void *c
     if (sms <= 0) return fail("sfb_clip_grad_norm: cannot query the device");
     uint32_t parts = 0;
     List<M> l;
+    uint64_t all = 0;
+    for (uint32_t i = 0; i < count; i++) all += numel[i];
+    l.chunk = kMostChunk;                            // a list that gives the SMs few chunks is cut finer
+    while (l.chunk > kLeastChunk && all / l.chunk < 4ull * most_ctas(sms)) l.chunk /= 2;
     for (uint32_t from = 0; from < count || from == 0; from += M) {
         fill<M>(l, from, count - from < M ? count - from : M, grads, out, numel, dtypes, out_dtypes);
         const uint32_t chunks = l.first[l.count], ctas = chunks < most_ctas(sms) ? (chunks ? chunks : 1) : most_ctas(sms);
-        launch_overlapped(square_sums_kernel<M>, dim3(ctas), dim3(kThreads), 0, s, l, sums + parts);
+        launch_overlapped(square_sums_kernel<M>, dim3(ctas), dim3(kThreads), kRoom, s, l, sums + parts);
         parts += ctas;
     }
     for (uint32_t from = 0; from < count || from == 0; from += M) {
         if (count > M) fill<M>(l, from, count - from < M ? count - from : M, grads, out, numel, dtypes, out_dtypes);
         const uint32_t chunks = write ? l.first[l.count] : 0, ctas = chunks < most_ctas(sms) ? (chunks ? chunks : 1) : most_ctas(sms);
         if (!write) l.count = 0, l.first[0] = 0;
-        launch_overlapped(clip_kernel<M>, dim3(ctas), dim3(kThreads), 0, s, l, sums, parts, from ? nullptr : norm, max_norm, scale, (int)(out == nullptr));
+        launch_overlapped(clip_kernel<M>, dim3(ctas), dim3(kThreads), kRoom, s, l, sums, parts, from ? nullptr : norm, max_norm, scale, (int)(out == nullptr));
         if (!write) break;
     }
     return check_launch("sfb_clip_grad_norm");
@@ -278,7 +324,7 @@ static int grad_norm_common(const char *who, sfb_stream_t stream, uint32_t count
         SFB_REQUIRE(numel[i] == 0 || (grads[i] && (!out || out[i])), "%s: tensor %u: NULL pointer", who, i);
         SFB_REQUIRE(((uintptr_t)grads[i] & (elem_size(dtypes[i]) - 1)) == 0 && (!out || ((uintptr_t)out[i] & (elem_size(out_dtypes[i]) - 1)) == 0),
                     "%s: tensor %u is not aligned to its elements", who, i);
-        chunks += numel[i] / gn::kChunk + 1;
+        chunks += numel[i] / gn::kLeastChunk + 1;
         SFB_REQUIRE(chunks < (1ull << 31), "%s: too many elements", who);
     }
     cudaStream_t s = as_stream(stream);
