@@ -241,27 +241,31 @@ __global__ void __launch_bounds__(tile::kThreads, 3) recompute_blocks_kernel(con
         }
 }
 
+constexpr uint64_t kMostSms = 148;
 // How many (batch, head) pairs go through the workspace at a time: as many as keep P and dS within what L2 holds beside the operands
-// (48 MB), one at least, whole batch elements or a part of one's heads.
-static uint32_t pairs_at_a_time(int dtype, uint32_t bs, uint32_t blocks, uint32_t B, uint32_t H)
+// (48 MB), but enough block-rows for every SM to have eight (fewer leave SMs without work: that costs more than a way through HBM) as long as that
+// takes no more than 512 MB; one at least; whole batch elements or a part of one's heads.
+static uint32_t pairs_at_a_time(int dtype, uint32_t bs, uint32_t nb, uint32_t blocks, uint32_t B, uint32_t H)
 {
-    const uint64_t one = 2ull * blocks * bs * bs * elem_size(dtype);
-    uint64_t n = one ? (48ull << 20) / one : (uint64_t)B * H;
+    const uint64_t one = 2ull * blocks * bs * bs * elem_size(dtype), all = (uint64_t)B * H;
+    if (one == 0) return (uint32_t)(all < 65535 ? all : 65535 / H * H);
+    const uint64_t fill = (kMostSms * 8 + nb - 1) / nb;
+    uint64_t n = (48ull << 20) / one;
+    if (n < fill) n = fill * one <= (512ull << 20) ? fill : (512ull << 20) / one;
     if (n < 1) n = 1;
-    if (n >= H) n = n / H * H;
-    const uint64_t all = (uint64_t)B * H;
+    if (n >= H) n = (n + H - 1) / H * H;
     if (n > all) n = all;
     return (uint32_t)(n < 65535 ? n : 65535 / H ? 65535 / H * H : 65535);
 }
-uint64_t simt_backward_workspace(int dtype, uint32_t bs, uint32_t blocks, uint32_t B, uint32_t H)
+uint64_t simt_backward_workspace(int dtype, uint32_t bs, uint32_t nb, uint32_t blocks, uint32_t B, uint32_t H)
 {
-    return 2ull * pairs_at_a_time(dtype, bs, blocks, B, H) * blocks * bs * bs * elem_size(dtype);
+    return 2ull * pairs_at_a_time(dtype, bs, nb, blocks, B, H) * blocks * bs * bs * elem_size(dtype);
 }
 
 int simt_backward_recompute(cudaStream_t s, const BackwardArgs &a, float *neg_lse, float *neg_delta, void *blocks_ws)
 {
     const AttnDims &p = a.p;
-    const uint32_t bs = a.bs, per = bs == 32 ? 4 : 1, n = pairs_at_a_time(a.dtype, bs, p.blocks, p.B, p.H);
+    const uint32_t bs = a.bs, per = bs == 32 ? 4 : 1, n = pairs_at_a_time(a.dtype, bs, p.nb_a, p.blocks, p.B, p.H);
     const size_t e = elem_size(a.dtype);
     const uint32_t L = p.nb_a * bs, unit = a.dtype == SFB_F32 ? 4 : 8;
     void *P = blocks_ws, *dS = (char *)blocks_ws + (size_t)n * p.blocks * bs * bs * e;

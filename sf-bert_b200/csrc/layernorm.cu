@@ -456,12 +456,13 @@ __global__ void __launch_bounds__(256) bias_gelu_kernel(void *out, const void *x
 constexpr int kEmbUnroll = 4;
 constexpr uint32_t kNoColumn = 0xffffffffu;
 // Who counts the ids outside the table.  Up to this many ids: one CTA beside the others, which reads them all and writes the
-// count, so that nothing has to clear it first.  It reads 2048 ids per trip of about half a microsecond, one after the other,
-// so beyond that the threads that read the ids anyway add to a counter cleared by a memset in front of the kernel, which costs
-// the overlap with the kernel before.  Measured (bf16, hidden 8 / 64 / 768, calls back to back), one CTA against memset: 4096
-// ids 2.1 / 2.1 / 4.2 against 5.4 / 4.5 / 8.2 us, 16384 5.3 / 5.5 / 7.1 against 5.6 / 6.2 / 10.3, 32768 9.6 / 10.1 / 17.3
-// against 5.7 / 6.2 / 14.4, a million at hidden 8 / 64 271 / 275 against 11 / 27.
-constexpr uint64_t kEmbOneCtaIds = 16384;
+// count, so that nothing has to clear it first.  It reads 8192 ids per trip of about half a microsecond (2048 where they are not 16-byte
+// aligned), one after the other, so beyond that the threads that read the ids anyway add to a counter cleared by a memset in front of the kernel,
+// which costs the overlap with the kernel before.  Measured with trips of 2048 (bf16, hidden 8 / 64 / 768, calls back to back), one CTA against
+// memset: 4096 ids 2.1 / 2.1 / 4.2 against 5.4 / 4.5 / 8.2 us, 16384 5.3 / 5.5 / 7.1 against 5.6 / 6.2 / 10.3, 32768 9.6 / 10.1 / 17.3
+// against 5.7 / 6.2 / 14.4, a million at hidden 8 / 64 271 / 275 against 11 / 27.  With trips of 8192, from Python: 65536 ids 6.4 / 6.5 / 26.5, with
+// the memset 8.2 / 8.3 / 29.8; 32768 of hidden 768 11.9.
+constexpr uint64_t kEmbOneCtaIds = 65536, kEmbOneCtaIdsApart = 16384;
 template <int DT>
 __global__ void __launch_bounds__(256) embedding_kernel(void *__restrict__ out, const void *__restrict__ table,
                                                        const int32_t *__restrict__ ids, const void *__restrict__ pos, uint32_t batch,
@@ -478,8 +479,20 @@ __global__ void __launch_bounds__(256) embedding_kernel(void *__restrict__ out, 
         // the extra column of CTAs: its first one counts the ids outside the table (nobody has to clear the counter first)
         if (blockIdx.y) return;
         const uint32_t total = batch * seq_len;                            // < 2^31 (checked by the host)
-        uint32_t bad = 0;
-        for (uint32_t t = threadIdx.x; t < total; t += 256 * 8) {
+        uint32_t bad = 0, done = 0;
+        if (((uintptr_t)ids & 15) == 0) {
+            const uint32_t pieces = total / 4;
+            for (uint32_t t = threadIdx.x; t < pieces; t += 256 * 8) {
+                int4 v[8];
+#pragma unroll
+                for (int u = 0; u < 8; u++) v[u] = t + u * 256 < pieces ? __ldg((const int4 *)ids + t + u * 256) : make_int4(0, 0, 0, 0);
+#pragma unroll
+                for (int u = 0; u < 8; u++)
+                    if (t + u * 256 < pieces) bad += ((uint32_t)v[u].x >= vocab) + ((uint32_t)v[u].y >= vocab) + ((uint32_t)v[u].z >= vocab) + ((uint32_t)v[u].w >= vocab);
+            }
+            done = pieces * 4;
+        }
+        for (uint32_t t = done + threadIdx.x; t < total; t += 256 * 8) {
             int32_t v[8];
 #pragma unroll
             for (int u = 0; u < 8; u++) v[u] = t + u * 256 < total ? __ldg(ids + t + u * 256) : 0;
@@ -588,7 +601,7 @@ int embedding_lookup(cudaStream_t s, void *out, const void *table, const int32_t
     if (split > 65535u) split = 65535u;
     if (split < 1) split = 1;
     const uint32_t per_y = (batch + split - 1) / split;
-    const bool one_cta = bad_ids && (uint64_t)batch * seq_len <= kEmbOneCtaIds;
+    const bool one_cta = bad_ids && (uint64_t)batch * seq_len <= (((uintptr_t)ids & 15) == 0 ? kEmbOneCtaIds : kEmbOneCtaIdsApart);
     const uint32_t column = one_cta ? (uint32_t)ctas_x : kNoColumn;
     if (bad_ids && !one_cta) {
         const cudaError_t e = cudaMemsetAsync(bad_ids, 0, sizeof(uint32_t), s);

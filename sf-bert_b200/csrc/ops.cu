@@ -170,7 +170,7 @@ extern "C" uint64_t sfb_attention_backward_workspace(int dtype, uint32_t block_s
     const uint64_t rows = 2 * constants_bytes(batch_dim, ctx_blks * block_size, head_dim);
     const AttnDims p = {batch_dim, head_dim, state_dim, ctx_blks, ctx_blks, blocks, 0, 0};
     if (aligned && tc_backward_recompute_supported(dtype, block_size, p, nn_max, tn_max)) return rows;
-    return rows + simt_backward_workspace(dtype, block_size, blocks, batch_dim, head_dim);
+    return rows + simt_backward_workspace(dtype, block_size, ctx_blks, blocks, batch_dim, head_dim);
 }
 
 extern "C" int sfb_attention_backward_recompute(sfb_stream_t stream, const void *nt_lut, const void *nn_lut, const void *tn_lut, const void *q,
@@ -202,7 +202,7 @@ extern "C" int sfb_attention_backward_recompute(sfb_stream_t stream, const void 
     const uintptr_t all = (uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)dout | (uintptr_t)mask | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv;
     const bool tc = (all & 15) == 0 && ((in_pitch | dout_pitch | grad_pitch) & 7) == 0 && tc_backward_recompute_supported(dtype, block_size, p, nn_max, tn_max);
     const uint64_t rows = constants_bytes(batch_dim, ctx_blks * block_size, head_dim);
-    const uint64_t need = 2 * rows + (tc ? 0 : simt_backward_workspace(dtype, block_size, blocks, batch_dim, head_dim));
+    const uint64_t need = 2 * rows + (tc ? 0 : simt_backward_workspace(dtype, block_size, ctx_blks, blocks, batch_dim, head_dim));
     SFB_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= need, "%s: needs a 16-byte aligned workspace of %llu bytes", who, (unsigned long long)need);
     const BackwardArgs a = {nt_lut, nn_lut, tn_lut, q, k, v, o, dout, mask, dq, dk, dv, dtype, block_size, lut_heads > 1 ? lut_dim : 0, nn_max, tn_max,
                             in_pitch, o_pitch, dout_pitch, grad_pitch, scale, p};

@@ -17,7 +17,7 @@ struct BackwardArgs {
 
 int attention_row_constants(cudaStream_t s, const void *o, const void *dout, const float *lse, float *neg_lse, float *neg_delta, int dtype, uint32_t B,
                             uint32_t L, uint32_t H, uint32_t d, uint64_t o_pitch, uint64_t do_pitch, float scale);
-uint64_t simt_backward_workspace(int dtype, uint32_t bs, uint32_t blocks, uint32_t B, uint32_t H);
+uint64_t simt_backward_workspace(int dtype, uint32_t bs, uint32_t nb, uint32_t blocks, uint32_t B, uint32_t H);
 int simt_backward_recompute(cudaStream_t s, const BackwardArgs &a, float *neg_lse, float *neg_delta, void *blocks_ws);
 
 
