@@ -12,48 +12,71 @@
 namespace sfb {
 
 // ---- the rows' constants: neg_lse = -lse log2(e), neg_delta = -scale rowsum(dO * O), both [B, H, L] ------------------------------
-// 32 rows of one (batch, head) per CTA, eight lanes each.  A row without kept elements has lse = -inf, and P = 0 of it: exp2(x + neg_lse)
-// with neg_lse = -inf too.
-template <int DT>
+// Eight lanes per row, 32 R rows of one (batch, head) per CTA; R = 4 where that leaves the SMs enough CTAs: a lane's loads of four rows are on their way
+// together.  100 MB of O and dO (8 x 4096 rows of 12 heads of 64): 25 us with cold caches, most of a copy's rate.  A row without kept
+// elements has lse = -inf, and P = 0 of it: exp2(x + neg_lse) with neg_lse = -inf too.
+template <int DT, uint32_t R>
 __global__ void __launch_bounds__(256) row_constants_kernel(const void *__restrict__ O, const void *__restrict__ dO, const float *__restrict__ lse,
                                                            float *__restrict__ neg_lse, float *__restrict__ neg_delta, uint32_t L, uint32_t H, uint32_t d,
                                                            size_t o_pitch, size_t do_pitch, float scale, bool vec)
 {
     grid_dependency_wait();
     grid_launch_dependents();
-    const uint32_t b = blockIdx.z, h = blockIdx.y, l = blockIdx.x * 32 + threadIdx.x / 8, part = threadIdx.x & 7;
-    const size_t at_o = ((size_t)b * L + l) * o_pitch + (size_t)h * d, at_do = ((size_t)b * L + l) * do_pitch + (size_t)h * d;
-    float sum = 0.f;
-    if (l < L) {
-        if (vec) {
-            constexpr uint32_t N = DT == SFB_F32 ? 4 : 8;
-            for (uint32_t c = part * N; c < d; c += 8 * N) {
-                const uint4 x = __ldg((const uint4 *)((const typename Elem<DT>::type *)O + at_o + c)), y = __ldg((const uint4 *)((const typename Elem<DT>::type *)dO + at_do + c));
-                const uint32_t xw[4] = {x.x, x.y, x.z, x.w}, yw[4] = {y.x, y.y, y.z, y.w};
+    // the heads of the same positions side by side: they lie in the same rows of memory
+    const uint32_t b = blockIdx.y, chunk = blockIdx.x / H, h = blockIdx.x - chunk * H, l0 = chunk * 32 * R + threadIdx.x / 8, part = threadIdx.x & 7;
+    float sum[R] = {};
+    if (vec) {
+        constexpr uint32_t N = DT == SFB_F32 ? 4 : 8;
+        for (uint32_t c = part * N; c < d; c += 8 * N) {
+            uint4 x[R], y[R];
+#pragma unroll
+            for (uint32_t k = 0; k < R; k++) {
+                const uint32_t l = l0 + 32 * k;
+                x[k] = y[k] = make_uint4(0u, 0u, 0u, 0u);
+                if (l < L) {
+                    x[k] = __ldg((const uint4 *)((const typename Elem<DT>::type *)O + ((size_t)b * L + l) * o_pitch + (size_t)h * d + c));
+                    y[k] = __ldg((const uint4 *)((const typename Elem<DT>::type *)dO + ((size_t)b * L + l) * do_pitch + (size_t)h * d + c));
+                }
+            }
+#pragma unroll
+            for (uint32_t k = 0; k < R; k++) {
+                const uint32_t xw[4] = {x[k].x, x[k].y, x[k].z, x[k].w}, yw[4] = {y[k].x, y[k].y, y[k].z, y[k].w};
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     if constexpr (DT == SFB_F32) {
-                        sum = fmaf(__uint_as_float(xw[i]), __uint_as_float(yw[i]), sum);
+                        sum[k] = fmaf(__uint_as_float(xw[i]), __uint_as_float(yw[i]), sum[k]);
                     } else {
                         float x0, x1, y0, y1;
                         tile::widen2<DT>(x0, x1, xw[i]);
                         tile::widen2<DT>(y0, y1, yw[i]);
-                        sum = fmaf(x0, y0, fmaf(x1, y1, sum));
+                        sum[k] = fmaf(x0, y0, fmaf(x1, y1, sum[k]));
                     }
                 }
             }
-        } else {
-            for (uint32_t c = part; c < d; c += 8) sum = fmaf(Elem<DT>::load(O, at_o + c), Elem<DT>::load(dO, at_do + c), sum);
+        }
+    } else {
+#pragma unroll
+        for (uint32_t k = 0; k < R; k++) {
+            const uint32_t l = l0 + 32 * k;
+            if (l < L)
+                for (uint32_t c = part; c < d; c += 8)
+                    sum[k] = fmaf(Elem<DT>::load(O, ((size_t)b * L + l) * o_pitch + (size_t)h * d + c), Elem<DT>::load(dO, ((size_t)b * L + l) * do_pitch + (size_t)h * d + c), sum[k]);
         }
     }
 #pragma unroll
-    for (int o = 4; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (l >= L || part) return;
-    const size_t row = ((size_t)b * H + h) * L + l;
-    const float s = lse[row];
-    // nothing kept (-inf): the row's dS is empty whatever dO and O hold
-    neg_lse[row] = s == -INFINITY ? s : s * -1.4426950408889634f;
-    neg_delta[row] = s == -INFINITY ? 0.f : sum * -scale;
+    for (uint32_t k = 0; k < R; k++)
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) sum[k] += __shfl_xor_sync(0xffffffffu, sum[k], o);
+#pragma unroll
+    for (uint32_t k = 0; k < R; k++) {
+        const uint32_t l = l0 + 32 * k;
+        if (part != k || l >= L) continue;
+        const size_t row = ((size_t)b * H + h) * L + l;
+        const float s = lse[row];
+        // nothing kept (-inf): the row's dS is empty whatever dO and O hold
+        neg_lse[row] = s == -INFINITY ? s : s * -1.4426950408889634f;
+        neg_delta[row] = s == -INFINITY ? 0.f : sum[k] * -scale;
+    }
 }
 
 int attention_row_constants(cudaStream_t s, const void *o, const void *dout, const float *lse, float *neg_lse, float *neg_delta, int dtype, uint32_t B,
@@ -61,12 +84,18 @@ int attention_row_constants(cudaStream_t s, const void *o, const void *dout, con
 {
     const uint32_t per = dtype == SFB_F32 ? 4 : 8;
     const bool vec = (((uintptr_t)o | (uintptr_t)dout) & 15) == 0 && o_pitch % per == 0 && do_pitch % per == 0 && d % per == 0;
-    const dim3 grid((L + 31) / 32, H, B);
-#define RC_LAUNCH(DT) launch_overlapped_few(row_constants_kernel<DT>, grid, dim3(256), 0, s, o, dout, lse, neg_lse, neg_delta, L, H, d, (size_t)o_pitch, (size_t)do_pitch, scale, vec)
-    if (dtype == SFB_F32) RC_LAUNCH(SFB_F32);
-    else if (dtype == SFB_BF16) RC_LAUNCH(SFB_BF16);
-    else RC_LAUNCH(SFB_F16);
+    const int sms = device_sm_count(current_device());
+    const uint32_t R = (uint64_t)L * H * B >= 128ull * 8 * (uint64_t)(sms > 0 ? sms : 1) ? 4 : 1;
+    const uint64_t chunks = ((uint64_t)L + 32 * R - 1) / (32 * R);
+    SFB_REQUIRE(chunks * H < (1ull << 31), "sfb_attention_backward_recompute: too many rows for one launch");
+    const dim3 grid((unsigned)(chunks * H), B);
+#define RC_LAUNCH_R(DT, RV) launch_overlapped_few(row_constants_kernel<DT, RV>, grid, dim3(256), 0, s, o, dout, lse, neg_lse, neg_delta, L, H, d, (size_t)o_pitch, (size_t)do_pitch, scale, vec)
+#define RC_LAUNCH(DT) { if (R == 4) RC_LAUNCH_R(DT, 4); else RC_LAUNCH_R(DT, 1); }
+    if (dtype == SFB_F32) RC_LAUNCH(SFB_F32)
+    else if (dtype == SFB_BF16) RC_LAUNCH(SFB_BF16)
+    else RC_LAUNCH(SFB_F16)
 #undef RC_LAUNCH
+#undef RC_LAUNCH_R
     return check_launch("sfb_attention_backward_recompute");
 }
 
