@@ -14,6 +14,8 @@ namespace sfb {
 namespace emb {
 
 constexpr uint32_t kSortThreads = 512, kSortWarps = kSortThreads / 32;
+constexpr uint32_t kStride = kSortWarps + 1;         // counters per id: neighbouring ids in different banks
+constexpr uint32_t kNear = 2048;                     // tokens of a CTA that it keeps in shared memory
 constexpr uint32_t kMaxRange = 1024;                 // ids that one CTA sorts
 
 struct GradArgs {
@@ -43,8 +45,9 @@ __device__ __forceinline__ uint32_t warp_scan(uint32_t v, uint32_t lane)      //
 // A CTA owns `range` consecutive ids and looks at all tokens: it counts those below its range, which is where its part of the sorted
 // list begins, and collects its own in order, a share of the tokens per warp.  These are then sorted by counting, per warp and id, so
 // that equal ids stay in order.  No CTA waits for another.  The ids come from L2 (4 bytes per token and CTA).
-__device__ __forceinline__ void sort_ids(const GradArgs &a, uint32_t *count)      // count: [range][kSortWarps]
+__device__ __forceinline__ void sort_ids(const GradArgs &a, uint32_t *count)      // count: [range][kStride]
 {
+    __shared__ int2 near_list[kNear];
     __shared__ uint32_t s_below[kSortWarps], s_mine[kSortWarps], s_bad[kSortWarps], s_sum[kSortWarps];
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t lo = blockIdx.x * a.range, width = min(a.range, a.vocab - lo);
@@ -82,7 +85,7 @@ __device__ __forceinline__ void sort_ids(const GradArgs &a, uint32_t *count)    
         s_mine[warp] = mine;
         s_bad[warp] = bad;
     }
-    for (uint32_t i = threadIdx.x; i < width * kSortWarps; i += kSortThreads) count[i] = 0;
+    for (uint32_t i = threadIdx.x; i < width * kStride; i += kSortThreads) count[i] = 0;
     __syncthreads();
     uint32_t base = 0, total = 0, before = 0, bad_all = 0;
 #pragma unroll
@@ -94,7 +97,7 @@ __device__ __forceinline__ void sort_ids(const GradArgs &a, uint32_t *count)    
     }
     if (blockIdx.x == 0 && threadIdx.x == 0 && a.bad) *a.bad = bad_all;
     // own tokens, in order of position
-    int2 *list = a.unsorted + base;
+    int2 *list = total <= kNear ? near_list : a.unsorted + base;
     if (total) {
         uint32_t at = before;
         for (uint32_t t = t0; t < t1; t += 512) {
@@ -120,12 +123,13 @@ __device__ __forceinline__ void sort_ids(const GradArgs &a, uint32_t *count)    
     __syncthreads();
     // how often each warp's share of them has each id
     const uint32_t part = ((total + kSortWarps - 1) / kSortWarps + 31) / 32 * 32, i0 = min(total, warp * part), i1 = min(total, i0 + part);
-    for (uint32_t i = i0 + lane; i < i1; i += 32) atomicAdd(&count[((uint32_t)list[i].y - lo) * kSortWarps + warp], 1u);
+    for (uint32_t i = i0 + lane; i < i1; i += 32) atomicAdd(&count[((uint32_t)list[i].y - lo) * kStride + warp], 1u);
     __syncthreads();
     // where each (id, warp) begins: an exclusive scan, ids outermost; a thread takes neighbouring ids
     const uint32_t per = (width + kSortThreads - 1) / kSortThreads, v0 = min(width, threadIdx.x * per), v1 = min(width, v0 + per);
     uint32_t sum = 0;
-    for (uint32_t i = v0 * kSortWarps; i < v1 * kSortWarps; i++) sum += count[i];
+    for (uint32_t v = v0; v < v1; v++)
+        for (uint32_t w = 0; w < kSortWarps; w++) sum += count[v * kStride + w];
     const uint32_t upto = warp_scan(sum, lane);
     if (lane == 31) s_sum[warp] = upto;
     __syncthreads();
@@ -136,8 +140,8 @@ __device__ __forceinline__ void sort_ids(const GradArgs &a, uint32_t *count)    
     for (uint32_t v = v0; v < v1; v++) {
         a.starts[lo + v] = base + off;
         for (uint32_t w = 0; w < kSortWarps; w++) {
-            const uint32_t c = count[v * kSortWarps + w];
-            count[v * kSortWarps + w] = off;
+            const uint32_t c = count[v * kStride + w];
+            count[v * kStride + w] = off;
             off += c;
         }
     }
@@ -147,7 +151,7 @@ __device__ __forceinline__ void sort_ids(const GradArgs &a, uint32_t *count)    
         const bool in = i + lane < i1;
         const int2 e = in ? list[i + lane] : make_int2(0, -1);
         const uint32_t same = __match_any_sync(0xffffffffu, e.y), rank = __popc(same & ((1u << lane) - 1u));
-        uint32_t *c = &count[(in ? (uint32_t)e.y - lo : 0u) * kSortWarps + warp];
+        uint32_t *c = &count[(in ? (uint32_t)e.y - lo : 0u) * kStride + warp];
         const uint32_t at = in ? *c + rank : 0u;
         __syncwarp();
         if (in && rank == 0) *c += __popc(same);
@@ -440,11 +444,11 @@ static int launch(cudaStream_t s, GradArgs a)
         while (a.ways < kSortWarps && warps * a.ways < want && a.batch >= 16 * a.ways) a.ways *= 2;
         pos_ctas = groups * ((a.len + kSortWarps / a.ways - 1) / (kSortWarps / a.ways));
     }
-    size_t smem = (size_t)a.range * kSortWarps * 4;
+    size_t smem = (size_t)a.range * kStride * 4;
     if (a.dpos && a.ways > 1 && smem < sizeof(float) * kSortWarps * N * 33) smem = sizeof(float) * kSortWarps * N * 33;
     static DeviceOnce once;
     if (!once.done(dev)) {
-        if (cudaFuncSetAttribute(sort_and_positions_kernel<DT, GT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(kMaxRange * kSortWarps * 4)) != cudaSuccess)
+        if (cudaFuncSetAttribute(sort_and_positions_kernel<DT, GT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(kMaxRange * kStride * 4)) != cudaSuccess)
             return fail("sfb_embedding_grad: cannot reserve shared memory");
         once.mark(dev);
     }
