@@ -5,7 +5,7 @@
 // Three launches.  (1) sort_and_positions_kernel: some CTAs bring the tokens into the order of their ids, equal ids by position, while the others
 // add up the batch, reading dout in order.  (2) table_grad_kernel walks the sorted tokens in pieces of equal length, so that a word that
 // is a tenth of the text does not hang on one CTA; a run of equal ids that lies in one piece is written at once, the parts of
-// one that does not go to the workspace.  The rows of tokens that do not occur are written as zeros by the same launch.
+// one that does not go to the workspace.  The rows of tokens that do not occur are zeros from the first launch (or the second, for few tokens).
 // (3) join_kernel adds up the parts.  Bound by memory: dout is read by (1) and gathered by (2), from L2 where it fits, and the table's
 // gradient is written once (a fill runs at 3.8 TB/s on this part, where a copy runs at 6.5).
 #include "common.cuh"
@@ -16,13 +16,15 @@ namespace emb {
 constexpr uint32_t kSortThreads = 512, kSortWarps = kSortThreads / 32;
 constexpr uint32_t kStride = kSortWarps + 1;         // counters per id: neighbouring ids in different banks
 constexpr uint32_t kNear = 2048;                     // tokens of a CTA that it keeps in shared memory
+constexpr uint32_t kFill = 8192;                     // 16-byte pieces of zeros per CTA
+constexpr uint32_t kFewTokens = 2048;
 constexpr uint32_t kMaxRange = 1024;                 // ids that one CTA sorts
 
 struct GradArgs {
     const void *dout;
     const int32_t *ids;
     void *dtable, *dpos;
-    uint32_t n, batch, len, hidden, vocab, range, sorters, ways, piece, pieces;
+    uint32_t n, batch, len, hidden, vocab, range, sorters, pos_ctas, fillers, ways, piece, pieces;      // fillers: CTAs that write the table's zeros ahead
     float scale;
     int accumulate;
     uint32_t *bad;
@@ -258,7 +260,6 @@ __global__ void __launch_bounds__(256) table_grad_kernel(const GradArgs a)
     const bool zeros = y >= piece_ctas;
     const uint32_t at = zeros ? y - piece_ctas : y;
     if (zeros) {
-        if (a.accumulate) return;
         const uint32_t v0 = (at * 8 + warp) * 32;
         const bool empty = v0 + lane < a.vocab && a.starts[v0 + lane] == a.starts[v0 + lane + 1];
         uint32_t todo = __ballot_sync(0xffffffffu, empty);
@@ -411,15 +412,27 @@ __device__ __forceinline__ void add_positions(const GradArgs &a, uint32_t cta, f
     if (live) write_sums<GT, N>(a.dpos, (size_t)l * a.hidden + col, s, 1.f, a.accumulate);
 }
 
-// The first CTAs sort, the others add up positions: one waits for latencies while the other moves data.
+// The first CTAs sort, the others add up positions or write zeros: one waits for latencies while the others move data.
 template <int DT, int GT>
 __global__ void __launch_bounds__(kSortThreads) sort_and_positions_kernel(const GradArgs a)
 {
     extern __shared__ __align__(16) uint32_t dynamic[];
     grid_dependency_wait();
     grid_launch_dependents();
-    if (blockIdx.x < a.sorters) sort_ids(a, dynamic);
-    else add_positions<DT, GT>(a, blockIdx.x - a.sorters, (float *)dynamic);
+    if (blockIdx.x < a.sorters) {
+        sort_ids(a, dynamic);
+        return;
+    }
+    const uint32_t y = blockIdx.x - a.sorters, both = 2 * min(a.pos_ctas, a.fillers), at = y < both ? y >> 1 : y - both / 2;
+    if (y < both ? y & 1 : a.fillers > a.pos_ctas) {
+        const size_t pieces = (size_t)a.vocab * a.hidden * sizeof(typename Elem<GT>::type) / 16, i0 = (size_t)at * kFill;
+        uint4 *out = (uint4 *)a.dtable + i0;
+        const uint32_t n = (uint32_t)(pieces - i0 < kFill ? pieces - i0 : kFill);
+#pragma unroll 8
+        for (uint32_t i = threadIdx.x; i < n; i += kSortThreads) __stcs(out + i, make_uint4(0u, 0u, 0u, 0u));
+    } else {
+        add_positions<DT, GT>(a, at, (float *)dynamic);
+    }
 }
 
 // sorted tokens per piece: short enough for a long run to spread, long enough for its parts to be few
@@ -433,17 +446,26 @@ static int launch(cudaStream_t s, GradArgs a)
     const int dev = current_device(), sms = device_sm_count(dev);
     if (sms <= 0) return fail("sfb_embedding_grad: cannot query the device");
     constexpr uint32_t N = Piece<DT>::N;
-    const uint64_t groups = (a.hidden / N + 31) / 32, rows = (a.pieces + 7) / 8 + ((uint64_t)a.vocab + 255) / 256;
-    SFB_REQUIRE(groups * a.len < (1ull << 31) && groups * rows < (1ull << 31) && (uint64_t)((a.hidden / 4 + 31) / 32) * a.pieces < (1ull << 31),
+    const uint64_t groups = (a.hidden / N + 31) / 32;
+    SFB_REQUIRE(groups * a.len < (1ull << 31) && groups * ((a.pieces + 7) / 8 + ((uint64_t)a.vocab + 255) / 256) < (1ull << 31) && (uint64_t)((a.hidden / 4 + 31) / 32) * a.pieces < (1ull << 31),
                 "sfb_embedding_grad: too many rows for one launch");
     // positions enough to fill the SMs: a warp each; otherwise several share the batch of one
-    uint64_t pos_ctas = 0;
+    uint64_t pos_ctas = 0, fillers = 0;
     if (a.dpos) {
         const uint64_t warps = groups * a.len, want = 16ull * sms;
         a.ways = 1;
         while (a.ways < kSortWarps && warps * a.ways < want && a.batch >= 16 * a.ways) a.ways *= 2;
         pos_ctas = groups * ((a.len + kSortWarps / a.ways - 1) / (kSortWarps / a.ways));
     }
+    // The rows of tokens that do not occur: all rows are zeroed beside the sorting, and those of tokens that do occur are written again (bf16, fp32
+    // gradients, 30522 x 768: 1024 tokens 31 us, 32768 55; zeroed after the sorting, by its counts, 43 and 60).  Few tokens, whose sorting is over
+    // soon, where a lane's zeros are 16 bytes: by the counts (fp32, 320 tokens 25 us, zeroed beside 28).
+    constexpr bool narrow = sizeof(typename Elem<GT>::type) * N == 16;
+    if (!a.accumulate && (!narrow || a.n >= kFewTokens)) fillers = ((uint64_t)a.vocab * a.hidden * sizeof(typename Elem<GT>::type) / 16 + kFill - 1) / kFill;
+    SFB_REQUIRE(a.sorters + pos_ctas + fillers < (1ull << 31), "sfb_embedding_grad: too many rows for one launch");
+    a.pos_ctas = (uint32_t)pos_ctas;
+    a.fillers = (uint32_t)fillers;
+    const uint64_t rows = (a.pieces + 7) / 8 + (fillers || a.accumulate ? 0 : ((uint64_t)a.vocab + 255) / 256);
     size_t smem = (size_t)a.range * kStride * 4;
     if (a.dpos && a.ways > 1 && smem < sizeof(float) * kSortWarps * N * 33) smem = sizeof(float) * kSortWarps * N * 33;
     static DeviceOnce once;
@@ -452,7 +474,7 @@ static int launch(cudaStream_t s, GradArgs a)
             return fail("sfb_embedding_grad: cannot reserve shared memory");
         once.mark(dev);
     }
-    launch_overlapped(sort_and_positions_kernel<DT, GT>, dim3((unsigned)(a.sorters + pos_ctas)), dim3(kSortThreads), smem, s, a);
+    launch_overlapped(sort_and_positions_kernel<DT, GT>, dim3((unsigned)(a.sorters + pos_ctas + fillers)), dim3(kSortThreads), smem, s, a);
     launch_overlapped(table_grad_kernel<DT, GT>, dim3((unsigned)(groups * rows)), dim3(256), 0, s, a);
     if (a.pieces > 1) launch_overlapped(join_kernel<GT>, dim3((a.hidden / 4 + 31) / 32 * ((a.pieces - 1 + 7) / 8)), dim3(256), 0, s, a);
     return check_launch("sfb_embedding_grad");
@@ -495,7 +517,7 @@ extern "C" int sfb_embedding_grad(sfb_stream_t stream, void *dtable, void *dpos,
         clear_error();
         return 0;
     }
-    GradArgs a = {dout, ids, dtable, dpos, (uint32_t)n, batch, seq_len, hidden, vocab, 0, 0, 1, piece_length((uint32_t)n), piece_count((uint32_t)n), scale, accumulate, bad_ids};
+    GradArgs a = {dout, ids, dtable, dpos, (uint32_t)n, batch, seq_len, hidden, vocab, 0, 0, 0, 0, 1, piece_length((uint32_t)n), piece_count((uint32_t)n), scale, accumulate, bad_ids};
     // a CTA per SM sorts, more where its counters would not fit
     const int sms = device_sm_count(current_device());
     const uint32_t ctas = max((uint32_t)(sms > 0 ? sms : 1), (vocab + kMaxRange - 1) / kMaxRange);
