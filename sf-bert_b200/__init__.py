@@ -339,7 +339,8 @@ def attention_backward_recompute(q, k, v, o, do, lse, lay, scale=None, use_mask=
     """The gradients (dq, dk, dv) of fused_attention_stats' output, with the probabilities made again from lse: nothing of the size
     of the scores was kept.  Any type, block and head size of the forward call; scale and use_mask as there.  q, k, v share a pitch, o and do
     have their own; out: three views to write to, of one pitch (such as the three parts of a packed [B, L, 3, H, d] gradient).  The same
-    inputs give the same bits.  With 16-bit operands P and dS are rounded to their type as operands of the products."""
+    inputs give the same bits.  With 16-bit operands P and dS are rounded to their type as operands of the products.  The layout's tables
+    by columns are built on first use (lay.tn_lut), which reads a number back: once before a call is captured in a graph."""
     return _host.attention_backward_recompute(q, k, v, o, do, lse, lay, scale, use_mask, out)
 
 

@@ -270,20 +270,22 @@ __global__ void __launch_bounds__(tile::kThreads, 3) recompute_blocks_kernel(con
         }
 }
 
-constexpr uint64_t kMostSms = 148;
-// How many (batch, head) pairs go through the workspace at a time: as many as keep P and dS within what L2 holds beside the operands
-// (48 MB), but enough block-rows for every SM to have eight (fewer leave SMs without work: that costs more than a way through HBM) as long as that
-// takes no more than 512 MB; one at least; whole batch elements or a part of one's heads.
+// How many (batch, head) pairs go through the workspace at a time: block-rows for every SM to have 32 (us with 8 / 16 / 32, each a share of what
+// follows: bf16, blocks of 32, d 64, 4 x 12 heads of 2048 positions, strided 1119 / 793 / 622; fp16, blocks of 64, d 128 1635 / 1308 / 1307; what L2 could
+// have kept of P and dS counts for less than the SMs that have nothing left to do at the end of each launch), as long as P and dS take no more
+// than 512 MB; one at least; whole batch elements or a part of one's heads, in parts of about the same size.
+constexpr uint64_t kRowsPerSm = 32, kMostSms = 148, kMostBytes = 512ull << 20;
 static uint32_t pairs_at_a_time(int dtype, uint32_t bs, uint32_t nb, uint32_t blocks, uint32_t B, uint32_t H)
 {
-    const uint64_t one = 2ull * blocks * bs * bs * elem_size(dtype), all = (uint64_t)B * H;
-    if (one == 0) return (uint32_t)(all < 65535 ? all : 65535 / H * H);
-    const uint64_t fill = (kMostSms * 8 + nb - 1) / nb;
-    uint64_t n = (48ull << 20) / one;
-    if (n < fill) n = fill * one <= (512ull << 20) ? fill : (512ull << 20) / one;
-    if (n < 1) n = 1;
-    if (n >= H) n = (n + H - 1) / H * H;
+    const uint64_t one = 2ull * blocks * bs * bs * elem_size(dtype), all = (uint64_t)B * H, most = one ? kMostBytes / one : all;
+    uint64_t n = (kMostSms * kRowsPerSm + nb - 1) / nb;
+    if (n > most) n = most;
     if (n > all) n = all;
+    if (n < 1) n = 1;
+    if (n >= H) {
+        const uint64_t elems = n / H, parts = (B + elems - 1) / elems;
+        n = (B + parts - 1) / parts * H;
+    }
     return (uint32_t)(n < 65535 ? n : 65535 / H ? 65535 / H * H : 65535);
 }
 uint64_t simt_backward_workspace(int dtype, uint32_t bs, uint32_t nb, uint32_t blocks, uint32_t B, uint32_t H)

@@ -8,18 +8,24 @@
 // positions:
 //     S  = own1 . Z^T      own1: Q (K), Z: the step's rows of K (Q)
 //     dP = own2 . Y^T      own2: dO (V), Y: the step's rows of V (dO)
-//     P and dS             256 threads, one own position and 32 of the 64 others each, straight out of TMEM and back, as 16-bit operands
+//     P and dS             128 threads, one own position each, straight out of TMEM and back, as 16-bit operands
 //     out += dS . Z        dQ (dK)
 //     COL: dV += P . Y     (for COL S and dP are already transposed: their lanes are keys)
-// One persistent CTA per SM with three groups of four worker warps that take the steps in turn, each with S and dP buffers of its own.  What a warp
-// pays for a step is mostly fixed: a satisfied barrier wait or an arrival costs it 100 to 200 cycles on a loaded SM, a trip to
-// TMEM 85.  So a thread has a whole row of 64 (half a row per thread, eight warps per group, took 1060 and 1515 cycles per step and SM), with two waits
-// and two arrivals per step, and the third group fills what the other two wait.
+// One persistent CTA per SM with three groups of four worker warps that take the steps in turn.  What bounds it is a warp's way through a step: at
+// 64 full block-rows 1010 cycles per step and SM (rows) and 1230 (columns), of which the exponentials would take 512 by
+// themselves and the products 432 and 590; without exponentials 790 and 1190, with a quarter of each product 960 and 1180 (measured in copies
+// of this code).  What counts is therefore how little a warp does besides:
+//   - a thread has a whole row of 64, with two waits and two arrivals per step (half a row per thread in eight warps per group: 1060 and 1515);
+//   - nothing is done for a half of the own positions that has not the step's block, in one branch around all of it;
+//   - own1 and own2 are copied to TMEM, so that a product reads 8 KB of shared memory instead of 24; the columns' constants are read
+//     there by 16-byte loads of that address space (through a generic pointer: + 17 %);
+//   - a chain of MMAs on one accumulator takes 115 cycles per MMA whatever its N up to 128, so the next S and dP are issued by threads of their own as
+//     soon as their buffer is free.  Rows: three buffers of each.  Columns, whose accumulators take twice the room: three of S
+//     and two of dP (two and three: + 15 %; P apart from S: + 12 %; four groups with a P and a dS for all: + 30 %).
 // A CTA starts with the item of its own index and takes over items that have not been started (cluster launch control), long rows and
 // columns paired with each other and first.  An item's epilogue falls to the groups in turn, the others go on.
-// Warps: 0-11 P, dS and the epilogue; 12 TMA; 13 issues S, 14 dP, 15 out, 16 dV; 17 plans the unions of the coming items.  The control warpgroups hand registers to
-// the workers (setmaxnreg): 640 threads x 96 = 12 x 32 x 128 + 8 x 32 x 48.
-// TMEM (512 columns): per group S 64 (columns: P over it) and dP 64 (dS over it); then dK and dV, or dQ of two items in turn.
+// Warps: 0-11 P, dS and the epilogue; 12 TMA; 13 issues S, 14 dP, 15 out, 16 dV; 17 plans the unions of the coming items.  The control warpgroups hand
+// registers to the workers (setmaxnreg): 640 threads x 96 = 12 x 32 x 128 + 8 x 32 x 48.
 #include "recompute.cuh"
 #include "tc_common.cuh"
 #include <stddef.h>
@@ -182,159 +188,159 @@ recompute_tc_kernel(const __grid_constant__ CUtensorMap own1_map, const __grid_c
     };
 
     if (warp >= kRcWorkers) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
-    if (warp == 17) {
-        // ===== planner: the coming items and their unions, up to two ahead =====
-        uint32_t id = blockIdx.x;
-        const uint32_t first_pairs = p.lut_stride == 0 ? long_pairs(p.lut, p.nb, p.blocks, lane) : 0;
-        for (uint32_t k = 0;; k++) {
-            const uint32_t slot = k & 1;
-            if (id != kNoItem && lane == 0) {
-                fence_proxy_async();                          // the last answer has been read
-                clc_request(st->clc_response, &st->clc_bar);
-            }
-            if (k >= 2 && !mbar_wait_warp(&st->list_free[slot], ((k >> 1) - 1) & 1, abort_flag, 110)) break;
-            uint32_t n = 0, bh = kNoItem, rows[2] = {kNoItem, kNoItem};
-            if (id != kNoItem) {
-                const ItemAt it = locate_item(p.lut, p.lut_stride, p.B, p.H, p.nb, p.blocks, first_pairs, id, lane, !COL);
-                bh = it.b * p.H + it.h;
-                rows[0] = it.own[0];
-                rows[1] = it.own[1];
-                n = warp_union(p.lut + (size_t)it.h * p.lut_stride, rows, st->lists[slot], kRcMaxUnion, lane);
-                if (n == kNoItem) {                           // more blocks than the caller's maximum: recorded, zeros written
-                    if (lane == 0) atomicCAS(&g_status, 0u, (9u << 24) | (blockIdx.x & 0xffffffu));
-                    n = 0;
-                }
-            }
-            if (lane == 0) {
-                st->list_n[slot] = n;
-                st->list_bh[slot] = bh;
-                st->list_own[slot][0] = rows[0];
-                st->list_own[slot][1] = rows[1];
-                mbar_arrive(&st->list_ready[slot]);
-            }
-            if (id == kNoItem) break;
-            if (!mbar_wait_warp(&st->clc_bar, k & 1, abort_flag, 111)) break;
-            id = clc_item(st->clc_response);
-            __syncwarp();
-        }
-    } else if (warp == 12) {
-        // ===== TMA producer =====
-        if (elect_one()) {
-            uint32_t g = 0, kq = 0;                           // steps, items with blocks
-            bool alive = true;
-            for (uint32_t k = 0; alive; k++) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
+        if (warp == 17) {
+            // ===== planner: the coming items and their unions, up to two ahead =====
+            uint32_t id = blockIdx.x;
+            const uint32_t first_pairs = p.lut_stride == 0 ? long_pairs(p.lut, p.nb, p.blocks, lane) : 0;
+            for (uint32_t k = 0;; k++) {
                 const uint32_t slot = k & 1;
-                if (!mbar_wait(&st->list_ready[slot], (k >> 1) & 1, abort_flag, 112)) break;
-                const uint32_t bh = st->list_bh[slot], T = st->list_n[slot];
-                if (bh == kNoItem) break;
-                const uint32_t b = bh / p.H, h = bh - b * p.H;
-                const int32_t x = (int32_t)(h * 64), row0 = (int32_t)(b * L), beyond = (int32_t)(p.B * L);
-                if (T > 0) {
-                    // the item two before has gone on to TMEM
-                    const uint32_t ob = kq & 1;
-                    if (kq >= 2 && !mbar_wait(&st->own_free[ob], ((kq >> 1) - 1) & 1, abort_flag, 114)) break;
-                    mbar_expect_tx(&st->own_full[ob], 2 * kQBytes);
-                    const uint32_t base = smem_u32(own + ob * 2 * kQBytes);
-#pragma unroll
-                    for (uint32_t o = 0; o < 2; o++) {
-                        const int32_t y = st->list_own[slot][o] == kNoItem ? beyond : row0 + (int32_t)(st->list_own[slot][o] * 64);
-                        tma_load_2d(base + o * kTileBytes, &own1_map, &st->own_full[ob], x, y);
-                        tma_load_2d(base + kQBytes + o * kTileBytes, &own2_map, &st->own_full[ob], x, y);
-                    }
-                    kq++;
+                if (id != kNoItem && lane == 0) {
+                    fence_proxy_async();                          // the last answer has been read
+                    clc_request(st->clc_response, &st->clc_bar);
                 }
-                for (uint32_t t = 0; t < T; t++, g++) {
-                    const uint32_t s = g % kRcStages;
-                    if (g >= kRcStages && !mbar_wait(&st->in_empty[s], ((g / kRcStages) - 1) & 1, abort_flag, 113)) { alive = false; break; }
-                    const uint32_t base = smem_u32(stages + s * kRcStageBytes);
-                    const UnionEntry ent = st->lists[slot][t];
-                    const uint32_t words = COL && MASK ? 512u * __popc(ent.flags & 3u) : 0u;
-                    mbar_expect_tx(&st->in_full[s], kRcStageBytes + (COL ? 512u : 0u) + words);
-                    tma_load_2d(base, &zmap, &st->in_full[s], x, row0 + (int32_t)(ent.col * 64));
-                    tma_load_2d(base + kTileBytes, &ymap, &st->in_full[s], x, row0 + (int32_t)(ent.col * 64));
-                    if (COL) {
-                        const size_t at = (size_t)bh * L + (size_t)ent.col * 64;
-                        bulk_load(smem_u32(st->neg_lse[s]), p.neg_lse + at, 256, &st->in_full[s]);
-                        bulk_load(smem_u32(st->neg_delta[s]), p.neg_delta + at, 256, &st->in_full[s]);
-                        if (MASK) {
-                            const uint64_t *m = p.mask + (size_t)h * p.mask_stride;
+                if (k >= 2 && !mbar_wait_warp(&st->list_free[slot], ((k >> 1) - 1) & 1, abort_flag, 110)) break;
+                uint32_t n = 0, bh = kNoItem, rows[2] = {kNoItem, kNoItem};
+                if (id != kNoItem) {
+                    const ItemAt it = locate_item(p.lut, p.lut_stride, p.B, p.H, p.nb, p.blocks, first_pairs, id, lane, !COL);
+                    bh = it.b * p.H + it.h;
+                    rows[0] = it.own[0];
+                    rows[1] = it.own[1];
+                    n = warp_union(p.lut + (size_t)it.h * p.lut_stride, rows, st->lists[slot], kRcMaxUnion, lane);
+                    if (n == kNoItem) {                           // more blocks than the caller's maximum: recorded, zeros written
+                        if (lane == 0) atomicCAS(&g_status, 0u, (9u << 24) | (blockIdx.x & 0xffffffu));
+                        n = 0;
+                    }
+                }
+                if (lane == 0) {
+                    st->list_n[slot] = n;
+                    st->list_bh[slot] = bh;
+                    st->list_own[slot][0] = rows[0];
+                    st->list_own[slot][1] = rows[1];
+                    mbar_arrive(&st->list_ready[slot]);
+                }
+                if (id == kNoItem) break;
+                if (!mbar_wait_warp(&st->clc_bar, k & 1, abort_flag, 111)) break;
+                id = clc_item(st->clc_response);
+                __syncwarp();
+            }
+        } else if (warp == 12) {
+            // ===== TMA producer =====
+            if (elect_one()) {
+                uint32_t g = 0, kq = 0;                           // steps, items with blocks
+                bool alive = true;
+                for (uint32_t k = 0; alive; k++) {
+                    const uint32_t slot = k & 1;
+                    if (!mbar_wait(&st->list_ready[slot], (k >> 1) & 1, abort_flag, 112)) break;
+                    const uint32_t bh = st->list_bh[slot], T = st->list_n[slot];
+                    if (bh == kNoItem) break;
+                    const uint32_t b = bh / p.H, h = bh - b * p.H;
+                    const int32_t x = (int32_t)(h * 64), row0 = (int32_t)(b * L), beyond = (int32_t)(p.B * L);
+                    if (T > 0) {
+                        // the item two before has gone on to TMEM
+                        const uint32_t ob = kq & 1;
+                        if (kq >= 2 && !mbar_wait(&st->own_free[ob], ((kq >> 1) - 1) & 1, abort_flag, 114)) break;
+                        mbar_expect_tx(&st->own_full[ob], 2 * kQBytes);
+                        const uint32_t base = smem_u32(own + ob * 2 * kQBytes);
 #pragma unroll
-                            for (uint32_t o = 0; o < 2; o++)
-                                if ((ent.flags >> o) & 1u) bulk_load(smem_u32(st->mask[s][o]), m + (size_t)ent.blk[o] * 64, 512, &st->in_full[s]);
+                        for (uint32_t o = 0; o < 2; o++) {
+                            const int32_t y = st->list_own[slot][o] == kNoItem ? beyond : row0 + (int32_t)(st->list_own[slot][o] * 64);
+                            tma_load_2d(base + o * kTileBytes, &own1_map, &st->own_full[ob], x, y);
+                            tma_load_2d(base + kQBytes + o * kTileBytes, &own2_map, &st->own_full[ob], x, y);
+                        }
+                        kq++;
+                    }
+                    for (uint32_t t = 0; t < T; t++, g++) {
+                        const uint32_t s = g % kRcStages;
+                        if (g >= kRcStages && !mbar_wait(&st->in_empty[s], ((g / kRcStages) - 1) & 1, abort_flag, 113)) { alive = false; break; }
+                        const uint32_t base = smem_u32(stages + s * kRcStageBytes);
+                        const UnionEntry ent = st->lists[slot][t];
+                        const uint32_t words = COL && MASK ? 512u * __popc(ent.flags & 3u) : 0u;
+                        mbar_expect_tx(&st->in_full[s], kRcStageBytes + (COL ? 512u : 0u) + words);
+                        tma_load_2d(base, &zmap, &st->in_full[s], x, row0 + (int32_t)(ent.col * 64));
+                        tma_load_2d(base + kTileBytes, &ymap, &st->in_full[s], x, row0 + (int32_t)(ent.col * 64));
+                        if (COL) {
+                            const size_t at = (size_t)bh * L + (size_t)ent.col * 64;
+                            bulk_load(smem_u32(st->neg_lse[s]), p.neg_lse + at, 256, &st->in_full[s]);
+                            bulk_load(smem_u32(st->neg_delta[s]), p.neg_delta + at, 256, &st->in_full[s]);
+                            if (MASK) {
+                                const uint64_t *m = p.mask + (size_t)h * p.mask_stride;
+#pragma unroll
+                                for (uint32_t o = 0; o < 2; o++)
+                                    if ((ent.flags >> o) & 1u) bulk_load(smem_u32(st->mask[s][o]), m + (size_t)ent.blk[o] * 64, 512, &st->in_full[s]);
+                            }
                         }
                     }
+                    if (alive) mbar_arrive(&st->list_free[slot]);
                 }
-                if (alive) mbar_arrive(&st->list_free[slot]);
+            }
+        } else if (warp == 13 || warp == 14) {
+            // ===== S = own1 . Z^T: as soon as the group's last one is in registers (COL: as P, which lies over it, has been multiplied);
+            // dP = own2 . Y^T: as soon as dS, which lies over the group's last one, has been multiplied =====
+            const bool is_s = warp == 13;
+            if (elect_one()) {
+                const uint32_t idesc = instr_desc(fmt, fmt, 128, 64, 0), a = tmem + Cols::own + (is_s ? 0 : 32);
+                uint64_t *full = is_s ? st->s_full : st->dp_full, *free_ = is_s ? (COL ? st->p_free : st->s_free) : st->ds_free, *done = &st->own_done[is_s ? 0 : 1];
+                const uint32_t ring = is_s ? 3 : Cols::dps, ring0 = is_s ? 0 : Cols::dp;
+                uint32_t at = 0, lap = 0;                         // buffer of the step, times round modulo 2
+                issue_all(is_s ? 115 : 123,
+                          [&](uint32_t kq) {
+                              // the item's own tile to TMEM, where the item before is no longer read
+                              if (kq >= 1 && !mbar_wait(done, (kq - 1) & 1, abort_flag, is_s ? 136 : 137)) return false;
+                              if (!mbar_wait(&st->own_full[kq & 1], (kq >> 1) & 1, abort_flag, is_s ? 116 : 124)) return false;
+                              tcgen05_fence_after();
+                              const uint64_t desc = smem_desc_sw128(smem_u32(own + (kq & 1) * 2 * kQBytes + (is_s ? 0 : kQBytes)));
+#pragma unroll
+                              for (uint32_t kk = 0; kk < 4; kk++) copy_to_tmem(a + 8 * kk, desc + 2 * kk);
+                              umma_commit(&st->own_free[kq & 1]);
+                              return true;
+                          },
+                          [&](bool last, bool, uint32_t g, uint32_t q, uint32_t, uint32_t) {
+                              const uint32_t s = g % kRcStages;
+                              const bool ready = mbar_try_wait(&st->in_full[s], (g / kRcStages) & 1);
+                              if (g >= ring && !mbar_wait(&free_[at], lap ^ 1, abort_flag, is_s ? 117 : 121)) return false;
+                              if (!ready && !mbar_wait(&st->in_full[s], (g / kRcStages) & 1, abort_flag, is_s ? 118 : 122)) return false;
+                              tcgen05_fence_after();
+                              const uint64_t b_desc = smem_desc_sw128(smem_u32(stages + s * kRcStageBytes + (is_s ? 0 : kTileBytes)));
+#pragma unroll
+                              for (uint32_t kk = 0; kk < 4; kk++) umma_f16_ts(tmem + ring0 + 64 * at, a + 8 * kk, b_desc + 2 * kk, idesc, kk);
+                              umma_commit(&full[q]);
+                              if (last) umma_commit(done);
+                              if (++at == ring) {
+                                  at = 0;
+                                  lap ^= 1;
+                              }
+                              return true;
+                          });
+            }
+        } else if (warp == 15 || (COL && warp == 16)) {
+            // ===== out += dS . Z, dV += P . Y =====
+            const bool is_dv = warp == 16;
+            if (elect_one()) {
+                const uint32_t idesc = instr_desc(fmt, fmt, 128, 64, 1), acc = tmem + Cols::out + (is_dv ? 64 : 0);
+                uint64_t *full = is_dv ? st->p_full : st->ds_full, *free_ = is_dv ? st->p_free : st->ds_free;
+                const uint32_t ring = is_dv ? 3 : Cols::dps, ring0 = is_dv ? 0 : Cols::dp;
+                uint32_t at = 0;
+                issue_all(is_dv ? 119 : 125, [&](uint32_t) { return true; },
+                          [&](bool last, bool first, uint32_t g, uint32_t q, uint32_t ph, uint32_t kq) {
+                              const uint32_t s = g % kRcStages;
+                              // the accumulator still holds the item before until its epilogue has read it
+                              if (first && kq >= 1 && !mbar_wait(&st->o_free, (kq - 1) & 1, abort_flag, is_dv ? 120 : 126)) return false;
+                              if (!mbar_wait(&full[q], ph, abort_flag, is_dv ? 129 : 127)) return false;
+                              tcgen05_fence_after();
+                              const uint64_t b_desc = smem_desc_sw128(smem_u32(stages + s * kRcStageBytes + (is_dv ? kTileBytes : 0)));
+                              // 16 words of each half of the others lie over the first 16 columns of that half
+#pragma unroll
+                              for (uint32_t kk = 0; kk < 4; kk++)
+                                  umma_f16_ts(acc, tmem + ring0 + 64 * at + 32 * (kk >> 1) + 8 * (kk & 1), b_desc + 128 * kk, idesc, first && kk == 0 ? 0u : 1u);
+                              umma_commit(&free_[at]);
+                              umma_commit(&st->in_empty[s]);      // S and dP of this step are complete: their values made this operand
+                              if (last) umma_commit(&st->o_final[kq % kRcGroups]);
+                              if (++at == ring) at = 0;
+                              return true;
+                          });
             }
         }
-    } else if (warp == 13 || warp == 14) {
-        // ===== S = own1 . Z^T: as soon as the group's last one is in registers (COL: as P, which lies over it, has been multiplied);
-        // dP = own2 . Y^T: as soon as dS, which lies over the group's last one, has been multiplied =====
-        const bool is_s = warp == 13;
-        if (elect_one()) {
-            const uint32_t idesc = instr_desc(fmt, fmt, 128, 64, 0), a = tmem + Cols::own + (is_s ? 0 : 32);
-            uint64_t *full = is_s ? st->s_full : st->dp_full, *free_ = is_s ? (COL ? st->p_free : st->s_free) : st->ds_free, *done = &st->own_done[is_s ? 0 : 1];
-            const uint32_t ring = is_s ? 3 : Cols::dps, ring0 = is_s ? 0 : Cols::dp;
-            uint32_t at = 0, lap = 0;                         // buffer of the step, times round modulo 2
-            issue_all(is_s ? 115 : 123,
-                      [&](uint32_t kq) {
-                          // the item's own tile to TMEM, where the item before is no longer read
-                          if (kq >= 1 && !mbar_wait(done, (kq - 1) & 1, abort_flag, is_s ? 136 : 137)) return false;
-                          if (!mbar_wait(&st->own_full[kq & 1], (kq >> 1) & 1, abort_flag, is_s ? 116 : 124)) return false;
-                          tcgen05_fence_after();
-                          const uint64_t desc = smem_desc_sw128(smem_u32(own + (kq & 1) * 2 * kQBytes + (is_s ? 0 : kQBytes)));
-#pragma unroll
-                          for (uint32_t kk = 0; kk < 4; kk++) copy_to_tmem(a + 8 * kk, desc + 2 * kk);
-                          umma_commit(&st->own_free[kq & 1]);
-                          return true;
-                      },
-                      [&](bool last, bool, uint32_t g, uint32_t q, uint32_t, uint32_t) {
-                          const uint32_t s = g % kRcStages;
-                          const bool ready = mbar_try_wait(&st->in_full[s], (g / kRcStages) & 1);
-                          if (g >= ring && !mbar_wait(&free_[at], lap ^ 1, abort_flag, is_s ? 117 : 121)) return false;
-                          if (!ready && !mbar_wait(&st->in_full[s], (g / kRcStages) & 1, abort_flag, is_s ? 118 : 122)) return false;
-                          tcgen05_fence_after();
-                          const uint64_t b_desc = smem_desc_sw128(smem_u32(stages + s * kRcStageBytes + (is_s ? 0 : kTileBytes)));
-#pragma unroll
-                          for (uint32_t kk = 0; kk < 4; kk++) umma_f16_ts(tmem + ring0 + 64 * at, a + 8 * kk, b_desc + 2 * kk, idesc, kk);
-                          umma_commit(&full[q]);
-                          if (last) umma_commit(done);
-                          if (++at == ring) {
-                              at = 0;
-                              lap ^= 1;
-                          }
-                          return true;
-                      });
-        }
-    } else if (warp == 15 || (COL && warp == 16)) {
-        // ===== out += dS . Z, dV += P . Y =====
-        const bool is_dv = warp == 16;
-        if (elect_one()) {
-            const uint32_t idesc = instr_desc(fmt, fmt, 128, 64, 1), acc = tmem + Cols::out + (is_dv ? 64 : 0);
-            uint64_t *full = is_dv ? st->p_full : st->ds_full, *free_ = is_dv ? st->p_free : st->ds_free;
-            const uint32_t ring = is_dv ? 3 : Cols::dps, ring0 = is_dv ? 0 : Cols::dp;
-            uint32_t at = 0;
-            issue_all(is_dv ? 119 : 125, [&](uint32_t) { return true; },
-                      [&](bool last, bool first, uint32_t g, uint32_t q, uint32_t ph, uint32_t kq) {
-                          const uint32_t s = g % kRcStages;
-                          // the accumulator still holds the item before until its epilogue has read it
-                          if (first && kq >= 1 && !mbar_wait(&st->o_free, (kq - 1) & 1, abort_flag, is_dv ? 120 : 126)) return false;
-                          if (!mbar_wait(&full[q], ph, abort_flag, is_dv ? 129 : 127)) return false;
-                          tcgen05_fence_after();
-                          const uint64_t b_desc = smem_desc_sw128(smem_u32(stages + s * kRcStageBytes + (is_dv ? kTileBytes : 0)));
-                          // 16 words of each half of the others lie over the first 16 columns of that half
-#pragma unroll
-                          for (uint32_t kk = 0; kk < 4; kk++)
-                              umma_f16_ts(acc, tmem + ring0 + 64 * at + 32 * (kk >> 1) + 8 * (kk & 1), b_desc + 128 * kk, idesc, first && kk == 0 ? 0u : 1u);
-                          umma_commit(&free_[at]);
-                          umma_commit(&st->in_empty[s]);      // S and dP of this step are complete: their values made this operand
-                          if (last) umma_commit(&st->o_final[kq % kRcGroups]);
-                          if (++at == ring) at = 0;
-                          return true;
-                      });
-        }
-    }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 128;");
         // ===== P, dS and the epilogue: own position r, every third step =====
@@ -553,6 +559,10 @@ static int launch_side(cudaStream_t s, const CUtensorMap &own1, const CUtensorMa
     if (!once.done(dev)) {
         if (cudaFuncSetAttribute(recompute_tc_kernel<COL, MASK, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kRcSmem) != cudaSuccess)
             return fail("sfb_attention_backward_recompute: cannot reserve %zu bytes of shared memory", kRcSmem);
+        // what the warpgroups hand to each other is what the block is launched with: with less the workers would wait for ever
+        cudaFuncAttributes attr;
+        if (cudaFuncGetAttributes(&attr, recompute_tc_kernel<COL, MASK, BF16>) != cudaSuccess || attr.numRegs < 96)
+            return fail("sfb_attention_backward_recompute: built with too few registers for its warpgroups");
         once.mark(dev);
     }
     const dim3 grid((prm.nb + 1) / 2 * prm.B * prm.H);

@@ -985,7 +985,6 @@ FUNCTION(py_clip_grad_norm, 5)
             out[i] = ptr(o);
         }
     }
-    require_cuda(first);
     if (write) {
         // what is written shares memory with nothing else, but for a gradient that stays where it is
         struct Span {
@@ -1009,6 +1008,7 @@ FUNCTION(py_clip_grad_norm, 5)
             if (x.written) written_end = std::max(written_end, x.end);
         }
     }
+    require_cuda(first);
     const c10::cuda::CUDAGuard on(first.device());
     at::Tensor norm = empty({1}, at::kFloat, first), ws = empty({(int64_t)L.sfb_clip_grad_norm_workspace((uint32_t)count)}, at::kByte, first);
     if (write)

@@ -314,6 +314,25 @@ def test_long_rows_of_many_blocks(sfb):
     assert sfb.device_status() == 0
 
 
+@pytest.mark.parametrize("B,H,heads", [(3, 40, 1), (2, 100, 1), (1, 130, 130)])
+def test_more_heads_than_go_through_the_workspace_at_once(sfb, B, H, heads):
+    """Whole batch elements at a time, and some heads of one: the same bits as calls for a few heads each, in place."""
+    bs, nb, d = 32, 64, 8
+    i, j = np.arange(nb)[:, None], np.arange(nb)[None, :]
+    blocks = np.stack([(i == j) | (j == (i + 1 + h % 5) % nb) for h in range(heads)]).astype(np.uint8)
+    q, k, v, do = (x.cuda() for x in operands(B, nb * bs, H, d, "f32", 13))
+    lay = plan(sfb, blocks, bs)
+    o, lse = sfb.fused_attention_stats(q, k, v, lay)
+    whole = sfb.attention_backward_recompute(q, k, v, o, do, lse, lay)
+    for h0 in range(0, H, 37):
+        h1 = min(H, h0 + 37)
+        part = plan(sfb, blocks[h0:h1] if heads > 1 else blocks, bs)
+        cut = [x[:, :, h0:h1] for x in (q, k, v, o, do)]
+        got = sfb.attention_backward_recompute(*cut, lse[:, h0:h1].contiguous(), part)
+        for a, b in zip(got, whole):
+            assert torch.equal(a, b[:, :, h0:h1])
+
+
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
 @pytest.mark.parametrize("kind", ["diagonal", "two", "three", "mixed", "empty rows"])
 def test_many_short_rows(sfb, dtype, kind):

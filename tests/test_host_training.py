@@ -158,15 +158,22 @@ def test_workspaces(sfb):
     rows = 2 * 2 * 4 * 128 * 4
     assert f(1, 64, 4, 2, 2, 4, 64, 2, 2, 1) >= rows and f(0, 32, 8, 2, 4, 4, 64, 2, 2, 1) >= rows + 2 * 8 * 32 * 32 * 4
     assert f(9, 64, 4, 2, 2, 4, 64, 2, 2, 1) == 0
-    assert f(0, 32, 1 << 12, 64, 64, 16, 64, 64, 64, 1) < (1 << 28)                 # P and dS go through it a few heads at a time
+    # P and dS go through it a few heads at a time: in 512 MB, beside two numbers per row
+    assert f(0, 32, 1 << 12, 64, 64, 16, 64, 64, 64, 1) <= (512 << 20) + 2 * 64 * 2048 * 16 * 4
     g = sfb.lib.sfb_embedding_grad_workspace
     assert g(0, 5, 16, 9) >= 40 and g(8, 4096, 768, 30522) >= 32768 * 16 + 30523 * 4 + 1024 * 2 * 768 * 4
     assert sfb.lib.sfb_clip_grad_norm_workspace(1) >= 8
 
 
-def test_arguments_that_need_no_gpu_to_be_refused_by_overlap(sfb):
-    """Tensors that share memory: found on the host, before the device is."""
+def test_tensors_that_share_memory(sfb):
+    """Found on the host, before the device is: what is written shares memory with nothing but the gradient that it takes the place of."""
     flat = z(100)
-    for grads in ([flat, flat], [flat[:60], flat[50:]], [flat[10:20], flat]):
-        with pytest.raises(AssertionError, match="CUDA device|shares memory"):
-            sfb.clip_grad_norm(grads, 1.0)
+    for grads, out in (([flat, flat], None), ([flat[:60], flat[50:]], None), ([flat[10:20], flat], None), ([flat[:50], z(50)], [z(50), flat[40:90]]),
+                       ([flat[:50], flat[50:]], [flat[50:], flat[:50]])):
+        with pytest.raises(AssertionError, match="shares memory"):
+            sfb.clip_grad_norm(grads, 1.0, out=out)
+    for grads, out in (([flat[:50], flat[50:]], None), ([flat, flat], [z(100), z(100)]), ([flat], [flat]), ([flat[:50], flat[50:]], [flat[:50], z(50)])):
+        with pytest.raises(AssertionError, match="CUDA device"):
+            sfb.clip_grad_norm(grads, 1.0, out=out)
+    with pytest.raises(AssertionError, match="CUDA device"):
+        sfb.grad_norm([flat, flat])                          # nothing is written
