@@ -8,8 +8,8 @@ struct AttnDims {
     uint32_t B, H, d, nb_a, nb_b, blocks;
     uint32_t lut_stride;   // uint2 per head in the LUT handed to the kernel (0 = shared by all heads)
     uint32_t mask_stride;  // words per head in the mask (0 = shared)
-    uint64_t in_pitch;     // elements between consecutive rows of q, k, v, or of a product's second operand (0 = H * d: the tensors hold these heads only)
-    uint64_t out_pitch;    // the same for o, or the product's result
+    uint64_t in_pitch;     // elements between consecutive rows of q, k, v (0 = H * d: the tensors hold these heads only)
+    uint64_t out_pitch;    // the same for o
 };
 
 // fp32 operands and the shapes that the tcgen05 kernels do not take (attn_simt.cu)

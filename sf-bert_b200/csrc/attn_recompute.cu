@@ -2,10 +2,9 @@
 // scores is kept from the forward pass.  With x = scale Q.K^T on the kept elements and lse the log of a row's sum of exp(x),
 //   P = exp(x - lse),  delta = rowsum(dO * O),  dS = P * (dO.V^T - delta) * scale,  dQ = dS.K,  dK = dS^T.Q,  dV = P^T.dO.
 // Here are the rows' constants for every path, and the path of fp32 operands and of every shape that the tcgen05 kernels
-// (attn_tc_recompute.cu) do not take.  That one makes P and dS of some (batch, head) pairs at a time in the caller's workspace, in the
-// operands' type, and multiplies them by the products of attn_simt.cu: five products per block.  Two kernels that keep both on
-// chip, one by rows and one by columns, would make two of them twice, and at fp32 precision a product costs more than a block's
-// way through L2.
+// (attn_tc_recompute.cu) do not take.  That one makes P and dS of some (batch, head) pairs at a time in the caller's workspace, 16-bit types as
+// operands of the products that follow, fp32 as three bf16 numbers each, and one launch makes the three products from them: five products per
+// block.  Two kernels that keep both on chip, one by rows and one by columns, would make two of them twice.
 #include "recompute.cuh"
 #include "simt_tile.cuh"
 #include <initializer_list>
@@ -109,7 +108,6 @@ struct BlockArgs {
     size_t in_pitch, do_pitch;
     uint32_t first, H, d, nb, blocks, lut_stride, mask_stride;        // first: (batch, head) pair of blockIdx.y = 0
     float scale, scale_log2e;
-    bool vec;
 };
 template <int BS> struct BlockCfg {
     static constexpr int TEAMS = BS == 32 ? 4 : 2, TT = 128 / TEAMS;      // teams that stage keys of their own
@@ -184,7 +182,7 @@ __device__ __forceinline__ void store_eight(void *out, size_t at, uint32_t plane
 // Both products on the warp tiles of simt_tile.cuh, 32 elements of d at a time: the rows of Q (dO) straight to fragments, a chunk ahead
 // in registers, the rows of K (V) through a ring of two chunks per team.  A thread holds eight neighbouring columns of four rows.
 // P and dS leave as three bf16 numbers each, whose sum they are.
-template <int BS>
+template <int BS, bool VEC>
 __global__ void __launch_bounds__(tile::kThreads, 3) recompute_blocks_kernel(const __grid_constant__ BlockArgs a)
 {
     using namespace tile;
@@ -214,16 +212,16 @@ __global__ void __launch_bounds__(tile::kThreads, 3) recompute_blocks_kernel(con
 #pragma unroll
             for (int i = 0; i < 8; i++) {
                 const uint32_t k = c * kChunk + 16 * (i >> 2) + 4 * t;
-                load_raw4<DT>(held_a[i], A, rowA + (size_t)(8 * (i & 3) + g) * pitchA + k, k < a.d ? a.d - k : 0u, a.vec);
+                load_raw4<DT>(held_a[i], A, rowA + (size_t)(8 * (i & 3) + g) * pitchA + k, k < a.d ? a.d - k : 0u, VEC);
             }
         };
         auto issue = [&](uint32_t c) {
-            stage_begin(held_b, rank, bufs + (c & 1) * Cfg::buf, kStride, B, rowB + c * kChunk, a.in_pitch, a.d - c * kChunk, a.vec);
+            stage_begin(held_b, rank, bufs + (c & 1) * Cfg::buf, kStride, B, rowB + c * kChunk, a.in_pitch, a.d - c * kChunk, VEC);
             cp_commit();
         };
         issue(0);
         load_a(0);
-        stage_end(held_b, rank, bufs, kStride, a.vec);
+        stage_end(held_b, rank, bufs, kStride, VEC);
         for (uint32_t c = 0; c < chunks; c++) {
             cp_wait<0>();
             meet<TT>(1 + team);
@@ -246,7 +244,7 @@ __global__ void __launch_bounds__(tile::kThreads, 3) recompute_blocks_kernel(con
 #pragma unroll
                 for (int m = 0; m < 2; m++) mma16<4, T, T>(acc[m], fa[k][m], fb);
             }
-            if (c + 1 < chunks) stage_end(held_b, rank, bufs + ((c + 1) & 1) * Cfg::buf, kStride, a.vec);
+            if (c + 1 < chunks) stage_end(held_b, rank, bufs + ((c + 1) & 1) * Cfg::buf, kStride, VEC);
         }
     };
     float x[2][4][4] = {}, y[2][4][4] = {};
@@ -308,7 +306,13 @@ __device__ __forceinline__ uint4 load_eight(const uint16_t *p, uint32_t n, bool 
         if (i < n) w[i >> 1] |= (uint32_t)p[i] << (16 * (i & 1));
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
-template <int BS, int DT>
+__device__ __forceinline__ float ex2(float x)           // 2 units of 2^-23, and 0 below 2^-126: P is rounded to 16 bits
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+template <int BS, int DT, bool VEC>
 __global__ void __launch_bounds__(tile::kThreads, 4) recompute_blocks16_kernel(const __grid_constant__ BlockArgs a)
 {
     constexpr uint32_t PER = BS == 32 ? 4 : 1;               // blocks per CTA
@@ -331,8 +335,8 @@ __global__ void __launch_bounds__(tile::kThreads, 4) recompute_blocks16_kernel(c
             uint4 x[4], y[4];
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                x[i] = load_eight(pa + (size_t)(8 * i) * pitchA + k, n, a.vec);
-                y[i] = load_eight(pb + (size_t)(2 * i) * a.in_pitch + k, n, a.vec);
+                x[i] = load_eight(pa + (size_t)(8 * i) * pitchA + k, n, VEC);
+                y[i] = load_eight(pb + (size_t)(2 * i) * a.in_pitch + k, n, VEC);
             }
 #pragma unroll
             for (int m = 0; m < 2; m++)
@@ -363,7 +367,7 @@ __global__ void __launch_bounds__(tile::kThreads, 4) recompute_blocks16_kernel(c
 #pragma unroll
             for (int k = 0; k < 8; k++) {
                 const bool in = (bits >> k) & 1u;
-                p[k] = in ? exp2f(fmaf(x[m][k >> 1][2 * half + (k & 1)], a.scale_log2e, nl)) : 0.f;
+                p[k] = in ? ex2(fmaf(x[m][k >> 1][2 * half + (k & 1)], a.scale_log2e, nl)) : 0.f;
                 ds[k] = in ? p[k] * fmaf(y[m][k >> 1][2 * half + (k & 1)], a.scale, nd) : 0.f;
             }
             store_eight<DT>(a.p, baseC + (size_t)r * BS + 8 * t, 0, p);
@@ -374,8 +378,8 @@ __global__ void __launch_bounds__(tile::kThreads, 4) recompute_blocks16_kernel(c
 // ---- the three products with P and dS: dV = P^T.dO, dK = dS^T.Q, dQ = dS.K -------------------------------------------------------------
 // A CTA makes one block-row (column) of one of them, all of d: a warp 32 x 32 outputs.  The contraction goes 32 elements at a time through a ring of
 // kStages stages of shared memory, brought by cp.async.  P and dS are 16-bit there and become fragments by ldmatrix, transposed or not; so do
-// 16-bit operands.  fp32: P and dS are three bf16 planes whose sum they are, split once by the kernel that made them (by FMAs on
-// fp32 blocks, which every warp would have to split again, the three products of 7680 blocks of 32, d 128, took 115 us), and a warp
+// 16-bit operands.  fp32: P and dS are three bf16 planes whose sum they are, split once by the kernel that made them (fp32
+// blocks would be split again by every warp, or multiplied by FMAs: 7680 blocks of 32, d 128, the whole backward pass 295 us, 273 so), and a warp
 // splits its own columns of the other operand.  Each 32 elements are added up from zero and then to the sum, rounded to
 // nearest: the tensor core's additions truncate.  Sums have a fixed order.
 struct ProductArgs {
@@ -383,7 +387,7 @@ struct ProductArgs {
     const void *p, *ds, *q, *k, *dout;
     void *dq, *dk, *dv;
     size_t in_pitch, do_pitch, grad_pitch;
-    uint32_t first, H, d, nb, blocks, lut_stride;
+    uint32_t first, pairs, H, d, nb, blocks, lut_stride;      // pairs: (batch, head) pairs of this launch, from `first` on
     bool in_vec, do_vec, out_vec;
 };
 constexpr uint32_t kStages = 3;
@@ -425,12 +429,12 @@ __device__ __noinline__ void product_again(float (&acc)[2][4][4], const uint16_t
         }
 }
 template <int BS, int W, int DT, bool TRANS>
-__device__ __forceinline__ void product_rows(char *sm, const ProductArgs &a, uint32_t i, const void *P, const void *V, size_t pitch, bool vec, void *out)
+__device__ __forceinline__ void product_rows(char *sm, const ProductArgs &a, uint32_t i, uint32_t y, const void *P, const void *V, size_t pitch, bool vec, void *out)
 {
     typedef ProductCfg<BS, W, DT, TRANS> Cfg;
     constexpr uint32_t T = Cfg::T, E = Cfg::E, PARTS = BS / 32;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const uint32_t bh = a.first + blockIdx.y, b = bh / a.H, h = bh - b * a.H;
+    const uint32_t bh = a.first + y, b = bh / a.H, h = bh - b * a.H;
     const uint32_t r0 = 32 * (warp / W), n0 = 32 * (warp % W);
     const uint2 *lut = (TRANS ? a.tn : a.nn) + (size_t)h * a.lut_stride;
     const uint2 head = lut[i], *ents = lut + head.x;
@@ -442,7 +446,7 @@ __device__ __forceinline__ void product_rows(char *sm, const ProductArgs &a, uin
         if (c < chunks) {
             const uint32_t part = c % PARTS;
             char *buf = sm + (c % kStages) * Cfg::stage;
-            const uint16_t *pa = (const uint16_t *)P + ((size_t)blockIdx.y * a.blocks + ent.x) * BS * BS * T + (TRANS ? part * 32 * BS : part * 32);
+            const uint16_t *pa = (const uint16_t *)P + ((size_t)y * a.blocks + ent.x) * BS * BS * T + (TRANS ? part * 32 * BS : part * 32);
             constexpr uint32_t PA = Cfg::a_cols / 8;          // 16-byte pieces per row
 #pragma unroll
             for (uint32_t x = threadIdx.x; x < T * Cfg::a_rows * PA; x += Cfg::threads) {
@@ -540,7 +544,7 @@ __device__ __forceinline__ void product_rows(char *sm, const ProductArgs &a, uin
     if constexpr (DT == SFB_F32) {
         const bool odd = !(tile::zero_if_finite<4>(acc[1], tile::zero_if_finite<4>(acc[0], 0.f)) == 0.f);
         if (__any_sync(0xffffffffu, odd))
-            product_again<BS, TRANS>(acc, (const uint16_t *)P, (const float *)V + baseV + n0, ents, head.y, (size_t)blockIdx.y * a.blocks, pitch, r0, left, g, t);
+            product_again<BS, TRANS>(acc, (const uint16_t *)P, (const float *)V + baseV + n0, ents, head.y, (size_t)y * a.blocks, pitch, r0, left, g, t);
     }
     // rows (columns) without blocks are written as zeros
 #pragma unroll
@@ -576,22 +580,25 @@ __device__ __forceinline__ void product_rows(char *sm, const ProductArgs &a, uin
             }
         }
 }
-// dV, dK and dQ of a block side by side: P and dS come from HBM once where they do not fit into L2
+// dV, dK and dQ of a block side by side: P and dS come from HBM once where they do not fit into L2.  The same block-row of all pairs before the
+// next one, and the last eighth of them first: a launch then ends with rows of the middle, and rows and columns that keep everything lie
+// at the ends in most layouts (us, pair after pair / row after row / that and the last eighth first / both ends inwards: bf16, blocks of 32, d 64,
+// 4 x 12 heads of 2048 positions, strided 212 / 199 / 202 / 208, causal 466 / 463 / 466 / 456; fp32, 4 x 8 heads, BigBird 450 / 437 / 374 / 375).
 template <int BS, int W, int DT>
 __global__ void __launch_bounds__(32 * W * (BS / 32), 512 / (32 * W * (BS / 32))) products_kernel(const __grid_constant__ ProductArgs a)
 {
     extern __shared__ __align__(16) char psm[];
     grid_dependency_wait();
     grid_launch_dependents();
-    const uint32_t i = blockIdx.x / 3, which = blockIdx.x - 3 * i;
+    const uint32_t n = blockIdx.x / 3, which = blockIdx.x - 3 * n, at = n / a.pairs, y = n - at * a.pairs, i = at < (a.nb + 7) / 8 ? a.nb - 1 - at : at - (a.nb + 7) / 8;
     if (which == 2) {
-        product_rows<BS, W, DT, false>(psm, a, i, a.ds, a.k, a.in_pitch, a.in_vec, a.dq);
+        product_rows<BS, W, DT, false>(psm, a, i, y, a.ds, a.k, a.in_pitch, a.in_vec, a.dq);
     } else {
-        product_rows<BS, W, DT, true>(psm, a, i, which ? a.ds : a.p, which ? a.q : a.dout, which ? a.in_pitch : a.do_pitch, which ? a.in_vec : a.do_vec, which ? a.dk : a.dv);
+        product_rows<BS, W, DT, true>(psm, a, i, y, which ? a.ds : a.p, which ? a.q : a.dout, which ? a.in_pitch : a.do_pitch, which ? a.in_vec : a.do_vec, which ? a.dk : a.dv);
     }
 }
 template <int BS, int W, int DT>
-static int launch_products(cudaStream_t s, const ProductArgs &k, uint32_t pairs)
+static int launch_products(cudaStream_t s, const ProductArgs &k)
 {
     constexpr size_t bytes = kStages * (ProductCfg<BS, W, DT, true>::stage > ProductCfg<BS, W, DT, false>::stage ? ProductCfg<BS, W, DT, true>::stage
                                                                                                              : ProductCfg<BS, W, DT, false>::stage);
@@ -602,15 +609,15 @@ static int launch_products(cudaStream_t s, const ProductArgs &k, uint32_t pairs)
             return fail("sfb_attention_backward_recompute: shared memory configuration failed");
         once.mark(dev);
     }
-    launch_overlapped_few(products_kernel<BS, W, DT>, dim3(3 * k.nb, pairs), dim3(ProductCfg<BS, W, DT, true>::threads), bytes, s, k);
+    launch_overlapped_few(products_kernel<BS, W, DT>, dim3(3 * k.nb * k.pairs), dim3(ProductCfg<BS, W, DT, true>::threads), bytes, s, k);
     return 0;
 }
 
-// How many (batch, head) pairs go through the workspace at a time: block-rows for every SM to have 32 (us with 8 / 16 / 32, each a share of what
-// follows: bf16, blocks of 32, d 64, 4 x 12 heads of 2048 positions, strided 1119 / 793 / 622; fp16, blocks of 64, d 128 1635 / 1308 / 1307; what L2 could
-// have kept of P and dS counts for less than the SMs that have nothing left to do at the end of each launch), as long as P and dS take no more
+// How many (batch, head) pairs go through the workspace at a time: block-rows for every SM to have 64 (us with 16 / 32 / 64:
+// bf16, blocks of 32, d 64, strided, 4 x 12 heads of 2048 positions 242 / 212 / 210, 8 x 16 heads 598 / 528 / 496; what L2 could have kept of P and dS
+// counts for less than the SMs that have nothing left to do at the end of each launch), as long as P and dS take no more
 // than 512 MB; one at least; parts of about the same size.
-constexpr uint64_t kRowsPerSm = 32, kMostSms = 148, kMostBytes = 512ull << 20;
+constexpr uint64_t kRowsPerSm = 64, kMostSms = 148, kMostBytes = 512ull << 20;
 static uint64_t score_bytes(int dtype) { return dtype == SFB_F32 ? 6 : 2; }      // three planes, or the operands' type
 static uint32_t pairs_at_a_time(int dtype, uint32_t bs, uint32_t nb, uint32_t blocks, uint32_t B, uint32_t H)
 {
@@ -629,19 +636,20 @@ uint64_t simt_backward_workspace(int dtype, uint32_t bs, uint32_t nb, uint32_t b
 }
 
 template <int BS, int DT>
-static int backward_parts(cudaStream_t s, BlockArgs &k, ProductArgs &o, uint32_t all, uint32_t n)
+static int backward_parts(cudaStream_t s, BlockArgs &k, ProductArgs &o, uint32_t all, uint32_t n, bool vec)
 {
     constexpr uint32_t per = BS == 32 ? 4 : 1;
     for (uint32_t first = 0; first < all; first += n) {
         const uint32_t pairs = all - first < n ? all - first : n;
         k.first = o.first = first;
+        o.pairs = pairs;
         if (k.blocks) {
             const dim3 grid((k.blocks + per - 1) / per, pairs);
-            if constexpr (DT == SFB_F32) launch_overlapped_few(recompute_blocks_kernel<BS>, grid, dim3(tile::kThreads), BlockCfg<BS>::bytes, s, k);
-            else launch_overlapped_few(recompute_blocks16_kernel<BS, DT>, grid, dim3(tile::kThreads), 0, s, k);
+            if constexpr (DT == SFB_F32) launch_overlapped_few(vec ? recompute_blocks_kernel<BS, true> : recompute_blocks_kernel<BS, false>, grid, dim3(tile::kThreads), BlockCfg<BS>::bytes, s, k);
+            else launch_overlapped_few(vec ? recompute_blocks16_kernel<BS, DT, true> : recompute_blocks16_kernel<BS, DT, false>, grid, dim3(tile::kThreads), 0, s, k);
         }
-        if (k.d <= 32 ? launch_products<BS, 1, DT>(s, o, pairs) : k.d <= 64 ? launch_products<BS, 2, DT>(s, o, pairs)
-            : k.d <= 96 ? launch_products<BS, 3, DT>(s, o, pairs) : launch_products<BS, 4, DT>(s, o, pairs)) return 1;
+        if (k.d <= 32 ? launch_products<BS, 1, DT>(s, o) : k.d <= 64 ? launch_products<BS, 2, DT>(s, o)
+            : k.d <= 96 ? launch_products<BS, 3, DT>(s, o) : launch_products<BS, 4, DT>(s, o)) return 1;
         if (check_launch("sfb_attention_backward_recompute")) return 1;
     }
     return 0;
@@ -658,12 +666,12 @@ int simt_backward_recompute(cudaStream_t s, const BackwardArgs &a, float *neg_ls
     };
     const bool in = rows({a.q, a.k, a.v}, a.in_pitch), dout = rows({a.dout}, a.do_pitch);
     BlockArgs k = {(const uint2 *)a.nt_lut, a.q, a.k, a.v, a.dout, a.mask, neg_lse, neg_delta, P, dS, (size_t)a.in_pitch, (size_t)a.do_pitch, 0, p.H, p.d, p.nb_a,
-                   p.blocks, a.nt_stride, p.mask_stride, a.scale, a.scale * 1.4426950408889634f, in && dout};
-    ProductArgs o = {(const uint2 *)a.nn_lut, (const uint2 *)a.tn_lut, P, dS, a.q, a.k, a.dout, a.dq, a.dk, a.dv, (size_t)a.in_pitch, (size_t)a.do_pitch, (size_t)a.grad_pitch, 0,
+                   p.blocks, a.nt_stride, p.mask_stride, a.scale, a.scale * 1.4426950408889634f};
+    ProductArgs o = {(const uint2 *)a.nn_lut, (const uint2 *)a.tn_lut, P, dS, a.q, a.k, a.dout, a.dq, a.dk, a.dv, (size_t)a.in_pitch, (size_t)a.do_pitch, (size_t)a.grad_pitch, 0, 0,
                      p.H, p.d, p.nb_a, p.blocks, p.lut_stride, in, dout, rows({a.dq, a.dk, a.dv}, a.grad_pitch)};
     const uint32_t all = p.B * p.H;
-#define BP(BS) (a.dtype == SFB_F32 ? backward_parts<BS, SFB_F32>(s, k, o, all, n) : a.dtype == SFB_BF16 ? backward_parts<BS, SFB_BF16>(s, k, o, all, n) \
-                                                                                                    : backward_parts<BS, SFB_F16>(s, k, o, all, n))
+#define BP(BS) (a.dtype == SFB_F32 ? backward_parts<BS, SFB_F32>(s, k, o, all, n, in && dout) : a.dtype == SFB_BF16 ? backward_parts<BS, SFB_BF16>(s, k, o, all, n, in && dout) \
+                                                                                                    : backward_parts<BS, SFB_F16>(s, k, o, all, n, in && dout))
     return a.bs == 32 ? BP(32) : BP(64);
 #undef BP
 }

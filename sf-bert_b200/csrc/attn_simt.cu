@@ -556,7 +556,7 @@ __device__ __forceinline__ void spmm_fma(float *sm, const uint2 *__restrict__ lu
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, lr = lane_row(lane), lc = lane_quad(lane);
     const uint2 *nn = lut + (size_t)h * p.lut_stride;
     const uint2 head = nn[i];
-    const size_t HD = p.in_pitch ? (size_t)p.in_pitch : (size_t)p.H * p.d, HDo = p.out_pitch ? (size_t)p.out_pitch : (size_t)p.H * p.d;      // row pitches of V and O
+    const size_t HD = (size_t)p.H * p.d;
     const size_t bh = (size_t)b * p.H + h;
     const uint32_t r0 = BS == 64 ? 32 * (warp >> 1) : 0, n0 = (BS == 64 ? warp & 1 : warp) * (DS / Cfg::WC);
     const uint32_t chunks = head.y * PARTS;
@@ -587,12 +587,12 @@ __device__ __forceinline__ void spmm_fma(float *sm, const uint2 *__restrict__ lu
         else mma_nn<TN>(acc, buf + (r0 + lr) * a_stride, a_stride, v, DS + 4);
     }
     // rows without blocks are written as zeros (blocksparse.h:949-962)
-    const size_t baseO = ((size_t)b * p.nb_a + i) * BS * HDo + (size_t)h * p.d + d0 + n0;
+    const size_t baseO = ((size_t)b * p.nb_a + i) * BS * HD + (size_t)h * p.d + d0 + n0;
     const uint32_t left = p.d > d0 + n0 ? p.d - d0 - n0 : 0;
 #pragma unroll
     for (int m = 0; m < 4; m++) {
         const uint32_t r = r0 + (TRANS ? 4 * lr + m : lr + 8 * m);
-        store_row<BC_DT, TN, AGAIN>(O, baseO + (size_t)r * HDo, lc, acc[m], left, vec);
+        store_row<BC_DT, TN, AGAIN>(O, baseO + (size_t)r * HD, lc, acc[m], left, vec);
     }
 }
 template <int BS, int DS, int A_DT, int BC_DT, bool TRANS>
@@ -607,9 +607,9 @@ __global__ void __launch_bounds__(tile::kThreads, 4) spmm_fma_kernel(const uint2
 // Not inlined, and from the kernel's parameters alone: nothing is kept for it in registers while the split products are made
 template <int BS, int DS, int A_DT, int BC_DT, bool TRANS>
 __device__ __noinline__ void spmm_again(float *sm, const uint2 *lut, const void *Pm, const void *V, void *O, uint32_t H, uint32_t d, uint32_t nb_a, uint32_t nb_b,
-                                        uint32_t blocks, uint32_t lut_stride, uint64_t in_pitch, uint64_t out_pitch, bool avec, bool vec)
+                                        uint32_t blocks, uint32_t lut_stride, bool avec, bool vec)
 {
-    const AttnDims p = {0, H, d, nb_a, nb_b, blocks, lut_stride, 0, in_pitch, out_pitch};
+    const AttnDims p = {0, H, d, nb_a, nb_b, blocks, lut_stride, 0, 0, 0};
     spmm_fma<BS, DS, A_DT, BC_DT, TRANS, true>(sm, lut, Pm, V, O, p, avec, vec);
 }
 
@@ -640,7 +640,7 @@ spmm_nn_kernel(const uint2 *__restrict__ lut, const void *__restrict__ Pm, const
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const uint2 *nn = lut + (size_t)h * p.lut_stride;
     const uint2 head = nn[i];
-    const size_t HD = p.in_pitch ? (size_t)p.in_pitch : (size_t)p.H * p.d, HDo = p.out_pitch ? (size_t)p.out_pitch : (size_t)p.H * p.d;      // row pitches of V and O
+    const size_t HD = (size_t)p.H * p.d;
     const size_t bh = (size_t)b * p.H + h;
     const uint32_t r0 = BS == 64 ? 32 * (warp >> 1) : 0, team = BS == 64 ? warp & 1 : warp, n0 = d0 + team * Cfg::NW;
     const uint32_t rank = BS == 64 ? 32 * (warp >> 1) + lane : lane;
@@ -722,16 +722,16 @@ spmm_nn_kernel(const uint2 *__restrict__ lut, const void *__restrict__ Pm, const
         land(c + 2);
     }
     // rows without blocks are written as zeros (blocksparse.h:949-962)
-    const size_t baseO = ((size_t)b * p.nb_a + i) * BS * HDo + (size_t)h * p.d + n0;
+    const size_t baseO = ((size_t)b * p.nb_a + i) * BS * HD + (size_t)h * p.d + n0;
     const bool odd = (TP > 1 || TV > 1) && !(zero_if_finite<N>(acc[1], zero_if_finite<N>(acc[0], 0.f)) == 0.f);
 #pragma unroll
     for (int m = 0; m < 2; m++)
 #pragma unroll
         for (int half = 0; half < 2; half++) {
             const uint32_t r = r0 + (TRANS ? 4 * g + 2 * m + half : 16 * m + 8 * half + g);
-            store_cols<BC_DT, N>(O, baseO + (size_t)r * HDo, t, acc[m], half, 1.f, left, vec);
+            store_cols<BC_DT, N>(O, baseO + (size_t)r * HD, t, acc[m], half, 1.f, left, vec);
         }
-    if ((TP > 1 || TV > 1) && __syncthreads_or(odd)) spmm_again<BS, DS, A_DT, BC_DT, TRANS>(sm, lut, Pm, V, O, p.H, p.d, p.nb_a, p.nb_b, p.blocks, p.lut_stride, p.in_pitch, p.out_pitch, avec, vec);
+    if ((TP > 1 || TV > 1) && __syncthreads_or(odd)) spmm_again<BS, DS, A_DT, BC_DT, TRANS>(sm, lut, Pm, V, O, p.H, p.d, p.nb_a, p.nb_b, p.blocks, p.lut_stride, avec, vec);
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -1527,8 +1527,7 @@ int simt_spmm_nn(cudaStream_t s, const void *lut, const void *a, const void *b, 
                  uint32_t bs, const AttnDims &p, bool trans)
 {
     const uint64_t HD = (uint64_t)p.H * p.d;
-    const bool avec = ((uintptr_t)a & 15) == 0;
-    const bool vec = rows_vec(b, bc_dtype, p.in_pitch ? p.in_pitch : HD, p.d) && rows_vec(c, bc_dtype, p.out_pitch ? p.out_pitch : HD, p.d);
+    const bool avec = ((uintptr_t)a & 15) == 0, vec = rows_vec(b, bc_dtype, HD, p.d) && rows_vec(c, bc_dtype, HD, p.d);
 #define SP_LAUNCH(DSV) { if (trans ? launch_spmm<BS, DSV, AD, BD, true>(s, lut, a, b, c, p, avec, vec) : launch_spmm<BS, DSV, AD, BD, false>(s, lut, a, b, c, p, avec, vec)) return 1; }
     DISPATCH_BS(bs, DISPATCH_DT(a_dtype, AD, DISPATCH_DT(bc_dtype, BD, {
         if (p.d <= 32) SP_LAUNCH(32) else if (p.d <= 64) SP_LAUNCH(64) else SP_LAUNCH(128)

@@ -228,6 +228,38 @@ def test_one_tensor_as_q_k_and_v(sfb):
         assert torch.equal(y, z)
 
 
+@pytest.mark.parametrize("dtype", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("bs,d", [(32, 8), (32, 72), (32, 96), (32, 100), (32, 126), (32, 128), (64, 16), (64, 48), (64, 96), (64, 104), (64, 127)])
+def test_widths_of_the_general_path(sfb, bs, d, dtype):
+    """Head sizes in every number of 32 columns, whole and not, with rows that can be read 16 bytes at a time and ones that cannot."""
+    check_attention(sfb, layout("long", 5), bs, 2, 3, d, dtype, seed=d)
+    at = torch.arange(5 * bs)
+    check_attention(sfb, layout("causal", 5), bs, 1, 2, d, dtype, keep=(at[:, None] >= at[None, :])[None], packed=True, seed=d)
+
+
+@pytest.mark.parametrize("bs,d", [(32, 40), (64, 128)])
+def test_fp32_operands_whose_first_bf16_number_is_infinite(sfb, bs, d):
+    """The largest fp32 number rounds to infinity in bf16: products of terms are NaN, the sum is not."""
+    nb, big = 3, 3.4e38
+    q, k, v, do = operands(1, nb * bs, 1, d, "f32", 4)
+    do = do * 0
+    do[0, 5, 0, 1], do[0, bs + 3, 0, 2], v = big, -big, v * 0
+    blocks = layout("full", nb)
+    lay = plan(sfb, blocks, bs)
+    cuda = [x.cuda() for x in (q, k, v, do)]
+    o, lse = sfb.fused_attention_stats(*cuda[:3], lay)
+    dq, dk, dv = sfb.attention_backward_recompute(*cuda[:3], o, cuda[3], lse, lay)
+    assert (dq == 0).all() and (dk == 0).all()
+    scale = 1 / math.sqrt(d)
+    want = attend_grad(q, k, v, o.cpu(), do, lse.cpu(), torch.ones(1, nb * bs, nb * bs, dtype=torch.bool), scale)[0][2]
+    qk = float(torch.einsum("blhd,bmhd->bhlm", q.double().abs(), k.double().abs()).max())
+    top = float(lse.abs().max())
+    # P as in grad_tolerance; a sum of one product, rounded
+    e = 2.0 ** -23 * (scale * qk * (2 + d / 16) + 2 * top + 4) + 2.0 ** -22 + 2.0 ** -23
+    assert torch.isfinite(dv).all()
+    assert ((dv.cpu().double() - want).abs() <= e * want.abs() + 1e-30).all()
+
+
 def test_a_layout_of_no_blocks_but_one(sfb):
     blocks = np.zeros((1, 6, 6), np.uint8)
     blocks[0, 3, 2] = 1
