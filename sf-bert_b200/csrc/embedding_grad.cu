@@ -246,11 +246,13 @@ __device__ __forceinline__ void write_sums(void *out, size_t at, const float (&s
 }
 
 // A warp takes `piece` sorted tokens and 32 lanes' columns.  The first CTAs do this, the others write the rows of
-// tokens that do not occur (in turn, one of each kind: 70 -> 72 us).
+// tokens that do not occur (in turn, one of each kind: 70 -> 72 us).  Four tokens' loads are on their way together: what ends a run stands there as
+// often, and with eight of them registers and code made the whole call slower (32768 x 1024 fp16 58 -> 45 us).  fp32 writes zeros here: five CTAs per
+// SM (320 tokens 26.4 -> 23.3; 16-bit types spill then, 53 -> 62).
 template <int DT, int GT>
-__global__ void __launch_bounds__(256) table_grad_kernel(const GradArgs a)
+__global__ void __launch_bounds__(256, DT == SFB_F32 ? 5 : 1) table_grad_kernel(const GradArgs a)
 {
-    constexpr int N = Piece<DT>::N, U = 8;
+    constexpr int N = Piece<DT>::N, U = 4;
     grid_dependency_wait();
     grid_launch_dependents();
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -435,10 +437,16 @@ __global__ void __launch_bounds__(kSortThreads) sort_and_positions_kernel(const 
     }
 }
 
-// sorted tokens per piece: short enough for a long run to spread, long enough for its parts to be few
-static uint32_t piece_length(uint32_t n) { return n <= (1u << 16) ? 32u : 128u; }
+// Sorted tokens per piece: as many as leave 3000 warps with 32 lanes' columns of a piece each, so that long runs have few parts (us, pieces of 8 / 16 /
+// 32 / 64 tokens: 32768 x 1024 fp16 55 / 49 / 45, 8192 x 512 fp32 17.6 / 19.3 / 21.8); from 8 to 64 (262144 x 768 fp16, 32 / 64 / 128: 245 / 240 / 257).
+static uint32_t piece_length(uint32_t n, uint32_t hidden)
+{
+    uint32_t len = 64;
+    while (len > 8 && (uint64_t)n / len * ((hidden + 255) / 256) < 3000) len /= 2;
+    return len;
+}
 static uint64_t padded(uint64_t bytes) { return (bytes + 63) / 64 * 64; }
-static uint32_t piece_count(uint32_t n) { return (uint32_t)(((uint64_t)n + piece_length(n) - 1) / piece_length(n)); }
+static uint32_t piece_count(uint32_t n, uint32_t hidden) { return (uint32_t)(((uint64_t)n + piece_length(n, hidden) - 1) / piece_length(n, hidden)); }
 
 template <int DT, int GT>
 static int launch(cudaStream_t s, GradArgs a)
@@ -458,8 +466,8 @@ static int launch(cudaStream_t s, GradArgs a)
         pos_ctas = groups * ((a.len + kSortWarps / a.ways - 1) / (kSortWarps / a.ways));
     }
     // The rows of tokens that do not occur: all rows are zeroed beside the sorting, and those of tokens that do occur are written again (bf16, fp32
-    // gradients, 30522 x 768: 1024 tokens 31 us, 32768 55; zeroed after the sorting, by its counts, 43 and 60).  Few tokens, whose sorting is over
-    // soon, where a lane's zeros are 16 bytes: by the counts (fp32, 320 tokens 25 us, zeroed beside 28).
+    // gradients, 30522 x 768: 1024 tokens 31 us, 32768 53; zeroed after the sorting, by its counts, 43 and 60).  Few tokens, whose sorting is over
+    // soon, where a lane's zeros are 16 bytes: by the counts (fp32, 320 tokens 23 us, zeroed beside 28).
     constexpr bool narrow = sizeof(typename Elem<GT>::type) * N == 16;
     if (!a.accumulate && (!narrow || a.n >= kFewTokens)) fillers = ((uint64_t)a.vocab * a.hidden * sizeof(typename Elem<GT>::type) / 16 + kFill - 1) / kFill;
     SFB_REQUIRE(a.sorters + pos_ctas + fillers < (1ull << 31), "sfb_embedding_grad: too many rows for one launch");
@@ -490,7 +498,7 @@ extern "C" uint64_t sfb_embedding_grad_workspace(uint32_t batch, uint32_t seq_le
     using namespace emb;
     const uint64_t n = (uint64_t)batch * seq_len;
     if (n >= (1ull << 31)) return 0;
-    return 2 * padded(n * 8) + padded(((uint64_t)vocab + 1) * 4) + (uint64_t)piece_count((uint32_t)n) * 2 * hidden * 4;
+    return 2 * padded(n * 8) + padded(((uint64_t)vocab + 1) * 4) + (uint64_t)piece_count((uint32_t)n, hidden) * 2 * hidden * 4;
 }
 
 extern "C" int sfb_embedding_grad(sfb_stream_t stream, void *dtable, void *dpos, const void *dout, const int32_t *ids, uint32_t batch,
@@ -517,7 +525,7 @@ extern "C" int sfb_embedding_grad(sfb_stream_t stream, void *dtable, void *dpos,
         clear_error();
         return 0;
     }
-    GradArgs a = {dout, ids, dtable, dpos, (uint32_t)n, batch, seq_len, hidden, vocab, 0, 0, 0, 0, 1, piece_length((uint32_t)n), piece_count((uint32_t)n), scale, accumulate, bad_ids};
+    GradArgs a = {dout, ids, dtable, dpos, (uint32_t)n, batch, seq_len, hidden, vocab, 0, 0, 0, 0, 1, piece_length((uint32_t)n, hidden), piece_count((uint32_t)n, hidden), scale, accumulate, bad_ids};
     // a CTA per SM sorts, more where its counters would not fit
     const int sms = device_sm_count(current_device());
     const uint32_t ctas = max((uint32_t)(sms > 0 ? sms : 1), (vocab + kMaxRange - 1) / kMaxRange);
