@@ -346,7 +346,7 @@ def test_long_rows_of_many_blocks(sfb):
     assert sfb.device_status() == 0
 
 
-@pytest.mark.parametrize("B,H,heads", [(3, 40, 1), (2, 100, 1), (1, 130, 130)])
+@pytest.mark.parametrize("B,H,heads", [(3, 40, 1), (2, 100, 1), (1, 130, 130), (5, 40, 1), (7, 43, 1), (1, 310, 310)])
 def test_more_heads_than_go_through_the_workspace_at_once(sfb, B, H, heads):
     """Whole batch elements at a time, and some heads of one: the same bits as calls for a few heads each, in place."""
     bs, nb, d = 32, 64, 8
@@ -363,6 +363,28 @@ def test_more_heads_than_go_through_the_workspace_at_once(sfb, B, H, heads):
         got = sfb.attention_backward_recompute(*cut, lse[:, h0:h1].contiguous(), part)
         for a, b in zip(got, whole):
             assert torch.equal(a, b[:, :, h0:h1])
+
+
+@pytest.mark.parametrize("flip", [False, True])
+@pytest.mark.parametrize("nb", [2, 13, 33, 64])
+def test_heads_in_groups(sfb, nb, flip):
+    """Rows that grow from one end to the other: the same bits as calls for one batch element or a few heads, whichever group they are in."""
+    B, H, bs, d = 3, 61, 64, 64
+    blocks = np.ascontiguousarray(layout("causal", nb)[:, ::-1, ::-1] if flip else layout("causal", nb))
+    if nb == 64:
+        B, H = 2, 23
+    q, k, v, do = (x.cuda() for x in operands(B, nb * bs, H, d, "bf16", 14))
+    lay = plan(sfb, blocks, bs)
+    o, lse = sfb.fused_attention_stats(q, k, v, lay)
+    whole = sfb.attention_backward_recompute(q, k, v, o, do, lse, lay)
+    for b in range(B):
+        for h0 in range(0, H, 7):
+            h1 = min(H, h0 + 7)
+            cut = [x[b:b + 1, :, h0:h1] for x in (q, k, v, o, do)]
+            got = sfb.attention_backward_recompute(*cut, lse[b:b + 1, h0:h1].contiguous(), lay)
+            for x, y in zip(got, whole):
+                assert torch.equal(x, y[b:b + 1, :, h0:h1])
+    assert sfb.device_status() == 0
 
 
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
