@@ -5,9 +5,9 @@
 // Three launches.  (1) sort_and_positions_kernel: some CTAs bring the tokens into the order of their ids, equal ids by position, while the others
 // add up the batch, reading dout in order.  (2) table_grad_kernel walks the sorted tokens in pieces of equal length, so that a word that
 // is a tenth of the text does not hang on one CTA; a run of equal ids that lies in one piece is written at once, the parts of
-// one that does not go to the workspace.  The rows of tokens that do not occur are zeros from the first launch (or the second, for few tokens).
+// one that does not go to the workspace.  The rows of tokens that do not occur are zeros from the first launch.
 // (3) join_kernel adds up the parts.  Bound by memory: dout is read by (1) and gathered by (2), from L2 where it fits, and the table's
-// gradient is written once (a fill runs at 3.8 TB/s on this part, where a copy runs at 6.5).
+// gradient is written once.  Few tokens: one launch (few_tokens_kernel).
 #include "common.cuh"
 
 namespace sfb {
@@ -17,7 +17,7 @@ constexpr uint32_t kSortThreads = 512, kSortWarps = kSortThreads / 32;
 constexpr uint32_t kStride = kSortWarps + 1;         // counters per id: neighbouring ids in different banks
 constexpr uint32_t kNear = 2048;                     // tokens of a CTA that it keeps in shared memory
 constexpr uint32_t kFill = 8192;                     // 16-byte pieces of zeros per CTA
-constexpr uint32_t kFewTokens = 2048;
+constexpr uint32_t kFew = 2048, kFewCtas = 2560;     // tokens, and CTAs for them, up to which one launch makes everything
 constexpr uint32_t kMaxRange = 1024;                 // ids that one CTA sorts
 
 struct GradArgs {
@@ -245,10 +245,9 @@ __device__ __forceinline__ void write_sums(void *out, size_t at, const float (&s
     }
 }
 
-// A warp takes `piece` sorted tokens and 32 lanes' columns.  The first CTAs do this, the others write the rows of
-// tokens that do not occur (in turn, one of each kind: 70 -> 72 us).  Four tokens' loads are on their way together: what ends a run stands there as
-// often, and with eight of them registers and code made the whole call slower (32768 x 1024 fp16 58 -> 45 us).  fp32 writes zeros here: five CTAs per
-// SM (320 tokens 26.4 -> 23.3; 16-bit types spill then, 53 -> 62).
+// A warp takes `piece` sorted tokens and 32 lanes' columns.  Four tokens' loads are on their way together: what ends a run stands there as
+// often, and with eight of them registers and code made the whole call slower (32768 x 1024 fp16 58 -> 45 us).  fp32: five CTAs per
+// SM (32768 x 768 76 -> 65; 16-bit types spill then, 53 -> 62).
 template <int DT, int GT>
 __global__ void __launch_bounds__(256, DT == SFB_F32 ? 5 : 1) table_grad_kernel(const GradArgs a)
 {
@@ -258,19 +257,7 @@ __global__ void __launch_bounds__(256, DT == SFB_F32 ? 5 : 1) table_grad_kernel(
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t groups = (a.hidden / N + 31) / 32, y = blockIdx.x / groups, col = ((blockIdx.x - y * groups) * 32 + lane) * N;
     const bool live = col < a.hidden;
-    const uint32_t piece_ctas = (a.pieces + 7) / 8;
-    const bool zeros = y >= piece_ctas;
-    const uint32_t at = zeros ? y - piece_ctas : y;
-    if (zeros) {
-        const uint32_t v0 = (at * 8 + warp) * 32;
-        const bool empty = v0 + lane < a.vocab && a.starts[v0 + lane] == a.starts[v0 + lane + 1];
-        uint32_t todo = __ballot_sync(0xffffffffu, empty);
-        const float none[N] = {};
-        for (; todo; todo &= todo - 1)
-            if (live) write_sums<GT, N>(a.dtable, (size_t)(v0 + __ffs(todo) - 1) * a.hidden + col, none, 1.f, false);
-        return;
-    }
-    const uint32_t c = at * 8 + warp, total = a.starts[a.vocab];
+    const uint32_t c = y * 8 + warp, total = a.starts[a.vocab];
     const uint32_t i0 = c * a.piece, i1 = min(total, i0 + a.piece);
     if (i0 >= total) return;
     const int before = i0 ? a.sorted[i0 - 1].y : -1, after = i1 < total ? a.sorted[i1].y : -1;
@@ -437,6 +424,105 @@ __global__ void __launch_bounds__(kSortThreads) sort_and_positions_kernel(const 
     }
 }
 
+// ---- few tokens: one launch ------------------------------------------------------------------------------------------------------------
+// A CTA per token and 32 lanes' columns: where an earlier token has the same id there is nothing to do, otherwise its warps look for the id among
+// shares of the tokens from there on and add up what they find, and their sums meet in shared memory.  Beside them the positions' sums, and CTAs that
+// write zeros to ranges of rows, all but those whose id they find among the tokens.  Every CTA reads all ids, 4 bytes each from L2.
+template <int DT, int GT>
+__global__ void __launch_bounds__(kSortThreads) few_tokens_kernel(const GradArgs a, uint32_t token_ctas, uint32_t rows)
+{
+    constexpr int N = Piece<DT>::N, U = 8;
+    extern __shared__ __align__(16) uint32_t dynamic[];
+    __shared__ uint32_t any[kSortWarps];
+    grid_dependency_wait();
+    grid_launch_dependents();
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (blockIdx.x >= token_ctas) {
+        const uint32_t y = blockIdx.x - token_ctas, both = 2 * min(a.pos_ctas, a.fillers), at = y < both ? y >> 1 : y - both / 2;
+        if (!(y < both ? y & 1 : a.fillers > a.pos_ctas)) {
+            add_positions<DT, GT>(a, at, (float *)dynamic);
+            return;
+        }
+        uint8_t *found = (uint8_t *)dynamic;
+        const uint32_t v0 = at * rows, n = min(rows, a.vocab - v0), per = (uint32_t)(a.hidden * sizeof(typename Elem<GT>::type) / 16);      // 16-byte pieces per row
+        for (uint32_t i = threadIdx.x; i < n; i += kSortThreads) found[i] = 0;
+        __syncthreads();
+        int here = 0;
+        for (uint32_t i = threadIdx.x; i < a.n; i += kSortThreads) {
+            const uint32_t v = (uint32_t)__ldg(a.ids + i) - v0;
+            if (v < n) {
+                found[v] = 1;
+                here = 1;
+            }
+        }
+        here = __syncthreads_or(here);
+        uint4 *out = (uint4 *)a.dtable + (size_t)v0 * per;
+        const uint32_t pieces = n * per;
+        if (!here) {
+#pragma unroll 8
+            for (uint32_t i = threadIdx.x; i < pieces; i += kSortThreads) __stcs(out + i, make_uint4(0u, 0u, 0u, 0u));
+        } else {
+            uint32_t r = threadIdx.x / per, c = threadIdx.x % per;
+            const uint32_t dr = kSortThreads / per, dc = kSortThreads % per;
+            for (uint32_t i = threadIdx.x; i < pieces; i += kSortThreads) {
+                if (!found[r]) __stcs(out + i, make_uint4(0u, 0u, 0u, 0u));
+                r += dr;
+                c += dc;
+                if (c >= per) {
+                    c -= per;
+                    r++;
+                }
+            }
+        }
+        return;
+    }
+    const uint32_t groups = (a.hidden / N + 31) / 32, t = blockIdx.x / groups, col = ((blockIdx.x - t * groups) * 32 + lane) * N;
+    const bool live = col < a.hidden;
+    const int32_t id = __ldg(a.ids + t);
+    if (blockIdx.x == 0 && a.bad) {
+        uint32_t bad = 0;
+        for (uint32_t i0 = 0; i0 < a.n; i0 += kSortThreads) bad += __syncthreads_count(i0 + threadIdx.x < a.n && (uint32_t)__ldg(a.ids + min(i0 + threadIdx.x, a.n - 1)) >= a.vocab);
+        if (threadIdx.x == 0) *a.bad = bad;
+    }
+    if ((uint32_t)id >= a.vocab) return;
+    int earlier = 0;
+    for (uint32_t i = threadIdx.x; i < t; i += kSortThreads) earlier |= __ldg(a.ids + i) == id;
+    if (__syncthreads_or(earlier)) return;
+    const uint32_t share = ((a.n - t + kSortWarps - 1) / kSortWarps + 31) / 32 * 32, i0 = min(a.n, t + warp * share), i1 = min(a.n, i0 + share);
+    float s[N] = {};
+    uint32_t mine = 0;
+    for (uint32_t i = i0; i < i1; i += 32) {
+        uint32_t todo = __ballot_sync(0xffffffffu, i + lane < i1 && __ldg(a.ids + min(i + lane, a.n - 1)) == id);
+        mine |= todo;
+        while (todo) {
+            uint4 u[U];
+#pragma unroll
+            for (int k = 0; k < U; k++) {
+                u[k] = make_uint4(0u, 0u, 0u, 0u);
+                if (todo) {
+                    if (live) u[k] = __ldg((const uint4 *)((const typename Elem<DT>::type *)a.dout + (size_t)(i + __ffs(todo) - 1) * a.hidden + col));
+                    todo &= todo - 1;
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < U; k++) Piece<DT>::add(s, u[k]);
+        }
+    }
+    float *part = (float *)dynamic;                          // [warp][N][33]
+    if (mine && warp) {
+#pragma unroll
+        for (int i = 0; i < N; i++) part[(warp * N + i) * 33 + lane] = s[i];
+    }
+    if (lane == 0) any[warp] = mine;
+    __syncthreads();
+    if (warp) return;
+    for (uint32_t w = 1; w < kSortWarps; w++)
+        if (any[w])
+#pragma unroll
+            for (int i = 0; i < N; i++) s[i] += part[(w * N + i) * 33 + lane];
+    if (live) write_sums<GT, N>(a.dtable, (size_t)id * a.hidden + col, s, a.scale, a.accumulate);
+}
+
 // Sorted tokens per piece: as many as leave 3000 warps with 32 lanes' columns of a piece each, so that long runs have few parts (us, pieces of 8 / 16 /
 // 32 / 64 tokens: 32768 x 1024 fp16 55 / 49 / 45, 8192 x 512 fp32 17.6 / 19.3 / 21.8); from 8 to 64 (262144 x 768 fp16, 32 / 64 / 128: 245 / 240 / 257).
 static uint32_t piece_length(uint32_t n, uint32_t hidden)
@@ -455,7 +541,7 @@ static int launch(cudaStream_t s, GradArgs a)
     if (sms <= 0) return fail("sfb_embedding_grad: cannot query the device");
     constexpr uint32_t N = Piece<DT>::N;
     const uint64_t groups = (a.hidden / N + 31) / 32;
-    SFB_REQUIRE(groups * a.len < (1ull << 31) && groups * ((a.pieces + 7) / 8 + ((uint64_t)a.vocab + 255) / 256) < (1ull << 31) && (uint64_t)((a.hidden / 4 + 31) / 32) * a.pieces < (1ull << 31),
+    SFB_REQUIRE(groups * a.len < (1ull << 31) && groups * ((a.pieces + 7) / 8) < (1ull << 31) && (uint64_t)((a.hidden / 4 + 31) / 32) * a.pieces < (1ull << 31),
                 "sfb_embedding_grad: too many rows for one launch");
     // positions enough to fill the SMs: a warp each; otherwise several share the batch of one
     uint64_t pos_ctas = 0, fillers = 0;
@@ -465,15 +551,26 @@ static int launch(cudaStream_t s, GradArgs a)
         while (a.ways < kSortWarps && warps * a.ways < want && a.batch >= 16 * a.ways) a.ways *= 2;
         pos_ctas = groups * ((a.len + kSortWarps / a.ways - 1) / (kSortWarps / a.ways));
     }
-    // The rows of tokens that do not occur: all rows are zeroed beside the sorting, and those of tokens that do occur are written again (bf16, fp32
-    // gradients, 30522 x 768: 1024 tokens 31 us, 32768 53; zeroed after the sorting, by its counts, 43 and 60).  Few tokens, whose sorting is over
-    // soon, where a lane's zeros are 16 bytes: by the counts (fp32, 320 tokens 23 us, zeroed beside 28).
-    constexpr bool narrow = sizeof(typename Elem<GT>::type) * N == 16;
-    if (!a.accumulate && (!narrow || a.n >= kFewTokens)) fillers = ((uint64_t)a.vocab * a.hidden * sizeof(typename Elem<GT>::type) / 16 + kFill - 1) / kFill;
+    // Few tokens (graphs of calls, us, three launches / one: 64 tokens x 256 bf16, vocabulary 1000 11.3 / 4.0, 2048 tokens 14.9 / 9.0; 320 x 768 fp32, 30522
+    // 22.3 / 20.2, 768 25.2 / 28.2; 512 x 2048 fp16 10.8 / 9.9, 768 11.5 / 13.9).
+    if (a.n <= kFew && groups * a.n <= kFewCtas) {
+        const uint64_t row = (uint64_t)a.hidden * sizeof(typename Elem<GT>::type);
+        const uint32_t rows = (uint32_t)(row < 16 * kFill ? 16 * kFill / row : 1);
+        a.fillers = a.accumulate ? 0 : (a.vocab + rows - 1) / rows;
+        a.pos_ctas = (uint32_t)pos_ctas;
+        const uint64_t ctas = groups * a.n + pos_ctas + a.fillers;
+        SFB_REQUIRE(ctas < (1ull << 31), "sfb_embedding_grad: too many rows for one launch");
+        const size_t sums = sizeof(float) * kSortWarps * N * 33;
+        launch_overlapped(few_tokens_kernel<DT, GT>, dim3((unsigned)ctas), dim3(kSortThreads), rows > sums ? rows : sums, s, a, (uint32_t)(groups * a.n), rows);
+        return check_launch("sfb_embedding_grad");
+    }
+    // All rows are zeroed beside the sorting, and those of tokens that do occur are written again (30522 x 768, us: zeroed after the sorting, by its
+    // counts, bf16 1024 tokens 43, 32768 60, fp32 1024 tokens 28; beside it 31, 53 and 24).
+    if (!a.accumulate) fillers = ((uint64_t)a.vocab * a.hidden * sizeof(typename Elem<GT>::type) / 16 + kFill - 1) / kFill;
     SFB_REQUIRE(a.sorters + pos_ctas + fillers < (1ull << 31), "sfb_embedding_grad: too many rows for one launch");
     a.pos_ctas = (uint32_t)pos_ctas;
     a.fillers = (uint32_t)fillers;
-    const uint64_t rows = (a.pieces + 7) / 8 + (fillers || a.accumulate ? 0 : ((uint64_t)a.vocab + 255) / 256);
+    const uint64_t rows = (a.pieces + 7) / 8;
     size_t smem = (size_t)a.range * kStride * 4;
     if (a.dpos && a.ways > 1 && smem < sizeof(float) * kSortWarps * N * 33) smem = sizeof(float) * kSortWarps * N * 33;
     static DeviceOnce once;

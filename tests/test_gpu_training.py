@@ -444,7 +444,8 @@ def check_embed_grad(sfb, dout, ids, vocab, scale=1.0, grad="f32", positions=Tru
             continue
         if start:
             w, s = w + start[k], s + start[k].abs()
-        # each of the additions rounds in fp32: at most a share of 2^-24 of the magnitudes per level, pieces of 128 at most and their parts in turn
+        # each of the additions rounds in fp32: at most a share of 2^-24 of the magnitudes per level.  A piece has up to 64 tokens (few tokens: a warp up to
+        # 128), 16 parts are added up in turn or by eight warps; of a run of very many parts the roundings' signs differ, and less is allowed than their worst
         tol = half_step(g) * w.abs() + 2.0 ** -24 * (128 + ids.numel() / 128 / 8 + 16) * s + (2.0 ** -25 if g == torch.float16 else 0)
         off = (got.cpu().double() - w).abs()
         assert (off <= tol).all(), float((off / (tol + 1e-300)).max())
@@ -478,6 +479,22 @@ def test_runs_of_ids(sfb, what):
                "beyond": torch.where(torch.arange(n) % 3 == 0, 2 ** 31 - 1, -2 ** 31)}[what].to(torch.int32).view(B, L)
         dout = torch.randn(B, L, hidden, generator=g)
         check_embed_grad(sfb, dout.bfloat16() if B == 7 else dout, ids, vocab)
+
+
+@pytest.mark.parametrize("B,L,vocab,hidden,dtype", [(1, 2048, 700, 256, "bf16"), (1, 2049, 700, 256, "bf16"), (2, 213, 3000, 768, "f32"), (2, 214, 3000, 768, "f32"),
+                                                     (1, 100, 200000, 8, "f16"), (5, 64, 9000, 2048, "f16"), (40, 16, 63, 64, "f32"), (300, 1, 77, 520, "bf16")])
+@pytest.mark.parametrize("what", ["any", "one id", "last rows", "all missing"])
+def test_few_tokens(sfb, B, L, vocab, hidden, dtype, what):
+    """Numbers of tokens on both sides of what one launch takes, new gradients and added ones."""
+    g = torch.Generator().manual_seed(B * L)
+    ids = {"any": torch.randint(-1, vocab + 1, (B, L), generator=g), "one id": torch.full((B, L), vocab // 2), "last rows": vocab - 1 - torch.randint(0, 3, (B, L), generator=g),
+           "all missing": torch.full((B, L), vocab)}[what].to(torch.int32)
+    dout = torch.randn(B, L, hidden, generator=g).to(DTYPES[dtype])
+    for grad in ("f32", None):
+        check_embed_grad(sfb, dout, ids, vocab, -1.5, grad)
+        t = torch.float32 if grad else DTYPES[dtype]
+        out = [torch.randn(vocab, hidden, generator=g).to(t).cuda(), torch.randn(L, hidden, generator=g).to(t).cuda()]
+        check_embed_grad(sfb, dout, ids, vocab, -1.5, grad, out=out)
 
 
 @pytest.mark.parametrize("dtype,grad", [("f32", "f32"), ("bf16", "f32"), ("f16", None), ("bf16", None)])
