@@ -287,11 +287,12 @@ def test_infinities_outside_the_kept_blocks(sfb):
             assert torch.equal(a, b)
 
 
-def test_streams_graphs_and_two_calls_at_once(sfb):
-    bs, nb, d = 64, 8, 64
+@pytest.mark.parametrize("bs,d,dtype", [(64, 64, "f16"), (32, 40, "bf16"), (64, 128, "f16"), (32, 64, "f32")])
+def test_streams_graphs_and_two_calls_at_once(sfb, bs, d, dtype):
+    nb = 8
     lay = plan(sfb, layout("stride", nb), bs)
     lay.tn_lut
-    sets = [[x.cuda() for x in operands(2, nb * bs, 4, d, "f16", 10 + i)] for i in range(2)]
+    sets = [[x.cuda() for x in operands(2, nb * bs, 4, d, dtype, 10 + i)] for i in range(2)]
 
     def step(q, k, v, do):
         o, lse = sfb.fused_attention_stats(q, k, v, lay)
@@ -527,6 +528,25 @@ def test_embedding_grad_of_rows_that_are_not_finite(sfb):
     rest = [i for i in range(20) if i not in (3, 19)]
     assert (dtable[rest] == 4).all() and (dtable[20:] == 0).all()
     assert dpos[3].isnan().all() and (dpos[39] == math.inf).all() and (dpos[[i for i in range(40) if i not in (3, 39)]] == 2).all()
+
+
+def test_few_tokens_in_graphs(sfb):
+    """The one-launch form captured and replayed with other ids and other gradients in place."""
+    vocab, hidden = 500, 96
+    dout = torch.zeros(3, 20, hidden, dtype=torch.bfloat16, device="cuda")
+    ids = torch.zeros(3, 20, dtype=torch.int32, device="cuda")
+    sfb.embedding_grad(dout, ids, vocab, 2.0, True)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        dtable, dpos, bad = sfb.embedding_grad(dout, ids, vocab, 2.0, True)
+    for seed in range(3):
+        gen = torch.Generator().manual_seed(seed)
+        dout.copy_(torch.randn(3, 20, hidden, generator=gen).bfloat16())
+        ids.copy_(torch.randint(-1, vocab, (3, 20), generator=gen, dtype=torch.int32))
+        g.replay()
+        for a, b in zip((dtable, dpos, bad), sfb.embedding_grad(dout, ids, vocab, 2.0, True)):
+            assert torch.equal(a, b)
+        check_embed_grad(sfb, dout.cpu(), ids.cpu(), vocab, 2.0)
 
 
 # ---- norm and clipping ------------------------------------------------------------------------------------------------------------
