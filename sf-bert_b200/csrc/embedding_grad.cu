@@ -427,11 +427,14 @@ __global__ void __launch_bounds__(kSortThreads) sort_and_positions_kernel(const 
 // ---- few tokens: one launch ------------------------------------------------------------------------------------------------------------
 // A CTA per token and 32 lanes' columns: where an earlier token has the same id there is nothing to do, otherwise its warps look for the id among
 // shares of the tokens from there on and add up what they find, and their sums meet in shared memory.  Beside them the positions' sums, and CTAs that
-// write zeros to ranges of rows, all but those whose id they find among the tokens.  Every CTA reads all ids, 4 bytes each from L2.
+// write zeros to ranges of rows, all but those whose id they find among the tokens.  Every CTA reads all ids, 4 bytes each from L2.  Most CTAs only find
+// that they have nothing to do, so as many as possible are on an SM: 32 registers and two tokens' loads at once (us, 52 registers and eight / 32 and four
+// / 32 and two: 320 tokens x 768 fp32 22.6 / 19.4 / 19.2, 320 x 2048 fp16 9.5 / 7.1 / 6.6; 320 times the same id 6.4 / 7.1 / 7.7).  Zeros and tokens
+// in turn instead of the tokens first: 24.7.
 template <int DT, int GT>
-__global__ void __launch_bounds__(kSortThreads) few_tokens_kernel(const GradArgs a, uint32_t token_ctas, uint32_t rows)
+__global__ void __launch_bounds__(kSortThreads, 4) few_tokens_kernel(const GradArgs a, uint32_t token_ctas, uint32_t rows)
 {
-    constexpr int N = Piece<DT>::N, U = 8;
+    constexpr int N = Piece<DT>::N, U = 2;
     extern __shared__ __align__(16) uint32_t dynamic[];
     __shared__ uint32_t any[kSortWarps];
     grid_dependency_wait();
@@ -551,8 +554,8 @@ static int launch(cudaStream_t s, GradArgs a)
         while (a.ways < kSortWarps && warps * a.ways < want && a.batch >= 16 * a.ways) a.ways *= 2;
         pos_ctas = groups * ((a.len + kSortWarps / a.ways - 1) / (kSortWarps / a.ways));
     }
-    // Few tokens (graphs of calls, us, three launches / one: 64 tokens x 256 bf16, vocabulary 1000 11.3 / 4.0, 2048 tokens 14.9 / 9.0; 320 x 768 fp32, 30522
-    // 22.3 / 20.2, 768 25.2 / 28.2; 512 x 2048 fp16 10.8 / 9.9, 768 11.5 / 13.9).
+    // Few tokens (graphs of calls, us, three launches / one: 64 tokens x 256 bf16, vocabulary 1000 11.3 / 4.0, 2048 tokens 14.9 / 8.4; 426 x 768 fp32, 30522
+    // 22.0 / 20.7; 426 x 2048 fp16, 3408 CTAs 10.7 / 10.2 with eight loads at once; 768 x 768 fp32, 4608 CTAs 23 / 28).
     if (a.n <= kFew && groups * a.n <= kFewCtas) {
         const uint64_t row = (uint64_t)a.hidden * sizeof(typename Elem<GT>::type);
         const uint32_t rows = (uint32_t)(row < 16 * kFill ? 16 * kFill / row : 1);
