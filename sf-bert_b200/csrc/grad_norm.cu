@@ -167,9 +167,18 @@ template <int GT> __device__ __forceinline__ void put(void *out, uint64_t i, flo
     else if constexpr (GT == SFB_BF16) ((__nv_bfloat16 *)out)[i] = __float2bfloat16_rn(v);
     else ((__half *)out)[i] = __float2half_rn(v);
 }
-template <int GT, int N> __device__ __forceinline__ void put_vec(void *out, uint64_t i, const float (&v)[N])
+// wide: 32-byte pieces of fp32 results at their boundaries, one store (as two, each covers half of every sector)
+template <int GT, int N> __device__ __forceinline__ void put_vec(void *out, uint64_t i, const float (&v)[N], bool wide)
 {
     if constexpr (GT == SFB_F32) {
+        if constexpr (N == 8) {
+            if (wide) {
+                asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"((float *)out + i), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]),
+                             "f"(v[6]), "f"(v[7])
+                             : "memory");
+                return;
+            }
+        }
 #pragma unroll
         for (int j = 0; j < N; j += 4) __stcs((float4 *)((float *)out + i + j), make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]));
     } else {
@@ -202,14 +211,24 @@ __device__ __forceinline__ void chunk_scale(const void *in, void *out, uint64_t 
         if (begin + threadIdx.x < body) put<GT>(out, begin + threadIdx.x, widen<DT>(p[begin + threadIdx.x]) * factor);
         if (tail + threadIdx.x < end) put<GT>(out, tail + threadIdx.x, widen<DT>(p[tail + threadIdx.x]) * factor);
         const uint4 *q = (const uint4 *)(p + body);
-#pragma unroll 4
-        for (uint32_t i = threadIdx.x; i < pieces; i += kThreads) {
+        const bool wide = (((uintptr_t)out + body * G) & 31) == 0;
+        auto scale_piece = [&](uint32_t i, const uint4 &u) {
             float v[N];
-            Vec<DT>::decode(v, q[i]);
+            Vec<DT>::decode(v, u);
 #pragma unroll
             for (int j = 0; j < N; j++) v[j] *= factor;
-            put_vec<GT>(out, body + (uint64_t)i * N, v);
+            put_vec<GT>(out, body + (uint64_t)i * N, v, wide);
+        };
+        // the results may lie where the gradients do: what is on its way together has to be asked for before the first of it is written
+        uint32_t i = threadIdx.x;
+        for (; i + 3 * kThreads < pieces; i += 4 * kThreads) {
+            uint4 u[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++) u[k] = q[i + k * kThreads];
+#pragma unroll
+            for (int k = 0; k < 4; k++) scale_piece(i + k * kThreads, u[k]);
         }
+        for (; i < pieces; i += kThreads) scale_piece(i, q[i]);
     } else {
         uint64_t i = begin + threadIdx.x;
         for (; i + (kAhead - 1) * kThreads < end; i += kAhead * kThreads) {
