@@ -242,6 +242,7 @@ __device__ __forceinline__ void chunk_scale(const void *in, void *out, uint64_t 
     }
 }
 
+// 334 M fp16 gradients into fp32: 345 us, 2.0 GB at 5.8 TB/s (with one load at a time and two stores per 32 bytes 352; eight loads 355).
 // max_norm: infinity where only the norm is wanted.  parts: how many numbers the launches before left.
 template <uint32_t M>
 __global__ void __launch_bounds__(kThreads) clip_kernel(const __grid_constant__ List<M> l, const double *sums, uint32_t parts, float *norm_out, float max_norm, float scale,
