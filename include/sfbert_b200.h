@@ -225,7 +225,9 @@ int sfb_fused_attention_stats(sfb_stream_t stream, const void *nn_lut, const voi
  * All types, block sizes and head sizes (at most 128) of the forward call; mask, mask_heads and scale as there.  nt_lut, nn_lut and tn_lut
  * are the layout's three tables, lut_dim the nt_lut's stride (`blocks`; the others': blocks + ctx_blks), nn_max and tn_max the longest row
  * and column (0: unknown).  Rows (columns) that keep nothing get zeros.  P and dS are operands of the products in the type of q: with
- * 16-bit types each entry is rounded once.  Every sum has a fixed order: the same inputs give the same bits.
+ * 16-bit types each entry is rounded once, dS before it is multiplied by a scale of at most 1 in magnitude, which dQ and dK then are, in fp32:
+ * in fp16 P * (dO.V^T - rowsum(dO * O)) keeps its bits down to 2^-14 and is infinite from 65520 on.
+ * Every sum has a fixed order: the same inputs give the same bits.
  * q, k, v (in_pitch), o (o_pitch), dout (dout_pitch) and dq, dk, dv (grad_pitch) may be head slices of wider tensors, as in
  * sfb_fused_attention_slice (0: packed); dq, dk and dv share no memory with the operands.
  * Operands are finite: an infinity or NaN in a row of q, k, v or dout makes the gradients of all positions NaN that share its blocks or a

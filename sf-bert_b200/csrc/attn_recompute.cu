@@ -11,14 +11,14 @@
 
 namespace sfb {
 
-// ---- the rows' constants: neg_lse = -lse log2(e), neg_delta = -scale rowsum(dO * O), both [B, H, L] ------------------------------
+// ---- the rows' constants: neg_lse = -lse log2(e), neg_delta = -inside rowsum(dO * O), both [B, H, L] (inside: recompute.cuh) --------
 // Eight lanes per row, 32 R rows of one (batch, head) per CTA; R = 4 where that leaves the SMs enough CTAs: a lane's loads of four rows are on their way
 // together.  100 MB of O and dO (8 x 4096 rows of 12 heads of 64): 25 us with cold caches, most of a copy's rate.  A row without kept
 // elements has lse = -inf, and P = 0 of it: exp2(x + neg_lse) with neg_lse = -inf too.
 template <int DT, uint32_t R>
 __global__ void __launch_bounds__(256) row_constants_kernel(const void *__restrict__ O, const void *__restrict__ dO, const float *__restrict__ lse,
                                                            float *__restrict__ neg_lse, float *__restrict__ neg_delta, uint32_t L, uint32_t H, uint32_t d,
-                                                           size_t o_pitch, size_t do_pitch, float scale, bool vec)
+                                                           size_t o_pitch, size_t do_pitch, float inside, bool vec)
 {
     grid_dependency_wait();
     grid_launch_dependents();
@@ -75,12 +75,12 @@ __global__ void __launch_bounds__(256) row_constants_kernel(const void *__restri
         const float s = lse[row];
         // nothing kept (-inf): the row's dS is empty whatever dO and O hold
         neg_lse[row] = s == -INFINITY ? s : s * -1.4426950408889634f;
-        neg_delta[row] = s == -INFINITY ? 0.f : sum[k] * -scale;
+        neg_delta[row] = s == -INFINITY ? 0.f : sum[k] * -inside;
     }
 }
 
 int attention_row_constants(cudaStream_t s, const void *o, const void *dout, const float *lse, float *neg_lse, float *neg_delta, int dtype, uint32_t B,
-                            uint32_t L, uint32_t H, uint32_t d, uint64_t o_pitch, uint64_t do_pitch, float scale)
+                            uint32_t L, uint32_t H, uint32_t d, uint64_t o_pitch, uint64_t do_pitch, float inside)
 {
     const uint32_t per = dtype == SFB_F32 ? 4 : 8;
     const bool vec = (((uintptr_t)o | (uintptr_t)dout) & 15) == 0 && o_pitch % per == 0 && do_pitch % per == 0 && d % per == 0;
@@ -89,7 +89,7 @@ int attention_row_constants(cudaStream_t s, const void *o, const void *dout, con
     const uint64_t chunks = ((uint64_t)L + 32 * R - 1) / (32 * R);
     SFB_REQUIRE(chunks * H < (1ull << 31), "sfb_attention_backward_recompute: too many rows for one launch");
     const dim3 grid((unsigned)(chunks * H), B);
-#define RC_LAUNCH_R(DT, RV) launch_overlapped_few(row_constants_kernel<DT, RV>, grid, dim3(256), 0, s, o, dout, lse, neg_lse, neg_delta, L, H, d, (size_t)o_pitch, (size_t)do_pitch, scale, vec)
+#define RC_LAUNCH_R(DT, RV) launch_overlapped_few(row_constants_kernel<DT, RV>, grid, dim3(256), 0, s, o, dout, lse, neg_lse, neg_delta, L, H, d, (size_t)o_pitch, (size_t)do_pitch, inside, vec)
 #define RC_LAUNCH(DT) { if (R == 4) RC_LAUNCH_R(DT, 4); else RC_LAUNCH_R(DT, 1); }
     if (dtype == SFB_F32) RC_LAUNCH(SFB_F32)
     else if (dtype == SFB_BF16) RC_LAUNCH(SFB_BF16)
@@ -107,7 +107,7 @@ struct BlockArgs {
     void *p, *ds;
     size_t in_pitch, do_pitch;
     uint32_t first, H, d, nb, blocks, lut_stride, mask_stride;        // first: (batch, head) pair of blockIdx.y = 0
-    float scale, scale_log2e;
+    float inside, scale_log2e;
 };
 template <int BS> struct BlockCfg {
     static constexpr int TEAMS = BS == 32 ? 4 : 2, TT = 128 / TEAMS;      // teams that stage keys of their own
@@ -140,7 +140,7 @@ __device__ __noinline__ void blocks_again(float *buf, const BlockArgs &a, size_t
     }
 #pragma unroll
     for (int n = 0; n < 32; n += 2) {
-        const float s0 = (bits >> n) & 1u ? x[n] * fmaf(y[n], a.scale, nd) : 0.f, s1 = (bits >> (n + 1)) & 1u ? x[n + 1] * fmaf(y[n + 1], a.scale, nd) : 0.f;
+        const float s0 = (bits >> n) & 1u ? x[n] * fmaf(y[n], a.inside, nd) : 0.f, s1 = (bits >> (n + 1)) & 1u ? x[n + 1] * fmaf(y[n + 1], a.inside, nd) : 0.f;
         uint32_t p[3], ds[3];
         tile::split2<3>(p, x[n], x[n + 1]);
         tile::split2<3>(ds, s0, s1);
@@ -275,7 +275,7 @@ __global__ void __launch_bounds__(tile::kThreads, 3) recompute_blocks_kernel(con
             for (int k = 0; k < 8; k++) {
                 const bool in = (bits >> k) & 1u;
                 p[k] = in ? exp2f(fmaf(x[m][k >> 1][2 * half + (k & 1)], a.scale_log2e, nl)) : 0.f;
-                ds[k] = in ? p[k] * fmaf(y[m][k >> 1][2 * half + (k & 1)], a.scale, nd) : 0.f;
+                ds[k] = in ? p[k] * fmaf(y[m][k >> 1][2 * half + (k & 1)], a.inside, nd) : 0.f;
             }
             store_eight<DT>(a.p, baseC + (size_t)r * BS + 8 * t, BS * BS, p);
             store_eight<DT>(a.ds, baseC + (size_t)r * BS + 8 * t, BS * BS, ds);
@@ -368,7 +368,7 @@ __global__ void __launch_bounds__(tile::kThreads, 4) recompute_blocks16_kernel(c
             for (int k = 0; k < 8; k++) {
                 const bool in = (bits >> k) & 1u;
                 p[k] = in ? ex2(fmaf(x[m][k >> 1][2 * half + (k & 1)], a.scale_log2e, nl)) : 0.f;
-                ds[k] = in ? p[k] * fmaf(y[m][k >> 1][2 * half + (k & 1)], a.scale, nd) : 0.f;
+                ds[k] = in ? p[k] * fmaf(y[m][k >> 1][2 * half + (k & 1)], a.inside, nd) : 0.f;
             }
             store_eight<DT>(a.p, baseC + (size_t)r * BS + 8 * t, 0, p);
             store_eight<DT>(a.ds, baseC + (size_t)r * BS + 8 * t, 0, ds);
@@ -389,6 +389,7 @@ struct ProductArgs {
     size_t in_pitch, do_pitch, grad_pitch;
     uint32_t first, pairs, H, d, nb, blocks, lut_stride;      // pairs: (batch, head) pairs of this launch, from `first` on
     bool in_vec, do_vec, out_vec;
+    float outside;                                            // 16 bits: what dQ and dK are multiplied by
 };
 constexpr uint32_t kStages = 3;
 template <int BS, int W, int DT, bool TRANS> struct ProductCfg {
@@ -430,7 +431,7 @@ __device__ __noinline__ void product_again(float (&acc)[2][4][4], const uint16_t
         }
 }
 template <int BS, int W, int DT, bool TRANS>
-__device__ __forceinline__ void product_rows(char *sm, const ProductArgs &a, uint32_t i, uint32_t y, const void *P, const void *V, size_t pitch, bool vec, void *out)
+__device__ __forceinline__ void product_rows(char *sm, const ProductArgs &a, uint32_t i, uint32_t y, const void *P, const void *V, size_t pitch, bool vec, void *out, float factor)
 {
     typedef ProductCfg<BS, W, DT, TRANS> Cfg;
     constexpr uint32_t T = Cfg::T, E = Cfg::E, PARTS = BS / 32;
@@ -569,7 +570,7 @@ __device__ __forceinline__ void product_rows(char *sm, const ProductArgs &a, uin
             } else {
 #pragma unroll
                 for (int n = 0; n < 4; n++) {
-                    const uint32_t w = pack_own<DT>(acc[m][n][2 * half], acc[m][n][2 * half + 1]), col = 8 * n + 2 * t;
+                    const uint32_t w = pack_own<DT>(acc[m][n][2 * half] * factor, acc[m][n][2 * half + 1] * factor), col = 8 * n + 2 * t;
                     uint16_t *o = (uint16_t *)out + at + col;
                     if (a.out_vec) {
                         if (col < left) *(uint32_t *)o = w;
@@ -593,9 +594,9 @@ __global__ void __launch_bounds__(32 * W * (BS / 32), 512 / (32 * W * (BS / 32))
     grid_launch_dependents();
     const uint32_t n = blockIdx.x / 3, which = blockIdx.x - 3 * n, at = n / a.pairs, y = n - at * a.pairs, i = at < (a.nb + 7) / 8 ? a.nb - 1 - at : at - (a.nb + 7) / 8;
     if (which == 2) {
-        product_rows<BS, W, DT, false>(psm, a, i, y, a.ds, a.k, a.in_pitch, a.in_vec, a.dq);
+        product_rows<BS, W, DT, false>(psm, a, i, y, a.ds, a.k, a.in_pitch, a.in_vec, a.dq, a.outside);
     } else {
-        product_rows<BS, W, DT, true>(psm, a, i, y, which ? a.ds : a.p, which ? a.q : a.dout, which ? a.in_pitch : a.do_pitch, which ? a.in_vec : a.do_vec, which ? a.dk : a.dv);
+        product_rows<BS, W, DT, true>(psm, a, i, y, which ? a.ds : a.p, which ? a.q : a.dout, which ? a.in_pitch : a.do_pitch, which ? a.in_vec : a.do_vec, which ? a.dk : a.dv, which ? a.outside : 1.f);
     }
 }
 template <int BS, int W, int DT>
@@ -667,9 +668,9 @@ int simt_backward_recompute(cudaStream_t s, const BackwardArgs &a, float *neg_ls
     };
     const bool in = rows({a.q, a.k, a.v}, a.in_pitch), dout = rows({a.dout}, a.do_pitch);
     BlockArgs k = {(const uint2 *)a.nt_lut, a.q, a.k, a.v, a.dout, a.mask, neg_lse, neg_delta, P, dS, (size_t)a.in_pitch, (size_t)a.do_pitch, 0, p.H, p.d, p.nb_a,
-                   p.blocks, a.nt_stride, p.mask_stride, a.scale, a.scale * 1.4426950408889634f};
+                   p.blocks, a.nt_stride, p.mask_stride, a.inside, a.scale * 1.4426950408889634f};
     ProductArgs o = {(const uint2 *)a.nn_lut, (const uint2 *)a.tn_lut, P, dS, a.q, a.k, a.dout, a.dq, a.dk, a.dv, (size_t)a.in_pitch, (size_t)a.do_pitch, (size_t)a.grad_pitch, 0, 0,
-                     p.H, p.d, p.nb_a, p.blocks, p.lut_stride, in, dout, rows({a.dq, a.dk, a.dv}, a.grad_pitch)};
+                     p.H, p.d, p.nb_a, p.blocks, p.lut_stride, in, dout, rows({a.dq, a.dk, a.dv}, a.grad_pitch), a.scale / a.inside};
     const uint32_t all = p.B * p.H;
 #define BP(BS) (a.dtype == SFB_F32 ? backward_parts<BS, SFB_F32>(s, k, o, all, n, in && dout) : a.dtype == SFB_BF16 ? backward_parts<BS, SFB_BF16>(s, k, o, all, n, in && dout) \
                                                                                                     : backward_parts<BS, SFB_F16>(s, k, o, all, n, in && dout))

@@ -1,6 +1,7 @@
 // The backward pass that makes the probabilities again (recompute.cuh), on the tensor cores (tcgen05) for 16-bit operands, block_size 64,
-// head size 64.  neg_lse = -lse log2(e) and neg_delta = -scale rowsum(dO * O) come from attn_recompute.cu; then
-//   P = exp2(S scale log2(e) + neg_lse),  dS = P * (dP scale + neg_delta),   S = Q.K^T,  dP = dO.V^T,   dQ = dS.K,  dK = dS^T.Q,  dV = P^T.dO.
+// head size 64.  neg_lse = -lse log2(e) and neg_delta = -inside rowsum(dO * O) come from attn_recompute.cu; then
+//   P = exp2(S scale log2(e) + neg_lse),  dS = P * (dP inside + neg_delta),   S = Q.K^T,  dP = dO.V^T,
+//   dQ = outside dS.K,  dK = outside dS^T.Q,  dV = P^T.dO,   inside outside = scale (recompute.cuh).
 //
 // Two kernels, the same code seen from two sides (COL): an item is 128 "own" positions (queries of two block-rows, or keys of two
 // block-columns) of one (batch, head) and a walk over the union of their blocks.  Nothing of the size of the scores is written anywhere and no sum
@@ -64,7 +65,7 @@ struct RcParams {
     const uint64_t *mask;
     void *out1, *out2;         // dQ, - or dK, dV
     uint32_t B, H, nb, blocks, lut_stride, mask_stride, sms, pitch;   // pitch: elements between consecutive rows of the gradients
-    float scale, scale_log2e;
+    float inside, outside, scale_log2e;
 };
 
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint64_t *bar)
@@ -80,7 +81,6 @@ __device__ __forceinline__ void copy_to_tmem(uint32_t tmem, uint64_t desc)
     asm volatile("tcgen05.cp.cta_group::1.128x256b [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
 }
 // A wait that is mostly over when it begins: one look and a vote
-
 __device__ __forceinline__ bool look_or_wait(uint64_t *bar, uint32_t parity, volatile uint32_t *abort_flag, uint32_t code)
 {
     return __all_sync(0xffffffffu, mbar_try_wait(bar, parity)) || mbar_wait_warp(bar, parity, abort_flag, code);
@@ -97,11 +97,11 @@ __device__ __forceinline__ uint32_t lds_word(uint32_t addr)
     return v;
 }
 
-// P * (dP * scale + neg_delta) for a pair, rounded to the 16-bit type
+// P * (dP * inside + neg_delta) for a pair, rounded to the 16-bit type
 template <bool BF16>
-__device__ __forceinline__ uint32_t ds_pair(uint32_t dp0, uint32_t dp1, uint32_t p0, uint32_t p1, uint64_t scale2, uint64_t delta2)
+__device__ __forceinline__ uint32_t ds_pair(uint32_t dp0, uint32_t dp1, uint32_t p0, uint32_t p1, uint64_t inside2, uint64_t delta2)
 {
-    const uint64_t x = fma2p(pk64(__uint_as_float(dp0), __uint_as_float(dp1)), scale2, delta2);
+    const uint64_t x = fma2p(pk64(__uint_as_float(dp0), __uint_as_float(dp1)), inside2, delta2);
     float e0, e1;
     up64(mul2p(x, pk64(__uint_as_float(p0), __uint_as_float(p1))), e0, e1);
     return pack2(e0, e1, BF16);
@@ -370,7 +370,7 @@ recompute_tc_kernel(const __grid_constant__ CUtensorMap own1_map, const __grid_c
         const uint32_t r = quarter * 32 + lane, half = r >> 6;
         const uint32_t lane_field = (quarter * 32) << 16;
         const uint32_t t_s = tmem + 64 * grp + lane_field;
-        const uint64_t scale2 = pk64(p.scale, p.scale), sl2 = pk64(p.scale_log2e, p.scale_log2e);
+        const uint64_t inside2 = pk64(p.inside, p.inside), sl2 = pk64(p.scale_log2e, p.scale_log2e);
         uint32_t turn = 0, lap = 0, ph = 0;                  // whose epilogue, times round modulo 2 (of items with blocks); this group's steps modulo 2
         uint32_t g = 0, wait = grp;                          // steps of all groups; how many of them come before this group's next
         bool alive = true;
@@ -478,7 +478,7 @@ recompute_tc_kernel(const __grid_constant__ CUtensorMap own1_map, const __grid_c
                             if (COL) lds_pairs(n2, nd_at + 128 * c + 16 * j);
 #pragma unroll
                             for (int e = 0; e < 2; e++)
-                                w[2 * j + e] = ds_pair<BF16>(u[4 * j + 2 * e], u[4 * j + 2 * e + 1], v[32 * c + 4 * j + 2 * e], v[32 * c + 4 * j + 2 * e + 1], scale2, n2[e]);
+                                w[2 * j + e] = ds_pair<BF16>(u[4 * j + 2 * e], u[4 * j + 2 * e + 1], v[32 * c + 4 * j + 2 * e], v[32 * c + 4 * j + 2 * e + 1], inside2, n2[e]);
                         }
                         TMEM_ST_16(t_dp + 32 * c, (w));
                     }
@@ -523,12 +523,13 @@ recompute_tc_kernel(const __grid_constant__ CUtensorMap own1_map, const __grid_c
 #pragma unroll
                     for (int j = 0; j < 64; j++) v[j] = 0u;  // rows and columns without blocks have zero gradients
                 }
+                const float factor = what ? 1.f : p.outside;
                 if (blk != kNoItem)
 #pragma unroll
                     for (int c = 0; c < 8; c++) {
                         uint32_t y[4];
 #pragma unroll
-                        for (int j = 0; j < 4; j++) y[j] = pack2(__uint_as_float(v[8 * c + 2 * j]), __uint_as_float(v[8 * c + 2 * j + 1]), BF16);
+                        for (int j = 0; j < 4; j++) y[j] = pack2(__uint_as_float(v[8 * c + 2 * j]) * factor, __uint_as_float(v[8 * c + 2 * j + 1]) * factor, BF16);
                         *(uint4 *)(dst + 8 * c) = make_uint4(y[0], y[1], y[2], y[3]);
                     }
             }
@@ -603,7 +604,7 @@ int tc_backward_recompute(cudaStream_t s, const BackwardArgs &a, const float *ne
         make_map(&dm, a.dout, rows, p.H, bf, 64, a.do_pitch))
         return 1;
     RcParams row = {(const uint2 *)a.nn_lut, neg_lse, neg_delta, (const uint64_t *)a.mask, a.dq, nullptr, p.B, p.H, p.nb_a, p.blocks, p.lut_stride, p.mask_stride, (uint32_t)(sms > 0 ? sms : 1),
-                    (uint32_t)a.grad_pitch, a.scale, a.scale * 1.4426950408889634f};
+                    (uint32_t)a.grad_pitch, a.inside, a.scale / a.inside, a.scale * 1.4426950408889634f};
     RcParams col = row;
     col.lut = (const uint2 *)a.tn_lut;
     col.out1 = a.dk;

@@ -205,10 +205,10 @@ extern "C" int sfb_attention_backward_recompute(sfb_stream_t stream, const void 
     const uint64_t need = 2 * rows + (tc ? 0 : simt_backward_workspace(dtype, block_size, ctx_blks, blocks, batch_dim, head_dim));
     SFB_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= need, "%s: needs a 16-byte aligned workspace of %llu bytes", who, (unsigned long long)need);
     const BackwardArgs a = {nt_lut, nn_lut, tn_lut, q, k, v, o, dout, mask, dq, dk, dv, dtype, block_size, lut_heads > 1 ? lut_dim : 0, nn_max, tn_max,
-                            in_pitch, o_pitch, dout_pitch, grad_pitch, scale, p};
+                            in_pitch, o_pitch, dout_pitch, grad_pitch, scale, scale_inside(dtype, scale), p};
     float *neg_lse = (float *)workspace, *neg_delta = (float *)((char *)workspace + rows);
     const uint32_t L = ctx_blks * block_size;
-    if (attention_row_constants(as_stream(stream), o, dout, lse, neg_lse, neg_delta, dtype, batch_dim, L, head_dim, state_dim, o_pitch, dout_pitch, scale)) return 1;
+    if (attention_row_constants(as_stream(stream), o, dout, lse, neg_lse, neg_delta, dtype, batch_dim, L, head_dim, state_dim, o_pitch, dout_pitch, a.inside)) return 1;
     if (tc) return tc_backward_recompute(as_stream(stream), a, neg_lse, neg_delta);
     return simt_backward_recompute(as_stream(stream), a, neg_lse, neg_delta, (char *)workspace + 2 * rows);
 }
