@@ -248,7 +248,8 @@ def linear_nt(x, wt, bias=None, act=ACT_NONE, out=None):
 
 def embedding(table, ids, pos=None, scale=1.0):
     """out[b, l, :] = scale * table[ids[b, l], :] + pos[l, :] (embedding_lookup + tensor_add_matrix, embedding.h:5-12,
-    ewops.h:276-282).  Returns (out, number of ids that were outside the table)."""
+    ewops.h:276-282).  pos: of the table's type, L rows or more, of which the first L are read.  Returns (out, number of ids that were
+    outside the table)."""
     return _host.embedding(table, ids, pos, scale)
 
 

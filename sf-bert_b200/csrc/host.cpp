@@ -138,6 +138,9 @@ inline int tag(const at::Tensor &t)
     PyErr_SetString(PyExc_KeyError, c10::toString(s));
     throw Raised();
 }
+inline void require_cuda(const at::Tensor &t) { require(t.is_cuda(), "expected a tensor on a CUDA device"); }
+// of the device of a call's tensors, whichever is the current one (with a CUDAGuard beside it)
+inline sfb_stream_t stream_of(const at::Tensor &t) { return (sfb_stream_t)c10::cuda::getCurrentCUDAStream(t.device().index()).stream(); }
 inline sfb_stream_t stream() { return (sfb_stream_t)c10::cuda::getCurrentCUDAStream().stream(); }
 inline at::Tensor empty(at::IntArrayRef size, at::ScalarType type, const at::Tensor &like)
 {
@@ -329,9 +332,21 @@ FUNCTION(py_embedding, 4)
     require(ids.scalar_type() == at::kInt && ids.is_contiguous() && table.is_contiguous(), "ids must be int32 and contiguous, like the table");
     const int64_t B = ids.size(0), len = ids.size(1), vocab = table.size(0), hidden = table.size(1);
     const float scale = (float)number(a[3]);
+    const int t = tag(table);
+    require(ids.device() == table.device(), "ids must be on the table's device");
+    require(B < (1ll << 31) && len < (1ll << 31) && vocab < (1ll << 31) && hidden < (1ll << 31) && B * len < (1ll << 31), "too many tokens, or too large a table");
+    if (a[2] != Py_None) {
+        // the rows of the first len positions are read: a longer table serves shorter sequences
+        const at::Tensor &pos = tensor(a[2]);
+        require(pos.dim() >= 1 && pos.size(-1) == hidden && pos.numel() >= len * hidden && pos.is_contiguous() && pos.scalar_type() == table.scalar_type() &&
+                    pos.device() == table.device(),
+                "pos must hold a row like the table's for every position: contiguous, of its type, on its device");
+    }
+    require_cuda(table);
+    const c10::cuda::CUDAGuard on(table.device());
     at::Tensor out = empty({B, len, hidden}, table.scalar_type(), table), bad = empty({1}, at::kInt, table);
-    call(L.sfb_embedding_scaled, stream(), ptr(out), ptr(table), (const int32_t *)ptr(ids), ptr_or_null(a[2]), (uint32_t)B, (uint32_t)len,
-                                 (uint32_t)hidden, (uint32_t)vocab, tag(table), scale, (uint32_t *)ptr(bad));
+    call(L.sfb_embedding_scaled, stream_of(table), ptr(out), ptr(table), (const int32_t *)ptr(ids), ptr_or_null(a[2]), (uint32_t)B, (uint32_t)len,
+                                 (uint32_t)hidden, (uint32_t)vocab, t, scale, (uint32_t *)ptr(bad));
     Ref o(wrap(out)), n(wrap(bad));
     return PyTuple_Pack(2, o.o, n.o);
 }
@@ -586,9 +601,6 @@ inline int64_t vocab_or_width(PyObject *o, const LogitRows &x)
     require(v >= 1 && v <= x.width, "vocab must be 1 to the number of columns");
     return v;
 }
-inline void require_cuda(const at::Tensor &t) { require(t.is_cuda(), "expected a tensor on a CUDA device"); }
-// The calls below run on the device of their tensors, on its current stream, whichever device is the current one.
-inline sfb_stream_t stream_of(const at::Tensor &t) { return (sfb_stream_t)c10::cuda::getCurrentCUDAStream(t.device().index()).stream(); }
 // The results of a call, [...] or [..., last] of four-byte elements.  An allocation takes about a microsecond of host time, and a
 // call for one row has six results: together at most 64 KB they share one, each at 64 bytes of its own.
 struct Results {

@@ -83,3 +83,14 @@ def test_a_scale_of_zero(sfb, dtype, bs, d):
     t = torch.finfo(DTYPES[dtype])
     # P: half a step; the sums as in grad_tolerance; the result's rounding
     assert ((dv.double() - want).abs() <= t.eps / 2 * want.abs() * 1.01 + ((t.eps / 2 if dtype != "f32" else 0) + 2.0 ** -18) * size + 2.0 ** -24).all()
+
+
+# ---- embedding ------------------------------------------------------------------------------------------------------------------
+def test_a_position_table_longer_than_the_sequence(sfb):
+    """Its first rows are added, as a view of them would be."""
+    g = torch.Generator(device="cuda").manual_seed(25)
+    table, pos = torch.randn(50, 16, device="cuda", generator=g), torch.randn(512, 16, device="cuda", generator=g)
+    ids = torch.randint(0, 50, (3, 20), device="cuda", generator=g, dtype=torch.int32)
+    want = sfb.embedding(table, ids, pos[:20].contiguous(), scale=2.0)[0]
+    assert torch.equal(want, sfb.embedding(table, ids, pos, scale=2.0)[0])
+    assert torch.equal(want, sfb.embedding(table, ids, pos[None, :20], scale=2.0)[0])
