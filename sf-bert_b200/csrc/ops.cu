@@ -238,12 +238,17 @@ extern "C" int sfb_linear_residual(sfb_stream_t stream, void *out, const void *x
 static int embedding_common(const char *who, sfb_stream_t stream, void *out, const void *table, const int32_t *ids, const void *pos, uint32_t batch,
                             uint32_t seq_len, uint32_t hidden, uint32_t vocab, int dtype, float scale, uint32_t *bad_ids)
 {
-    SFB_REQUIRE(out && table && ids, "%s: NULL pointer", who);
+    const bool none = batch == 0 || seq_len == 0 || hidden == 0;                  // nothing is looked up
+    SFB_REQUIRE(none || (out && table && ids), "%s: NULL pointer", who);
     SFB_REQUIRE(valid_dtype(dtype), "%s: unknown dtype", who);
     SFB_REQUIRE(hidden % 8 == 0, "%s: hidden=%u must be a multiple of 8", who, hidden);
     SFB_REQUIRE(aligned16(out) && aligned16(table) && (!pos || aligned16(pos)), "%s: out, table and pos must be 16-byte aligned", who);
     SFB_REQUIRE((uint64_t)batch * seq_len < (1ull << 31), "%s: too many tokens", who);
-    if (batch == 0 || seq_len == 0 || hidden == 0) { clear_error(); return 0; }
+    if (none) {
+        if (bad_ids && cudaMemsetAsync(bad_ids, 0, sizeof(uint32_t), as_stream(stream)) != cudaSuccess) return fail("%s: cannot clear the count", who);
+        clear_error();
+        return 0;
+    }
     return embedding_lookup(as_stream(stream), out, table, ids, pos, batch, seq_len, hidden, vocab, dtype, scale, bad_ids);
 }
 

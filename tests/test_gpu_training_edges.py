@@ -94,3 +94,14 @@ def test_a_position_table_longer_than_the_sequence(sfb):
     want = sfb.embedding(table, ids, pos[:20].contiguous(), scale=2.0)[0]
     assert torch.equal(want, sfb.embedding(table, ids, pos, scale=2.0)[0])
     assert torch.equal(want, sfb.embedding(table, ids, pos[None, :20], scale=2.0)[0])
+
+
+@pytest.mark.parametrize("B,L", [(0, 5), (3, 0), (0, 0)])
+def test_a_lookup_of_no_tokens(sfb, B, L):
+    """Its count is 0, whatever was in that memory before."""
+    table, ids = torch.ones(9, 16, device="cuda"), torch.zeros(B, L, dtype=torch.int32, device="cuda")
+    for _ in range(4):
+        dirt = [torch.full((1,), 77, dtype=torch.int32, device="cuda") for _ in range(64)]
+        del dirt
+        out, bad = sfb.embedding(table, ids)
+        assert out.shape == (B, L, 16) and int(bad) == 0
