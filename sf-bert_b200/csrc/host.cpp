@@ -824,9 +824,9 @@ inline Bytes bytes_of(const at::Tensor &t)
     const int64_t rows = t.size(0) * t.size(1);
     return {p, rows ? p + ((rows - 1) * t.stride(1) + t.size(2) * t.size(3)) * t.element_size() : p};
 }
-inline at::Tensor like_operand(PyObject *out, const at::Tensor &q, const char *text)
+// a result that the caller gave.  All that can be wrong with it is found before the device is asked for
+inline const at::Tensor &like_operand(PyObject *out, const at::Tensor &q, const char *text)
 {
-    if (out == Py_None) return empty(q.sizes(), q.scalar_type(), q);
     const at::Tensor &o = tensor(out);
     require(o.sizes() == q.sizes() && o.scalar_type() == q.scalar_type() && o.device() == q.device(), text);
     return o;
@@ -840,13 +840,18 @@ FUNCTION(py_fused_attention_stats, 7)
     const uint64_t pitch = operand_pitch(q, k, v);
     const float scale = scale_or(a[4], n.d);
     require(n.d >= 1 && n.d <= 128, "heads must be 1 to 128 wide");
+    at::Tensor o;
+    if (a[6] != Py_None) {
+        o = like_operand(a[6], q, "out must be like q");
+        row_pitch(o);
+        const Bytes r = bytes_of(o);
+        require(!r.meets(bytes_of(q)) && !r.meets(bytes_of(k)) && !r.meets(bytes_of(v)), "out must not share memory with the operands");
+    }
     require_cuda(q);
     const c10::cuda::CUDAGuard on(q.device());
     void *nn = table_on(lay, n_nn_lut, 2ll * lay.heads * (lay.nb + lay.blocks), q, bad_layout), *mask = mask_on(lay, truth(a[5]), q);
-    at::Tensor o = like_operand(a[6], q, "out must be like q");
+    if (!o.defined()) o = empty(q.sizes(), q.scalar_type(), q);
     const uint64_t out_pitch = row_pitch(o);
-    const Bytes r = bytes_of(o);
-    require(!r.meets(bytes_of(q)) && !r.meets(bytes_of(k)) && !r.meets(bytes_of(v)), "out must not share memory with the operands");
     at::Tensor lse = empty({n.B, n.H, n.L}, at::kFloat, q);
     if (n.B && n.H)
         call(L.sfb_fused_attention_stats, stream_of(q), nn, ptr(q), ptr(k), ptr(v), ptr(o), (float *)ptr(lse), mask, tag(q), lay.bs, lay.blocks, n.B, lay.nb, n.H,
@@ -869,29 +874,31 @@ FUNCTION(py_attention_backward_recompute, 10)
     require(lse.scalar_type() == at::kFloat && lse.is_contiguous() && lse.device() == q.device() && lse.dim() == 3 && lse.size(0) == n.B && lse.size(1) == n.H &&
                 lse.size(2) == n.L,
             "lse must be the contiguous fp32 [B, H, L] tensor that the forward call gave");
-    require_cuda(q);
-    const c10::cuda::CUDAGuard on(q.device());
     at::Tensor grad[3];
-    if (a[9] == Py_None) {
-        for (at::Tensor &g : grad) g = empty(q.sizes(), q.scalar_type(), q);
-    } else {
+    if (a[9] != Py_None) {
         Ref list(PySequence_Fast(a[9], "out must be a sequence of three tensors"));
         require(PySequence_Fast_GET_SIZE(list.o) == 3, "out must be a sequence of three tensors");
         for (int i = 0; i < 3; i++) grad[i] = like_operand(PySequence_Fast_GET_ITEM(list.o, i), q, "out's tensors must be like q");
-    }
-    const uint64_t grad_pitch = row_pitch(grad[0]);
-    require(row_pitch(grad[1]) == grad_pitch && row_pitch(grad[2]) == grad_pitch, "out's tensors have different row pitches");
-    const Bytes in[6] = {bytes_of(q), bytes_of(k), bytes_of(v), bytes_of(o), bytes_of(dout), {(const char *)ptr(lse), (const char *)ptr(lse) + lse.numel() * 4}};
-    for (int i = 0; i < 3; i++) {
-        const Bytes r = bytes_of(grad[i]);
-        for (const Bytes &x : in) require(!r.meets(x), "out must not share memory with the operands");
-        for (int j = 0; j < i; j++) {
-            // apart, or side by side in the rows of one wider tensor
-            const Bytes r2 = bytes_of(grad[j]);
-            const int64_t off = (r.begin < r2.begin ? r2.begin - r.begin : r.begin - r2.begin) / q.element_size() % (int64_t)grad_pitch, width = (int64_t)n.H * n.d;
-            require(!r.meets(r2) || (off >= width && off + width <= (int64_t)grad_pitch), "out's tensors must not share memory");
+        const int64_t wide = (int64_t)row_pitch(grad[0]), width = (int64_t)n.H * n.d;
+        require((int64_t)row_pitch(grad[1]) == wide && (int64_t)row_pitch(grad[2]) == wide, "out's tensors have different row pitches");
+        const Bytes in[6] = {bytes_of(q), bytes_of(k), bytes_of(v), bytes_of(o), bytes_of(dout), {(const char *)ptr(lse), (const char *)ptr(lse) + lse.numel() * 4}};
+        for (int i = 0; i < 3; i++) {
+            const Bytes r = bytes_of(grad[i]);
+            for (const Bytes &x : in) require(!r.meets(x), "out must not share memory with the operands");
+            for (int j = 0; j < i; j++) {
+                // apart, or side by side in the rows of one wider tensor
+                const Bytes r2 = bytes_of(grad[j]);
+                if (!r.meets(r2)) continue;
+                const int64_t off = (r.begin < r2.begin ? r2.begin - r.begin : r.begin - r2.begin) / q.element_size() % wide;
+                require(off >= width && off + width <= wide, "out's tensors must not share memory");
+            }
         }
     }
+    require_cuda(q);
+    const c10::cuda::CUDAGuard on(q.device());
+    if (!grad[0].defined())
+        for (at::Tensor &g : grad) g = empty(q.sizes(), q.scalar_type(), q);
+    const uint64_t grad_pitch = row_pitch(grad[0]);
     const bool use_mask = truth(a[8]);
     if (n.B && n.H && n.L) {
         const uint32_t tn_max = attr_u32(lay.o, n_tn_max);
@@ -926,13 +933,8 @@ FUNCTION(py_embedding_grad, 7)
     require(vocab >= 1 && vocab <= (1 << 27), "vocab must be 1 to 2^27");
     require(hidden >= 8 && hidden % 8 == 0 && hidden < (1ll << 31), "hidden must be a multiple of 8");
     require(B * len < (1ll << 31) && B < (1ll << 31) && len < (1ll << 31), "too many tokens");
-    require_cuda(dout);
-    const c10::cuda::CUDAGuard on(dout.device());
     at::Tensor dtable, dpos;
-    if (a[6] == Py_None) {
-        dtable = empty({vocab, hidden}, scalar_type(g), dout);
-        if (positions) dpos = empty({len, hidden}, scalar_type(g), dout);
-    } else {
+    if (a[6] != Py_None) {
         const char *text = "out must be the table's gradient, or with positions a pair: contiguous, of the gradients' type and the tables' sizes, on dout's device";
         auto fits = [&](PyObject *o, int64_t rows) {
             const at::Tensor &x = tensor(o);
@@ -952,6 +954,12 @@ FUNCTION(py_embedding_grad, 7)
         const Bytes table = span(dtable);
         require(!table.meets(span(dout)) && !table.meets(span(ids)) && (!positions || (!span(dpos).meets(table) && !span(dpos).meets(span(dout)) && !span(dpos).meets(span(ids)))),
                 "out must not share memory with the operands");
+    }
+    require_cuda(dout);
+    const c10::cuda::CUDAGuard on(dout.device());
+    if (!dtable.defined()) {
+        dtable = empty({vocab, hidden}, scalar_type(g), dout);
+        if (positions) dpos = empty({len, hidden}, scalar_type(g), dout);
     }
     at::Tensor bad = empty({1}, at::kInt, dout);
     at::Tensor ws = empty({(int64_t)L.sfb_embedding_grad_workspace((uint32_t)B, (uint32_t)len, (uint32_t)hidden, (uint32_t)vocab)}, at::kByte, dout);

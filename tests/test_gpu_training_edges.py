@@ -85,6 +85,26 @@ def test_a_scale_of_zero(sfb, dtype, bs, d):
     assert ((dv.double() - want).abs() <= t.eps / 2 * want.abs() * 1.01 + ((t.eps / 2 if dtype != "f32" else 0) + 2.0 ** -18) * size + 2.0 ** -24).all()
 
 
+@pytest.mark.parametrize("dtype,bs,d", [("f16", 64, 64), ("bf16", 64, 64), ("bf16", 32, 40), ("f32", 32, 64)])
+def test_log_sums_with_an_output_in_a_wider_tensor(sfb, dtype, bs, d):
+    """Two heads of five: the neighbouring heads stay, the bits are those of a call without out."""
+    nb, H = 5, 2
+    q, k, v = (x.cuda() for x in operands(2, nb * bs, H, d, dtype, 23, n=3))
+    lay = plan(sfb, layout("stride", nb), bs)
+    want = sfb.fused_attention_stats(q, k, v, lay)
+    wider = torch.full((2, nb * bs, 5, d), 7.0, dtype=DTYPES[dtype], device="cuda")
+    o, lse = sfb.fused_attention_stats(q, k, v, lay, out=wider[:, :, 1:3])
+    assert o.data_ptr() == wider[:, :, 1:3].data_ptr() and torch.equal(o, want[0]) and torch.equal(lse, want[1])
+    assert (wider[:, :, :1] == 7).all() and (wider[:, :, 3:] == 7).all()
+    grads = sfb.attention_backward_recompute(q, k, v, *want[:1], q, lse, lay)
+    # gradients beside each other in rows that are wider still
+    wide = torch.full((2, nb * bs, 4, H, d), 7.0, dtype=DTYPES[dtype], device="cuda")
+    got = sfb.attention_backward_recompute(q, k, v, o, q, lse, lay, out=[wide[:, :, i] for i in (3, 0, 2)])
+    for a, b in zip(grads, got):
+        assert torch.equal(a, b)
+    assert (wide[:, :, 1] == 7).all()
+
+
 # ---- embedding ------------------------------------------------------------------------------------------------------------------
 def test_a_position_table_longer_than_the_sequence(sfb):
     """Its first rows are added, as a view of them would be."""
