@@ -6,7 +6,7 @@ import pytest
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
-from test_gpu_training import check_attention, layout, operands, plan                                            # noqa: E402
+from test_gpu_training import check_attention, check_embed_grad, layout, operands, plan                         # noqa: E402
 from training_reference import DTYPES                                                                         # noqa: E402
 
 
@@ -105,6 +105,33 @@ def test_log_sums_with_an_output_in_a_wider_tensor(sfb, dtype, bs, d):
     assert (wide[:, :, 1] == 7).all()
 
 
+def test_differences_of_the_fp32_forward(sfb):
+    """The gradient of <o, do> along a direction, by central differences of the package's own forward, without their second-order error."""
+    bs, nb, d, H = 32, 5, 64, 2
+    lay = plan(sfb, layout("stride", nb), bs)
+    q, k, v, do = (x.cuda() for x in operands(1, nb * bs, H, d, "f32", 3))
+    o, lse = sfb.fused_attention_stats(q, k, v, lay)
+    grads = sfb.attention_backward_recompute(q, k, v, o, do, lse, lay)
+    for which in range(3):
+        y = torch.randn(q.shape, generator=torch.Generator().manual_seed(9 + which)).cuda()
+
+        def slope(eps):
+            f = []
+            for e in (eps, -eps):
+                x = [q, k, v]
+                x[which] = x[which] + e * y
+                f.append(float((sfb.fused_attention_stats(*x, lay)[0].double() * do.double()).sum()))
+            return (f[0] - f[1]) / (2 * eps)
+
+        eps = 2.0 ** -6
+        near, far = (4 * slope(eps) - slope(2 * eps)) / 3, (4 * slope(2 * eps) - slope(4 * eps)) / 3
+        size = float((grads[which].double() * y.double()).abs().sum())
+        # what is left of the differences goes with eps^4: a fifteenth of what the doubled step changes.  The forward's entries are off by 2^-20 of
+        # the values' size (24 roundings of the scores and sums), independently, four times in a slope; the gradients by 1e-6
+        noise = 4 * 2.0 ** -20 * float((do.double().square().sum() * v.double().square().mean()).sqrt()) / eps
+        assert abs(near - float((grads[which].double() * y.double()).sum())) <= abs(near - far) / 15 * 2 + noise + 1e-6 * size
+
+
 # ---- embedding ------------------------------------------------------------------------------------------------------------------
 def test_a_position_table_longer_than_the_sequence(sfb):
     """Its first rows are added, as a view of them would be."""
@@ -125,3 +152,109 @@ def test_a_lookup_of_no_tokens(sfb, B, L):
         del dirt
         out, bad = sfb.embedding(table, ids)
         assert out.shape == (B, L, 16) and int(bad) == 0
+
+
+@pytest.mark.parametrize("n", [16383, 16384, 16385, 65535, 65536, 65537, 65541])
+@pytest.mark.parametrize("off", [0, 1, 3])
+@pytest.mark.parametrize("dtype,hidden", [("bf16", 8), ("f32", 24)])
+def test_counts_of_ids_at_every_alignment(sfb, n, off, dtype, hidden):
+    """One CTA counts, four ids per load where they are 16-byte aligned, or all that read them: on both sides of what decides, and ids that end inside a load."""
+    vocab = 300
+    g = torch.Generator(device="cuda").manual_seed(n)
+    table = torch.randn(vocab, hidden, device="cuda", generator=g).to(DTYPES[dtype])
+    flat = torch.full((n + 8,), -5, device="cuda", dtype=torch.int32)
+    ids = flat[off:off + n].view(1, n)
+    ids.copy_(torch.randint(-3, vocab + 3, (1, n), device="cuda", generator=g, dtype=torch.int32))
+    for edge in ((0, -1), (n - 1, vocab), (n - 2, -2 ** 31)):
+        ids[0, edge[0]] = edge[1]
+    there = (ids >= 0) & (ids < vocab)
+    for _ in range(2):
+        out, bad = sfb.embedding(table, ids, scale=1.0)
+        assert int(bad) == int((~there).sum())
+        assert torch.equal(out, table[ids.clamp(0, vocab - 1).long()] * there[..., None])
+
+
+def tokens(n, vocab, hidden, seed, B=1):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    ids = torch.randint(-1, vocab + 1, (B, n // B), device="cuda", generator=g, dtype=torch.int32)
+    return torch.randn(B, n // B, hidden, device="cuda", generator=g), ids
+
+
+def test_tables_of_many_tokens_in_graphs_and_on_streams(sfb):
+    """The three launches and their workspace: calls at once on two streams, captured, and replayed with other tokens in place."""
+    vocab, hidden = 700, 96
+    sets = [[x.clone() for x in tokens(4096, vocab, hidden, i, 4)] for i in range(2)]
+
+    def step(dout, ids):
+        return sfb.embedding_grad(dout, ids, vocab, 0.5, True)
+
+    want = [step(*s) for s in sets]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in sets], []
+    for s, x in zip(streams, sets):
+        with torch.cuda.stream(s):
+            got.append([step(*x) for _ in range(4)][-1])
+    torch.cuda.synchronize()
+    for a, b in zip(want, got):
+        for x, y in zip(a, b):
+            assert torch.equal(x, y)
+    graphs, outs = [], []
+    for x in sets:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(step(*x))
+        graphs.append(graph)
+    for seed in range(3):
+        for i, x in enumerate(sets):
+            for y, z in zip(x, tokens(4096, vocab, hidden, 10 * seed + i, 4)):
+                y.copy_(z)
+        torch.cuda.synchronize()
+        for s, graph in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                graph.replay()
+        torch.cuda.synchronize()
+        for x, o in zip(sets, outs):
+            for y, z in zip(o, step(*x)):
+                assert torch.equal(y, z)
+    check_embed_grad(sfb, sets[0][0].cpu(), sets[0][1].cpu(), vocab, 0.5)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_many_tokens_whose_rows_are_not_finite(sfb, dtype):
+    """They reach their own ids' and positions' rows only, beside others in their piece and over several pieces."""
+    n, vocab, hidden = 5000, 60, 40
+    ids = (torch.arange(n) % 50).to(torch.int32)
+    ids[7::50], ids[9::50] = -1, vocab
+    dout = torch.ones(n, hidden)
+    dout[3], dout[77], dout[4999], dout[7], dout[59] = math.nan, math.inf, -math.inf, math.nan, math.inf      # 7, 59: ids that have no row
+    dtable, dpos, bad = sfb.embedding_grad(dout.to(DTYPES[dtype]).view(1, n, hidden).cuda(), ids.view(1, n).cuda(), vocab, positions=True)
+    assert int(bad) == 200
+    assert dtable[3].isnan().all() and (dtable[27] == math.inf).all() and (dtable[49] == -math.inf).all()
+    rest = [i for i in range(50) if i not in (3, 7, 9, 27, 49)]
+    assert (dtable[rest] == 100).all() and (dtable[50:] == 0).all() and (dtable[[7, 9]] == 0).all()
+    assert torch.equal(dpos.cpu().nan_to_num(5.0), dout.nan_to_num(5.0))
+
+
+@pytest.mark.parametrize("n,piece", [(4096, 8), (65536, 16), (98304, 32), (196608, 64)])
+@pytest.mark.parametrize("shift", [0, 1, 5])
+def test_runs_at_the_ends_of_pieces(sfb, n, piece, shift):
+    """Whole numbers, whose sums are exact: runs of one piece and of several, that end with a piece or beside its end, runs of up to 16 parts
+    and of more, which a warp and a CTA add up, and a total that is a multiple of the piece."""
+    parts = [1, 1, 2, 16, 17, 3, 33, 15]
+    lengths = [shift] if shift else []
+    while sum(lengths) < n:
+        lengths += [p * piece for p in parts] + [piece // 2, piece // 2, 1, 16 * piece - 1, 17 * piece + 1, piece - 1]
+    ids = torch.repeat_interleave(torch.arange(len(lengths)) * 2 + 1, torch.tensor(lengths))[:n]      # every other row has no token
+    vocab, hidden = 2 * len(lengths) + 2, 24
+    g = torch.Generator().manual_seed(n + shift)
+    ids = ids[torch.randperm(n, generator=g)].to(torch.int32)
+    dout = torch.randint(-8, 9, (n, hidden), generator=g)
+    want = torch.zeros(vocab, hidden, dtype=torch.int64).index_add_(0, ids.long(), dout)
+    for t in (torch.float32, torch.bfloat16):
+        dtable, dpos, bad = sfb.embedding_grad(dout.to(t).view(2, n // 2, hidden).cuda(), ids.view(2, n // 2).cuda(), vocab, positions=True)
+        assert int(bad) == 0
+        assert torch.equal(dtable.cpu().long(), want)
+        assert torch.equal(dpos.cpu().long(), dout.view(2, n // 2, hidden).sum(0))
+    start = torch.randint(-8, 9, (vocab, hidden), generator=g).float().cuda()
+    added, _, _ = sfb.embedding_grad(dout.float().view(1, n, hidden).cuda(), ids.view(1, n).cuda(), vocab, out=start.clone())
+    assert torch.equal(added.cpu().long(), want + start.cpu().long())
