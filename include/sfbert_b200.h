@@ -234,7 +234,10 @@ int sfb_fused_attention_stats(sfb_stream_t stream, const void *nn_lut, const voi
  * pair of block-rows (columns) with one that does, masked or not.
  * workspace: device memory of sfb_attention_backward_workspace() bytes, 16-byte aligned, for this call alone; aligned is 1 where
  * q, k, v, dout, dq, dk, dv and mask are 16-byte aligned and the pitches multiples of 8 elements, 0 otherwise or where that is unknown
- * (which 16-bit operands with blocks and heads of 64 need more workspace for).  No counterpart in the reference. */
+ * (which 16-bit operands with blocks and heads of 64 need more workspace for).  It is 8 bytes per row and head for 16-bit operands with blocks and
+ * heads of 64 that are aligned, on at most 256 block-rows or with rows and columns of at most 128 blocks; other calls also keep P and dS of
+ * some (batch, head) pairs there at a time, 4 bytes per kept score (fp32: 12): up to 512 MB, or one pair's where that is more (16-bit, causal: 2 GB
+ * at 32768 positions).  No counterpart in the reference. */
 uint64_t sfb_attention_backward_workspace(int dtype, uint32_t block_size, uint32_t blocks, uint32_t batch_dim, uint32_t ctx_blks,
                                           uint32_t head_dim, uint32_t state_dim, uint32_t nn_max, uint32_t tn_max, int aligned);
 int sfb_attention_backward_recompute(sfb_stream_t stream, const void *nt_lut, const void *nn_lut, const void *tn_lut, const void *q,

@@ -338,7 +338,10 @@ def fused_attention_stats(q, k, v, lay, scale=None, use_mask=False, out=None):
 
 def attention_backward_recompute(q, k, v, o, do, lse, lay, scale=None, use_mask=False, out=None):
     """The gradients (dq, dk, dv) of fused_attention_stats' output, with the probabilities made again from lse: nothing of the size
-    of the scores was kept.  Any type, block and head size of the forward call; scale and use_mask as there.  q, k, v share a pitch, o and do
+    of the scores is kept from one call to the other.  16-bit operands with blocks and heads of 64, all 16-byte aligned, have nothing of that size
+    during the call either, as long as the layout has at most 256 block-rows or no row and column of more than 128 blocks.  Other calls go a slower
+    way, by way of P and dS of some heads at a time in memory that torch's allocator has back after the call: up to 512 MB, or one head's where that
+    is more (4 bytes per kept score, fp32 12: 2 GB for 16-bit causal heads of 32768 positions).  Any type, block and head size of the forward call; scale and use_mask as there.  q, k, v share a pitch, o and do
     have their own; out: three views to write to, of one pitch (such as the three parts of a packed [B, L, 3, H, d] gradient).  The same
     inputs give the same bits.  With 16-bit operands P and dS are rounded to their type as operands of the products.  The layout's tables
     by columns are built on first use (lay.tn_lut), which reads a number back: once before a call is captured in a graph."""

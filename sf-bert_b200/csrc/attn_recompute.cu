@@ -618,7 +618,8 @@ static int launch_products(cudaStream_t s, const ProductArgs &k)
 // How many (batch, head) pairs go through the workspace at a time: block-rows for every SM to have 64 (us with 16 / 32 / 64:
 // bf16, blocks of 32, d 64, strided, 4 x 12 heads of 2048 positions 242 / 212 / 210, 8 x 16 heads 598 / 528 / 496; what L2 could have kept of P and dS
 // counts for less than the SMs that have nothing left to do at the end of each launch), as long as P and dS take no more
-// than 512 MB; one at least; parts of about the same size.
+// than 512 MB, but one at least: a pair is not divided, so that the workspace is as large as P and dS of a whole one where that is more (bf16, blocks of
+// 64, causal: 0.5 GB at 16384 positions, 2 GB at 32768, 8 GB at 65536; fp32 three times as much).  Parts of about the same size.
 constexpr uint64_t kRowsPerSm = 64, kMostSms = 148, kMostBytes = 512ull << 20;
 static uint64_t score_bytes(int dtype) { return dtype == SFB_F32 ? 6 : 2; }      // three planes, or the operands' type
 static uint32_t pairs_at_a_time(int dtype, uint32_t bs, uint32_t nb, uint32_t blocks, uint32_t B, uint32_t H)

@@ -125,3 +125,27 @@ def test_what_is_not_a_sequence_of_tensors(sfb):
     for out in (3, (1.0, 2.0, 3.0)):
         with pytest.raises(TypeError):
             sfb.attention_backward_recompute(X, X, X, X, X, S, lay(), out=out)
+
+
+def test_workspaces_of_large_heads(sfb):
+    """8 bytes per row where nothing of the scores is in memory; otherwise P and dS of some (batch, head) pairs, up to 512 MB, or of one where that is more."""
+    f = sfb.lib.sfb_attention_backward_workspace
+    mb = 1 << 20
+
+    def asked(dtype, bs, nb, blocks, d, B=1, H=12, nn=None, tn=None, aligned=1):
+        return f(dtype, bs, blocks, B, nb, H, d, nb if nn is None else nn, nb if tn is None else tn, aligned) - 8 * B * H * nb * bs
+
+    def causal(nb):
+        return nb * (nb + 1) // 2
+
+    assert asked(1, 64, 256, causal(256), 64) == 0                                         # the tensor-core kernels up to 256 block-rows
+    assert asked(1, 64, 257, causal(257), 64) == 4 * causal(257) * 4096                    # one pair: 518 MB
+    assert asked(1, 64, 4096, 4096 * 20, 64, nn=128, tn=128) == 0                          # any number of short rows and columns
+    assert 0 < asked(1, 64, 4096, 4096 * 20, 64, nn=129, tn=128) <= 1280 * mb
+    assert 0 < asked(1, 64, 256, causal(256), 64, aligned=0) <= 514 * mb
+    assert asked(1, 64, 512, causal(512), 64) == 4 * causal(512) * 4096 > 2000 * mb        # 32768 positions
+    assert asked(2, 64, 1024, causal(1024), 128) == 4 * causal(1024) * 4096                # 65536
+    assert asked(0, 32, 512, causal(512), 64) == 12 * causal(512) * 1024 > 1500 * mb
+    for dtype, bs, nb, blocks, d in ((1, 32, 64, 64 * 20, 64), (2, 64, 32, 300, 128), (0, 32, 64, 2080, 64), (0, 64, 16, 256, 128)):
+        for H in (1, 12, 400):
+            assert 0 < asked(dtype, bs, nb, blocks, d, 8, H) <= 512 * mb
