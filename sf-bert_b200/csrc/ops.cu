@@ -166,7 +166,7 @@ static uint64_t constants_bytes(uint32_t B, uint32_t L, uint32_t H) { return ((u
 extern "C" uint64_t sfb_attention_backward_workspace(int dtype, uint32_t block_size, uint32_t blocks, uint32_t batch_dim, uint32_t ctx_blks,
                                                      uint32_t head_dim, uint32_t state_dim, uint32_t nn_max, uint32_t tn_max, int aligned)
 {
-    if (!valid_dtype(dtype) || (block_size != 32 && block_size != 64) || !batch_dim || !head_dim) return 0;
+    if (!valid_dtype(dtype) || (block_size != 32 && block_size != 64) || !batch_dim || !head_dim || !ctx_blks || (uint64_t)ctx_blks * block_size >= (1ull << 31)) return 0;
     const uint64_t rows = 2 * constants_bytes(batch_dim, ctx_blks * block_size, head_dim);
     const AttnDims p = {batch_dim, head_dim, state_dim, ctx_blks, ctx_blks, blocks, 0, 0};
     if (aligned && tc_backward_recompute_supported(dtype, block_size, p, nn_max, tn_max)) return rows;

@@ -149,3 +149,15 @@ def test_workspaces_of_large_heads(sfb):
     for dtype, bs, nb, blocks, d in ((1, 32, 64, 64 * 20, 64), (2, 64, 32, 300, 128), (0, 32, 64, 2080, 64), (0, 64, 16, 256, 128)):
         for H in (1, 12, 400):
             assert 0 < asked(dtype, bs, nb, blocks, d, 8, H) <= 512 * mb
+
+
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+@pytest.mark.parametrize("bs,d", [(32, 40), (64, 64)])
+def test_workspaces_of_nothing(sfb, dtype, bs, d):
+    """A sequence without blocks, a batch without elements, positions that no call takes: no memory, and no division by their number."""
+    f = sfb.lib.sfb_attention_backward_workspace
+    for blocks, B, nb, H in ((0, 2, 0, 4), (5, 2, 0, 4), (0, 0, 3, 4), (0, 2, 3, 0), (4, 1, 1 << 26, 1)):
+        for aligned in (0, 1):
+            assert f(dtype, bs, blocks, B, nb, H, d, 0, 0, aligned) == 0
+    assert f(dtype, bs, 0, 2, 3, 4, d, 0, 0, 0) == 2 * 4 * 2 * 3 * bs * 4                  # rows without blocks: two numbers each
+    assert sfb.lib.sfb_embedding_grad_workspace(0, 0, 0, 0) >= 0 and sfb.lib.sfb_clip_grad_norm_workspace(0) >= 8
