@@ -258,3 +258,48 @@ def test_runs_at_the_ends_of_pieces(sfb, n, piece, shift):
     start = torch.randint(-8, 9, (vocab, hidden), generator=g).float().cuda()
     added, _, _ = sfb.embedding_grad(dout.float().view(1, n, hidden).cuda(), ids.view(1, n).cuda(), vocab, out=start.clone())
     assert torch.equal(added.cpu().long(), want + start.cpu().long())
+
+
+# ---- threads ----------------------------------------------------------------------------------------------------------------------
+def test_calls_from_several_threads(sfb):
+    """Each thread on a stream of its own, all of them at once (a call lets other threads run while it launches): the bits of calls one by one."""
+    import threading
+    bs, nb, n = 64, 6, 4
+    lay = plan(sfb, layout("stride", nb), bs)
+    lay.tn_lut
+    sets = []
+    for i in range(n):
+        dtype = ("f16", "bf16", "f32", "f16")[i]
+        dout, ids = tokens(3000 if i % 2 else 300, 200, 64, 60 + i)
+        grads = [torch.randn(7000 + i, device="cuda"), torch.randn(33, 5, device="cuda")]
+        sets.append(([x.cuda() for x in operands(2, nb * bs, 3, 64, dtype, 50 + i)], dout, ids, grads))
+
+    def step(x, dout, ids, grads):
+        q, k, v, do = x
+        o, lse = sfb.fused_attention_stats(q, k, v, lay)
+        out = [torch.empty_like(g) for g in grads]
+        norm = sfb.clip_grad_norm(grads, 1.0, out=out)
+        return (o, lse, norm, *out, *sfb.attention_backward_recompute(q, k, v, o, do, lse, lay), *sfb.embedding_grad(dout, ids, 200, positions=True))
+
+    want = [step(*s) for s in sets]
+    torch.cuda.synchronize()
+    got, errors = [None] * n, []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(10):
+                    got[i] = step(*sets[i])
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:                               # reported by the main thread
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(n)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+    for a, b in zip(want, got):
+        for x, y in zip(a, b):
+            assert torch.equal(x, y)
